@@ -38,6 +38,10 @@ extern "C" {
 #define SGNN_ERR_HIP          -3   /* a HIP call failed; see sgnn_last_error() */
 #define SGNN_ERR_UNSUPPORTED  -4
 
+/* element types of the entry points that take more than fp32 */
+#define SGNN_F32               0
+#define SGNN_BF16              1
+
 /* build flags */
 #define SGNN_STRIP_DIAG        1   /* drop (i,i) entries of the input first: model/SGNN.py:497-501 */
 #define SGNN_DROP_ZEROS        2   /* drop entries whose merged value is 0 (scipy's sparse subtraction does) */
@@ -601,6 +605,43 @@ int sgnn_head_xent_f32(int64_t B, int64_t D, int64_t C, const float* E, int64_t 
                        const int64_t* labels, int64_t n_labels, const int64_t* idx, float* loss,
                        float* dE, int64_t ldde, float* dWt, int64_t lddw,
                        void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * A layer's input kept in 8 bits between forward and backward.  No reference counterpart (its
+ * autograd keeps every layer input in fp32: model/GCN.py:14-16, model/SGC.py:14).
+ *
+ * a = x > 0 ? x : slope * x, slope >= 0 (the layer's inner activation: 1 none, 0 ReLU), computed
+ * in 32 bits, is held as one byte per element and one byte per group of 32 consecutive features
+ * of a row:
+ *   codes  n rows of 32 * ceil(F / 32) bytes, 16-byte aligned; two's complement
+ *   steps  n rows of ceil(F / 32) bytes: s + 127 of the group's step 2^s, s >= -125; 255 marks a
+ *          group that holds a NaN or an infinity, all of which reads back as NaN
+ *   slope == 1:  code = rint(a / 2^s), value = code * 2^s, s the smallest with |code| <= 127 (at
+ *                most 121: what lies beyond 127.5 * 2^121 is held as 127 * 2^121);
+ *   otherwise:   code = ceil(a / 2^s) - 1, value = (code + 1/2) * 2^s, s the smallest with
+ *                |a| <= 128 * 2^s; code < 0 exactly where x > 0 is false (NaN groups too); with
+ *                slope 0 negative codes stand for 0.
+ * An element is off by at most half its group's step.  `dtype` is SGNN_F32 or SGNN_BF16 and holds
+ * for x, act, out, grad, dx and dW alike; each result is rounded once, to nearest even.
+ *
+ * sgnn_save8            x -> codes, steps and, when act is given, a itself.
+ * sgnn_restore8         the values, exact in either type.
+ * sgnn_saved8_input_grad  dx = code < 0 ? slope * grad : grad (slope 0: 0 there, whatever grad
+ *                       holds); dx may be grad itself; slope 1 is refused (nothing to do).
+ * sgnn_saved8_weight_grad  dW = grad^T . value, H x F, sums in 32 bits in a fixed order, products
+ *                       exact; `workspace` of sgnn_saved8_weight_grad_workspace_bytes bytes,
+ *                       contents irrelevant.  Any row strides; 16-byte aligned rows are faster.
+ */
+int sgnn_save8(int dtype, int64_t n, int64_t F, const void* x, int64_t ldx, float slope, void* codes, void* steps,
+               void* act, int64_t ldact, void* stream);
+int sgnn_restore8(int dtype, int64_t n, int64_t F, const void* codes, const void* steps, float slope, void* out,
+                  int64_t ldo, void* stream);
+int sgnn_saved8_input_grad(int dtype, int64_t n, int64_t F, const void* codes, float slope, const void* grad,
+                           int64_t ldg, void* dx, int64_t lddx, void* stream);
+size_t sgnn_saved8_weight_grad_workspace_bytes(int64_t n, int64_t F, int64_t H);
+int sgnn_saved8_weight_grad(int dtype, int64_t n, int64_t F, int64_t H, const void* codes, const void* steps,
+                            float slope, const void* grad, int64_t ldg, void* dW, int64_t lddw, void* workspace,
+                            size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -23,6 +23,8 @@ SAMPLE_SKIP_SELF = 1
 ADAM_STATE_WORDS = 1026
 LOOPS_NONE, LOOPS_ADD, LOOPS_REMAINING = 0, 1, 2
 EPI_SCALE_ROW, EPI_SCALE_ROW2 = 0, 1
+F32, BF16 = 0, 1
+SAVED8_GROUP = 32
 # tile-group operand state (sgnn_tilegroup_state_bytes): 32-bit words; the per-feature maxima follow the header
 TG_STATE_FLAG, TG_STATE_TINY, TG_STATE_TINY_LIMIT, TG_STATE_HEAD_WORDS = 1, 4, 6, 16
 # words 2 and 3: the exact max / split passes ran behind a provisional split; the maxima are a sample's
@@ -124,6 +126,14 @@ SIGNATURES = {
                                       c_void_p, c_int64, c_void_p, c_size_t, c_void_p]),
     "sgnn_sq_err_f32": (c_int, [c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_float,
                                 c_void_p, c_void_p, c_int64, c_void_p, c_size_t, c_void_p]),
+    "sgnn_save8": (c_int, [c_int, c_int64, c_int64, c_void_p, c_int64, c_float, c_void_p, c_void_p, c_void_p, c_int64,
+                           c_void_p]),
+    "sgnn_restore8": (c_int, [c_int, c_int64, c_int64, c_void_p, c_void_p, c_float, c_void_p, c_int64, c_void_p]),
+    "sgnn_saved8_input_grad": (c_int, [c_int, c_int64, c_int64, c_void_p, c_float, c_void_p, c_int64, c_void_p, c_int64,
+                                       c_void_p]),
+    "sgnn_saved8_weight_grad_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
+    "sgnn_saved8_weight_grad": (c_int, [c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_float, c_void_p, c_int64,
+                                        c_void_p, c_int64, c_void_p, c_size_t, c_void_p]),
     "sgnn_sample_block_f32": (c_int, [c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int,
                                       c_void_p, c_int64, c_void_p]),
 }

@@ -1,0 +1,625 @@
+// A layer's input kept in 8 bits between its forward and its backward pass.
+//
+// a = x > 0 ? x : slope * x (the inner activation of a layer) is held as one byte per element
+// plus one byte per group of 32 consecutive features of a row, the group's power-of-two step
+// 2^s (biased by 127; 255 marks a group that holds a NaN or an infinity and decodes to NaN):
+//   slope == 1 : code = rint(a / 2^s),     value = code * 2^s,         s = smallest with |code| <= 127
+//                (s <= 121: the last numbers before infinity are held as +-127 * 2^121)
+//   otherwise  : code = ceil(a / 2^s) - 1, value = (code + 1/2) 2^s,   s = smallest with |a| <= 128 * 2^s
+// In the second form a code is negative exactly where "x > 0" is false, so the same byte also
+// answers for the activation's derivative; with slope 0 the negative codes stand for 0 and the
+// group's range is that of its positive elements.  Either form is off by at most half a step.
+//
+// Steps are powers of two so that every value (at most 8 significant bits) is a bf16 number
+// without any rounding: the weight gradient dW = grad^T . value runs on the bf16 matrix
+// instructions with an exact left operand, and coding is exact in 32 bits, too (a multiplication
+// by a power of two, one rounding to a whole number).
+#include "common.h"
+
+namespace {
+
+constexpr int kGroup = 32;
+constexpr int kMinBiased = 2;                     // s >= -125: half a step is still a normal number
+constexpr int kMaxBiased = 248;                   // s <= 121: 127.5 steps are still finite
+constexpr int kBadGroup = 255;
+
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+struct Bf16 { uint16_t bits; };
+
+__device__ __forceinline__ float widen(float v) { return v; }
+__device__ __forceinline__ float widen(Bf16 v) { return __uint_as_float(unsigned(v.bits) << 16); }
+template <typename T> __device__ __forceinline__ T narrow(float v);
+template <> __device__ __forceinline__ float narrow<float>(float v) { return v; }
+template <> __device__ __forceinline__ Bf16 narrow<Bf16>(float v) {          // nearest even, the only rounding of a result
+  unsigned u = __float_as_uint(v);
+  if ((u & 0x7fffffffu) > 0x7f800000u) return Bf16{uint16_t(0x7fc0u)};
+  return Bf16{uint16_t((u + 0x7fffu + ((u >> 16) & 1u)) >> 16)};
+}
+
+// slope 0 is a selection, not a product: -inf becomes 0 there, NaN stays NaN
+__device__ __forceinline__ float activate(float x, float slope) {
+  if (x > 0.f) return x;
+  if (slope == 0.f) return x != x ? x : 0.f;
+  return slope * x;
+}
+
+__device__ __forceinline__ int step_of(unsigned peak_bits, bool plain) {      // peak = max |a|, as bits
+  const int e = int(peak_bits >> 23);
+  const unsigned frac = peak_bits & 0x7fffffu;
+  if (e == 255) return kBadGroup;
+  // plain: 127.5 of 128 would round to 128; else a power of two is still held by its own exponent
+  const int b = plain ? e - 6 + (frac >= 0x7f0000u ? 1 : 0) : e - 6 - (frac == 0u ? 1 : 0);
+  return b < kMinBiased ? kMinBiased : b > kMaxBiased ? kMaxBiased : b;
+}
+__device__ __forceinline__ float step_value(int biased) {      // NaN for a bad group
+  return biased == kBadGroup ? __uint_as_float(0x7fc00000u) : __uint_as_float(unsigned(biased) << 23);
+}
+
+// `u` = code + 128 as a number: value = (u - (plain ? 128 : 127.5)) * step, exact.  With slope 0
+// the clamp at 127.5 makes the negative codes exactly 0 and leaves a NaN step NaN.
+__device__ __forceinline__ float decode(float u, float step, float offset, float floor_u) {
+  return (fmaxf(u, floor_u) + offset) * step;
+}
+
+// Elements per thread of the element-wise passes: 16 bytes of the wide operand.
+template <typename T> struct Lane { static constexpr int kElems = 16 / sizeof(T); };
+
+template <typename T, int V>
+__device__ __forceinline__ void load_row(const T* p, int left, bool wide, T (&out)[V]) {
+  if (wide && left >= V) {
+    const u32x4 w = *reinterpret_cast<const u32x4*>(p);
+    __builtin_memcpy(&out, &w, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = i < left ? p[i] : narrow<T>(0.f);
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_row(T* p, int left, bool wide, const T (&v)[V]) {
+  if (wide && left >= V) {
+    u32x4 w;
+    __builtin_memcpy(&w, &v, 16);
+    *reinterpret_cast<u32x4*>(p) = w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i < left) p[i] = v[i];
+  }
+}
+
+// A workgroup owns `rows` whole rows; `per_row` = lanes a row takes (a multiple of a group's
+// lanes, so that a group never leaves its wavefront's aligned block of lanes).
+constexpr int kEltThreads = 256;
+
+template <typename T>
+__global__ __launch_bounds__(kEltThreads) void k_save8(int64_t n, int F, const T* __restrict__ x, int64_t ldx,
+                                                       bool wide, float slope, int rows, int per_row,
+                                                       uint8_t* __restrict__ codes, uint8_t* __restrict__ steps,
+                                                       T* __restrict__ act, int64_t ldact, bool act_wide) {
+  constexpr int V = Lane<T>::kElems, kPer = kGroup / V;
+  const bool plain = slope == 1.f;
+  const int groups = (F + kGroup - 1) / kGroup;
+  const int64_t row0 = int64_t(blockIdx.x) * rows;
+  const int count = int(n - row0 < rows ? n - row0 : rows) * per_row;
+  for (int i = threadIdx.x; i < count; i += kEltThreads) {
+    const int lr = i / per_row, at = i - lr * per_row;
+    const int64_t r = row0 + lr;
+    const int f = at * V, left = F - f;
+    T raw[V];
+    load_row<T, V>(x + r * ldx + f, left, wide, raw);
+    float a[V];
+    unsigned peak = 0;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      a[e] = activate(widen(raw[e]), slope);
+      const unsigned m = __float_as_uint(a[e]) & 0x7fffffffu;                 // a NaN is larger than any number here
+      peak = m > peak ? m : peak;
+    }
+    if (act != nullptr) {
+      T out[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) out[e] = narrow<T>(a[e]);
+      store_row<T, V>(act + r * ldact + f, left, act_wide, out);
+    }
+#pragma unroll
+    for (int off = 1; off < kPer; off <<= 1) {
+      const unsigned o = unsigned(__shfl_xor(int(peak), off));
+      peak = o > peak ? o : peak;
+    }
+    const int biased = step_of(peak, plain);
+    const float inv = biased == kBadGroup ? 0.f : __uint_as_float(unsigned(254 - biased) << 23);
+    unsigned packed[V / 4];
+#pragma unroll
+    for (int w = 0; w < V / 4; ++w) {
+      packed[w] = 0;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const float s = biased == kBadGroup ? 0.f : a[4 * w + b] * inv;
+        int q;
+        if (plain) {
+          q = int(rintf(s));
+          q = q > 127 ? 127 : q < -127 ? -127 : q;             // beyond 127.5 * 2^121 only
+        } else {
+          q = int(ceilf(s)) - 1;
+          if (widen(raw[4 * w + b]) > 0.f) q = q < 0 ? 0 : (q > 127 ? 127 : q);
+          else q = q > -1 ? -1 : (q < -128 ? -128 : q);
+        }
+        packed[w] |= (unsigned(q) & 0xffu) << (8 * b);
+      }
+    }
+    unsigned* dst = reinterpret_cast<unsigned*>(codes + r * (int64_t(groups) * kGroup) + f);
+    if constexpr (V == 4) dst[0] = packed[0];
+    else *reinterpret_cast<u32x2*>(dst) = u32x2{packed[0], packed[1]};
+    if (at % kPer == 0) steps[r * groups + at / kPer] = uint8_t(biased);
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kEltThreads) void k_restore8(int64_t n, int F, const uint8_t* __restrict__ codes,
+                                                          const uint8_t* __restrict__ steps, float slope, int rows,
+                                                          int per_row, T* __restrict__ out, int64_t ldo, bool wide) {
+  constexpr int V = Lane<T>::kElems, kPer = kGroup / V;
+  const float offset = slope == 1.f ? -128.f : -127.5f, floor_u = slope == 0.f ? 127.5f : 0.f;
+  const int groups = (F + kGroup - 1) / kGroup;
+  const int64_t row0 = int64_t(blockIdx.x) * rows;
+  const int count = int(n - row0 < rows ? n - row0 : rows) * per_row;
+  for (int i = threadIdx.x; i < count; i += kEltThreads) {
+    const int lr = i / per_row, at = i - lr * per_row;
+    const int64_t r = row0 + lr;
+    const int f = at * V;
+    const unsigned* src = reinterpret_cast<const unsigned*>(codes + r * (int64_t(groups) * kGroup) + f);
+    const float step = step_value(steps[r * groups + at / kPer]);
+    T v[V];
+#pragma unroll
+    for (int w = 0; w < V / 4; ++w) {
+      const unsigned u = src[w] ^ 0x80808080u;
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        v[4 * w + b] = narrow<T>(decode(float((u >> (8 * b)) & 0xffu), step, offset, floor_u));
+    }
+    store_row<T, V>(out + r * ldo + f, F - f, wide, v);
+  }
+}
+
+// dx = grad where the code says x > 0, slope * grad elsewhere; dx may be grad itself.
+template <typename T>
+__global__ __launch_bounds__(kEltThreads) void k_input_grad8(int64_t n, int F, const uint8_t* __restrict__ codes,
+                                                             float slope, int rows, int per_row, const T* g,
+                                                             int64_t ldg, bool g_wide, T* dx, int64_t lddx,
+                                                             bool dx_wide) {
+  constexpr int V = Lane<T>::kElems;
+  const int groups = (F + kGroup - 1) / kGroup;
+  const int64_t row0 = int64_t(blockIdx.x) * rows;
+  const int count = int(n - row0 < rows ? n - row0 : rows) * per_row;
+  for (int i = threadIdx.x; i < count; i += kEltThreads) {
+    const int lr = i / per_row, at = i - lr * per_row;
+    const int64_t r = row0 + lr;
+    const int f = at * V, left = F - f;
+    if (left <= 0) continue;
+    const unsigned* src = reinterpret_cast<const unsigned*>(codes + r * (int64_t(groups) * kGroup) + f);
+    T v[V];
+    load_row<T, V>(g + r * ldg + f, left, g_wide, v);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const bool negative = (src[e / 4] >> (8 * (e % 4) + 7)) & 1u;
+      if (negative) v[e] = slope == 0.f ? narrow<T>(0.f) : narrow<T>(slope * widen(v[e]));
+    }
+    store_row<T, V>(dx + r * lddx + f, left, dx_wide, v);
+  }
+}
+
+// ---------------------------------------------------------------------------------
+// dW[h][f] = sum_r grad[r][h] * value[r][f]: a product whose reduction runs over the rows, both
+// operands row-major over it.  A workgroup forms a BH x BF tile of dW over a chunk of rows, 32
+// rows at a time: codes are decoded and grad split into bf16 planes on the way from registers to
+// LDS, both kept row-major there, and the matrix instructions' operands (8 consecutive rows of
+// one column per lane) come out of the transposing LDS read.  grad in 32 bits is the sum of three
+// bf16 numbers (8 + 8 + 8 bits of its mantissa, cut off, not rounded, so the sum is exact), which
+// makes every product exact and the sums those of 32-bit arithmetic; bf16 grad takes one plane.
+// Chunks go to the workspace and are added in chunk order by a second launch.
+constexpr int kRowsStep = 32;
+
+template <int COLS>                               // byte offset of (row, col) in a row-major bf16 slab of COLS columns
+__device__ __forceinline__ int slab_at(int k, int col) {
+  // 64-byte blocks of a row are permuted by the row so that the 4 rows x 64 bytes which a
+  // transposing read touches at once fall into different banks
+  constexpr int nb = COLS / 32;
+  const int swz = nb >= 4 ? (k & 3) : nb == 2 ? ((k >> 1) & 1) : 0;
+  return k * (COLS * 2) + (((col >> 5) ^ swz) << 6) + (col & 31) * 2;
+}
+
+template <int COLS>
+__device__ __forceinline__ bf16x8 slab_frag(const char* slab, int k0, int c0, int lane) {
+  const int k = k0 + 8 * (lane >> 5) + ((lane & 15) >> 2);
+  const int c = c0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(slab + slab_at<COLS>(k, c)));
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(slab + slab_at<COLS>(k + 4, c)));
+  bf16x8 r;
+  __builtin_memcpy(&r, &lo, 8);
+  __builtin_memcpy(reinterpret_cast<char*>(&r) + 8, &hi, 8);
+  return r;
+}
+
+// the high halves of two floats as a bf16 pair
+__device__ __forceinline__ unsigned high_halves(float lo, float hi) {
+  return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+}
+
+__device__ __forceinline__ void split3(float v, float& a, float& b, float& c) {
+  const unsigned u = __float_as_uint(v);
+  a = __uint_as_float(u & 0xffff0000u);
+  const float r = v - a;
+  b = __uint_as_float(__float_as_uint(r) & 0xffff0000u);
+  c = r - b;
+  if ((u & 0x7f800000u) == 0x7f800000u) {         // infinities and NaN live in the first plane only
+    a = (u & 0x7fffffu) ? __uint_as_float(0x7fc00000u) : v;
+    b = c = 0.f;
+  }
+}
+
+template <typename T, int BH, int BF, int WH, int WF>
+__global__ __launch_bounds__(64 * WH * WF) void k_weight_grad8(
+    int64_t n, int F, int H, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ steps, float slope,
+    const T* __restrict__ g, int64_t ldg, bool wide, int64_t chunk_rows, int chunks, int tiles_f, int tiles_h,
+    T* __restrict__ dW, int64_t lddw, float* __restrict__ partial) {
+  constexpr int kThreads = 64 * WH * WF;
+  constexpr int P = sizeof(T) == 4 ? 3 : 1;
+  constexpr int MH = BH / (32 * WH), MF = BF / (32 * WF);       // 32 x 32 blocks of a wavefront
+  constexpr int kCodeLoads = kRowsStep * BF / 16 / kThreads;    // 16 codes each
+  constexpr int GV = 8;                                         // grad elements a thread loads at once
+  constexpr int kGradSlots = kRowsStep * BH / GV;
+  constexpr int kGradLoads = (kGradSlots + kThreads - 1) / kThreads;
+  __shared__ __align__(128) char sB[kRowsStep * BF * 2];
+  __shared__ __align__(128) char sA[P * kRowsStep * BH * 2];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int wh = wave / WF, wf = wave % WF;
+  // the tiles of one chunk of rows go to one XCD, one after the other: they share grad and codes through its L2
+  const int tiles = tiles_f * tiles_h;
+  const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
+  const int tile = slot % tiles, chunk = (slot / tiles) * 8 + xcd;
+  if (chunk >= chunks) return;                    // the whole workgroup
+  const int f0 = (tile % tiles_f) * BF, h0 = (tile / tiles_f) * BH;
+  const int groups = (F + kGroup - 1) / kGroup, ldq = groups * kGroup;
+  const int64_t first = int64_t(chunk) * chunk_rows;
+  const int64_t last = first + chunk_rows < n ? first + chunk_rows : n;
+  const float offset = slope == 1.f ? -128.f : -127.5f, floor_u = slope == 0.f ? 127.5f : 0.f;
+
+  u32x4 rc[kCodeLoads];
+  int rs[kCodeLoads];
+  T rg[kGradLoads][GV];
+  const auto fetch = [&](int64_t r0) {
+#pragma unroll
+    for (int l = 0; l < kCodeLoads; ++l) {
+      const int s = t + l * kThreads, k = s / (BF / 16), f = f0 + (s % (BF / 16)) * 16;
+      const int64_t r = r0 + k;
+      rc[l] = u32x4{0, 0, 0, 0};
+      rs[l] = kMinBiased;
+      if (r < last && f < ldq) {
+        rc[l] = *reinterpret_cast<const u32x4*>(codes + r * ldq + f);
+        rs[l] = steps[r * groups + (f >> 5)];
+      }
+    }
+#pragma unroll
+    for (int l = 0; l < kGradLoads; ++l) {
+      const int s = t + l * kThreads, k = s / (BH / GV), h = h0 + (s % (BH / GV)) * GV;
+      const int64_t r = r0 + k;
+#pragma unroll
+      for (int e = 0; e < GV; ++e) rg[l][e] = narrow<T>(0.f);
+      if (s < kGradSlots && r < last && h < H) {
+        const T* p = g + r * ldg + h;
+        if (wide && h + GV <= H) {
+#pragma unroll
+          for (int q = 0; q < GV * int(sizeof(T)) / 16; ++q) {
+            const u32x4 w = reinterpret_cast<const u32x4*>(p)[q];
+            __builtin_memcpy(reinterpret_cast<char*>(&rg[l][0]) + 16 * q, &w, 16);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < GV; ++e)
+            if (h + e < H) rg[l][e] = p[e];
+        }
+      }
+    }
+  };
+  const auto stage = [&]() {
+#pragma unroll
+    for (int l = 0; l < kCodeLoads; ++l) {
+      const int s = t + l * kThreads, k = s / (BF / 16), c = (s % (BF / 16)) * 16;
+      const float step = step_value(rs[l]);
+      unsigned out[8];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const unsigned u = rc[l][w] ^ 0x80808080u;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const float lo = decode(float((u >> (16 * b)) & 0xffu), step, offset, floor_u);
+          const float hi = decode(float((u >> (16 * b + 8)) & 0xffu), step, offset, floor_u);
+          out[2 * w + b] = high_halves(lo, hi);
+        }
+      }
+      u32x4* dst = reinterpret_cast<u32x4*>(sB + slab_at<BF>(k, c));
+      dst[0] = u32x4{out[0], out[1], out[2], out[3]};
+      dst[1] = u32x4{out[4], out[5], out[6], out[7]};
+    }
+#pragma unroll
+    for (int l = 0; l < kGradLoads; ++l) {
+      const int s = t + l * kThreads, k = s / (BH / GV), c = (s % (BH / GV)) * GV;
+      if (s < kGradSlots) {
+        if constexpr (P == 1) {
+          u32x4 w;
+          __builtin_memcpy(&w, &rg[l][0], 16);
+          *reinterpret_cast<u32x4*>(sA + slab_at<BH>(k, c)) = w;
+        } else {
+          u32x4 pl[3];
+#pragma unroll
+          for (int e = 0; e < GV; e += 2) {
+            float a0, b0, c0, a1, b1, c1;
+            split3(widen(rg[l][e]), a0, b0, c0);
+            split3(widen(rg[l][e + 1]), a1, b1, c1);
+            pl[0][e / 2] = high_halves(a0, a1);
+            pl[1][e / 2] = high_halves(b0, b1);
+            pl[2][e / 2] = high_halves(c0, c1);
+          }
+#pragma unroll
+          for (int p = 0; p < 3; ++p)
+            *reinterpret_cast<u32x4*>(sA + p * (kRowsStep * BH * 2) + slab_at<BH>(k, c)) = pl[p];
+        }
+      }
+    }
+  };
+
+  f32x16 acc[MH][MF];
+#pragma unroll
+  for (int i = 0; i < MH; ++i)
+#pragma unroll
+    for (int j = 0; j < MF; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+
+  fetch(first);
+  for (int64_t r0 = first; r0 < last; r0 += kRowsStep) {
+    __syncthreads();                              // the previous step's reads are done
+    stage();
+    if (r0 + kRowsStep < last) fetch(r0 + kRowsStep);
+    __syncthreads();
+#pragma unroll
+    for (int k0 = 0; k0 < kRowsStep; k0 += 16) {
+      bf16x8 b[MF];
+#pragma unroll
+      for (int j = 0; j < MF; ++j) b[j] = slab_frag<BF>(sB, k0, (wf * MF + j) * 32, lane);
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+#pragma unroll
+        for (int i = 0; i < MH; ++i) {
+          const bf16x8 a = slab_frag<BH>(sA + p * (kRowsStep * BH * 2), k0, (wh * MH + i) * 32, lane);
+#pragma unroll
+          for (int j = 0; j < MF; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b[j], acc[i][j], 0, 0, 0);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < MH; ++i)
+#pragma unroll
+    for (int j = 0; j < MF; ++j) {
+      const int f = f0 + (wf * MF + j) * 32 + (lane & 31);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int h = h0 + (wh * MH + i) * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+        if (h < H && f < F) {
+          if (chunks > 1) partial[(int64_t(chunk) * H + h) * F + f] = acc[i][j][e];
+          else dW[int64_t(h) * lddw + f] = narrow<T>(acc[i][j][e]);
+        }
+      }
+    }
+}
+
+// dW = sum of the chunks' tiles: four quarters of the chunks in order, then the quarters in order.
+template <typename T>
+__global__ __launch_bounds__(256) void k_weight_grad_sum8(int F, int64_t total, int chunks,
+                                                          const float* __restrict__ partial, T* __restrict__ dW,
+                                                          int64_t lddw) {
+  __shared__ float part[4][64];
+  const int c = threadIdx.x & 63, q = threadIdx.x >> 6;
+  const int64_t e = int64_t(blockIdx.x) * 64 + c;
+  const int lo = int(int64_t(chunks) * q / 4), hi = int(int64_t(chunks) * (q + 1) / 4);
+  float s = 0.f;
+  if (e < total) {
+#pragma unroll 8
+    for (int z = lo; z < hi; ++z) s += partial[int64_t(z) * total + e];
+  }
+  part[q][c] = s;
+  __syncthreads();
+  if (q == 0 && e < total)
+    dW[(e / F) * lddw + e % F] = narrow<T>((part[0][c] + part[1][c]) + (part[2][c] + part[3][c]));
+}
+
+struct GradPlan {
+  int bh, bf, tiles_h, tiles_f, chunks;
+  int64_t chunk_rows;
+};
+
+GradPlan grad_plan(int64_t n, int64_t F, int64_t H) {
+  GradPlan p;
+  p.bh = H <= 32 ? 32 : H <= 64 ? 64 : 128;
+  p.bf = 256;
+  p.tiles_h = int((H + p.bh - 1) / p.bh);
+  p.tiles_f = int((F + p.bf - 1) / p.bf);
+  const int64_t steps = (n + kRowsStep - 1) / kRowsStep;
+  int64_t want = 512 / (int64_t(p.tiles_h) * p.tiles_f);
+  if (want < 1) want = 1;
+  if (want > steps) want = steps;
+  int64_t per = (steps + want - 1) / want;
+  if (per < 1) per = 1;
+  p.chunk_rows = per * kRowsStep;
+  p.chunks = int((n + p.chunk_rows - 1) / p.chunk_rows);
+  if (p.chunks < 1) p.chunks = 1;
+  return p;
+}
+
+int check_saved(int dtype, int64_t n, int64_t F, float slope) {
+  using sgnn::fail;
+  if (dtype != SGNN_F32 && dtype != SGNN_BF16) return fail(SGNN_ERR_INVALID, "unknown element type");
+  if (n < 0 || F <= 0) return fail(SGNN_ERR_INVALID, "need n >= 0 and F > 0");
+  if (F > (int64_t(1) << 24)) return fail(SGNN_ERR_UNSUPPORTED, "more than 2^24 features");
+  if (n > (int64_t(1) << 31) * 64) return fail(SGNN_ERR_UNSUPPORTED, "too many rows");
+  if (!(slope >= 0.f) || !(slope <= 3.4e38f)) return fail(SGNN_ERR_INVALID, "the activation's slope must be finite and not negative");
+  return SGNN_OK;
+}
+
+bool wide_ok(const void* p, int64_t ld, size_t elem) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (size_t(ld) * elem) % 16 == 0;
+}
+
+struct EltGrid { int rows, per_row; unsigned blocks; };
+int elt_grid(int64_t n, int64_t F, int elems, EltGrid* g) {
+  const int64_t per_row = (F + kGroup - 1) / kGroup * (kGroup / elems);
+  // about four trips of the workgroup: enough loads in flight, and n * F / 4096 workgroups to spread
+  int64_t rows = (4 * kEltThreads) / per_row;
+  if (rows < 1) rows = 1;
+  const int64_t blocks = (n + rows - 1) / rows;
+  if (blocks > 0x7fffffff) return sgnn::fail(SGNN_ERR_UNSUPPORTED, "too many rows for one launch");
+  *g = {int(rows), int(per_row), unsigned(blocks)};
+  return SGNN_OK;
+}
+
+template <typename T>
+int launch_weight_grad(const GradPlan& p, int64_t n, int64_t F, int64_t H, const uint8_t* codes, const uint8_t* steps,
+                       float slope, const void* grad, int64_t ldg, void* dW, int64_t lddw, float* partial,
+                       hipStream_t st) {
+  const T* g = static_cast<const T*>(grad);
+  T* out = static_cast<T*>(dW);
+  const bool wide = wide_ok(grad, ldg, sizeof(T));
+  const unsigned blocks = unsigned((p.chunks + 7) / 8 * 8) * unsigned(p.tiles_f * p.tiles_h);
+#define SGNN_WG8(BH, BF, WH, WF)                                                                                  \
+  hipLaunchKernelGGL((k_weight_grad8<T, BH, BF, WH, WF>), dim3(blocks), dim3(64 * WH * WF), 0, st, n, int(F),     \
+                     int(H), codes, steps, slope, g, ldg, wide, p.chunk_rows, p.chunks, p.tiles_f, p.tiles_h, out, \
+                     lddw, partial)
+  if (p.bh == 32) SGNN_WG8(32, 256, 1, 4);
+  else if (p.bh == 64) SGNN_WG8(64, 256, 1, 4);
+  else SGNN_WG8(128, 256, 2, 4);
+#undef SGNN_WG8
+  HIP_TRY(hipGetLastError());
+  if (p.chunks > 1) {
+    const int64_t total = F * H;
+    hipLaunchKernelGGL((k_weight_grad_sum8<T>), dim3(unsigned((total + 63) / 64)), dim3(256), 0, st, int(F), total,
+                       p.chunks, partial, out, lddw);
+    HIP_TRY(hipGetLastError());
+  }
+  return SGNN_OK;
+}
+
+}  // namespace
+
+extern "C" int sgnn_save8(int dtype, int64_t n, int64_t F, const void* x, int64_t ldx, float slope, void* codes,
+                          void* steps, void* act, int64_t ldact, void* stream) {
+  using sgnn::fail;
+  if (int rc = check_saved(dtype, n, F, slope)) return rc;
+  if (ldx < F || (act && ldact < F)) return fail(SGNN_ERR_INVALID, "row stride smaller than the width");
+  if (n == 0) return SGNN_OK;
+  if (!x || !codes || !steps) return fail(SGNN_ERR_INVALID, "null pointer");
+  if (reinterpret_cast<uintptr_t>(codes) % 16) return fail(SGNN_ERR_INVALID, "codes must be 16-byte aligned");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  EltGrid g;
+  uint8_t* q = static_cast<uint8_t*>(codes);
+  uint8_t* s = static_cast<uint8_t*>(steps);
+  if (dtype == SGNN_F32) {
+    if (int rc = elt_grid(n, F, Lane<float>::kElems, &g)) return rc;
+    hipLaunchKernelGGL((k_save8<float>), dim3(g.blocks), dim3(kEltThreads), 0, st, n, int(F),
+                       static_cast<const float*>(x), ldx, wide_ok(x, ldx, 4), slope, g.rows, g.per_row, q, s,
+                       static_cast<float*>(act), ldact, wide_ok(act, ldact, 4));
+  } else {
+    if (int rc = elt_grid(n, F, Lane<Bf16>::kElems, &g)) return rc;
+    hipLaunchKernelGGL((k_save8<Bf16>), dim3(g.blocks), dim3(kEltThreads), 0, st, n, int(F),
+                       static_cast<const Bf16*>(x), ldx, wide_ok(x, ldx, 2), slope, g.rows, g.per_row, q, s,
+                       static_cast<Bf16*>(act), ldact, wide_ok(act, ldact, 2));
+  }
+  HIP_TRY(hipGetLastError());
+  return SGNN_OK;
+}
+
+extern "C" int sgnn_restore8(int dtype, int64_t n, int64_t F, const void* codes, const void* steps, float slope,
+                             void* out, int64_t ldo, void* stream) {
+  using sgnn::fail;
+  if (int rc = check_saved(dtype, n, F, slope)) return rc;
+  if (ldo < F) return fail(SGNN_ERR_INVALID, "row stride smaller than the width");
+  if (n == 0) return SGNN_OK;
+  if (!codes || !steps || !out) return fail(SGNN_ERR_INVALID, "null pointer");
+  if (reinterpret_cast<uintptr_t>(codes) % 16) return fail(SGNN_ERR_INVALID, "codes must be 16-byte aligned");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  EltGrid g;
+  const uint8_t* q = static_cast<const uint8_t*>(codes);
+  const uint8_t* s = static_cast<const uint8_t*>(steps);
+  if (dtype == SGNN_F32) {
+    if (int rc = elt_grid(n, F, Lane<float>::kElems, &g)) return rc;
+    hipLaunchKernelGGL((k_restore8<float>), dim3(g.blocks), dim3(kEltThreads), 0, st, n, int(F), q, s, slope, g.rows,
+                       g.per_row, static_cast<float*>(out), ldo, wide_ok(out, ldo, 4));
+  } else {
+    if (int rc = elt_grid(n, F, Lane<Bf16>::kElems, &g)) return rc;
+    hipLaunchKernelGGL((k_restore8<Bf16>), dim3(g.blocks), dim3(kEltThreads), 0, st, n, int(F), q, s, slope, g.rows,
+                       g.per_row, static_cast<Bf16*>(out), ldo, wide_ok(out, ldo, 2));
+  }
+  HIP_TRY(hipGetLastError());
+  return SGNN_OK;
+}
+
+extern "C" int sgnn_saved8_input_grad(int dtype, int64_t n, int64_t F, const void* codes, float slope,
+                                      const void* grad, int64_t ldg, void* dx, int64_t lddx, void* stream) {
+  using sgnn::fail;
+  if (int rc = check_saved(dtype, n, F, slope)) return rc;
+  if (slope == 1.f) return fail(SGNN_ERR_INVALID, "codes of slope 1 hold no sign of the input");
+  if (ldg < F || lddx < F) return fail(SGNN_ERR_INVALID, "row stride smaller than the width");
+  if (n == 0) return SGNN_OK;
+  if (!codes || !grad || !dx) return fail(SGNN_ERR_INVALID, "null pointer");
+  if (reinterpret_cast<uintptr_t>(codes) % 16) return fail(SGNN_ERR_INVALID, "codes must be 16-byte aligned");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  EltGrid g;
+  const uint8_t* q = static_cast<const uint8_t*>(codes);
+  if (dtype == SGNN_F32) {
+    if (int rc = elt_grid(n, F, Lane<float>::kElems, &g)) return rc;
+    hipLaunchKernelGGL((k_input_grad8<float>), dim3(g.blocks), dim3(kEltThreads), 0, st, n, int(F), q, slope, g.rows,
+                       g.per_row, static_cast<const float*>(grad), ldg, wide_ok(grad, ldg, 4),
+                       static_cast<float*>(dx), lddx, wide_ok(dx, lddx, 4));
+  } else {
+    if (int rc = elt_grid(n, F, Lane<Bf16>::kElems, &g)) return rc;
+    hipLaunchKernelGGL((k_input_grad8<Bf16>), dim3(g.blocks), dim3(kEltThreads), 0, st, n, int(F), q, slope, g.rows,
+                       g.per_row, static_cast<const Bf16*>(grad), ldg, wide_ok(grad, ldg, 2),
+                       static_cast<Bf16*>(dx), lddx, wide_ok(dx, lddx, 2));
+  }
+  HIP_TRY(hipGetLastError());
+  return SGNN_OK;
+}
+
+extern "C" size_t sgnn_saved8_weight_grad_workspace_bytes(int64_t n, int64_t F, int64_t H) {
+  if (n <= 0 || F <= 0 || H <= 0) return 0;
+  const GradPlan p = grad_plan(n, F, H);
+  return p.chunks > 1 ? size_t(p.chunks) * size_t(F) * size_t(H) * sizeof(float) : 0;
+}
+
+extern "C" int sgnn_saved8_weight_grad(int dtype, int64_t n, int64_t F, int64_t H, const void* codes,
+                                       const void* steps, float slope, const void* grad, int64_t ldg, void* dW,
+                                       int64_t lddw, void* workspace, size_t workspace_bytes, void* stream) {
+  using sgnn::fail;
+  if (int rc = check_saved(dtype, n, F, slope)) return rc;
+  if (n == 0 || H <= 0) return fail(SGNN_ERR_INVALID, "need n > 0 and H > 0");
+  if (H > (int64_t(1) << 24) || F * H > (int64_t(1) << 31)) return fail(SGNN_ERR_UNSUPPORTED, "weight too large");
+  if (ldg < H || lddw < F) return fail(SGNN_ERR_INVALID, "row stride smaller than the width");
+  if (!codes || !steps || !grad || !dW) return fail(SGNN_ERR_INVALID, "null pointer");
+  if (reinterpret_cast<uintptr_t>(codes) % 16) return fail(SGNN_ERR_INVALID, "codes must be 16-byte aligned");
+  if (workspace_bytes < sgnn_saved8_weight_grad_workspace_bytes(n, F, H))
+    return fail(SGNN_ERR_WORKSPACE, "weight-gradient workspace too small");
+  const GradPlan p = grad_plan(n, F, H);
+  if (p.chunks > 1 && !workspace) return fail(SGNN_ERR_INVALID, "null pointer");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const uint8_t* q = static_cast<const uint8_t*>(codes);
+  const uint8_t* s = static_cast<const uint8_t*>(steps);
+  float* part = static_cast<float*>(workspace);
+  if (dtype == SGNN_F32) return launch_weight_grad<float>(p, n, F, H, q, s, slope, grad, ldg, dW, lddw, part, st);
+  return launch_weight_grad<Bf16>(p, n, F, H, q, s, slope, grad, ldg, dW, lddw, part, st);
+}

@@ -15,6 +15,7 @@ import torch
 from torch import nn
 
 from .norm_adj import NormAdj
+from .saved8 import SavedInt8, activated, checked_slope, linear_saved_int8, save_int8  # noqa: F401
 
 
 class _Propagate(torch.autograd.Function):
@@ -40,10 +41,15 @@ def propagate(x, adj, K=1):
 
 
 class _GraphConvBase(nn.Module):
-    def __init__(self, add_self_loops=True, cached=False):
+    def __init__(self, add_self_loops=True, cached=False, checkpoint=None):
         super().__init__()
+        if checkpoint not in (None, "int8"):
+            raise ValueError(f"checkpoint must be None or 'int8', got {checkpoint!r}")
+        if checkpoint is not None and cached:
+            raise ValueError("cached=True keeps the propagated features in full: there is nothing to checkpoint")
         self.add_self_loops = add_self_loops
         self.cached = cached
+        self.checkpoint = checkpoint
         self._adj = None
         self._adj_src = None
 
@@ -74,11 +80,14 @@ class SGConv(_GraphConvBase):
     map is applied first and the K hops run at the output width — the same result to fp32
     rounding at a fraction of the gather traffic (``reorder=False`` keeps the literal
     order).  With ``cached=True`` the propagated features are kept at the input width and
-    only the linear map runs per forward, as in torch_geometric."""
+    only the linear map runs per forward, as in torch_geometric.
+
+    ``checkpoint="int8"`` keeps the linear map's input for the backward pass in 8 bits
+    (``linear_saved_int8``)."""
 
     def __init__(self, in_channels, out_channels, K=1, cached=False, add_self_loops=True, bias=True,
-                 reorder=True):
-        super().__init__(add_self_loops, cached)
+                 reorder=True, checkpoint=None):
+        super().__init__(add_self_loops, cached, checkpoint)
         self.in_channels, self.out_channels, self.K = in_channels, out_channels, K
         self.reorder = reorder
         self.lin = nn.Linear(in_channels, out_channels, bias=bias)
@@ -93,19 +102,30 @@ class SGConv(_GraphConvBase):
             return self.lin(self._cached_x)
         adj = self._norm_adj(x, edge_index, edge_weight)
         if not self.cached and self.reorder and self.out_channels < self.in_channels:
-            out = propagate(torch.nn.functional.linear(x, self.lin.weight), adj, self.K)
+            h = linear_saved_int8(x, self.lin.weight) if self.checkpoint else nn.functional.linear(x, self.lin.weight)
+            out = propagate(h, adj, self.K)
             return out if self.lin.bias is None else out + self.lin.bias
         h = propagate(x, adj, self.K)
+        if self.checkpoint:
+            out = linear_saved_int8(h, self.lin.weight)
+            return out if self.lin.bias is None else out + self.lin.bias
         if self.cached:
             self._cached_x = h.detach()
         return self.lin(h)
 
 
 class GCNConv(_GraphConvBase):
-    """``A_hat (x W^T) + b`` — torch_geometric.nn.GCNConv as used at model/GCN.py:9-10."""
+    """``A_hat (x W^T) + b`` — torch_geometric.nn.GCNConv as used at model/GCN.py:9-10.
 
-    def __init__(self, in_channels, out_channels, cached=False, add_self_loops=True, bias=True):
-        super().__init__(add_self_loops, cached)
+    ``checkpoint="int8"`` keeps the layer's input for the backward pass in 8 bits.  ``input_slope``
+    folds the activation in front of the layer (model/GCN.py:15) into it: the layer takes the
+    pre-activation and applies ``x if x > 0 else input_slope * x`` itself (1: none, 0: ReLU), so
+    that nothing else of it has to be kept."""
+
+    def __init__(self, in_channels, out_channels, cached=False, add_self_loops=True, bias=True, checkpoint=None,
+                 input_slope=1.0):
+        super().__init__(add_self_loops, cached, checkpoint)
+        self.input_slope = checked_slope(input_slope)
         self.in_channels, self.out_channels = in_channels, out_channels
         self.lin = nn.Linear(in_channels, out_channels, bias=False)
         self.bias = nn.Parameter(torch.zeros(out_channels)) if bias else None
@@ -118,7 +138,10 @@ class GCNConv(_GraphConvBase):
             nn.init.zeros_(self.bias)
 
     def forward(self, x, edge_index, edge_weight=None):
-        h = self.lin(x)
+        if self.checkpoint:
+            h = linear_saved_int8(x, self.lin.weight, slope=self.input_slope)
+        else:
+            h = self.lin(activated(x, self.input_slope))
         out = propagate(h, self._norm_adj(x, edge_index, edge_weight), 1)
         if self.bias is not None:
             out = out + self.bias

@@ -1,0 +1,207 @@
+"""A layer's input kept in 8 bits for its backward pass.
+
+Training a layer stack on a whole graph is bound by what autograd keeps: every linear map holds
+its ``n x F`` input in full until the weight gradient is formed (model/GCN.py:14-16,
+model/SGC.py:14).  ``save_int8`` keeps it as one byte per element and one byte per group of 32
+features, and the weight gradient is formed from those bytes (``SavedInt8.weight_grad``).  An
+activation ``x if x > 0 else slope * x`` in front of the map is folded in: the sign of a code is
+the sign of ``x``, so the activation keeps nothing of its own (``SavedInt8.input_grad``).
+
+``linear_saved_int8`` is the layer built of these; ``nn.GCNConv`` and ``nn.SGConv`` use it with
+``checkpoint="int8"``.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _lib
+
+_TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
+
+
+def _type(t, what):
+    if not t.is_cuda:
+        raise ValueError(f"{what} must be on the GPU, got {t.device}")
+    code = _TYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{what} must be float32 or bfloat16, got {t.dtype}")
+    return code
+
+
+def checked_slope(slope):
+    """``slope`` as the kernels hold it; what they cannot hold is refused."""
+    slope = float(slope)
+    if not (math.isfinite(slope) and slope >= 0.0):
+        raise ValueError(f"the activation's slope must be finite and not negative, got {slope}")
+    # what the kernels compute with; a slope that 32 bits cannot hold is refused, not turned into another one
+    held = torch.tensor(slope, dtype=torch.float32).item()
+    if math.isinf(held) or (held == 0.0) != (slope == 0.0) or (held == 1.0) != (slope == 1.0):
+        raise ValueError(f"the activation's slope is not a 32-bit number: {slope}")
+    return held
+
+
+def activated(x, slope):
+    """``x if x > 0 else slope * x`` by torch's operators."""
+    if slope == 1.0:
+        return x
+    return torch.relu(x) if slope == 0.0 else torch.nn.functional.leaky_relu(x, slope)
+
+
+def _rows(t):
+    """``t`` with unit stride along its rows and rows that do not overlap (a copy if need be)."""
+    n, f = t.shape
+    if (f > 1 and t.stride(1) != 1) or (n > 1 and t.stride(0) < f):
+        return t.contiguous()
+    return t
+
+
+def _ld(t):
+    return max(t.stride(0), t.shape[1])
+
+
+class SavedInt8:
+    """An ``n x F`` activation in 8 bits: ``codes`` int8 ``[n, 32 * ceil(F / 32)]``, ``steps``
+    uint8 ``[n, ceil(F / 32)]`` (the group's exponent plus 127), ``slope`` and the ``dtype`` it
+    came from."""
+
+    def __init__(self, codes, steps, shape, slope, dtype):
+        self.codes, self.steps, self.shape = codes, steps, tuple(shape)
+        self.slope, self.dtype = checked_slope(slope), dtype
+        n, F = self.shape
+        groups = -(-F // _lib.SAVED8_GROUP)
+        for name, t, kind, width in (("codes", codes, torch.int8, groups * _lib.SAVED8_GROUP),
+                                     ("steps", steps, torch.uint8, groups)):
+            if t.dtype != kind or tuple(t.shape) != (n, width) or not t.is_contiguous() or not t.is_cuda:
+                raise ValueError(f"{name} must be a contiguous {kind} tensor of shape {(n, width)} on the GPU")
+        if steps.device != codes.device:
+            raise ValueError("codes and steps are on different devices")
+        if codes.data_ptr() % 16:
+            raise ValueError("codes must be 16-byte aligned")
+        if dtype not in _TYPES:
+            raise TypeError(f"saved activations are float32 or bfloat16, got {dtype}")
+
+    @property
+    def nbytes(self):
+        return self.codes.numel() + self.steps.numel()
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def restore(self, dtype=None):
+        """The values the codes stand for, ``n x F`` (exact in either type)."""
+        dtype = self.dtype if dtype is None else dtype
+        if dtype not in _TYPES:
+            raise TypeError(f"saved activations are restored as float32 or bfloat16, not {dtype}")
+        n, F = self.shape
+        out = torch.empty(n, F, dtype=dtype, device=self.device)
+        with torch.cuda.device(self.device):
+            _lib.check(_lib.load().sgnn_restore8(_TYPES[dtype], n, F, _lib.ptr(self.codes), _lib.ptr(self.steps),
+                                                 self.slope, _lib.ptr(out), F, _lib.current_stream(self.device)))
+        return out
+
+    def _grad(self, grad, width, what):
+        _type(grad, what)
+        if grad.dim() != 2 or grad.shape[0] != self.shape[0] or (width is not None and grad.shape[1] != width):
+            raise ValueError(f"{what} must have shape ({self.shape[0]}, {'H' if width is None else width}), "
+                             f"got {tuple(grad.shape)}")
+        if grad.device != self.device:
+            raise ValueError(f"{what} is on {grad.device}, the saved activation on {self.device}")
+        return _rows(grad.detach())
+
+    def weight_grad(self, grad):
+        """``grad.T @ values``: the gradient ``[H, F]`` of a weight applied to the activation, from
+        the gradient ``[n, H]`` of its output, in ``grad``'s type."""
+        grad = self._grad(grad, None, "the output's gradient")
+        (n, F), H = self.shape, grad.shape[1]
+        if n == 0 or H == 0:
+            return torch.zeros(H, F, dtype=grad.dtype, device=self.device)
+        lib = _lib.load()
+        dW = torch.empty(H, F, dtype=grad.dtype, device=self.device)
+        ws = torch.empty(lib.sgnn_saved8_weight_grad_workspace_bytes(n, F, H), dtype=torch.uint8, device=self.device)
+        with torch.cuda.device(self.device):
+            _lib.check(lib.sgnn_saved8_weight_grad(_TYPES[grad.dtype], n, F, H, _lib.ptr(self.codes),
+                                                   _lib.ptr(self.steps), self.slope, _lib.ptr(grad), _ld(grad),
+                                                   _lib.ptr(dW), F, _lib.ptr(ws), ws.numel(),
+                                                   _lib.current_stream(self.device)))
+        return dW
+
+    def input_grad(self, grad):
+        """``grad * act'(x)``: the gradient of the activation's input from that of its output."""
+        return self._input_grad(self._grad(grad, self.shape[1], "the activation's gradient"), in_place=False)
+
+    def _input_grad(self, grad, in_place):
+        if self.slope == 1.0:
+            return grad
+        n, F = self.shape
+        out = grad if in_place else torch.empty(n, F, dtype=grad.dtype, device=self.device)
+        with torch.cuda.device(self.device):
+            _lib.check(_lib.load().sgnn_saved8_input_grad(_TYPES[grad.dtype], n, F, _lib.ptr(self.codes), self.slope,
+                                                          _lib.ptr(grad), _ld(grad), _lib.ptr(out), _ld(out),
+                                                          _lib.current_stream(self.device)))
+        return out
+
+
+def _save(x, slope, with_act):
+    code = _type(x, "the activation")
+    if x.dim() != 2 or x.shape[1] == 0:
+        raise ValueError(f"the activation must be a matrix with at least one column, got {tuple(x.shape)}")
+    slope = checked_slope(slope)
+    x = _rows(x.detach())
+    n, F = x.shape
+    groups = -(-F // _lib.SAVED8_GROUP)
+    codes = torch.empty(n, groups * _lib.SAVED8_GROUP, dtype=torch.int8, device=x.device)
+    steps = torch.empty(n, groups, dtype=torch.uint8, device=x.device)
+    act = torch.empty(n, F, dtype=x.dtype, device=x.device) if with_act and slope != 1.0 else None
+    with torch.cuda.device(x.device):
+        _lib.check(_lib.load().sgnn_save8(code, n, F, _lib.ptr(x), _ld(x), slope, _lib.ptr(codes), _lib.ptr(steps),
+                                          _lib.ptr(act), F, _lib.current_stream(x.device)))
+    return SavedInt8(codes, steps, (n, F), slope, x.dtype), (x if act is None else act)
+
+
+def save_int8(x, slope=1.0):
+    """``x if x > 0 else slope * x`` in 8 bits (``slope`` 1: no activation, 0: ReLU)."""
+    return _save(x, slope, with_act=False)[0]
+
+
+class _LinearSaved(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, slope):
+        saved, act = _save(x, slope, with_act=True)
+        ctx.save_for_backward(saved.codes, saved.steps, weight)
+        ctx.meta = (saved.shape, saved.slope, saved.dtype)
+        with torch.autocast("cuda", enabled=False):          # in the operands' own type
+            return torch.nn.functional.linear(act, weight.detach())
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        codes, steps, weight = ctx.saved_tensors
+        saved = SavedInt8(codes, steps, *ctx.meta)
+        dx = dw = None
+        if ctx.needs_input_grad[0]:
+            dx = saved._input_grad(grad.matmul(weight), in_place=True)
+        if ctx.needs_input_grad[1]:
+            dw = saved.weight_grad(grad)
+        return dx, dw, None
+
+
+def linear_saved_int8(x, weight, slope=1.0):
+    """``act(x) @ weight.T`` with ``act(x) = x if x > 0 else slope * x``, keeping nothing of its
+    input but the 8-bit codes for the backward pass.  The output and ``x``'s gradient are those of
+    the full activation; the weight's gradient is formed from the codes (off by half a step of
+    their group at most, element by element)."""
+    code = _type(x, "the input")
+    if _type(weight, "the weight") != code:
+        raise TypeError(f"the input is {x.dtype}, the weight {weight.dtype}")
+    if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1]:
+        raise ValueError(f"need an (n, F) input and an (H, F) weight, got {tuple(x.shape)} and {tuple(weight.shape)}")
+    if weight.device != x.device:
+        raise ValueError(f"the input is on {x.device}, the weight on {weight.device}")
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        return _LinearSaved.apply(x, weight, slope)
+    act = activated(x, checked_slope(slope))
+    with torch.autocast("cuda", enabled=False):
+        return torch.nn.functional.linear(act, weight)
