@@ -643,6 +643,35 @@ int sgnn_saved8_weight_grad(int dtype, int64_t n, int64_t F, int64_t H, const vo
                             float slope, const void* grad, int64_t ldg, void* dW, int64_t lddw, void* workspace,
                             size_t workspace_bytes, void* stream);
 
+/*
+ * Softmax cross-entropy of a label head of any width, without the logits (model/SGNN.py:397-399
+ * keeps them and their gradient; sgnn_head_xent_f32 serves heads of up to 64 classes).
+ *   z = x . weight^T,  row_loss[b] = logsumexp_v(z_bv) - z_b,y(b),
+ *   dx = dz . weight,  dweight = dz^T . x,  dz_bv = g_b (softmax(z_b)_v - [v = y(b)])
+ * x is B x D (row stride ldx), weight is V x D with element (v, d) at v * sv + d * sd, unit stride
+ * along one of the two; dweight likewise (dsv, dsd).  `dtype` (SGNN_F32 or SGNN_BF16) holds for x,
+ * weight, dx and dweight; losses, statistics and gradients of losses are fp32.  y(b) = labels[idx[b]]
+ * when idx is given, else labels[b]; a row whose index or label is out of range has no class: its
+ * loss is 0, it adds nothing to either gradient and does not count in the mean.
+ *
+ * forward: stats[b] = (max, sum of exp(z - max)) (2 floats a row), row_loss; with `loss` also
+ *   loss[0] = mean of the counted rows (0 if there are none) and share[0] = 1 / their number (0).
+ * backward: from the same operands and the forward's stats.  share given: g_b = grad[0] * share[0]
+ *   (the mean's gradient); share NULL: g_b = grad[b].  dx or dweight may be NULL.
+ * Sums are formed in 32 bits in a fixed order.  `workspace`: sgnn_class_xent_workspace_bytes bytes
+ * (backward = 0 or 1), contents irrelevant.
+ */
+size_t sgnn_class_xent_workspace_bytes(int dtype, int64_t B, int64_t D, int64_t V, int backward);
+int sgnn_class_xent_forward(int dtype, int64_t B, int64_t D, int64_t V, const void* x, int64_t ldx,
+                            const void* weight, int64_t sv, int64_t sd, const int64_t* labels, int64_t n_labels,
+                            const int64_t* idx, float* stats, float* row_loss, float* loss, float* share,
+                            void* workspace, size_t workspace_bytes, void* stream);
+int sgnn_class_xent_backward(int dtype, int64_t B, int64_t D, int64_t V, const void* x, int64_t ldx,
+                             const void* weight, int64_t sv, int64_t sd, const int64_t* labels, int64_t n_labels,
+                             const int64_t* idx, const float* stats, const float* grad, const float* share, void* dx,
+                             int64_t lddx, void* dweight, int64_t dsv, int64_t dsd, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -134,6 +134,13 @@ SIGNATURES = {
     "sgnn_saved8_weight_grad_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
     "sgnn_saved8_weight_grad": (c_int, [c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_float, c_void_p, c_int64,
                                         c_void_p, c_int64, c_void_p, c_size_t, c_void_p]),
+    "sgnn_class_xent_workspace_bytes": (c_size_t, [c_int, c_int64, c_int64, c_int64, c_int]),
+    "sgnn_class_xent_forward": (c_int, [c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64,
+                                        c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                        c_size_t, c_void_p]),
+    "sgnn_class_xent_backward": (c_int, [c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64,
+                                         c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                         c_int64, c_void_p, c_int64, c_int64, c_void_p, c_size_t, c_void_p]),
     "sgnn_sample_block_f32": (c_int, [c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int,
                                       c_void_p, c_int64, c_void_p]),
 }

@@ -1,0 +1,708 @@
+// Softmax cross-entropy of x . weight^T over many classes, and its gradients, without the logits.
+//
+//   z = x . weight^T (B x V),  loss_b = log sum_v exp(z_bv) - z_b,y(b),
+//   dz_bv = g_b (exp(z_bv) / sum_v exp(z_bv) - [v = y(b)]),  dx = dz . weight,  dweight = dz^T . x
+//
+// The forward pass runs over the classes once and keeps a running maximum and sum per row; the
+// backward pass forms the logits again, a piece of the classes at a time, writes that piece of dz
+// in bf16 and multiplies it from either side.  A piece is sized to stay in the last-level cache
+// between the launch that writes it and the two that read it.
+//
+// All four products run on the bf16 matrix instructions.  bf16 operands go in as they are, their
+// products are exact and summed in 32 bits; dz is rounded to bf16 there (relative 2^-9 per
+// element, below the half step that each result is rounded by).  fp32 operands, and dz with
+// them, are the sum of three bf16 numbers each (8 + 8 + 8 bits of the mantissa, cut off, so the
+// sum is exact); of the nine products the three smallest, below 2^-24 of the whole, are left out.
+#include "common.h"
+
+namespace {
+
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+struct Bf16 { uint16_t bits; };
+
+__device__ __forceinline__ float widen(float v) { return v; }
+__device__ __forceinline__ float widen(Bf16 v) { return __uint_as_float(unsigned(v.bits) << 16); }
+__device__ __forceinline__ uint16_t to_bf16(float v) {                       // nearest even
+  const unsigned u = __float_as_uint(v);
+  if ((u & 0x7fffffffu) > 0x7f800000u) return 0x7fc0u;
+  return uint16_t((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+}
+template <typename T> __device__ __forceinline__ T narrow(float v);
+template <> __device__ __forceinline__ float narrow<float>(float v) { return v; }
+template <> __device__ __forceinline__ Bf16 narrow<Bf16>(float v) { return Bf16{to_bf16(v)}; }
+
+// v = plane 0 + plane 1 + plane 2 exactly; infinities and NaN live in plane 0 only
+__device__ __forceinline__ void split3(float v, uint16_t (&p)[3]) {
+  const unsigned u = __float_as_uint(v);
+  if ((u & 0x7f800000u) == 0x7f800000u) {
+    p[0] = (u & 0x7fffffu) ? uint16_t(0x7fc0u) : uint16_t(u >> 16);
+    p[1] = p[2] = 0;
+    return;
+  }
+  const float r = v - __uint_as_float(u & 0xffff0000u);
+  const unsigned ur = __float_as_uint(r);
+  p[0] = uint16_t(u >> 16);
+  p[1] = uint16_t(ur >> 16);
+  p[2] = uint16_t(__float_as_uint(r - __uint_as_float(ur & 0xffff0000u)) >> 16);
+}
+template <int P>
+__device__ __forceinline__ void to_planes(float v, uint16_t (&p)[P]) {
+  if constexpr (P == 1) p[0] = to_bf16(v);
+  else split3(v, p);
+}
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ int64_t label_of(int64_t b, const int64_t* labels, const int64_t* idx, int64_t n_labels,
+                                            int64_t V) {
+  const int64_t at = idx ? idx[b] : b;
+  const int64_t y = (at >= 0 && at < n_labels) ? labels[at] : -1;
+  return (y >= 0 && y < V) ? y : -1;
+}
+
+// ------------------------------------------------------------------ operands as bf16 planes
+struct Labels {
+  const int64_t *labels, *idx;
+  int64_t n_labels, V;
+};
+// in[r][d] at r * sr + d * sd  ->  out[plane][r][Dp], columns D .. Dp zero.  A 64 x 64 tile goes
+// through LDS, read along whichever of its directions is contiguous.  Rows of x without a class
+// become zeros, so that whatever a padded row holds (NaN too) reaches no gradient.
+template <typename T, int P>
+__global__ __launch_bounds__(256) void k_planes(int64_t R, int D, int Dp, const T* __restrict__ in, int64_t sr,
+                                                int64_t sd, Labels of, uint16_t* __restrict__ out) {
+  __shared__ float tile[64][65];
+  const int64_t r0 = int64_t(blockIdx.x) * 64;
+  const int d0 = blockIdx.y * 64, t = threadIdx.x;
+  for (int i = t; i < 64 * 64; i += 256) {
+    const int fast = i & 63, slow = i >> 6;
+    const int lr = sd == 1 ? slow : fast, ld = sd == 1 ? fast : slow;
+    const int64_t r = r0 + lr;
+    const int d = d0 + ld;
+    const bool live = r < R && d < D && (of.V == 0 || label_of(r, of.labels, of.idx, of.n_labels, of.V) >= 0);
+    tile[lr][ld] = live ? widen(in[r * sr + d * sd]) : 0.f;
+  }
+  __syncthreads();
+  for (int i = t; i < 64 * 8; i += 256) {
+    const int lr = i >> 3, c = (i & 7) * 8;
+    const int64_t r = r0 + lr;
+    if (r >= R) continue;
+    uint16_t pl[P][8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      uint16_t p[P];
+      to_planes<P>(tile[lr][c + e], p);
+#pragma unroll
+      for (int q = 0; q < P; ++q) pl[q][e] = p[q];
+    }
+#pragma unroll
+    for (int q = 0; q < P; ++q) {
+      u32x4 w;
+      __builtin_memcpy(&w, &pl[q][0], 16);
+      *reinterpret_cast<u32x4*>(out + (int64_t(q) * R + r) * Dp + d0 + c) = w;
+    }
+  }
+}
+
+// ------------------------------------------------------------------ the product's inner loop
+// A workgroup of four wavefronts forms a 128 x 128 tile, 64 x 64 a wavefront, K steps of kBK.
+// Operands travel from memory to LDS without passing registers, one step ahead.  An operand is
+// "deep" when its memory is contiguous along the reduction (LDS holds [128][kBK], read directly)
+// and "flat" when it is contiguous along the tile ([kBK][128], read through the transposing LDS
+// load).  16-byte chunks are permuted on the way in so that neither read meets bank conflicts.
+constexpr int kTile = 128;
+constexpr int kThreads = 256;
+
+struct Operand {
+  const uint16_t* base;
+  int64_t ld, plane;       // row stride and distance between planes, in elements
+  int64_t rows;            // rows that exist: reads beyond repeat the last one
+  int64_t cols;            // columns that exist (flat operands; a multiple of 8)
+};
+
+template <int P> struct Depth { static constexpr int kBK = P == 1 ? 64 : 32; };
+
+template <int P> constexpr int stage_bytes() { return P * kTile * Depth<P>::kBK * 2; }
+
+typedef __attribute__((address_space(3))) void lds_void;
+typedef const __attribute__((address_space(1))) void global_void;
+
+// deep: rows r0 .. r0 + 127 at reduction offset k0;  flat: reduction rows k0 .. at columns r0 ..
+template <int P, bool DEEP>
+__device__ __forceinline__ void stage_operand(const Operand& op, int64_t r0, int64_t k0, char* lds, int wave,
+                                              int lane) {
+  constexpr int BK = Depth<P>::kBK;
+  constexpr int kChunks = P * kTile * BK / 8;
+#pragma unroll
+  for (int l = 0; l < kChunks / kThreads; ++l) {
+    const int first = (l * 4 + wave) * 64, q = first + lane;
+    constexpr int per_plane = kTile * BK / 8;
+    const int p = q / per_plane, at = q % per_plane;
+    const uint16_t* src;
+    if constexpr (DEEP) {
+      constexpr int cpr = BK / 8;
+      const int row = at / cpr, c = at % cpr;
+      const int cl = c ^ (cpr == 8 ? (row & 7) : ((row >> 2) & 3));
+      int64_t r = r0 + row;
+      r = r < op.rows ? r : op.rows - 1;
+      src = op.base + p * op.plane + r * op.ld + k0 + cl * 8;
+    } else {
+      const int row = at / 16, c = at % 16;
+      const int cl = c ^ ((row & 3) << 2);
+      int64_t r = k0 + row, col = r0 + cl * 8;
+      r = r < op.rows ? r : op.rows - 1;
+      col = col < op.cols ? col : op.cols - 8;
+      src = op.base + p * op.plane + r * op.ld + col;
+    }
+    __builtin_amdgcn_global_load_lds((global_void*)src, (lds_void*)(lds + first * 16), 16, 0, 0);
+  }
+}
+
+// the operand of one 32 x 32 x 16 instruction: element `lane & 31` of the block at m0, eight
+// reduction indexes from k0 + 8 * (lane / 32)
+template <int P, bool DEEP>
+__device__ __forceinline__ bf16x8 fragment(const char* lds, int p, int m0, int k0, int lane) {
+  constexpr int BK = Depth<P>::kBK;
+  const char* slab = lds + p * (kTile * BK * 2);
+  if constexpr (DEEP) {
+    constexpr int cpr = BK / 8;
+    const int row = m0 + (lane & 31), c = k0 / 8 + (lane >> 5);
+    const int cl = c ^ (cpr == 8 ? (row & 7) : ((row >> 2) & 3));
+    return *reinterpret_cast<const bf16x8*>(slab + row * (BK * 2) + cl * 16);
+  } else {
+    const int k = k0 + 8 * (lane >> 5) + ((lane & 15) >> 2);
+    const int m = m0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    const int at = ((m >> 3) ^ ((k & 3) << 2)) * 16 + (m & 7) * 2;       // k and k + 4 share k & 3
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(slab + k * (kTile * 2) + at));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(slab + (k + 4) * (kTile * 2) + at));
+    bf16x8 r;
+    __builtin_memcpy(&r, &lo, 8);
+    __builtin_memcpy(reinterpret_cast<char*>(&r) + 8, &hi, 8);
+    return r;
+  }
+}
+
+typedef f32x16 Tile[2][2];
+
+__device__ __forceinline__ void clear(Tile& acc) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+}
+
+// acc += A[m0 .., k0 .. k1] . B[n0 .., k0 .. k1]; k1 - k0 a multiple of kBK.  `lds` holds two
+// stages of both operands; every wavefront has left them when this returns.
+template <int P, bool ADEEP, bool BDEEP>
+__device__ __forceinline__ void multiply(const Operand& A, int64_t m0, const Operand& B, int64_t n0, int64_t k0,
+                                         int64_t k1, char* lds, Tile& acc) {
+  constexpr int BK = Depth<P>::kBK;
+  constexpr int kStage = stage_bytes<P>();
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
+  stage_operand<P, ADEEP>(A, m0, k0, lds, wave, lane);
+  stage_operand<P, BDEEP>(B, n0, k0, lds + kStage, wave, lane);
+  int cur = 0;
+  for (int64_t k = k0; k < k1; k += BK) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // this wavefront's part of the stage has landed
+    __syncthreads();                                         // everybody's has, and the other stage is free
+    const char* a = lds + cur * 2 * kStage;
+    const char* b = a + kStage;
+    if (k + BK < k1) {
+      char* next = lds + (cur ^ 1) * 2 * kStage;
+      stage_operand<P, ADEEP>(A, m0, k + BK, next, wave, lane);
+      stage_operand<P, BDEEP>(B, n0, k + BK, next + kStage, wave, lane);
+    }
+#pragma unroll
+    for (int kk = 0; kk < BK; kk += 16) {
+      bf16x8 fa[P][2], fb[P][2];
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          fa[p][i] = fragment<P, ADEEP>(a, p, wm + 32 * i, kk, lane);
+          fb[p][i] = fragment<P, BDEEP>(b, p, wn + 32 * i, kk, lane);
+        }
+#pragma unroll
+      for (int pa = 0; pa < P; ++pa)
+#pragma unroll
+        for (int pb = 0; pa + pb < P; ++pb)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[pa][i], fb[pb][j], acc[i][j], 0, 0, 0);
+    }
+    cur ^= 1;
+  }
+  __syncthreads();
+}
+
+// row of element e of a 32 x 32 block (its column is lane & 31)
+__device__ __forceinline__ int block_row(int e, int lane) { return 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3); }
+
+// ------------------------------------------------------------------ forward
+// A workgroup takes 128 rows of x and a range of the classes, 128 at a time.  The tile is formed
+// as classes x rows, so that a lane holds 32 classes of each of two rows and its running maximum
+// and sum need no other lane until the end.  part[split][row] = (max, sum of exp relative to it).
+template <int P>
+__global__ __launch_bounds__(kThreads) void k_class_stats(int64_t B, int64_t V, int Dp, Operand x, Operand w,
+                                                          const int64_t* __restrict__ labels,
+                                                          const int64_t* __restrict__ idx, int64_t n_labels,
+                                                          int64_t tiles_v, int splits, float2* __restrict__ part,
+                                                          float* __restrict__ picked) {
+  __shared__ __align__(128) char lds[4 * stage_bytes<P>()];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wv = (wave >> 1) * 64, wb = (wave & 1) * 64;
+  const int split = blockIdx.x % splits;
+  const int64_t b0 = int64_t(blockIdx.x / splits) * kTile;
+  const int64_t t0 = tiles_v * split / splits, t1 = tiles_v * (split + 1) / splits;
+  float top[2], sum[2];
+  int64_t y[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int64_t b = b0 + wb + 32 * j + (lane & 31);
+    top[j] = -INFINITY;
+    sum[j] = 0.f;
+    y[j] = b < B ? label_of(b, labels, idx, n_labels, V) : -1;
+  }
+  for (int64_t t = t0; t < t1; ++t) {
+    Tile acc;
+    clear(acc);
+    multiply<P, true, true>(w, t * kTile, x, b0, 0, Dp, lds, acc);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float m = top[j];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int64_t v = t * kTile + wv + 32 * i + block_row(e, lane);
+          if (v == y[j]) picked[b0 + wb + 32 * j + (lane & 31)] = acc[i][j][e];
+          if (v >= V) acc[i][j][e] = -INFINITY;
+          m = acc[i][j][e] > m || acc[i][j][e] != acc[i][j][e] ? acc[i][j][e] : m;      // a NaN stays
+        }
+      // while everything is -inf the sum stays 0
+      const float ref = m == -INFINITY ? 0.f : m;
+      float s = sum[j] * exp2f((top[j] - ref) * kLog2e);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s += exp2f((acc[i][j][e] - ref) * kLog2e);
+      top[j] = m;
+      sum[j] = s;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const float om = __shfl_xor(top[j], 32), os = __shfl_xor(sum[j], 32);
+    const float m = (om > top[j] || om != om) ? om : top[j], ref = m == -INFINITY ? 0.f : m;
+    const float s = sum[j] * exp2f((top[j] - ref) * kLog2e) + os * exp2f((om - ref) * kLog2e);
+    const int64_t b = b0 + wb + 32 * j + (lane & 31);
+    if (lane < 32 && b < B) part[(int64_t(split) * 2 + (wave >> 1)) * B + b] = make_float2(m, s);
+  }
+}
+
+// One row's pieces joined: stats[b] = (max, sum), row_loss[b] (0 where the row has no class).
+__global__ __launch_bounds__(256) void k_class_rows(int64_t B, int64_t V, int parts, const float2* __restrict__ part,
+                                                    const float* __restrict__ picked,
+                                                    const int64_t* __restrict__ labels,
+                                                    const int64_t* __restrict__ idx, int64_t n_labels,
+                                                    float2* __restrict__ stats, float* __restrict__ row_loss) {
+  const int64_t b = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (b >= B) return;
+  float m = -INFINITY;
+  for (int q = 0; q < parts; ++q) {
+    const float o = part[int64_t(q) * B + b].x;
+    m = (o > m || o != o) ? o : m;
+  }
+  const float ref = m == -INFINITY ? 0.f : m;
+  float s = 0.f;
+  for (int q = 0; q < parts; ++q) {
+    const float2 o = part[int64_t(q) * B + b];
+    s += o.y * exp2f((o.x - ref) * kLog2e);
+  }
+  stats[b] = make_float2(m, s);
+  row_loss[b] = label_of(b, labels, idx, n_labels, V) >= 0 ? (m - picked[b]) + log2f(s) * kLn2 : 0.f;
+}
+
+// loss[0] = mean loss of the counted rows (0 if there are none), share[0] = 1 / their number.
+__global__ __launch_bounds__(1024) void k_class_mean(int64_t B, int64_t V, const float* __restrict__ row_loss,
+                                                     const int64_t* __restrict__ labels,
+                                                     const int64_t* __restrict__ idx, int64_t n_labels,
+                                                     float* __restrict__ loss, float* __restrict__ share) {
+  __shared__ double s_sum[16];
+  __shared__ int64_t s_count[16];
+  double sum = 0.0;
+  int64_t count = 0;
+  for (int64_t b = threadIdx.x; b < B; b += 1024)
+    if (label_of(b, labels, idx, n_labels, V) >= 0) {
+      sum += double(row_loss[b]);
+      ++count;
+    }
+  for (int off = 32; off >= 1; off >>= 1) {
+    sum += __shfl_xor(sum, off);
+    count += __shfl_xor(count, off);
+  }
+  if ((threadIdx.x & 63) == 0) {
+    s_sum[threadIdx.x >> 6] = sum;
+    s_count[threadIdx.x >> 6] = count;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int q = 1; q < 16; ++q) {
+      sum += s_sum[q];
+      count += s_count[q];
+    }
+    loss[0] = count ? float(sum / double(count)) : 0.f;
+    share[0] = count ? float(1.0 / double(count)) : 0.f;
+  }
+}
+
+// ------------------------------------------------------------------ backward
+// dz of the classes v0 .. v0 + 128 * tiles and all rows, as bf16 planes [plane][Bp][ldz]; rows and
+// classes beyond the last are 0.
+template <int P>
+__global__ __launch_bounds__(kThreads) void k_class_dz(int64_t B, int64_t V, int Dp, Operand x, Operand w,
+                                                       const int64_t* __restrict__ labels,
+                                                       const int64_t* __restrict__ idx, int64_t n_labels,
+                                                       const float2* __restrict__ stats,
+                                                       const float* __restrict__ grad, const float* __restrict__ share,
+                                                       int64_t v0, int tiles, uint16_t* __restrict__ dz, int64_t ldz,
+                                                       int64_t plane) {
+  constexpr int kRow = kTile * 2 + 16;             // bytes of a staged row of dz
+  constexpr int kLds = 4 * stage_bytes<P>() > kTile * kRow ? 4 * stage_bytes<P>() : kTile * kRow;
+  __shared__ __align__(128) char lds[kLds];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wv = (wave >> 1) * 64, wb = (wave & 1) * 64;
+  const int64_t vt = v0 + int64_t(blockIdx.x % tiles) * kTile;
+  const int64_t b0 = int64_t(blockIdx.x / tiles) * kTile;
+  Tile acc;
+  clear(acc);
+  multiply<P, true, true>(w, vt, x, b0, 0, Dp, lds, acc);
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int64_t b = b0 + wb + 32 * j + (lane & 31);
+    const int64_t y = b < B ? label_of(b, labels, idx, n_labels, V) : -1;
+    // share given: the mean's gradient over the counted rows; else a gradient for each row
+    const float g = y >= 0 ? (share ? grad[0] * share[0] : grad[b]) : 0.f;
+    const float2 st = b < B ? stats[b] : make_float2(0.f, 1.f);
+    const float scale = g / st.y;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int64_t v = vt + wv + 32 * i + block_row(e, lane);
+        float d = exp2f((acc[i][j][e] - st.x) * kLog2e) * scale;
+        if (v == y) d -= g;
+        acc[i][j][e] = y >= 0 && v < V ? d : 0.f;
+      }
+  }
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          uint16_t four[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint16_t pl[P];
+            to_planes<P>(acc[i][j][e + q], pl);
+            four[q] = pl[p];
+          }
+          u32x2 u;
+          __builtin_memcpy(&u, &four, 8);
+          *reinterpret_cast<u32x2*>(lds + (wb + 32 * j + (lane & 31)) * kRow + (wv + 32 * i + block_row(e, lane)) * 2) = u;
+        }
+    __syncthreads();
+    uint16_t* out = dz + p * plane + b0 * ldz + (vt - v0);
+    for (int c = threadIdx.x; c < kTile * kTile / 8; c += kThreads) {
+      const int row = c >> 4, col = (c & 15) * 8;
+      *reinterpret_cast<u32x4*>(out + row * ldz + col) = *reinterpret_cast<const u32x4*>(lds + row * kRow + col * 2);
+    }
+    __syncthreads();
+  }
+}
+
+// C[m][n] += or = A . B over this workgroup's share of the reduction, 32 bits, one buffer per share:
+// out[split][Mp][Np].
+template <int P, bool ADEEP>
+__global__ __launch_bounds__(kThreads) void k_class_product(Operand A, Operand B, int tiles_m, int tiles_n,
+                                                            int64_t K, int splits, int add, float* __restrict__ out,
+                                                            int64_t plane, int64_t ldo) {
+  __shared__ __align__(128) char lds[4 * stage_bytes<P>()];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
+  const int tn = blockIdx.x % tiles_n, rest = blockIdx.x / tiles_n;
+  const int split = rest % splits, tm = rest / splits;
+  const int64_t m0 = int64_t(tm) * kTile, n0 = int64_t(tn) * kTile;
+  const int64_t steps = K / Depth<P>::kBK;
+  const int64_t k0 = steps * split / splits * Depth<P>::kBK, k1 = steps * (split + 1) / splits * Depth<P>::kBK;
+  Tile acc;
+  clear(acc);
+  if (k0 < k1) multiply<P, ADEEP, false>(A, m0, B, n0, k0, k1, lds, acc);
+  float* dst = out + split * plane;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        float* at = dst + (m0 + wm + 32 * i + block_row(e, lane)) * ldo + n0 + wn + 32 * j + (lane & 31);
+        *at = add ? *at + acc[i][j][e] : acc[i][j][e];
+      }
+}
+
+// out[r][d] = sum over the shares, in order; out at r * sr + d * sd
+template <typename T>
+__global__ __launch_bounds__(256) void k_class_join(int64_t R, int D, int splits, const float* __restrict__ in,
+                                                    int64_t plane, int64_t ldi, T* __restrict__ out, int64_t sr,
+                                                    int64_t sd) {
+  __shared__ float tile[32][33];
+  const int64_t r0 = int64_t(blockIdx.x) * 32;
+  const int d0 = blockIdx.y * 32, t = threadIdx.x;
+  for (int i = t; i < 32 * 32; i += 256) {
+    const int lr = i >> 5, ld = i & 31;
+    float s = 0.f;
+    if (r0 + lr < R && d0 + ld < D) {
+      const float* src = in + (r0 + lr) * ldi + d0 + ld;
+#pragma unroll 4
+      for (int q = 0; q < splits; ++q) s += src[q * plane];
+    }
+    tile[lr][ld] = s;
+  }
+  __syncthreads();
+  for (int i = t; i < 32 * 32; i += 256) {
+    const int fast = i & 31, slow = i >> 5;
+    const int lr = sd == 1 ? slow : fast, ld = sd == 1 ? fast : slow;
+    if (r0 + lr < R && d0 + ld < D) out[(r0 + lr) * sr + (d0 + ld) * sd] = narrow<T>(tile[lr][ld]);
+  }
+}
+
+// ------------------------------------------------------------------ plans
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+struct Plan {
+  int P, Dp;
+  int64_t Bp, tiles_b, tiles_v;
+  int stat_splits;
+  // backward
+  int64_t piece;                     // classes of a piece, a multiple of kTile
+  int tiles_d;
+  int dx_splits, dw_splits;
+};
+
+constexpr int64_t kPieceBytes = int64_t(96) << 20;      // of dz: stays in the 256 MB last-level cache with its operands
+constexpr int kWant = 512;                              // workgroups a launch should have: two per CU
+
+Plan make_plan(int dtype, int64_t B, int64_t D, int64_t V) {
+  Plan p;
+  p.P = dtype == SGNN_F32 ? 3 : 1;
+  p.Dp = int(ceil_div(D, 64) * 64);
+  p.tiles_b = ceil_div(B, kTile);
+  p.tiles_v = ceil_div(V, kTile);
+  p.Bp = p.tiles_b * kTile;
+  int64_t s = ceil_div(kWant, p.tiles_b);
+  p.stat_splits = int(s < p.tiles_v ? s : p.tiles_v);
+  int64_t tiles = kPieceBytes / (p.Bp * 2 * p.P * kTile);
+  if (tiles < 1) tiles = 1;
+  if (tiles > p.tiles_v) tiles = p.tiles_v;
+  p.piece = tiles * kTile;
+  p.tiles_d = int(ceil_div(D, kTile));
+  const int bk = p.P == 1 ? 64 : 32;
+  s = ceil_div(kWant, p.tiles_b * p.tiles_d);
+  int64_t most = p.piece / bk / 2;
+  p.dx_splits = int(s < most ? s : most);
+  s = ceil_div(kWant, tiles * p.tiles_d);
+  most = p.Bp / bk / 2;
+  p.dw_splits = int(s < most ? s : most);
+  if (p.dx_splits < 1) p.dx_splits = 1;
+  if (p.dw_splits < 1) p.dw_splits = 1;
+  return p;
+}
+
+struct Buffers {
+  uint16_t *x, *w, *dz;
+  float2* part;
+  float *picked, *dx, *dw;
+  size_t bytes;
+};
+
+Buffers carve(const Plan& p, int64_t B, int64_t V, bool backward, void* base) {
+  sgnn::Carver c(base);
+  Buffers b{};
+  b.x = c.take<uint16_t>(size_t(p.P) * B * p.Dp);
+  b.w = c.take<uint16_t>(size_t(p.P) * V * p.Dp);
+  if (!backward) {
+    b.part = c.take<float2>(size_t(p.stat_splits) * 2 * B);
+    b.picked = c.take<float>(size_t(B));
+  } else {
+    const size_t Np = size_t(p.tiles_d) * kTile;
+    b.dz = c.take<uint16_t>(size_t(p.P) * p.Bp * p.piece);
+    b.dx = c.take<float>(size_t(p.dx_splits) * p.Bp * Np);
+    b.dw = c.take<float>(size_t(p.dw_splits) * p.piece * Np);
+  }
+  b.bytes = c.off;
+  return b;
+}
+
+struct Call {
+  int dtype;
+  int64_t B, D, V;
+  const void* x;
+  int64_t ldx;
+  const void* w;
+  int64_t sv, sd;
+  const int64_t* labels;
+  int64_t n_labels;
+  const int64_t* idx;
+};
+
+int check_call(const Call& c) {
+  using sgnn::fail;
+  if (c.dtype != SGNN_F32 && c.dtype != SGNN_BF16) return fail(SGNN_ERR_INVALID, "unknown element type");
+  if (c.B <= 0 || c.D <= 0 || c.V <= 0) return fail(SGNN_ERR_INVALID, "need B > 0, D > 0, V > 0");
+  if (c.B > (int64_t(1) << 30) || c.V > (int64_t(1) << 30) || c.D > (int64_t(1) << 16))
+    return fail(SGNN_ERR_UNSUPPORTED, "head larger than 2^30 rows, 2^30 classes or 65536 features");
+  if (c.ldx < c.D) return fail(SGNN_ERR_INVALID, "row stride smaller than the width");
+  if (!((c.sd == 1 && c.sv >= c.D) || (c.sv == 1 && c.sd >= c.V)))
+    return fail(SGNN_ERR_INVALID, "the weight must have unit stride along its features or its classes");
+  if (c.n_labels < 0 || (!c.idx && c.n_labels < c.B)) return fail(SGNN_ERR_INVALID, "fewer labels than rows");
+  if (!c.x || !c.w || !c.labels) return fail(SGNN_ERR_INVALID, "null pointer");
+  return SGNN_OK;
+}
+
+template <typename T, int P>
+int planes(int64_t R, int64_t D, int Dp, const void* in, int64_t sr, int64_t sd, const Labels& of, uint16_t* out,
+           Operand* op, hipStream_t st) {
+  const int64_t bx = ceil_div(R, 64);
+  hipLaunchKernelGGL((k_planes<T, P>), dim3(unsigned(bx), unsigned(Dp / 64)), dim3(256), 0, st, R, int(D), Dp,
+                     static_cast<const T*>(in), sr, sd, of, out);
+  HIP_TRY(hipGetLastError());
+  *op = Operand{out, Dp, R * Dp, R, Dp};
+  return SGNN_OK;
+}
+
+template <typename T, int P>
+int forward(const Call& c, const Plan& p, const Buffers& b, float2* stats, float* row_loss, float* loss,
+            float* share, hipStream_t st) {
+  Operand x, w;
+  if (int rc = planes<T, P>(c.B, c.D, p.Dp, c.x, c.ldx, 1, Labels{c.labels, c.idx, c.n_labels, c.V}, b.x, &x, st)) return rc;
+  if (int rc = planes<T, P>(c.V, c.D, p.Dp, c.w, c.sv, c.sd, Labels{}, b.w, &w, st)) return rc;
+  hipLaunchKernelGGL((k_class_stats<P>), dim3(unsigned(p.tiles_b * p.stat_splits)), dim3(kThreads), 0, st, c.B, c.V,
+                     p.Dp, x, w, c.labels, c.idx, c.n_labels, p.tiles_v, p.stat_splits, b.part, b.picked);
+  HIP_TRY(hipGetLastError());
+  hipLaunchKernelGGL(k_class_rows, dim3(unsigned(ceil_div(c.B, 256))), dim3(256), 0, st, c.B, c.V, 2 * p.stat_splits,
+                     b.part, b.picked, c.labels, c.idx, c.n_labels, stats, row_loss);
+  HIP_TRY(hipGetLastError());
+  if (loss) {
+    hipLaunchKernelGGL(k_class_mean, dim3(1), dim3(1024), 0, st, c.B, c.V, row_loss, c.labels, c.idx, c.n_labels, loss,
+                       share);
+    HIP_TRY(hipGetLastError());
+  }
+  return SGNN_OK;
+}
+
+template <typename T>
+int join(int64_t R, int64_t D, int splits, const float* in, int64_t plane, int64_t ldi, T* out, int64_t sr, int64_t sd,
+         hipStream_t st) {
+  hipLaunchKernelGGL((k_class_join<T>), dim3(unsigned(ceil_div(R, 32)), unsigned(ceil_div(D, 32))), dim3(256), 0, st, R,
+                     int(D), splits, in, plane, ldi, out, sr, sd);
+  HIP_TRY(hipGetLastError());
+  return SGNN_OK;
+}
+
+template <typename T, int P>
+int backward(const Call& c, const Plan& p, const Buffers& b, const float2* stats, const float* grad,
+             const float* share, void* dx, int64_t lddx, void* dw, int64_t dsv, int64_t dsd, hipStream_t st) {
+  Operand x, w;
+  if (int rc = planes<T, P>(c.B, c.D, p.Dp, c.x, c.ldx, 1, Labels{c.labels, c.idx, c.n_labels, c.V}, b.x, &x, st)) return rc;
+  if (int rc = planes<T, P>(c.V, c.D, p.Dp, c.w, c.sv, c.sd, Labels{}, b.w, &w, st)) return rc;
+  const int64_t Np = int64_t(p.tiles_d) * kTile;
+  const int64_t dz_plane = p.Bp * p.piece;
+  for (int64_t v0 = 0; v0 < c.V; v0 += p.piece) {
+    const int64_t left = ceil_div(c.V - v0, kTile);
+    const int tiles = int(left < p.piece / kTile ? left : p.piece / kTile);
+    const int64_t width = int64_t(tiles) * kTile;
+    hipLaunchKernelGGL((k_class_dz<P>), dim3(unsigned(p.tiles_b * tiles)), dim3(kThreads), 0, st, c.B, c.V, p.Dp, x, w,
+                       c.labels, c.idx, c.n_labels, stats, grad, share, v0, tiles, b.dz, p.piece, dz_plane);
+    HIP_TRY(hipGetLastError());
+    if (dx) {                                    // dx[b][d] += dz[b][v] . w[v][d]
+      const Operand a{b.dz, p.piece, dz_plane, p.Bp, p.piece};
+      const Operand wv{w.base + v0 * w.ld, w.ld, w.plane, c.V - v0, w.cols};
+      hipLaunchKernelGGL((k_class_product<P, true>), dim3(unsigned(p.tiles_b * p.dx_splits * p.tiles_d)),
+                         dim3(kThreads), 0, st, a, wv, int(p.tiles_b), p.tiles_d, width, p.dx_splits, v0 > 0 ? 1 : 0,
+                         b.dx, p.Bp * Np, Np);
+      HIP_TRY(hipGetLastError());
+    }
+    if (dw) {                                    // dw[v][d] = dz[b][v] . x[b][d]
+      const Operand a{b.dz, p.piece, dz_plane, p.Bp, p.piece};
+      hipLaunchKernelGGL((k_class_product<P, false>), dim3(unsigned(tiles * p.dw_splits * p.tiles_d)), dim3(kThreads),
+                         0, st, a, x, tiles, p.tiles_d, p.Bp, p.dw_splits, 0, b.dw, p.piece * Np, Np);
+      HIP_TRY(hipGetLastError());
+      const int64_t rows = c.V - v0 < width ? c.V - v0 : width;
+      if (int rc = join<T>(rows, c.D, p.dw_splits, b.dw, p.piece * Np, Np, static_cast<T*>(dw) + v0 * dsv, dsv, dsd, st))
+        return rc;
+    }
+  }
+  if (dx) return join<T>(c.B, c.D, p.dx_splits, b.dx, p.Bp * Np, Np, static_cast<T*>(dx), lddx, 1, st);
+  return SGNN_OK;
+}
+
+}  // namespace
+
+extern "C" size_t sgnn_class_xent_workspace_bytes(int dtype, int64_t B, int64_t D, int64_t V, int backward) {
+  if (B <= 0 || D <= 0 || V <= 0 || (dtype != SGNN_F32 && dtype != SGNN_BF16)) return 0;
+  return carve(make_plan(dtype, B, D, V), B, V, backward != 0, nullptr).bytes;
+}
+
+extern "C" int sgnn_class_xent_forward(int dtype, int64_t B, int64_t D, int64_t V, const void* x, int64_t ldx,
+                                       const void* weight, int64_t sv, int64_t sd, const int64_t* labels,
+                                       int64_t n_labels, const int64_t* idx, float* stats, float* row_loss,
+                                       float* loss, float* share, void* workspace, size_t workspace_bytes,
+                                       void* stream) {
+  using sgnn::fail;
+  const Call c{dtype, B, D, V, x, ldx, weight, sv, sd, labels, n_labels, idx};
+  if (int rc = check_call(c)) return rc;
+  if (!stats || !row_loss || !workspace || (loss && !share)) return fail(SGNN_ERR_INVALID, "null pointer");
+  const Plan p = make_plan(dtype, B, D, V);
+  const Buffers b = carve(p, B, V, false, workspace);
+  if (workspace_bytes < b.bytes) return fail(SGNN_ERR_WORKSPACE, "class-loss workspace too small");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  float2* s = reinterpret_cast<float2*>(stats);
+  if (dtype == SGNN_F32) return forward<float, 3>(c, p, b, s, row_loss, loss, share, st);
+  return forward<Bf16, 1>(c, p, b, s, row_loss, loss, share, st);
+}
+
+extern "C" int sgnn_class_xent_backward(int dtype, int64_t B, int64_t D, int64_t V, const void* x, int64_t ldx,
+                                        const void* weight, int64_t sv, int64_t sd, const int64_t* labels,
+                                        int64_t n_labels, const int64_t* idx, const float* stats, const float* grad,
+                                        const float* share, void* dx, int64_t lddx, void* dweight, int64_t dsv,
+                                        int64_t dsd, void* workspace, size_t workspace_bytes, void* stream) {
+  using sgnn::fail;
+  const Call c{dtype, B, D, V, x, ldx, weight, sv, sd, labels, n_labels, idx};
+  if (int rc = check_call(c)) return rc;
+  if (!stats || !grad || !workspace) return fail(SGNN_ERR_INVALID, "null pointer");
+  if (dx && lddx < D) return fail(SGNN_ERR_INVALID, "row stride smaller than the width");
+  if (dweight && !((dsd == 1 && dsv >= D) || (dsv == 1 && dsd >= V)))
+    return fail(SGNN_ERR_INVALID, "the weight's gradient must have unit stride along its features or its classes");
+  if (!dx && !dweight) return SGNN_OK;
+  const Plan p = make_plan(dtype, B, D, V);
+  const Buffers b = carve(p, B, V, true, workspace);
+  if (workspace_bytes < b.bytes) return fail(SGNN_ERR_WORKSPACE, "class-loss workspace too small");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const float2* s = reinterpret_cast<const float2*>(stats);
+  if (dtype == SGNN_F32) return backward<float, 3>(c, p, b, s, grad, share, dx, lddx, dweight, dsv, dsd, st);
+  return backward<Bf16, 1>(c, p, b, s, grad, share, dx, lddx, dweight, dsv, dsd, st);
+}

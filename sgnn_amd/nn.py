@@ -14,6 +14,7 @@ import math
 import torch
 from torch import nn
 
+from .class_loss import class_cross_entropy  # noqa: F401
 from .norm_adj import NormAdj
 from .saved8 import SavedInt8, activated, checked_slope, linear_saved_int8, save_int8  # noqa: F401
 

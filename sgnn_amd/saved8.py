@@ -21,7 +21,8 @@ from . import _lib
 _TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 
 
-def _type(t, what):
+def element_type(t, what):
+    """The library's code of a GPU tensor's element type."""
     if not t.is_cuda:
         raise ValueError(f"{what} must be on the GPU, got {t.device}")
     code = _TYPES.get(t.dtype)
@@ -49,7 +50,7 @@ def activated(x, slope):
     return torch.relu(x) if slope == 0.0 else torch.nn.functional.leaky_relu(x, slope)
 
 
-def _rows(t):
+def unit_rows(t):
     """``t`` with unit stride along its rows and rows that do not overlap (a copy if need be)."""
     n, f = t.shape
     if (f > 1 and t.stride(1) != 1) or (n > 1 and t.stride(0) < f):
@@ -103,13 +104,13 @@ class SavedInt8:
         return out
 
     def _grad(self, grad, width, what):
-        _type(grad, what)
+        element_type(grad, what)
         if grad.dim() != 2 or grad.shape[0] != self.shape[0] or (width is not None and grad.shape[1] != width):
             raise ValueError(f"{what} must have shape ({self.shape[0]}, {'H' if width is None else width}), "
                              f"got {tuple(grad.shape)}")
         if grad.device != self.device:
             raise ValueError(f"{what} is on {grad.device}, the saved activation on {self.device}")
-        return _rows(grad.detach())
+        return unit_rows(grad.detach())
 
     def weight_grad(self, grad):
         """``grad.T @ values``: the gradient ``[H, F]`` of a weight applied to the activation, from
@@ -145,11 +146,11 @@ class SavedInt8:
 
 
 def _save(x, slope, with_act):
-    code = _type(x, "the activation")
+    code = element_type(x, "the activation")
     if x.dim() != 2 or x.shape[1] == 0:
         raise ValueError(f"the activation must be a matrix with at least one column, got {tuple(x.shape)}")
     slope = checked_slope(slope)
-    x = _rows(x.detach())
+    x = unit_rows(x.detach())
     n, F = x.shape
     groups = -(-F // _lib.SAVED8_GROUP)
     codes = torch.empty(n, groups * _lib.SAVED8_GROUP, dtype=torch.int8, device=x.device)
@@ -193,8 +194,8 @@ def linear_saved_int8(x, weight, slope=1.0):
     input but the 8-bit codes for the backward pass.  The output and ``x``'s gradient are those of
     the full activation; the weight's gradient is formed from the codes (off by half a step of
     their group at most, element by element)."""
-    code = _type(x, "the input")
-    if _type(weight, "the weight") != code:
+    code = element_type(x, "the input")
+    if element_type(weight, "the weight") != code:
         raise TypeError(f"the input is {x.dtype}, the weight {weight.dtype}")
     if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1]:
         raise ValueError(f"need an (n, F) input and an (H, F) weight, got {tuple(x.shape)} and {tuple(weight.shape)}")
