@@ -36,25 +36,29 @@ template <typename T> __device__ __forceinline__ T narrow(float v);
 template <> __device__ __forceinline__ float narrow<float>(float v) { return v; }
 template <> __device__ __forceinline__ Bf16 narrow<Bf16>(float v) { return Bf16{to_bf16(v)}; }
 
-// v = plane 0 + plane 1 + plane 2 exactly; infinities and NaN live in plane 0 only
-__device__ __forceinline__ void split3(float v, uint16_t (&p)[3]) {
-  const unsigned u = __float_as_uint(v);
-  if ((u & 0x7f800000u) == 0x7f800000u) {
-    p[0] = (u & 0x7fffffu) ? uint16_t(0x7fc0u) : uint16_t(u >> 16);
-    p[1] = p[2] = 0;
-    return;
-  }
-  const float r = v - __uint_as_float(u & 0xffff0000u);
-  const unsigned ur = __float_as_uint(r);
-  p[0] = uint16_t(u >> 16);
-  p[1] = uint16_t(ur >> 16);
-  p[2] = uint16_t(__float_as_uint(r - __uint_as_float(ur & 0xffff0000u)) >> 16);
+// v = plane 0 + plane 1 + plane 2 exactly; an infinity or NaN leaves a NaN behind
+__device__ __forceinline__ void split3(float v, float& a, float& b, float& c) {
+  a = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
+  const float r = v - a;
+  b = __uint_as_float(__float_as_uint(r) & 0xffff0000u);
+  c = r - b;
+}
+__device__ __forceinline__ uint16_t high_half(float v) { return uint16_t(__float_as_uint(v) >> 16); }
+// the high halves of two floats as a bf16 pair
+__device__ __forceinline__ unsigned high_halves(float lo, float hi) {
+  return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
 }
 template <int P>
 __device__ __forceinline__ void to_planes(float v, uint16_t (&p)[P]) {
-  if constexpr (P == 1) p[0] = to_bf16(v);
-  else split3(v, p);
+  if constexpr (P == 1) {
+    p[0] = to_bf16(v);
+  } else {
+    float a, b, c;
+    split3(v, a, b, c);
+    p[0] = high_half(a); p[1] = high_half(b); p[2] = high_half(c);
+  }
 }
+__device__ __forceinline__ float exp2_raw(float v) { return __builtin_amdgcn_exp2f(v); }   // 0 below 2^-126
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -70,33 +74,65 @@ struct Labels {
   const int64_t *labels, *idx;
   int64_t n_labels, V;
 };
-// in[r][d] at r * sr + d * sd  ->  out[plane][r][Dp], columns D .. Dp zero.  A 64 x 64 tile goes
-// through LDS, read along whichever of its directions is contiguous.  Rows of x without a class
-// become zeros, so that whatever a padded row holds (NaN too) reaches no gradient.
+// in[r][d] at r * sr + d * sd  ->  out[plane][r][Dp], columns D .. Dp zero.  Rows of x without a
+// class become zeros, so that whatever a padded row holds (NaN too) reaches no gradient.
+struct Source {
+  const void* in;
+  int64_t rows, sr, sd;
+  uint16_t* out;
+  int64_t blocks;          // workgroups it takes: one for 64 x 64 elements
+};
+
+// x and the weight in one launch.  Rows that are contiguous go straight through registers, eight
+// elements a lane; a weight stored by feature goes through a tile in LDS.
 template <typename T, int P>
-__global__ __launch_bounds__(256) void k_planes(int64_t R, int D, int Dp, const T* __restrict__ in, int64_t sr,
-                                                int64_t sd, Labels of, uint16_t* __restrict__ out) {
+__global__ __launch_bounds__(256) void k_planes(int D, int Dp, Source first, Source second, Labels of) {
   __shared__ float tile[64][65];
-  const int64_t r0 = int64_t(blockIdx.x) * 64;
-  const int d0 = blockIdx.y * 64, t = threadIdx.x;
-  for (int i = t; i < 64 * 64; i += 256) {
-    const int fast = i & 63, slow = i >> 6;
-    const int lr = sd == 1 ? slow : fast, ld = sd == 1 ? fast : slow;
-    const int64_t r = r0 + lr;
-    const int d = d0 + ld;
-    const bool live = r < R && d < D && (of.V == 0 || label_of(r, of.labels, of.idx, of.n_labels, of.V) >= 0);
-    tile[lr][ld] = live ? widen(in[r * sr + d * sd]) : 0.f;
+  const bool is_x = int64_t(blockIdx.x) < first.blocks;
+  const Source src = is_x ? first : second;
+  const int64_t block = is_x ? blockIdx.x : blockIdx.x - first.blocks;
+  const int across = Dp / 64;
+  const int64_t r0 = block / across * 64;
+  const int d0 = int(block % across) * 64, t = threadIdx.x;
+  const T* in = static_cast<const T*>(src.in);
+  const auto live = [&](int64_t r) {
+    return r < src.rows && (!is_x || label_of(r, of.labels, of.idx, of.n_labels, of.V) >= 0);
+  };
+  if (src.sd != 1) {
+    for (int i = t; i < 64 * 64; i += 256) {
+      const int lr = i & 63, ld = i >> 6;
+      const int64_t r = r0 + lr;
+      const int d = d0 + ld;
+      tile[lr][ld] = (d < D && live(r)) ? widen(in[r * src.sr + d * src.sd]) : 0.f;
+    }
+    __syncthreads();
   }
-  __syncthreads();
+#pragma unroll
   for (int i = t; i < 64 * 8; i += 256) {
-    const int lr = i >> 3, c = (i & 7) * 8;
+    const int lr = i >> 3, c = (i & 7) * 8, d = d0 + c;
     const int64_t r = r0 + lr;
-    if (r >= R) continue;
+    if (r >= src.rows) continue;
+    float v[8];
+    if (src.sd != 1) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = tile[lr][c + e];
+    } else if (!live(r)) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = 0.f;
+    } else if (d + 8 <= D) {
+      T raw[8];
+      __builtin_memcpy(&raw, in + r * src.sr + d, sizeof(raw));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = widen(raw[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = d + e < D ? widen(in[r * src.sr + d + e]) : 0.f;
+    }
     uint16_t pl[P][8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       uint16_t p[P];
-      to_planes<P>(tile[lr][c + e], p);
+      to_planes<P>(v[e], p);
 #pragma unroll
       for (int q = 0; q < P; ++q) pl[q][e] = p[q];
     }
@@ -104,7 +140,7 @@ __global__ __launch_bounds__(256) void k_planes(int64_t R, int D, int Dp, const 
     for (int q = 0; q < P; ++q) {
       u32x4 w;
       __builtin_memcpy(&w, &pl[q][0], 16);
-      *reinterpret_cast<u32x4*>(out + (int64_t(q) * R + r) * Dp + d0 + c) = w;
+      *reinterpret_cast<u32x4*>(src.out + (int64_t(q) * src.rows + r) * Dp + d) = w;
     }
   }
 }
@@ -250,9 +286,32 @@ __device__ __forceinline__ void multiply(const Operand& A, int64_t m0, const Ope
 __device__ __forceinline__ int block_row(int e, int lane) { return 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3); }
 
 // ------------------------------------------------------------------ forward
+// (m, s) = (maximum, sum of exp relative to it).  While everything is -inf the sum stays 0; a NaN
+// never becomes the maximum but makes the sum NaN.
+__device__ __forceinline__ void join_stats(float& m, float& s, float om, float os) {
+  const float top = fmaxf(m, om), ref = top == -INFINITY ? 0.f : top;
+  s = s * exp2_raw((m - ref) * kLog2e) + os * exp2_raw((om - ref) * kLog2e);
+  m = top;
+}
+__device__ __forceinline__ void accumulate(const f32x16& a, const f32x16& b, float& m, float& s) {
+  float top = m;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) top = fmaxf(fmaxf(a[e], b[e]), top);
+  const float ref = top == -INFINITY ? 0.f : top;
+  s *= exp2_raw((m - ref) * kLog2e);
+  float s1 = 0.f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    s += exp2_raw((a[e] - ref) * kLog2e);
+    s1 += exp2_raw((b[e] - ref) * kLog2e);
+  }
+  s += s1;
+  m = top;
+}
+
 // A workgroup takes 128 rows of x and a range of the classes, 128 at a time.  The tile is formed
 // as classes x rows, so that a lane holds 32 classes of each of two rows and its running maximum
-// and sum need no other lane until the end.  part[split][row] = (max, sum of exp relative to it).
+// and sum need no other lane until the end.  part[row][split][half] = (max, sum of exp relative to it).
 template <int P>
 __global__ __launch_bounds__(kThreads) void k_class_stats(int64_t B, int64_t V, int Dp, Operand x, Operand w,
                                                           const int64_t* __restrict__ labels,
@@ -278,60 +337,58 @@ __global__ __launch_bounds__(kThreads) void k_class_stats(int64_t B, int64_t V, 
     Tile acc;
     clear(acc);
     multiply<P, true, true>(w, t * kTile, x, b0, 0, Dp, lds, acc);
+    const int64_t vw = t * kTile + wv;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      float m = top[j];
+      if (__any(y[j] >= vw && y[j] < vw + 64)) {       // one tile in V / 64 holds a row's label
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int64_t v = t * kTile + wv + 32 * i + block_row(e, lane);
-          if (v == y[j]) picked[b0 + wb + 32 * j + (lane & 31)] = acc[i][j][e];
-          if (v >= V) acc[i][j][e] = -INFINITY;
-          m = acc[i][j][e] > m || acc[i][j][e] != acc[i][j][e] ? acc[i][j][e] : m;      // a NaN stays
-        }
-      // while everything is -inf the sum stays 0
-      const float ref = m == -INFINITY ? 0.f : m;
-      float s = sum[j] * exp2f((top[j] - ref) * kLog2e);
+          for (int e = 0; e < 16; ++e)
+            if (vw + 32 * i + block_row(e, lane) == y[j]) picked[b0 + wb + 32 * j + (lane & 31)] = acc[i][j][e];
+      }
+      if (vw + 64 > V) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s += exp2f((acc[i][j][e] - ref) * kLog2e);
-      top[j] = m;
-      sum[j] = s;
+          for (int e = 0; e < 16; ++e)
+            if (vw + 32 * i + block_row(e, lane) >= V) acc[i][j][e] = -INFINITY;
+      }
+      accumulate(acc[0][j], acc[1][j], top[j], sum[j]);
     }
   }
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const float om = __shfl_xor(top[j], 32), os = __shfl_xor(sum[j], 32);
-    const float m = (om > top[j] || om != om) ? om : top[j], ref = m == -INFINITY ? 0.f : m;
-    const float s = sum[j] * exp2f((top[j] - ref) * kLog2e) + os * exp2f((om - ref) * kLog2e);
+    join_stats(top[j], sum[j], om, os);
     const int64_t b = b0 + wb + 32 * j + (lane & 31);
-    if (lane < 32 && b < B) part[(int64_t(split) * 2 + (wave >> 1)) * B + b] = make_float2(m, s);
+    if (lane < 32 && b < B) part[b * (2 * splits) + split * 2 + (wave >> 1)] = make_float2(top[j], sum[j]);
   }
 }
 
-// One row's pieces joined: stats[b] = (max, sum), row_loss[b] (0 where the row has no class).
+// A row's pieces joined by one wavefront: stats[b] = (max, sum), row_loss[b] (0 where the row has no class).
 __global__ __launch_bounds__(256) void k_class_rows(int64_t B, int64_t V, int parts, const float2* __restrict__ part,
                                                     const float* __restrict__ picked,
                                                     const int64_t* __restrict__ labels,
                                                     const int64_t* __restrict__ idx, int64_t n_labels,
                                                     float2* __restrict__ stats, float* __restrict__ row_loss) {
-  const int64_t b = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  const int lane = threadIdx.x & 63;
+  const int64_t b = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (b >= B) return;
-  float m = -INFINITY;
-  for (int q = 0; q < parts; ++q) {
-    const float o = part[int64_t(q) * B + b].x;
-    m = (o > m || o != o) ? o : m;
+  float m = -INFINITY, s = 0.f;
+  for (int q = lane; q < parts; q += 64) {
+    const float2 o = part[b * parts + q];
+    join_stats(m, s, o.x, o.y);
   }
-  const float ref = m == -INFINITY ? 0.f : m;
-  float s = 0.f;
-  for (int q = 0; q < parts; ++q) {
-    const float2 o = part[int64_t(q) * B + b];
-    s += o.y * exp2f((o.x - ref) * kLog2e);
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) {
+    const float om = __shfl_xor(m, off), os = __shfl_xor(s, off);
+    join_stats(m, s, om, os);
   }
-  stats[b] = make_float2(m, s);
-  row_loss[b] = label_of(b, labels, idx, n_labels, V) >= 0 ? (m - picked[b]) + log2f(s) * kLn2 : 0.f;
+  if (lane == 0) {
+    stats[b] = make_float2(m, s);
+    row_loss[b] = label_of(b, labels, idx, n_labels, V) >= 0 ? (m - picked[b]) + log2f(s) * kLn2 : 0.f;
+  }
 }
 
 // loss[0] = mean loss of the counted rows (0 if there are none), share[0] = 1 / their number.
@@ -369,13 +426,15 @@ __global__ __launch_bounds__(1024) void k_class_mean(int64_t B, int64_t V, const
 
 // ------------------------------------------------------------------ backward
 // dz of the classes v0 .. v0 + 128 * tiles and all rows, as bf16 planes [plane][Bp][ldz]; rows and
-// classes beyond the last are 0.
+// classes beyond the last are 0.  `grad` NULL leaves the mean's factor to the gradients' last step.
+// The label's element dominates a row and is the one whose rounding to bf16 would be felt in dx:
+// what it loses is kept in rest[b] and joins dx in 32 bits.
 template <int P>
 __global__ __launch_bounds__(kThreads) void k_class_dz(int64_t B, int64_t V, int Dp, Operand x, Operand w,
                                                        const int64_t* __restrict__ labels,
                                                        const int64_t* __restrict__ idx, int64_t n_labels,
                                                        const float2* __restrict__ stats,
-                                                       const float* __restrict__ grad, const float* __restrict__ share,
+                                                       const float* __restrict__ grad, float* __restrict__ rest,
                                                        int64_t v0, int tiles, uint16_t* __restrict__ dz, int64_t ldz,
                                                        int64_t plane) {
   constexpr int kRow = kTile * 2 + 16;             // bytes of a staged row of dz
@@ -388,23 +447,36 @@ __global__ __launch_bounds__(kThreads) void k_class_dz(int64_t B, int64_t V, int
   Tile acc;
   clear(acc);
   multiply<P, true, true>(w, vt, x, b0, 0, Dp, lds, acc);
+  const int64_t vw = vt + wv;
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const int64_t b = b0 + wb + 32 * j + (lane & 31);
     const int64_t y = b < B ? label_of(b, labels, idx, n_labels, V) : -1;
-    // share given: the mean's gradient over the counted rows; else a gradient for each row
-    const float g = y >= 0 ? (share ? grad[0] * share[0] : grad[b]) : 0.f;
+    const float g = y >= 0 ? (grad ? grad[b] : 1.f) : 0.f;
     const float2 st = b < B ? stats[b] : make_float2(0.f, 1.f);
     const float scale = g / st.y;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int64_t v = vt + wv + 32 * i + block_row(e, lane);
-        float d = exp2f((acc[i][j][e] - st.x) * kLog2e) * scale;
-        if (v == y) d -= g;
-        acc[i][j][e] = y >= 0 && v < V ? d : 0.f;
-      }
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = exp2_raw((acc[i][j][e] - st.x) * kLog2e) * scale;
+    if (__any(y >= vw && y < vw + 64)) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (vw + 32 * i + block_row(e, lane) == y) {
+            const float d = acc[i][j][e] - g;
+            acc[i][j][e] = d;
+            if constexpr (P == 1) rest[b] = d - widen(Bf16{to_bf16(d)});
+          }
+    }
+    if (vw + 64 > V || __any(y < 0)) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (y < 0 || vw + 32 * i + block_row(e, lane) >= V) acc[i][j][e] = 0.f;
+    }
   }
 #pragma unroll
   for (int p = 0; p < P; ++p) {
@@ -464,28 +536,45 @@ __global__ __launch_bounds__(kThreads) void k_class_product(Operand A, Operand B
       }
 }
 
-// out[r][d] = sum over the shares, in order; out at r * sr + d * sd
+// out[r][d] = factor * (sum over the shares, in order, + rest[r] * weight[y(r)][d]), out at r * sr +
+// d * sd; factor = grad[0] * share[0] or 1; `rest` (dx in bf16) may be NULL.  With `of` rows without
+// a class are 0 whatever the weight holds.
 template <typename T>
 __global__ __launch_bounds__(256) void k_class_join(int64_t R, int D, int splits, const float* __restrict__ in,
-                                                    int64_t plane, int64_t ldi, T* __restrict__ out, int64_t sr,
-                                                    int64_t sd) {
+                                                    int64_t plane, int64_t ldi, const float* __restrict__ grad,
+                                                    const float* __restrict__ share, const float* __restrict__ rest,
+                                                    Labels of, const T* __restrict__ weight, int64_t sv, int64_t sdw,
+                                                    T* __restrict__ out, int64_t sr, int64_t sd) {
   __shared__ float tile[32][33];
   const int64_t r0 = int64_t(blockIdx.x) * 32;
   const int d0 = blockIdx.y * 32, t = threadIdx.x;
+  const float factor = share ? grad[0] * share[0] : 1.f;
+#pragma unroll
   for (int i = t; i < 32 * 32; i += 256) {
     const int lr = i >> 5, ld = i & 31;
+    const int64_t r = r0 + lr;
     float s = 0.f;
-    if (r0 + lr < R && d0 + ld < D) {
-      const float* src = in + (r0 + lr) * ldi + d0 + ld;
+    if (r < R && d0 + ld < D) {
+      const float* src = in + r * ldi + d0 + ld;
 #pragma unroll 4
       for (int q = 0; q < splits; ++q) s += src[q * plane];
+      if (of.V) {
+        const int64_t y = label_of(r, of.labels, of.idx, of.n_labels, of.V);
+        if (y < 0) s = 0.f;
+        else if (rest) s += rest[r] * widen(weight[y * sv + (d0 + ld) * sdw]);
+      }
+      s *= factor;
     }
-    tile[lr][ld] = s;
+    if (sd == 1) {
+      if (r < R && d0 + ld < D) out[r * sr + d0 + ld] = narrow<T>(s);
+    } else {
+      tile[lr][ld] = s;
+    }
   }
+  if (sd == 1) return;
   __syncthreads();
   for (int i = t; i < 32 * 32; i += 256) {
-    const int fast = i & 31, slow = i >> 5;
-    const int lr = sd == 1 ? slow : fast, ld = sd == 1 ? fast : slow;
+    const int lr = i & 31, ld = i >> 5;
     if (r0 + lr < R && d0 + ld < D) out[(r0 + lr) * sr + (d0 + ld) * sd] = narrow<T>(tile[lr][ld]);
   }
 }
@@ -535,7 +624,7 @@ Plan make_plan(int dtype, int64_t B, int64_t D, int64_t V) {
 struct Buffers {
   uint16_t *x, *w, *dz;
   float2* part;
-  float *picked, *dx, *dw;
+  float *picked, *rest, *dx, *dw;
   size_t bytes;
 };
 
@@ -550,6 +639,7 @@ Buffers carve(const Plan& p, int64_t B, int64_t V, bool backward, void* base) {
   } else {
     const size_t Np = size_t(p.tiles_d) * kTile;
     b.dz = c.take<uint16_t>(size_t(p.P) * p.Bp * p.piece);
+    b.rest = c.take<float>(size_t(B));
     b.dx = c.take<float>(size_t(p.dx_splits) * p.Bp * Np);
     b.dw = c.take<float>(size_t(p.dw_splits) * p.piece * Np);
   }
@@ -575,6 +665,9 @@ int check_call(const Call& c) {
   if (c.B <= 0 || c.D <= 0 || c.V <= 0) return fail(SGNN_ERR_INVALID, "need B > 0, D > 0, V > 0");
   if (c.B > (int64_t(1) << 30) || c.V > (int64_t(1) << 30) || c.D > (int64_t(1) << 16))
     return fail(SGNN_ERR_UNSUPPORTED, "head larger than 2^30 rows, 2^30 classes or 65536 features");
+  const int64_t width = ceil_div(c.D, 64) * 64;
+  if (c.B * width > (int64_t(1) << 35) || c.V * width > (int64_t(1) << 35))      // one launch lays either out
+    return fail(SGNN_ERR_UNSUPPORTED, "an operand of more than 2^35 elements");
   if (c.ldx < c.D) return fail(SGNN_ERR_INVALID, "row stride smaller than the width");
   if (!((c.sd == 1 && c.sv >= c.D) || (c.sv == 1 && c.sd >= c.V)))
     return fail(SGNN_ERR_INVALID, "the weight must have unit stride along its features or its classes");
@@ -583,14 +676,25 @@ int check_call(const Call& c) {
   return SGNN_OK;
 }
 
+// A bf16 weight whose rows are whole 128-byte lines can be staged as it lies.
+bool weight_as_is(const Call& c, const Plan& p) {
+  return p.P == 1 && c.sd == 1 && c.D == p.Dp && c.sv % 8 == 0 && reinterpret_cast<uintptr_t>(c.w) % 16 == 0;
+}
+
 template <typename T, int P>
-int planes(int64_t R, int64_t D, int Dp, const void* in, int64_t sr, int64_t sd, const Labels& of, uint16_t* out,
-           Operand* op, hipStream_t st) {
-  const int64_t bx = ceil_div(R, 64);
-  hipLaunchKernelGGL((k_planes<T, P>), dim3(unsigned(bx), unsigned(Dp / 64)), dim3(256), 0, st, R, int(D), Dp,
-                     static_cast<const T*>(in), sr, sd, of, out);
+int planes(const Call& c, const Plan& p, const Buffers& b, Operand* x, Operand* w, hipStream_t st) {
+  const int across = p.Dp / 64;
+  const Source sx{c.x, c.B, c.ldx, 1, b.x, ceil_div(c.B, 64) * across};
+  Source sw{c.w, c.V, c.sv, c.sd, b.w, ceil_div(c.V, 64) * across};
+  *x = Operand{b.x, p.Dp, c.B * p.Dp, c.B, p.Dp};
+  *w = Operand{b.w, p.Dp, c.V * p.Dp, c.V, p.Dp};
+  if (weight_as_is(c, p)) {
+    sw.blocks = 0;
+    *w = Operand{static_cast<const uint16_t*>(c.w), c.sv, 0, c.V, c.D};
+  }
+  hipLaunchKernelGGL((k_planes<T, P>), dim3(unsigned(sx.blocks + sw.blocks)), dim3(256), 0, st, int(c.D), p.Dp, sx, sw,
+                     Labels{c.labels, c.idx, c.n_labels, c.V});
   HIP_TRY(hipGetLastError());
-  *op = Operand{out, Dp, R * Dp, R, Dp};
   return SGNN_OK;
 }
 
@@ -598,12 +702,11 @@ template <typename T, int P>
 int forward(const Call& c, const Plan& p, const Buffers& b, float2* stats, float* row_loss, float* loss,
             float* share, hipStream_t st) {
   Operand x, w;
-  if (int rc = planes<T, P>(c.B, c.D, p.Dp, c.x, c.ldx, 1, Labels{c.labels, c.idx, c.n_labels, c.V}, b.x, &x, st)) return rc;
-  if (int rc = planes<T, P>(c.V, c.D, p.Dp, c.w, c.sv, c.sd, Labels{}, b.w, &w, st)) return rc;
+  if (int rc = planes<T, P>(c, p, b, &x, &w, st)) return rc;
   hipLaunchKernelGGL((k_class_stats<P>), dim3(unsigned(p.tiles_b * p.stat_splits)), dim3(kThreads), 0, st, c.B, c.V,
                      p.Dp, x, w, c.labels, c.idx, c.n_labels, p.tiles_v, p.stat_splits, b.part, b.picked);
   HIP_TRY(hipGetLastError());
-  hipLaunchKernelGGL(k_class_rows, dim3(unsigned(ceil_div(c.B, 256))), dim3(256), 0, st, c.B, c.V, 2 * p.stat_splits,
+  hipLaunchKernelGGL(k_class_rows, dim3(unsigned(ceil_div(c.B, 4))), dim3(256), 0, st, c.B, c.V, 2 * p.stat_splits,
                      b.part, b.picked, c.labels, c.idx, c.n_labels, stats, row_loss);
   HIP_TRY(hipGetLastError());
   if (loss) {
@@ -614,21 +717,11 @@ int forward(const Call& c, const Plan& p, const Buffers& b, float2* stats, float
   return SGNN_OK;
 }
 
-template <typename T>
-int join(int64_t R, int64_t D, int splits, const float* in, int64_t plane, int64_t ldi, T* out, int64_t sr, int64_t sd,
-         hipStream_t st) {
-  hipLaunchKernelGGL((k_class_join<T>), dim3(unsigned(ceil_div(R, 32)), unsigned(ceil_div(D, 32))), dim3(256), 0, st, R,
-                     int(D), splits, in, plane, ldi, out, sr, sd);
-  HIP_TRY(hipGetLastError());
-  return SGNN_OK;
-}
-
 template <typename T, int P>
 int backward(const Call& c, const Plan& p, const Buffers& b, const float2* stats, const float* grad,
              const float* share, void* dx, int64_t lddx, void* dw, int64_t dsv, int64_t dsd, hipStream_t st) {
   Operand x, w;
-  if (int rc = planes<T, P>(c.B, c.D, p.Dp, c.x, c.ldx, 1, Labels{c.labels, c.idx, c.n_labels, c.V}, b.x, &x, st)) return rc;
-  if (int rc = planes<T, P>(c.V, c.D, p.Dp, c.w, c.sv, c.sd, Labels{}, b.w, &w, st)) return rc;
+  if (int rc = planes<T, P>(c, p, b, &x, &w, st)) return rc;
   const int64_t Np = int64_t(p.tiles_d) * kTile;
   const int64_t dz_plane = p.Bp * p.piece;
   for (int64_t v0 = 0; v0 < c.V; v0 += p.piece) {
@@ -636,7 +729,8 @@ int backward(const Call& c, const Plan& p, const Buffers& b, const float2* stats
     const int tiles = int(left < p.piece / kTile ? left : p.piece / kTile);
     const int64_t width = int64_t(tiles) * kTile;
     hipLaunchKernelGGL((k_class_dz<P>), dim3(unsigned(p.tiles_b * tiles)), dim3(kThreads), 0, st, c.B, c.V, p.Dp, x, w,
-                       c.labels, c.idx, c.n_labels, stats, grad, share, v0, tiles, b.dz, p.piece, dz_plane);
+                       c.labels, c.idx, c.n_labels, stats, share ? nullptr : grad, b.rest, v0, tiles, b.dz,
+                       p.piece, dz_plane);
     HIP_TRY(hipGetLastError());
     if (dx) {                                    // dx[b][d] += dz[b][v] . w[v][d]
       const Operand a{b.dz, p.piece, dz_plane, p.Bp, p.piece};
@@ -652,11 +746,19 @@ int backward(const Call& c, const Plan& p, const Buffers& b, const float2* stats
                          0, st, a, x, tiles, p.tiles_d, p.Bp, p.dw_splits, 0, b.dw, p.piece * Np, Np);
       HIP_TRY(hipGetLastError());
       const int64_t rows = c.V - v0 < width ? c.V - v0 : width;
-      if (int rc = join<T>(rows, c.D, p.dw_splits, b.dw, p.piece * Np, Np, static_cast<T*>(dw) + v0 * dsv, dsv, dsd, st))
-        return rc;
+      hipLaunchKernelGGL((k_class_join<T>), dim3(unsigned(ceil_div(rows, 32)), unsigned(ceil_div(c.D, 32))), dim3(256), 0,
+                         st, rows, int(c.D), p.dw_splits, b.dw, p.piece * Np, Np, grad, share, nullptr, Labels{}, nullptr,
+                         0, 0, static_cast<T*>(dw) + v0 * dsv, dsv, dsd);
+      HIP_TRY(hipGetLastError());
     }
   }
-  if (dx) return join<T>(c.B, c.D, p.dx_splits, b.dx, p.Bp * Np, Np, static_cast<T*>(dx), lddx, 1, st);
+  if (dx) {
+    hipLaunchKernelGGL((k_class_join<T>), dim3(unsigned(ceil_div(c.B, 32)), unsigned(ceil_div(c.D, 32))), dim3(256), 0, st,
+                       c.B, int(c.D), p.dx_splits, b.dx, p.Bp * Np, Np, grad, share, P == 1 ? b.rest : nullptr,
+                       Labels{c.labels, c.idx, c.n_labels, c.V}, static_cast<const T*>(c.w), c.sv, c.sd,
+                       static_cast<T*>(dx), lddx, int64_t(1));
+    HIP_TRY(hipGetLastError());
+  }
   return SGNN_OK;
 }
 
