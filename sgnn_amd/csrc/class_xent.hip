@@ -579,6 +579,253 @@ __global__ __launch_bounds__(256) void k_class_join(int64_t R, int D, int splits
   }
 }
 
+// ------------------------------------------------------------------ few rows
+// With up to 32 rows the weight is what counts: it is read once forward and twice backward (the
+// second time mostly from the last-level cache), as it lies, and its gradient written once.  x
+// waits in LDS as bf16 planes; a wavefront takes 32 classes at a time straight from memory into the
+// matrix instructions' operand, splitting them in registers.  Both gradients are plain 32-bit
+// multiply-adds: 2 * rows of them per element of the weight.
+constexpr int kFewRows = 32;
+constexpr int kFewBlocks = 768;                  // workgroups: three per CU
+constexpr int kFewSteps = 4;                     // 16-feature steps loaded together
+
+template <int P>
+__device__ __forceinline__ int few_at(int p, int row, int chunk, int Dk) {       // byte offset of 8 features in LDS
+  return ((p * kFewRows + row) * Dk) * 2 + ((chunk ^ (row & 7)) << 4);
+}
+
+// x's rows to LDS, features D .. Dk and rows without a class zero
+template <typename T, int P>
+__device__ __forceinline__ void few_stage(const Labels& of, int B, int D, int Dk, const T* __restrict__ x, int64_t ldx,
+                                          char* lds) {
+  for (int i = threadIdx.x; i < kFewRows * (Dk / 8); i += kThreads) {
+    const int row = i / (Dk / 8), chunk = i - row * (Dk / 8), d = chunk * 8;
+    const bool live = row < B && label_of(row, of.labels, of.idx, of.n_labels, of.V) >= 0;
+    uint16_t pl[P][8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      uint16_t p[P];
+      to_planes<P>(live && d + e < D ? widen(x[row * ldx + d + e]) : 0.f, p);
+#pragma unroll
+      for (int q = 0; q < P; ++q) pl[q][e] = p[q];
+    }
+#pragma unroll
+    for (int q = 0; q < P; ++q) {
+      u32x4 w;
+      __builtin_memcpy(&w, &pl[q][0], 16);
+      *reinterpret_cast<u32x4*>(lds + few_at<P>(q, row, chunk, Dk)) = w;
+    }
+  }
+  __syncthreads();
+}
+
+template <typename T, int P>
+__device__ __forceinline__ void few_operand(const T (&raw)[8], bf16x8 (&out)[P]) {
+  if constexpr (P == 1) {
+    __builtin_memcpy(&out[0], &raw, 16);
+  } else {
+    u32x4 pl[3];
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      float a0, b0, c0, a1, b1, c1;
+      split3(widen(raw[e]), a0, b0, c0);
+      split3(widen(raw[e + 1]), a1, b1, c1);
+      pl[0][e / 2] = high_halves(a0, a1);
+      pl[1][e / 2] = high_halves(b0, b1);
+      pl[2][e / 2] = high_halves(c0, c1);
+    }
+#pragma unroll
+    for (int q = 0; q < 3; ++q) __builtin_memcpy(&out[q], &pl[q], 16);
+  }
+}
+
+// logits of classes v0 .. v0 + 31 (rows of the block) and all 32 rows of x (columns)
+template <typename T, int P>
+__device__ __forceinline__ f32x16 few_logits(int D, int Dk, int64_t v0, int64_t V, const T* __restrict__ w, int64_t sv,
+                                             const char* lds, int lane) {
+  const int64_t v = v0 + (lane & 31) < V ? v0 + (lane & 31) : V - 1;
+  const int half = lane >> 5;
+  const T* src = w + v * sv + 8 * half;
+  f32x16 acc;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+  for (int k = 0; k < Dk; k += 16 * kFewSteps) {
+    T raw[kFewSteps][8];
+    if (k + 16 * kFewSteps <= D) {
+#pragma unroll
+      for (int u = 0; u < kFewSteps; ++u) __builtin_memcpy(&raw[u], src + k + 16 * u, sizeof(raw[u]));
+    } else {
+#pragma unroll
+      for (int u = 0; u < kFewSteps; ++u)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          raw[u][e] = k + 16 * u + 8 * half + e < D ? src[k + 16 * u + e] : narrow<T>(0.f);
+    }
+#pragma unroll
+    for (int u = 0; u < kFewSteps; ++u) {
+      if (k + 16 * u >= Dk) break;
+      bf16x8 a[P], b[P];
+      few_operand<T, P>(raw[u], a);
+#pragma unroll
+      for (int q = 0; q < P; ++q)
+        b[q] = *reinterpret_cast<const bf16x8*>(lds + few_at<P>(q, lane & 31, (k + 16 * u) / 8 + half, Dk));
+#pragma unroll
+      for (int pa = 0; pa < P; ++pa)
+#pragma unroll
+        for (int pb = 0; pa + pb < P; ++pb) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[pa], b[pb], acc, 0, 0, 0);
+    }
+  }
+  return acc;
+}
+
+template <typename T, int P>
+__global__ __launch_bounds__(kThreads) void k_few_stats(int B, int D, int Dk, int64_t V, const T* __restrict__ x,
+                                                        int64_t ldx, const T* __restrict__ w, int64_t sv, Labels of,
+                                                        float2* __restrict__ part, float* __restrict__ picked) {
+  extern __shared__ __align__(128) char few_lds[];
+  __shared__ float2 joined[4][kFewRows];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  few_stage<T, P>(of, B, D, Dk, x, ldx, few_lds);
+  const int b = lane & 31;
+  const int64_t y = b < B ? label_of(b, of.labels, of.idx, of.n_labels, of.V) : -1;
+  float m = -INFINITY, s = 0.f;
+  for (int64_t v0 = (int64_t(blockIdx.x) * 4 + wave) * 32; v0 < V; v0 += int64_t(gridDim.x) * 128) {
+    f32x16 z = few_logits<T, P>(D, Dk, v0, V, w, sv, few_lds, lane);
+    if (__any(y >= v0 && y < v0 + 32)) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (v0 + block_row(e, lane) == y) picked[b] = z[e];
+    }
+    if (v0 + 32 > V) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (v0 + block_row(e, lane) >= V) z[e] = -INFINITY;
+    }
+    float top = m;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) top = fmaxf(z[e], top);
+    const float ref = top == -INFINITY ? 0.f : top;
+    s *= exp2_raw((m - ref) * kLog2e);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s += exp2_raw((z[e] - ref) * kLog2e);
+    m = top;
+  }
+  const float om = __shfl_xor(m, 32), os = __shfl_xor(s, 32);
+  join_stats(m, s, om, os);
+  if (lane < kFewRows) joined[wave][lane] = make_float2(m, s);
+  __syncthreads();
+  if (threadIdx.x < unsigned(B)) {
+    m = -INFINITY;
+    s = 0.f;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) join_stats(m, s, joined[q][threadIdx.x].x, joined[q][threadIdx.x].y);
+    part[int64_t(threadIdx.x) * gridDim.x + blockIdx.x] = make_float2(m, s);
+  }
+}
+
+// dz[v][ROWS] in 32 bits, the rows' factors included
+template <typename T, int P>
+__global__ __launch_bounds__(kThreads) void k_few_dz(int B, int rows, int D, int Dk, int64_t V,
+                                                     const T* __restrict__ x, int64_t ldx, const T* __restrict__ w,
+                                                     int64_t sv, Labels of, const float2* __restrict__ stats,
+                                                     const float* __restrict__ grad, const float* __restrict__ share,
+                                                     float* __restrict__ dz) {
+  extern __shared__ __align__(128) char few_lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  few_stage<T, P>(of, B, D, Dk, x, ldx, few_lds);
+  const int b = lane & 31;
+  const int64_t y = b < B ? label_of(b, of.labels, of.idx, of.n_labels, of.V) : -1;
+  const float2 st = y >= 0 ? stats[b] : make_float2(0.f, 1.f);
+  const float g = y >= 0 ? (share ? grad[0] * share[0] : grad[b]) : 0.f;
+  const float scale = g / st.y;
+  for (int64_t v0 = (int64_t(blockIdx.x) * 4 + wave) * 32; v0 < V; v0 += int64_t(gridDim.x) * 128) {
+    const f32x16 z = few_logits<T, P>(D, Dk, v0, V, w, sv, few_lds, lane);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int64_t v = v0 + block_row(e, lane);
+      const float d = exp2_raw((z[e] - st.x) * kLog2e) * scale - (v == y ? g : 0.f);
+      if (b < rows && v < V) dz[v * rows + b] = y >= 0 ? d : 0.f;
+    }
+  }
+}
+
+// A wavefront owns 64 * VEC features and every gridDim.y * 4-th class; dz's row is the same for all
+// its lanes.  dweight leaves at once, dx's share of the workgroup goes to part[blockIdx.y][ROWS][D].
+template <typename T, int ROWS, int VEC>
+__global__ __launch_bounds__(kThreads) void k_few_grads(int B, int D, int64_t V, const T* __restrict__ x, int64_t ldx,
+                                                        const T* __restrict__ w, int64_t sv, Labels of,
+                                                        const float* __restrict__ dz, T* __restrict__ dw, int64_t dsv,
+                                                        int64_t dsd, float* __restrict__ part) {
+  __shared__ float joined[4][64 * VEC];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int d0 = (int(blockIdx.x) * 64 + lane) * VEC;
+  const int left = D - d0;
+  float xr[ROWS][VEC], dx[ROWS][VEC];
+#pragma unroll
+  for (int b = 0; b < ROWS; ++b) {
+    const bool live = b < B && label_of(b, of.labels, of.idx, of.n_labels, of.V) >= 0;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      xr[b][e] = live && e < left ? widen(x[b * ldx + d0 + e]) : 0.f;
+      dx[b][e] = 0.f;
+    }
+  }
+  const int64_t stride = int64_t(gridDim.y) * 4;
+  for (int64_t v = int64_t(blockIdx.y) * 4 + wave; v < V; v += stride) {
+    const float* row = dz + v * ROWS;
+    T raw[VEC];
+    if (left >= VEC) {
+      __builtin_memcpy(&raw, w + v * sv + d0, sizeof(raw));
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) raw[e] = e < left ? w[v * sv + d0 + e] : narrow<T>(0.f);
+    }
+    float out[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) out[e] = 0.f;
+#pragma unroll
+    for (int b = 0; b < ROWS; ++b) {
+      const float z = row[b];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        dx[b][e] = fmaf(z, widen(raw[e]), dx[b][e]);
+        out[e] = fmaf(z, xr[b][e], out[e]);
+      }
+    }
+    if (dw != nullptr) {
+      T res[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) res[e] = narrow<T>(out[e]);
+      T* dst = dw + v * dsv + d0 * dsd;
+      if (dsd == 1 && left >= VEC) {
+        __builtin_memcpy(dst, &res, sizeof(res));
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (e < left) dst[e * dsd] = res[e];
+      }
+    }
+  }
+  if (part == nullptr) return;                   // the whole launch
+  for (int b = 0; b < ROWS; ++b) {
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) joined[wave][lane * VEC + e] = 0.f;
+#pragma unroll
+    for (int q = 0; q < ROWS; ++q)               // constant indexes: dx stays in registers
+      if (q == b) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) joined[wave][lane * VEC + e] = dx[q][e];
+      }
+    __syncthreads();
+    for (int c = threadIdx.x; c < 64 * VEC; c += kThreads) {
+      const int d = int(blockIdx.x) * 64 * VEC + c;
+      if (d < D)
+        part[(int64_t(blockIdx.y) * ROWS + b) * D + d] = (joined[0][c] + joined[1][c]) + (joined[2][c] + joined[3][c]);
+    }
+  }
+}
+
 // ------------------------------------------------------------------ plans
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
@@ -621,6 +868,30 @@ Plan make_plan(int dtype, int64_t B, int64_t D, int64_t V) {
   return p;
 }
 
+// The few-rows kernels: sizes that fit them, 0 rows where they do not apply.
+struct Few {
+  int rows, Dk, vec;
+  size_t lds;
+  unsigned blocks, slabs, splits;
+};
+
+Few make_few(int dtype, int64_t B, int64_t D, int64_t V, int64_t sd) {
+  Few f{};
+  const int P = dtype == SGNN_F32 ? 3 : 1;
+  if (B > kFewRows || sd != 1 || D > 65536) return f;
+  f.Dk = int(ceil_div(D, 64) * 64);
+  f.lds = size_t(P) * kFewRows * f.Dk * 2;
+  if (f.lds > 150 * 1024) return f;              // of 160 KB
+  f.rows = B <= 2 ? 2 : B <= 4 ? 4 : B <= 8 ? 8 : B <= 16 ? 16 : 32;
+  f.vec = f.rows > 16 ? 2 : 4;
+  const int64_t blocks = ceil_div(V, 128);
+  f.blocks = unsigned(blocks < kFewBlocks ? blocks : kFewBlocks);
+  f.slabs = unsigned(ceil_div(D, 64 * f.vec));
+  const int64_t want = ceil_div(1024, f.slabs), most = ceil_div(V, 16);
+  f.splits = unsigned(want < most ? want : most);
+  return f;
+}
+
 struct Buffers {
   uint16_t *x, *w, *dz;
   float2* part;
@@ -642,6 +913,20 @@ Buffers carve(const Plan& p, int64_t B, int64_t V, bool backward, void* base) {
     b.rest = c.take<float>(size_t(B));
     b.dx = c.take<float>(size_t(p.dx_splits) * p.Bp * Np);
     b.dw = c.take<float>(size_t(p.dw_splits) * p.piece * Np);
+  }
+  b.bytes = c.off;
+  return b;
+}
+
+Buffers carve_few(const Few& f, int64_t B, int64_t D, int64_t V, bool backward, void* base) {
+  sgnn::Carver c(base);
+  Buffers b{};
+  if (!backward) {
+    b.part = c.take<float2>(size_t(f.blocks) * B);
+    b.picked = c.take<float>(size_t(B));
+  } else {
+    b.dw = c.take<float>(size_t(V) * f.rows);    // dz
+    b.dx = c.take<float>(size_t(f.splits) * f.rows * D);
   }
   b.bytes = c.off;
   return b;
@@ -698,6 +983,25 @@ int planes(const Call& c, const Plan& p, const Buffers& b, Operand* x, Operand* 
   return SGNN_OK;
 }
 
+int finish_forward(const Call& c, int parts, const Buffers& b, float2* stats, float* row_loss, float* loss,
+                   float* share, hipStream_t st) {
+  hipLaunchKernelGGL(k_class_rows, dim3(unsigned(ceil_div(c.B, 4))), dim3(256), 0, st, c.B, c.V, parts, b.part, b.picked,
+                     c.labels, c.idx, c.n_labels, stats, row_loss);
+  HIP_TRY(hipGetLastError());
+  if (loss) {
+    hipLaunchKernelGGL(k_class_mean, dim3(1), dim3(1024), 0, st, c.B, c.V, row_loss, c.labels, c.idx, c.n_labels, loss,
+                       share);
+    HIP_TRY(hipGetLastError());
+  }
+  return SGNN_OK;
+}
+
+// a kernel's dynamic LDS beyond the default limit has to be asked for
+int allow_lds(const void* kernel, size_t bytes) {
+  HIP_TRY(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes)));
+  return SGNN_OK;
+}
+
 template <typename T, int P>
 int forward(const Call& c, const Plan& p, const Buffers& b, float2* stats, float* row_loss, float* loss,
             float* share, hipStream_t st) {
@@ -706,15 +1010,7 @@ int forward(const Call& c, const Plan& p, const Buffers& b, float2* stats, float
   hipLaunchKernelGGL((k_class_stats<P>), dim3(unsigned(p.tiles_b * p.stat_splits)), dim3(kThreads), 0, st, c.B, c.V,
                      p.Dp, x, w, c.labels, c.idx, c.n_labels, p.tiles_v, p.stat_splits, b.part, b.picked);
   HIP_TRY(hipGetLastError());
-  hipLaunchKernelGGL(k_class_rows, dim3(unsigned(ceil_div(c.B, 4))), dim3(256), 0, st, c.B, c.V, 2 * p.stat_splits,
-                     b.part, b.picked, c.labels, c.idx, c.n_labels, stats, row_loss);
-  HIP_TRY(hipGetLastError());
-  if (loss) {
-    hipLaunchKernelGGL(k_class_mean, dim3(1), dim3(1024), 0, st, c.B, c.V, row_loss, c.labels, c.idx, c.n_labels, loss,
-                       share);
-    HIP_TRY(hipGetLastError());
-  }
-  return SGNN_OK;
+  return finish_forward(c, 2 * p.stat_splits, b, stats, row_loss, loss, share, st);
 }
 
 template <typename T, int P>
@@ -762,11 +1058,57 @@ int backward(const Call& c, const Plan& p, const Buffers& b, const float2* stats
   return SGNN_OK;
 }
 
+template <typename T, int P>
+int few_forward(const Call& c, const Few& f, const Buffers& b, float2* stats, float* row_loss, float* loss,
+                float* share, hipStream_t st) {
+  const Labels of{c.labels, c.idx, c.n_labels, c.V};
+  if (int rc = allow_lds(reinterpret_cast<const void*>(&k_few_stats<T, P>), f.lds)) return rc;
+  hipLaunchKernelGGL((k_few_stats<T, P>), dim3(f.blocks), dim3(kThreads), f.lds, st, int(c.B), int(c.D), f.Dk, c.V,
+                     static_cast<const T*>(c.x), c.ldx, static_cast<const T*>(c.w), c.sv, of, b.part, b.picked);
+  HIP_TRY(hipGetLastError());
+  return finish_forward(c, int(f.blocks), b, stats, row_loss, loss, share, st);
+}
+
+template <typename T, int P>
+int few_backward(const Call& c, const Few& f, const Buffers& b, const float2* stats, const float* grad,
+                 const float* share, void* dx, int64_t lddx, void* dw, int64_t dsv, int64_t dsd, hipStream_t st) {
+  const Labels of{c.labels, c.idx, c.n_labels, c.V};
+  const T* x = static_cast<const T*>(c.x);
+  const T* w = static_cast<const T*>(c.w);
+  if (int rc = allow_lds(reinterpret_cast<const void*>(&k_few_dz<T, P>), f.lds)) return rc;
+  hipLaunchKernelGGL((k_few_dz<T, P>), dim3(f.blocks), dim3(kThreads), f.lds, st, int(c.B), f.rows, int(c.D), f.Dk, c.V,
+                     x, c.ldx, w, c.sv, of, stats, grad, share, b.dw);
+  HIP_TRY(hipGetLastError());
+#define SGNN_FEW(ROWS, VEC)                                                                                          \
+  hipLaunchKernelGGL((k_few_grads<T, ROWS, VEC>), dim3(f.slabs, f.splits), dim3(kThreads), 0, st, int(c.B), int(c.D), \
+                     c.V, x, c.ldx, w, c.sv, of, b.dw, static_cast<T*>(dw), dsv, dsd, dx ? b.dx : nullptr)
+  switch (f.rows) {
+    case 2: SGNN_FEW(2, 4); break;
+    case 4: SGNN_FEW(4, 4); break;
+    case 8: SGNN_FEW(8, 4); break;
+    case 16: SGNN_FEW(16, 4); break;
+    default: SGNN_FEW(32, 2); break;
+  }
+#undef SGNN_FEW
+  HIP_TRY(hipGetLastError());
+  if (dx) {
+    hipLaunchKernelGGL((k_class_join<T>), dim3(1, unsigned(ceil_div(c.D, 32))), dim3(256), 0, st, c.B, int(c.D),
+                       int(f.splits), b.dx, int64_t(f.rows) * c.D, c.D, nullptr, nullptr, nullptr, of, nullptr, 0, 0,
+                       static_cast<T*>(dx), lddx, int64_t(1));
+    HIP_TRY(hipGetLastError());
+  }
+  return SGNN_OK;
+}
+
 }  // namespace
 
 extern "C" size_t sgnn_class_xent_workspace_bytes(int dtype, int64_t B, int64_t D, int64_t V, int backward) {
   if (B <= 0 || D <= 0 || V <= 0 || (dtype != SGNN_F32 && dtype != SGNN_BF16)) return 0;
-  return carve(make_plan(dtype, B, D, V), B, V, backward != 0, nullptr).bytes;
+  // the weight's layout is not known here: enough for either way
+  const size_t whole = carve(make_plan(dtype, B, D, V), B, V, backward != 0, nullptr).bytes;
+  const Few f = make_few(dtype, B, D, V, 1);
+  const size_t few = f.rows ? carve_few(f, B, D, V, backward != 0, nullptr).bytes : 0;
+  return whole > few ? whole : few;
 }
 
 extern "C" int sgnn_class_xent_forward(int dtype, int64_t B, int64_t D, int64_t V, const void* x, int64_t ldx,
@@ -778,11 +1120,17 @@ extern "C" int sgnn_class_xent_forward(int dtype, int64_t B, int64_t D, int64_t 
   const Call c{dtype, B, D, V, x, ldx, weight, sv, sd, labels, n_labels, idx};
   if (int rc = check_call(c)) return rc;
   if (!stats || !row_loss || !workspace || (loss && !share)) return fail(SGNN_ERR_INVALID, "null pointer");
-  const Plan p = make_plan(dtype, B, D, V);
-  const Buffers b = carve(p, B, V, false, workspace);
-  if (workspace_bytes < b.bytes) return fail(SGNN_ERR_WORKSPACE, "class-loss workspace too small");
+  if (workspace_bytes < sgnn_class_xent_workspace_bytes(dtype, B, D, V, 0))
+    return fail(SGNN_ERR_WORKSPACE, "class-loss workspace too small");
   hipStream_t st = static_cast<hipStream_t>(stream);
   float2* s = reinterpret_cast<float2*>(stats);
+  if (const Few f = make_few(dtype, B, D, V, sd); f.rows) {
+    const Buffers b = carve_few(f, B, D, V, false, workspace);
+    if (dtype == SGNN_F32) return few_forward<float, 3>(c, f, b, s, row_loss, loss, share, st);
+    return few_forward<Bf16, 1>(c, f, b, s, row_loss, loss, share, st);
+  }
+  const Plan p = make_plan(dtype, B, D, V);
+  const Buffers b = carve(p, B, V, false, workspace);
   if (dtype == SGNN_F32) return forward<float, 3>(c, p, b, s, row_loss, loss, share, st);
   return forward<Bf16, 1>(c, p, b, s, row_loss, loss, share, st);
 }
@@ -800,11 +1148,17 @@ extern "C" int sgnn_class_xent_backward(int dtype, int64_t B, int64_t D, int64_t
   if (dweight && !((dsd == 1 && dsv >= D) || (dsv == 1 && dsd >= V)))
     return fail(SGNN_ERR_INVALID, "the weight's gradient must have unit stride along its features or its classes");
   if (!dx && !dweight) return SGNN_OK;
-  const Plan p = make_plan(dtype, B, D, V);
-  const Buffers b = carve(p, B, V, true, workspace);
-  if (workspace_bytes < b.bytes) return fail(SGNN_ERR_WORKSPACE, "class-loss workspace too small");
+  if (workspace_bytes < sgnn_class_xent_workspace_bytes(dtype, B, D, V, 1))
+    return fail(SGNN_ERR_WORKSPACE, "class-loss workspace too small");
   hipStream_t st = static_cast<hipStream_t>(stream);
   const float2* s = reinterpret_cast<const float2*>(stats);
+  if (const Few f = make_few(dtype, B, D, V, sd); f.rows) {
+    const Buffers b = carve_few(f, B, D, V, true, workspace);
+    if (dtype == SGNN_F32) return few_backward<float, 3>(c, f, b, s, grad, share, dx, lddx, dweight, dsv, dsd, st);
+    return few_backward<Bf16, 1>(c, f, b, s, grad, share, dx, lddx, dweight, dsv, dsd, st);
+  }
+  const Plan p = make_plan(dtype, B, D, V);
+  const Buffers b = carve(p, B, V, true, workspace);
   if (dtype == SGNN_F32) return backward<float, 3>(c, p, b, s, grad, share, dx, lddx, dweight, dsv, dsd, st);
   return backward<Bf16, 1>(c, p, b, s, grad, share, dx, lddx, dweight, dsv, dsd, st);
 }
