@@ -8,56 +8,13 @@
 // in bf16 and multiplies it from either side.  A piece is sized to stay in the last-level cache
 // between the launch that writes it and the two that read it.
 //
-// All four products run on the bf16 matrix instructions.  bf16 operands go in as they are, their
-// products are exact and summed in 32 bits; dz is rounded to bf16 there (relative 2^-9 per
-// element, below the half step that each result is rounded by).  fp32 operands, and dz with
-// them, are the sum of three bf16 numbers each (8 + 8 + 8 bits of the mantissa, cut off, so the
-// sum is exact); of the nine products the three smallest, below 2^-24 of the whole, are left out.
-#include "common.h"
+// All four products run on the bf16 matrix instructions (tile_product.h): bf16 operands as they
+// are, fp32 ones as three bf16 numbers each.  dz of bf16 operands is rounded to bf16 there
+// (relative 2^-9 per element, below the half step that each result is rounded by).
+#include "tile_product.h"
 
 namespace {
 
-typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-
-struct Bf16 { uint16_t bits; };
-
-__device__ __forceinline__ float widen(float v) { return v; }
-__device__ __forceinline__ float widen(Bf16 v) { return __uint_as_float(unsigned(v.bits) << 16); }
-__device__ __forceinline__ uint16_t to_bf16(float v) {                       // nearest even
-  const unsigned u = __float_as_uint(v);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return 0x7fc0u;
-  return uint16_t((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
-}
-template <typename T> __device__ __forceinline__ T narrow(float v);
-template <> __device__ __forceinline__ float narrow<float>(float v) { return v; }
-template <> __device__ __forceinline__ Bf16 narrow<Bf16>(float v) { return Bf16{to_bf16(v)}; }
-
-// v = plane 0 + plane 1 + plane 2 exactly; an infinity or NaN leaves a NaN behind
-__device__ __forceinline__ void split3(float v, float& a, float& b, float& c) {
-  a = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
-  const float r = v - a;
-  b = __uint_as_float(__float_as_uint(r) & 0xffff0000u);
-  c = r - b;
-}
-__device__ __forceinline__ uint16_t high_half(float v) { return uint16_t(__float_as_uint(v) >> 16); }
-// the high halves of two floats as a bf16 pair
-__device__ __forceinline__ unsigned high_halves(float lo, float hi) {
-  return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
-}
-template <int P>
-__device__ __forceinline__ void to_planes(float v, uint16_t (&p)[P]) {
-  if constexpr (P == 1) {
-    p[0] = to_bf16(v);
-  } else {
-    float a, b, c;
-    split3(v, a, b, c);
-    p[0] = high_half(a); p[1] = high_half(b); p[2] = high_half(c);
-  }
-}
 __device__ __forceinline__ float exp2_raw(float v) { return __builtin_amdgcn_exp2f(v); }   // 0 below 2^-126
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -69,25 +26,26 @@ __device__ __forceinline__ int64_t label_of(int64_t b, const int64_t* labels, co
   return (y >= 0 && y < V) ? y : -1;
 }
 
-// ------------------------------------------------------------------ operands as bf16 planes
+// ------------------------------------------------------------------ operands
 struct Labels {
   const int64_t *labels, *idx;
   int64_t n_labels, V;
 };
-// in[r][d] at r * sr + d * sd  ->  out[plane][r][Dp], columns D .. Dp zero.  Rows of x without a
-// class become zeros, so that whatever a padded row holds (NaN too) reaches no gradient.
+
+// in[r][d] at r * sr + d * sd  ->  out[r][Dp], columns D .. Dp zero.  Rows of x without a class
+// become zeros, so that whatever a padded row holds (NaN too) reaches no gradient.
 struct Source {
   const void* in;
   int64_t rows, sr, sd;
-  uint16_t* out;
+  void* out;
   int64_t blocks;          // workgroups it takes: one for 64 x 64 elements
 };
 
 // x and the weight in one launch.  Rows that are contiguous go straight through registers, eight
 // elements a lane; a weight stored by feature goes through a tile in LDS.
-template <typename T, int P>
-__global__ __launch_bounds__(256) void k_planes(int D, int Dp, Source first, Source second, Labels of) {
-  __shared__ float tile[64][65];
+template <typename T>
+__global__ __launch_bounds__(256) void k_class_operands(int D, int Dp, Source first, Source second, Labels of) {
+  __shared__ T tile[64][sizeof(T) == 4 ? 65 : 66];
   const bool is_x = int64_t(blockIdx.x) < first.blocks;
   const Source src = is_x ? first : second;
   const int64_t block = is_x ? blockIdx.x : blockIdx.x - first.blocks;
@@ -103,7 +61,7 @@ __global__ __launch_bounds__(256) void k_planes(int D, int Dp, Source first, Sou
       const int lr = i & 63, ld = i >> 6;
       const int64_t r = r0 + lr;
       const int d = d0 + ld;
-      tile[lr][ld] = (d < D && live(r)) ? widen(in[r * src.sr + d * src.sd]) : 0.f;
+      tile[lr][ld] = (d < D && live(r)) ? in[r * src.sr + d * src.sd] : T{};
     }
     __syncthreads();
   }
@@ -112,178 +70,26 @@ __global__ __launch_bounds__(256) void k_planes(int D, int Dp, Source first, Sou
     const int lr = i >> 3, c = (i & 7) * 8, d = d0 + c;
     const int64_t r = r0 + lr;
     if (r >= src.rows) continue;
-    float v[8];
+    T v[8];
     if (src.sd != 1) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = tile[lr][c + e];
     } else if (!live(r)) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = 0.f;
+      for (int e = 0; e < 8; ++e) v[e] = T{};
     } else if (d + 8 <= D) {
-      T raw[8];
-      __builtin_memcpy(&raw, in + r * src.sr + d, sizeof(raw));
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = widen(raw[e]);
+      __builtin_memcpy(&v, in + r * src.sr + d, sizeof(v));
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = d + e < D ? widen(in[r * src.sr + d + e]) : 0.f;
+      for (int e = 0; e < 8; ++e) v[e] = d + e < D ? in[r * src.sr + d + e] : T{};
     }
-    uint16_t pl[P][8];
+    u32x4 w[sizeof(v) / 16];
+    __builtin_memcpy(&w, &v, sizeof(v));
+    u32x4* dst = reinterpret_cast<u32x4*>(static_cast<T*>(src.out) + r * Dp + d);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      uint16_t p[P];
-      to_planes<P>(v[e], p);
-#pragma unroll
-      for (int q = 0; q < P; ++q) pl[q][e] = p[q];
-    }
-#pragma unroll
-    for (int q = 0; q < P; ++q) {
-      u32x4 w;
-      __builtin_memcpy(&w, &pl[q][0], 16);
-      *reinterpret_cast<u32x4*>(src.out + (int64_t(q) * src.rows + r) * Dp + d) = w;
-    }
+    for (int q = 0; q < int(sizeof(v) / 16); ++q) dst[q] = w[q];
   }
 }
-
-// ------------------------------------------------------------------ the product's inner loop
-// A workgroup of four wavefronts forms a 128 x 128 tile, 64 x 64 a wavefront, K steps of kBK.
-// Operands travel from memory to LDS without passing registers, one step ahead.  An operand is
-// "deep" when its memory is contiguous along the reduction (LDS holds [128][kBK], read directly)
-// and "flat" when it is contiguous along the tile ([kBK][128], read through the transposing LDS
-// load).  16-byte chunks are permuted on the way in so that neither read meets bank conflicts.
-constexpr int kTile = 128;
-constexpr int kThreads = 256;
-
-struct Operand {
-  const uint16_t* base;
-  int64_t ld, plane;       // row stride and distance between planes, in elements
-  int64_t rows;            // rows that exist: reads beyond repeat the last one
-  int64_t cols;            // columns that exist (flat operands; a multiple of 8)
-};
-
-template <int P> struct Depth { static constexpr int kBK = P == 1 ? 64 : 32; };
-
-template <int P> constexpr int stage_bytes() { return P * kTile * Depth<P>::kBK * 2; }
-
-typedef __attribute__((address_space(3))) void lds_void;
-typedef const __attribute__((address_space(1))) void global_void;
-
-// deep: rows r0 .. r0 + 127 at reduction offset k0;  flat: reduction rows k0 .. at columns r0 ..
-template <int P, bool DEEP>
-__device__ __forceinline__ void stage_operand(const Operand& op, int64_t r0, int64_t k0, char* lds, int wave,
-                                              int lane) {
-  constexpr int BK = Depth<P>::kBK;
-  constexpr int kChunks = P * kTile * BK / 8;
-#pragma unroll
-  for (int l = 0; l < kChunks / kThreads; ++l) {
-    const int first = (l * 4 + wave) * 64, q = first + lane;
-    constexpr int per_plane = kTile * BK / 8;
-    const int p = q / per_plane, at = q % per_plane;
-    const uint16_t* src;
-    if constexpr (DEEP) {
-      constexpr int cpr = BK / 8;
-      const int row = at / cpr, c = at % cpr;
-      const int cl = c ^ (cpr == 8 ? (row & 7) : ((row >> 2) & 3));
-      int64_t r = r0 + row;
-      r = r < op.rows ? r : op.rows - 1;
-      src = op.base + p * op.plane + r * op.ld + k0 + cl * 8;
-    } else {
-      const int row = at / 16, c = at % 16;
-      const int cl = c ^ ((row & 3) << 2);
-      int64_t r = k0 + row, col = r0 + cl * 8;
-      r = r < op.rows ? r : op.rows - 1;
-      col = col < op.cols ? col : op.cols - 8;
-      src = op.base + p * op.plane + r * op.ld + col;
-    }
-    __builtin_amdgcn_global_load_lds((global_void*)src, (lds_void*)(lds + first * 16), 16, 0, 0);
-  }
-}
-
-// the operand of one 32 x 32 x 16 instruction: element `lane & 31` of the block at m0, eight
-// reduction indexes from k0 + 8 * (lane / 32)
-template <int P, bool DEEP>
-__device__ __forceinline__ bf16x8 fragment(const char* lds, int p, int m0, int k0, int lane) {
-  constexpr int BK = Depth<P>::kBK;
-  const char* slab = lds + p * (kTile * BK * 2);
-  if constexpr (DEEP) {
-    constexpr int cpr = BK / 8;
-    const int row = m0 + (lane & 31), c = k0 / 8 + (lane >> 5);
-    const int cl = c ^ (cpr == 8 ? (row & 7) : ((row >> 2) & 3));
-    return *reinterpret_cast<const bf16x8*>(slab + row * (BK * 2) + cl * 16);
-  } else {
-    const int k = k0 + 8 * (lane >> 5) + ((lane & 15) >> 2);
-    const int m = m0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-    const int at = ((m >> 3) ^ ((k & 3) << 2)) * 16 + (m & 7) * 2;       // k and k + 4 share k & 3
-    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(slab + k * (kTile * 2) + at));
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(slab + (k + 4) * (kTile * 2) + at));
-    bf16x8 r;
-    __builtin_memcpy(&r, &lo, 8);
-    __builtin_memcpy(reinterpret_cast<char*>(&r) + 8, &hi, 8);
-    return r;
-  }
-}
-
-typedef f32x16 Tile[2][2];
-
-__device__ __forceinline__ void clear(Tile& acc) {
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-}
-
-// acc += A[m0 .., k0 .. k1] . B[n0 .., k0 .. k1]; k1 - k0 a multiple of kBK.  `lds` holds two
-// stages of both operands; every wavefront has left them when this returns.
-template <int P, bool ADEEP, bool BDEEP>
-__device__ __forceinline__ void multiply(const Operand& A, int64_t m0, const Operand& B, int64_t n0, int64_t k0,
-                                         int64_t k1, char* lds, Tile& acc) {
-  constexpr int BK = Depth<P>::kBK;
-  constexpr int kStage = stage_bytes<P>();
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
-  stage_operand<P, ADEEP>(A, m0, k0, lds, wave, lane);
-  stage_operand<P, BDEEP>(B, n0, k0, lds + kStage, wave, lane);
-  int cur = 0;
-  for (int64_t k = k0; k < k1; k += BK) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // this wavefront's part of the stage has landed
-    __syncthreads();                                         // everybody's has, and the other stage is free
-    const char* a = lds + cur * 2 * kStage;
-    const char* b = a + kStage;
-    if (k + BK < k1) {
-      char* next = lds + (cur ^ 1) * 2 * kStage;
-      stage_operand<P, ADEEP>(A, m0, k + BK, next, wave, lane);
-      stage_operand<P, BDEEP>(B, n0, k + BK, next + kStage, wave, lane);
-    }
-#pragma unroll
-    for (int kk = 0; kk < BK; kk += 16) {
-      bf16x8 fa[P][2], fb[P][2];
-#pragma unroll
-      for (int p = 0; p < P; ++p)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          fa[p][i] = fragment<P, ADEEP>(a, p, wm + 32 * i, kk, lane);
-          fb[p][i] = fragment<P, BDEEP>(b, p, wn + 32 * i, kk, lane);
-        }
-#pragma unroll
-      for (int pa = 0; pa < P; ++pa)
-#pragma unroll
-        for (int pb = 0; pa + pb < P; ++pb)
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-              acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[pa][i], fb[pb][j], acc[i][j], 0, 0, 0);
-    }
-    cur ^= 1;
-  }
-  __syncthreads();
-}
-
-// row of element e of a 32 x 32 block (its column is lane & 31)
-__device__ __forceinline__ int block_row(int e, int lane) { return 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3); }
 
 // ------------------------------------------------------------------ forward
 // (m, s) = (maximum, sum of exp relative to it).  While everything is -inf the sum stays 0; a NaN
@@ -312,13 +118,13 @@ __device__ __forceinline__ void accumulate(const f32x16& a, const f32x16& b, flo
 // A workgroup takes 128 rows of x and a range of the classes, 128 at a time.  The tile is formed
 // as classes x rows, so that a lane holds 32 classes of each of two rows and its running maximum
 // and sum need no other lane until the end.  part[row][split][half] = (max, sum of exp relative to it).
-template <int P>
-__global__ __launch_bounds__(kThreads) void k_class_stats(int64_t B, int64_t V, int Dp, Operand x, Operand w,
+template <typename T>
+__global__ __launch_bounds__(kThreads) void k_class_stats(int64_t B, int64_t V, int Dp, Operand<T> x, Operand<T> w,
                                                           const int64_t* __restrict__ labels,
                                                           const int64_t* __restrict__ idx, int64_t n_labels,
                                                           int64_t tiles_v, int splits, float2* __restrict__ part,
                                                           float* __restrict__ picked) {
-  __shared__ __align__(128) char lds[4 * stage_bytes<P>()];
+  __shared__ __align__(128) char lds[kProductLds];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wv = (wave >> 1) * 64, wb = (wave & 1) * 64;
   const int split = blockIdx.x % splits;
@@ -336,7 +142,7 @@ __global__ __launch_bounds__(kThreads) void k_class_stats(int64_t B, int64_t V, 
   for (int64_t t = t0; t < t1; ++t) {
     Tile acc;
     clear(acc);
-    multiply<P, true, true>(w, t * kTile, x, b0, 0, Dp, lds, acc);
+    multiply<T, true, true>(w, t * kTile, x, b0, 0, Dp, lds, acc);
     const int64_t vw = t * kTile + wv;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -425,28 +231,25 @@ __global__ __launch_bounds__(1024) void k_class_mean(int64_t B, int64_t V, const
 }
 
 // ------------------------------------------------------------------ backward
-// dz of the classes v0 .. v0 + 128 * tiles and all rows, as bf16 planes [plane][Bp][ldz]; rows and
+// dz of the classes v0 .. v0 + 128 * tiles and all rows, [Bp][ldz]; rows and
 // classes beyond the last are 0.  `grad` NULL leaves the mean's factor to the gradients' last step.
 // The label's element dominates a row and is the one whose rounding to bf16 would be felt in dx:
 // what it loses is kept in rest[b] and joins dx in 32 bits.
-template <int P>
-__global__ __launch_bounds__(kThreads) void k_class_dz(int64_t B, int64_t V, int Dp, Operand x, Operand w,
+template <typename T>
+__global__ __launch_bounds__(kThreads) void k_class_dz(int64_t B, int64_t V, int Dp, Operand<T> x, Operand<T> w,
                                                        const int64_t* __restrict__ labels,
                                                        const int64_t* __restrict__ idx, int64_t n_labels,
                                                        const float2* __restrict__ stats,
                                                        const float* __restrict__ grad, float* __restrict__ rest,
-                                                       int64_t v0, int tiles, uint16_t* __restrict__ dz, int64_t ldz,
-                                                       int64_t plane) {
-  constexpr int kRow = kTile * 2 + 16;             // bytes of a staged row of dz
-  constexpr int kLds = 4 * stage_bytes<P>() > kTile * kRow ? 4 * stage_bytes<P>() : kTile * kRow;
-  __shared__ __align__(128) char lds[kLds];
+                                                       int64_t v0, int tiles, T* __restrict__ dz, int64_t ldz) {
+  __shared__ __align__(128) char lds[kProductLds];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wv = (wave >> 1) * 64, wb = (wave & 1) * 64;
   const int64_t vt = v0 + int64_t(blockIdx.x % tiles) * kTile;
   const int64_t b0 = int64_t(blockIdx.x / tiles) * kTile;
   Tile acc;
   clear(acc);
-  multiply<P, true, true>(w, vt, x, b0, 0, Dp, lds, acc);
+  multiply<T, true, true>(w, vt, x, b0, 0, Dp, lds, acc);
   const int64_t vw = vt + wv;
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
@@ -467,7 +270,7 @@ __global__ __launch_bounds__(kThreads) void k_class_dz(int64_t B, int64_t V, int
           if (vw + 32 * i + block_row(e, lane) == y) {
             const float d = acc[i][j][e] - g;
             acc[i][j][e] = d;
-            if constexpr (P == 1) rest[b] = d - widen(Bf16{to_bf16(d)});
+            if constexpr (sizeof(T) == 2) rest[b] = d - widen(Bf16{to_bf16(d)});
           }
     }
     if (vw + 64 > V || __any(y < 0)) {
@@ -478,8 +281,19 @@ __global__ __launch_bounds__(kThreads) void k_class_dz(int64_t B, int64_t V, int
           if (y < 0 || vw + 32 * i + block_row(e, lane) >= V) acc[i][j][e] = 0.f;
     }
   }
+  T* out = dz + b0 * ldz + (vt - v0);
+  if constexpr (sizeof(T) == 4) {                  // four classes a lane: whole 16 bytes
 #pragma unroll
-  for (int p = 0; p < P; ++p) {
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4)
+          *reinterpret_cast<f32x4*>(out + (wb + 32 * j + (lane & 31)) * ldz + wv + 32 * i + block_row(e, lane)) =
+              f32x4{acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
+  } else {
+    constexpr int kRow = kTile * 2 + 16;           // bytes of a staged row of dz
+    static_assert(kTile * kRow <= kProductLds, "a tile of dz fits the product's stages");
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -488,42 +302,36 @@ __global__ __launch_bounds__(kThreads) void k_class_dz(int64_t B, int64_t V, int
         for (int e = 0; e < 16; e += 4) {
           uint16_t four[4];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint16_t pl[P];
-            to_planes<P>(acc[i][j][e + q], pl);
-            four[q] = pl[p];
-          }
+          for (int q = 0; q < 4; ++q) four[q] = to_bf16(acc[i][j][e + q]);
           u32x2 u;
           __builtin_memcpy(&u, &four, 8);
           *reinterpret_cast<u32x2*>(lds + (wb + 32 * j + (lane & 31)) * kRow + (wv + 32 * i + block_row(e, lane)) * 2) = u;
         }
     __syncthreads();
-    uint16_t* out = dz + p * plane + b0 * ldz + (vt - v0);
     for (int c = threadIdx.x; c < kTile * kTile / 8; c += kThreads) {
       const int row = c >> 4, col = (c & 15) * 8;
       *reinterpret_cast<u32x4*>(out + row * ldz + col) = *reinterpret_cast<const u32x4*>(lds + row * kRow + col * 2);
     }
-    __syncthreads();
   }
 }
 
 // C[m][n] += or = A . B over this workgroup's share of the reduction, 32 bits, one buffer per share:
 // out[split][Mp][Np].
-template <int P, bool ADEEP>
-__global__ __launch_bounds__(kThreads) void k_class_product(Operand A, Operand B, int tiles_m, int tiles_n,
+template <typename T, bool ADEEP>
+__global__ __launch_bounds__(kThreads) void k_class_product(Operand<T> A, Operand<T> B, int tiles_m, int tiles_n,
                                                             int64_t K, int splits, int add, float* __restrict__ out,
                                                             int64_t plane, int64_t ldo) {
-  __shared__ __align__(128) char lds[4 * stage_bytes<P>()];
+  __shared__ __align__(128) char lds[kProductLds];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
   const int tn = blockIdx.x % tiles_n, rest = blockIdx.x / tiles_n;
   const int split = rest % splits, tm = rest / splits;
   const int64_t m0 = int64_t(tm) * kTile, n0 = int64_t(tn) * kTile;
-  const int64_t steps = K / Depth<P>::kBK;
-  const int64_t k0 = steps * split / splits * Depth<P>::kBK, k1 = steps * (split + 1) / splits * Depth<P>::kBK;
+  const int64_t steps = K / Step<T>::kDepth;
+  const int64_t k0 = steps * split / splits * Step<T>::kDepth, k1 = steps * (split + 1) / splits * Step<T>::kDepth;
   Tile acc;
   clear(acc);
-  if (k0 < k1) multiply<P, ADEEP, false>(A, m0, B, n0, k0, k1, lds, acc);
+  if (k0 < k1) multiply<T, ADEEP, false>(A, m0, B, n0, k0, k1, lds, acc);
   float* dst = out + split * plane;
 #pragma unroll
   for (int i = 0; i < 2; ++i)
@@ -595,56 +403,31 @@ __device__ __forceinline__ int few_at(int p, int row, int chunk, int Dk) {      
 }
 
 // x's rows to LDS, features D .. Dk and rows without a class zero
-template <typename T, int P>
+template <typename T>
 __device__ __forceinline__ void few_stage(const Labels& of, int B, int D, int Dk, const T* __restrict__ x, int64_t ldx,
                                           char* lds) {
+  constexpr int P = Planes<T>::kCount;
   for (int i = threadIdx.x; i < kFewRows * (Dk / 8); i += kThreads) {
     const int row = i / (Dk / 8), chunk = i - row * (Dk / 8), d = chunk * 8;
     const bool live = row < B && label_of(row, of.labels, of.idx, of.n_labels, of.V) >= 0;
-    uint16_t pl[P][8];
+    T v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      uint16_t p[P];
-      to_planes<P>(live && d + e < D ? widen(x[row * ldx + d + e]) : 0.f, p);
+    for (int e = 0; e < 8; ++e) v[e] = live && d + e < D ? x[row * ldx + d + e] : T{};
+    bf16x8 pl[P];
+    planes_of(v, pl);
 #pragma unroll
-      for (int q = 0; q < P; ++q) pl[q][e] = p[q];
-    }
-#pragma unroll
-    for (int q = 0; q < P; ++q) {
-      u32x4 w;
-      __builtin_memcpy(&w, &pl[q][0], 16);
-      *reinterpret_cast<u32x4*>(lds + few_at<P>(q, row, chunk, Dk)) = w;
-    }
+    for (int q = 0; q < P; ++q) *reinterpret_cast<bf16x8*>(lds + few_at<P>(q, row, chunk, Dk)) = pl[q];
   }
   __syncthreads();
 }
 
-template <typename T, int P>
-__device__ __forceinline__ void few_operand(const T (&raw)[8], bf16x8 (&out)[P]) {
-  if constexpr (P == 1) {
-    __builtin_memcpy(&out[0], &raw, 16);
-  } else {
-    u32x4 pl[3];
-#pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-      float a0, b0, c0, a1, b1, c1;
-      split3(widen(raw[e]), a0, b0, c0);
-      split3(widen(raw[e + 1]), a1, b1, c1);
-      pl[0][e / 2] = high_halves(a0, a1);
-      pl[1][e / 2] = high_halves(b0, b1);
-      pl[2][e / 2] = high_halves(c0, c1);
-    }
-#pragma unroll
-    for (int q = 0; q < 3; ++q) __builtin_memcpy(&out[q], &pl[q], 16);
-  }
-}
-
 // logits of classes v0 .. v0 + 31 (rows of the block) and all 32 rows of x (columns)
-template <typename T, int P>
+template <typename T>
 __device__ __forceinline__ f32x16 few_logits(int D, int Dk, int64_t v0, int64_t V, const T* __restrict__ w, int64_t sv,
                                              const char* lds, int lane) {
   const int64_t v = v0 + (lane & 31) < V ? v0 + (lane & 31) : V - 1;
   const int half = lane >> 5;
+  constexpr int P = Planes<T>::kCount;
   const T* src = w + v * sv + 8 * half;
   f32x16 acc;
 #pragma unroll
@@ -659,38 +442,35 @@ __device__ __forceinline__ f32x16 few_logits(int D, int Dk, int64_t v0, int64_t 
       for (int u = 0; u < kFewSteps; ++u)
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          raw[u][e] = k + 16 * u + 8 * half + e < D ? src[k + 16 * u + e] : narrow<T>(0.f);
+          raw[u][e] = k + 16 * u + 8 * half + e < D ? src[k + 16 * u + e] : T{};
     }
 #pragma unroll
     for (int u = 0; u < kFewSteps; ++u) {
       if (k + 16 * u >= Dk) break;
       bf16x8 a[P], b[P];
-      few_operand<T, P>(raw[u], a);
+      planes_of(raw[u], a);
 #pragma unroll
       for (int q = 0; q < P; ++q)
         b[q] = *reinterpret_cast<const bf16x8*>(lds + few_at<P>(q, lane & 31, (k + 16 * u) / 8 + half, Dk));
-#pragma unroll
-      for (int pa = 0; pa < P; ++pa)
-#pragma unroll
-        for (int pb = 0; pa + pb < P; ++pb) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[pa], b[pb], acc, 0, 0, 0);
+      multiply_planes<P>(a, b, acc);
     }
   }
   return acc;
 }
 
-template <typename T, int P>
+template <typename T>
 __global__ __launch_bounds__(kThreads) void k_few_stats(int B, int D, int Dk, int64_t V, const T* __restrict__ x,
                                                         int64_t ldx, const T* __restrict__ w, int64_t sv, Labels of,
                                                         float2* __restrict__ part, float* __restrict__ picked) {
   extern __shared__ __align__(128) char few_lds[];
   __shared__ float2 joined[4][kFewRows];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  few_stage<T, P>(of, B, D, Dk, x, ldx, few_lds);
+  few_stage<T>(of, B, D, Dk, x, ldx, few_lds);
   const int b = lane & 31;
   const int64_t y = b < B ? label_of(b, of.labels, of.idx, of.n_labels, of.V) : -1;
   float m = -INFINITY, s = 0.f;
   for (int64_t v0 = (int64_t(blockIdx.x) * 4 + wave) * 32; v0 < V; v0 += int64_t(gridDim.x) * 128) {
-    f32x16 z = few_logits<T, P>(D, Dk, v0, V, w, sv, few_lds, lane);
+    f32x16 z = few_logits<T>(D, Dk, v0, V, w, sv, few_lds, lane);
     if (__any(y >= v0 && y < v0 + 32)) {
 #pragma unroll
       for (int e = 0; e < 16; ++e)
@@ -724,7 +504,7 @@ __global__ __launch_bounds__(kThreads) void k_few_stats(int B, int D, int Dk, in
 }
 
 // dz[v][ROWS] in 32 bits, the rows' factors included
-template <typename T, int P>
+template <typename T>
 __global__ __launch_bounds__(kThreads) void k_few_dz(int B, int rows, int D, int Dk, int64_t V,
                                                      const T* __restrict__ x, int64_t ldx, const T* __restrict__ w,
                                                      int64_t sv, Labels of, const float2* __restrict__ stats,
@@ -732,14 +512,14 @@ __global__ __launch_bounds__(kThreads) void k_few_dz(int B, int rows, int D, int
                                                      float* __restrict__ dz) {
   extern __shared__ __align__(128) char few_lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  few_stage<T, P>(of, B, D, Dk, x, ldx, few_lds);
+  few_stage<T>(of, B, D, Dk, x, ldx, few_lds);
   const int b = lane & 31;
   const int64_t y = b < B ? label_of(b, of.labels, of.idx, of.n_labels, of.V) : -1;
   const float2 st = y >= 0 ? stats[b] : make_float2(0.f, 1.f);
   const float g = y >= 0 ? (share ? grad[0] * share[0] : grad[b]) : 0.f;
   const float scale = g / st.y;
   for (int64_t v0 = (int64_t(blockIdx.x) * 4 + wave) * 32; v0 < V; v0 += int64_t(gridDim.x) * 128) {
-    const f32x16 z = few_logits<T, P>(D, Dk, v0, V, w, sv, few_lds, lane);
+    const f32x16 z = few_logits<T>(D, Dk, v0, V, w, sv, few_lds, lane);
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       const int64_t v = v0 + block_row(e, lane);
@@ -749,8 +529,9 @@ __global__ __launch_bounds__(kThreads) void k_few_dz(int B, int rows, int D, int
   }
 }
 
-// A wavefront owns 64 * VEC features and every gridDim.y * 4-th class; dz's row is the same for all
-// its lanes.  dweight leaves at once, dx's share of the workgroup goes to part[blockIdx.y][ROWS][D].
+// A wavefront owns 64 * VEC features and four classes in every gridDim.y * 16; dz's rows are the
+// same for all its lanes.  dweight leaves at once, dx's share of the workgroup goes to
+// part[blockIdx.y][ROWS][D].
 template <typename T, int ROWS, int VEC>
 __global__ __launch_bounds__(kThreads) void k_few_grads(int B, int D, int64_t V, const T* __restrict__ x, int64_t ldx,
                                                         const T* __restrict__ w, int64_t sv, Labels of,
@@ -761,62 +542,67 @@ __global__ __launch_bounds__(kThreads) void k_few_grads(int B, int D, int64_t V,
   const int d0 = (int(blockIdx.x) * 64 + lane) * VEC;
   const int left = D - d0;
   float xr[ROWS][VEC], dx[ROWS][VEC];
+  // bit b: row b has a class; the loads below do not wait for each other
+  const uint64_t live = __ballot(lane < B && label_of(lane, of.labels, of.idx, of.n_labels, of.V) >= 0);
 #pragma unroll
-  for (int b = 0; b < ROWS; ++b) {
-    const bool live = b < B && label_of(b, of.labels, of.idx, of.n_labels, of.V) >= 0;
+  for (int b = 0; b < ROWS; ++b)
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      xr[b][e] = live && e < left ? widen(x[b * ldx + d0 + e]) : 0.f;
+      const int64_t at = int64_t(b < B ? b : B - 1) * ldx + (e < left ? d0 + e : D - 1);
+      const float v = widen(x[at]);
+      xr[b][e] = (live >> b & 1) && e < left ? v : 0.f;
       dx[b][e] = 0.f;
     }
-  }
-  const int64_t stride = int64_t(gridDim.y) * 4;
-  for (int64_t v = int64_t(blockIdx.y) * 4 + wave; v < V; v += stride) {
-    const float* row = dz + v * ROWS;
-    T raw[VEC];
-    if (left >= VEC) {
-      __builtin_memcpy(&raw, w + v * sv + d0, sizeof(raw));
-    } else {
+  const int64_t stride = int64_t(gridDim.y) * 16;
+  for (int64_t v0 = (int64_t(blockIdx.y) * 4 + wave) * 4; v0 < V; v0 += stride) {
+    T raw[4][VEC];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) raw[e] = e < left ? w[v * sv + d0 + e] : narrow<T>(0.f);
-    }
-    float out[VEC];
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) out[e] = 0.f;
-#pragma unroll
-    for (int b = 0; b < ROWS; ++b) {
-      const float z = row[b];
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        dx[b][e] = fmaf(z, widen(raw[e]), dx[b][e]);
-        out[e] = fmaf(z, xr[b][e], out[e]);
-      }
-    }
-    if (dw != nullptr) {
-      T res[VEC];
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) res[e] = narrow<T>(out[e]);
-      T* dst = dw + v * dsv + d0 * dsd;
-      if (dsd == 1 && left >= VEC) {
-        __builtin_memcpy(dst, &res, sizeof(res));
+    for (int u = 0; u < 4; ++u) {
+      const int64_t v = v0 + u < V ? v0 + u : V - 1;
+      if (left >= VEC) {
+        __builtin_memcpy(&raw[u], w + v * sv + d0, sizeof(raw[u]));
       } else {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e)
-          if (e < left) dst[e * dsd] = res[e];
+        for (int e = 0; e < VEC; ++e) raw[u][e] = e < left ? w[v * sv + d0 + e] : T{};
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (v0 + u >= V) break;
+      const float* row = dz + (v0 + u) * ROWS;
+      float out[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) out[e] = 0.f;
+#pragma unroll
+      for (int b = 0; b < ROWS; ++b) {
+        const float z = row[b];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          dx[b][e] = fmaf(z, widen(raw[u][e]), dx[b][e]);
+          out[e] = fmaf(z, xr[b][e], out[e]);
+        }
+      }
+      if (dw != nullptr) {
+        T res[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) res[e] = narrow<T>(out[e]);
+        T* dst = dw + (v0 + u) * dsv + d0 * dsd;
+        if (dsd == 1 && left >= VEC) {
+          __builtin_memcpy(dst, &res, sizeof(res));
+        } else {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e)
+            if (e < left) dst[e * dsd] = res[e];
+        }
       }
     }
   }
   if (part == nullptr) return;                   // the whole launch
+#pragma unroll
   for (int b = 0; b < ROWS; ++b) {
     __syncthreads();
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) joined[wave][lane * VEC + e] = 0.f;
-#pragma unroll
-    for (int q = 0; q < ROWS; ++q)               // constant indexes: dx stays in registers
-      if (q == b) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) joined[wave][lane * VEC + e] = dx[q][e];
-      }
+    for (int e = 0; e < VEC; ++e) joined[wave][lane * VEC + e] = dx[b][e];
     __syncthreads();
     for (int c = threadIdx.x; c < 64 * VEC; c += kThreads) {
       const int d = int(blockIdx.x) * 64 * VEC + c;
@@ -826,11 +612,33 @@ __global__ __launch_bounds__(kThreads) void k_few_grads(int B, int D, int64_t V,
   }
 }
 
+// dx[b][d] = sum over the shares: eight of them apart, each in order, then joined in order.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void k_few_join(int D, int rows, int splits, const float* __restrict__ part,
+                                                       Labels of, T* __restrict__ dx, int64_t lddx) {
+  __shared__ float joined[8][32];
+  const int c = threadIdx.x & 31, q = threadIdx.x >> 5;
+  const int b = blockIdx.x, d = int(blockIdx.y) * 32 + c;
+  float s = 0.f;
+  if (d < D) {
+#pragma unroll 8
+    for (int z = q; z < splits; z += 8) s += part[(int64_t(z) * rows + b) * D + d];
+  }
+  joined[q][c] = s;
+  __syncthreads();
+  if (q == 0 && d < D) {
+#pragma unroll
+    for (int z = 1; z < 8; ++z) s += joined[z][c];
+    dx[b * lddx + d] = label_of(b, of.labels, of.idx, of.n_labels, of.V) >= 0 ? narrow<T>(s) : T{};
+  }
+}
+
 // ------------------------------------------------------------------ plans
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 struct Plan {
-  int P, Dp;
+  int Dp, depth;                     // padded features, reduction step
+  size_t elem;
   int64_t Bp, tiles_b, tiles_v;
   int stat_splits;
   // backward
@@ -844,24 +652,24 @@ constexpr int kWant = 512;                              // workgroups a launch s
 
 Plan make_plan(int dtype, int64_t B, int64_t D, int64_t V) {
   Plan p;
-  p.P = dtype == SGNN_F32 ? 3 : 1;
+  p.elem = dtype == SGNN_F32 ? 4 : 2;
+  p.depth = int(128 / p.elem);
   p.Dp = int(ceil_div(D, 64) * 64);
   p.tiles_b = ceil_div(B, kTile);
   p.tiles_v = ceil_div(V, kTile);
   p.Bp = p.tiles_b * kTile;
   int64_t s = ceil_div(kWant, p.tiles_b);
   p.stat_splits = int(s < p.tiles_v ? s : p.tiles_v);
-  int64_t tiles = kPieceBytes / (p.Bp * 2 * p.P * kTile);
+  int64_t tiles = kPieceBytes / (p.Bp * int64_t(p.elem) * kTile);
   if (tiles < 1) tiles = 1;
   if (tiles > p.tiles_v) tiles = p.tiles_v;
   p.piece = tiles * kTile;
   p.tiles_d = int(ceil_div(D, kTile));
-  const int bk = p.P == 1 ? 64 : 32;
   s = ceil_div(kWant, p.tiles_b * p.tiles_d);
-  int64_t most = p.piece / bk / 2;
+  int64_t most = p.piece / p.depth / 2;
   p.dx_splits = int(s < most ? s : most);
   s = ceil_div(kWant, tiles * p.tiles_d);
-  most = p.Bp / bk / 2;
+  most = p.Bp / p.depth / 2;
   p.dw_splits = int(s < most ? s : most);
   if (p.dx_splits < 1) p.dx_splits = 1;
   if (p.dw_splits < 1) p.dw_splits = 1;
@@ -887,13 +695,13 @@ Few make_few(int dtype, int64_t B, int64_t D, int64_t V, int64_t sd) {
   const int64_t blocks = ceil_div(V, 128);
   f.blocks = unsigned(blocks < kFewBlocks ? blocks : kFewBlocks);
   f.slabs = unsigned(ceil_div(D, 64 * f.vec));
-  const int64_t want = ceil_div(1024, f.slabs), most = ceil_div(V, 16);
+  const int64_t want = ceil_div(f.rows > 8 ? 512 : 1024, f.slabs), most = ceil_div(V, 16);
   f.splits = unsigned(want < most ? want : most);
   return f;
 }
 
 struct Buffers {
-  uint16_t *x, *w, *dz;
+  char *x, *w, *dz;
   float2* part;
   float *picked, *rest, *dx, *dw;
   size_t bytes;
@@ -902,14 +710,14 @@ struct Buffers {
 Buffers carve(const Plan& p, int64_t B, int64_t V, bool backward, void* base) {
   sgnn::Carver c(base);
   Buffers b{};
-  b.x = c.take<uint16_t>(size_t(p.P) * B * p.Dp);
-  b.w = c.take<uint16_t>(size_t(p.P) * V * p.Dp);
+  b.x = c.take<char>(p.elem * B * p.Dp);
+  b.w = c.take<char>(p.elem * V * p.Dp);
   if (!backward) {
     b.part = c.take<float2>(size_t(p.stat_splits) * 2 * B);
     b.picked = c.take<float>(size_t(B));
   } else {
     const size_t Np = size_t(p.tiles_d) * kTile;
-    b.dz = c.take<uint16_t>(size_t(p.P) * p.Bp * p.piece);
+    b.dz = c.take<char>(p.elem * p.Bp * p.piece);
     b.rest = c.take<float>(size_t(B));
     b.dx = c.take<float>(size_t(p.dx_splits) * p.Bp * Np);
     b.dw = c.take<float>(size_t(p.dw_splits) * p.piece * Np);
@@ -961,24 +769,25 @@ int check_call(const Call& c) {
   return SGNN_OK;
 }
 
-// A bf16 weight whose rows are whole 128-byte lines can be staged as it lies.
+// A weight whose rows are whole steps and 16-byte aligned can be staged as it lies.
 bool weight_as_is(const Call& c, const Plan& p) {
-  return p.P == 1 && c.sd == 1 && c.D == p.Dp && c.sv % 8 == 0 && reinterpret_cast<uintptr_t>(c.w) % 16 == 0;
+  return c.sd == 1 && c.D % p.depth == 0 && size_t(c.sv) * p.elem % 16 == 0 &&
+         reinterpret_cast<uintptr_t>(c.w) % 16 == 0;
 }
 
-template <typename T, int P>
-int planes(const Call& c, const Plan& p, const Buffers& b, Operand* x, Operand* w, hipStream_t st) {
+template <typename T>
+int operands(const Call& c, const Plan& p, const Buffers& b, Operand<T>* x, Operand<T>* w, hipStream_t st) {
   const int across = p.Dp / 64;
   const Source sx{c.x, c.B, c.ldx, 1, b.x, ceil_div(c.B, 64) * across};
   Source sw{c.w, c.V, c.sv, c.sd, b.w, ceil_div(c.V, 64) * across};
-  *x = Operand{b.x, p.Dp, c.B * p.Dp, c.B, p.Dp};
-  *w = Operand{b.w, p.Dp, c.V * p.Dp, c.V, p.Dp};
+  *x = Operand<T>{reinterpret_cast<const T*>(b.x), p.Dp, c.B, p.Dp};
+  *w = Operand<T>{reinterpret_cast<const T*>(b.w), p.Dp, c.V, p.Dp};
   if (weight_as_is(c, p)) {
     sw.blocks = 0;
-    *w = Operand{static_cast<const uint16_t*>(c.w), c.sv, 0, c.V, c.D};
+    *w = Operand<T>{static_cast<const T*>(c.w), c.sv, c.V, c.D};
   }
-  hipLaunchKernelGGL((k_planes<T, P>), dim3(unsigned(sx.blocks + sw.blocks)), dim3(256), 0, st, int(c.D), p.Dp, sx, sw,
-                     Labels{c.labels, c.idx, c.n_labels, c.V});
+  hipLaunchKernelGGL((k_class_operands<T>), dim3(unsigned(sx.blocks + sw.blocks)), dim3(256), 0, st, int(c.D), p.Dp, sx,
+                     sw, Labels{c.labels, c.idx, c.n_labels, c.V});
   HIP_TRY(hipGetLastError());
   return SGNN_OK;
 }
@@ -1002,43 +811,44 @@ int allow_lds(const void* kernel, size_t bytes) {
   return SGNN_OK;
 }
 
-template <typename T, int P>
+template <typename T>
 int forward(const Call& c, const Plan& p, const Buffers& b, float2* stats, float* row_loss, float* loss,
             float* share, hipStream_t st) {
-  Operand x, w;
-  if (int rc = planes<T, P>(c, p, b, &x, &w, st)) return rc;
-  hipLaunchKernelGGL((k_class_stats<P>), dim3(unsigned(p.tiles_b * p.stat_splits)), dim3(kThreads), 0, st, c.B, c.V,
+  Operand<T> x, w;
+  if (int rc = operands<T>(c, p, b, &x, &w, st)) return rc;
+  const int depth = int(ceil_div(c.D, p.depth) * p.depth);
+  hipLaunchKernelGGL((k_class_stats<T>), dim3(unsigned(p.tiles_b * p.stat_splits)), dim3(kThreads), 0, st, c.B, c.V,
                      p.Dp, x, w, c.labels, c.idx, c.n_labels, p.tiles_v, p.stat_splits, b.part, b.picked);
   HIP_TRY(hipGetLastError());
   return finish_forward(c, 2 * p.stat_splits, b, stats, row_loss, loss, share, st);
 }
 
-template <typename T, int P>
+template <typename T>
 int backward(const Call& c, const Plan& p, const Buffers& b, const float2* stats, const float* grad,
              const float* share, void* dx, int64_t lddx, void* dw, int64_t dsv, int64_t dsd, hipStream_t st) {
-  Operand x, w;
-  if (int rc = planes<T, P>(c, p, b, &x, &w, st)) return rc;
+  Operand<T> x, w;
+  if (int rc = operands<T>(c, p, b, &x, &w, st)) return rc;
   const int64_t Np = int64_t(p.tiles_d) * kTile;
-  const int64_t dz_plane = p.Bp * p.piece;
+  T* const dz = reinterpret_cast<T*>(b.dz);
+  const int depth = int(ceil_div(c.D, p.depth) * p.depth);
   for (int64_t v0 = 0; v0 < c.V; v0 += p.piece) {
     const int64_t left = ceil_div(c.V - v0, kTile);
     const int tiles = int(left < p.piece / kTile ? left : p.piece / kTile);
     const int64_t width = int64_t(tiles) * kTile;
-    hipLaunchKernelGGL((k_class_dz<P>), dim3(unsigned(p.tiles_b * tiles)), dim3(kThreads), 0, st, c.B, c.V, p.Dp, x, w,
-                       c.labels, c.idx, c.n_labels, stats, share ? nullptr : grad, b.rest, v0, tiles, b.dz,
-                       p.piece, dz_plane);
+    hipLaunchKernelGGL((k_class_dz<T>), dim3(unsigned(p.tiles_b * tiles)), dim3(kThreads), 0, st, c.B, c.V, depth, x, w,
+                       c.labels, c.idx, c.n_labels, stats, share ? nullptr : grad, b.rest, v0, tiles, dz, p.piece);
     HIP_TRY(hipGetLastError());
     if (dx) {                                    // dx[b][d] += dz[b][v] . w[v][d]
-      const Operand a{b.dz, p.piece, dz_plane, p.Bp, p.piece};
-      const Operand wv{w.base + v0 * w.ld, w.ld, w.plane, c.V - v0, w.cols};
-      hipLaunchKernelGGL((k_class_product<P, true>), dim3(unsigned(p.tiles_b * p.dx_splits * p.tiles_d)),
+      const Operand<T> a{dz, p.piece, p.Bp, p.piece};
+      const Operand<T> wv{w.base + v0 * w.ld, w.ld, c.V - v0, w.cols};
+      hipLaunchKernelGGL((k_class_product<T, true>), dim3(unsigned(p.tiles_b * p.dx_splits * p.tiles_d)),
                          dim3(kThreads), 0, st, a, wv, int(p.tiles_b), p.tiles_d, width, p.dx_splits, v0 > 0 ? 1 : 0,
                          b.dx, p.Bp * Np, Np);
       HIP_TRY(hipGetLastError());
     }
     if (dw) {                                    // dw[v][d] = dz[b][v] . x[b][d]
-      const Operand a{b.dz, p.piece, dz_plane, p.Bp, p.piece};
-      hipLaunchKernelGGL((k_class_product<P, false>), dim3(unsigned(tiles * p.dw_splits * p.tiles_d)), dim3(kThreads),
+      const Operand<T> a{dz, p.piece, p.Bp, p.piece};
+      hipLaunchKernelGGL((k_class_product<T, false>), dim3(unsigned(tiles * p.dw_splits * p.tiles_d)), dim3(kThreads),
                          0, st, a, x, tiles, p.tiles_d, p.Bp, p.dw_splits, 0, b.dw, p.piece * Np, Np);
       HIP_TRY(hipGetLastError());
       const int64_t rows = c.V - v0 < width ? c.V - v0 : width;
@@ -1050,7 +860,7 @@ int backward(const Call& c, const Plan& p, const Buffers& b, const float2* stats
   }
   if (dx) {
     hipLaunchKernelGGL((k_class_join<T>), dim3(unsigned(ceil_div(c.B, 32)), unsigned(ceil_div(c.D, 32))), dim3(256), 0, st,
-                       c.B, int(c.D), p.dx_splits, b.dx, p.Bp * Np, Np, grad, share, P == 1 ? b.rest : nullptr,
+                       c.B, int(c.D), p.dx_splits, b.dx, p.Bp * Np, Np, grad, share, sizeof(T) == 2 ? b.rest : nullptr,
                        Labels{c.labels, c.idx, c.n_labels, c.V}, static_cast<const T*>(c.w), c.sv, c.sd,
                        static_cast<T*>(dx), lddx, int64_t(1));
     HIP_TRY(hipGetLastError());
@@ -1058,25 +868,25 @@ int backward(const Call& c, const Plan& p, const Buffers& b, const float2* stats
   return SGNN_OK;
 }
 
-template <typename T, int P>
+template <typename T>
 int few_forward(const Call& c, const Few& f, const Buffers& b, float2* stats, float* row_loss, float* loss,
                 float* share, hipStream_t st) {
   const Labels of{c.labels, c.idx, c.n_labels, c.V};
-  if (int rc = allow_lds(reinterpret_cast<const void*>(&k_few_stats<T, P>), f.lds)) return rc;
-  hipLaunchKernelGGL((k_few_stats<T, P>), dim3(f.blocks), dim3(kThreads), f.lds, st, int(c.B), int(c.D), f.Dk, c.V,
+  if (int rc = allow_lds(reinterpret_cast<const void*>(&k_few_stats<T>), f.lds)) return rc;
+  hipLaunchKernelGGL((k_few_stats<T>), dim3(f.blocks), dim3(kThreads), f.lds, st, int(c.B), int(c.D), f.Dk, c.V,
                      static_cast<const T*>(c.x), c.ldx, static_cast<const T*>(c.w), c.sv, of, b.part, b.picked);
   HIP_TRY(hipGetLastError());
   return finish_forward(c, int(f.blocks), b, stats, row_loss, loss, share, st);
 }
 
-template <typename T, int P>
+template <typename T>
 int few_backward(const Call& c, const Few& f, const Buffers& b, const float2* stats, const float* grad,
                  const float* share, void* dx, int64_t lddx, void* dw, int64_t dsv, int64_t dsd, hipStream_t st) {
   const Labels of{c.labels, c.idx, c.n_labels, c.V};
   const T* x = static_cast<const T*>(c.x);
   const T* w = static_cast<const T*>(c.w);
-  if (int rc = allow_lds(reinterpret_cast<const void*>(&k_few_dz<T, P>), f.lds)) return rc;
-  hipLaunchKernelGGL((k_few_dz<T, P>), dim3(f.blocks), dim3(kThreads), f.lds, st, int(c.B), f.rows, int(c.D), f.Dk, c.V,
+  if (int rc = allow_lds(reinterpret_cast<const void*>(&k_few_dz<T>), f.lds)) return rc;
+  hipLaunchKernelGGL((k_few_dz<T>), dim3(f.blocks), dim3(kThreads), f.lds, st, int(c.B), f.rows, int(c.D), f.Dk, c.V,
                      x, c.ldx, w, c.sv, of, stats, grad, share, b.dw);
   HIP_TRY(hipGetLastError());
 #define SGNN_FEW(ROWS, VEC)                                                                                          \
@@ -1092,9 +902,8 @@ int few_backward(const Call& c, const Few& f, const Buffers& b, const float2* st
 #undef SGNN_FEW
   HIP_TRY(hipGetLastError());
   if (dx) {
-    hipLaunchKernelGGL((k_class_join<T>), dim3(1, unsigned(ceil_div(c.D, 32))), dim3(256), 0, st, c.B, int(c.D),
-                       int(f.splits), b.dx, int64_t(f.rows) * c.D, c.D, nullptr, nullptr, nullptr, of, nullptr, 0, 0,
-                       static_cast<T*>(dx), lddx, int64_t(1));
+    hipLaunchKernelGGL((k_few_join<T>), dim3(unsigned(c.B), unsigned(ceil_div(c.D, 32))), dim3(kThreads), 0, st, int(c.D),
+                       f.rows, int(f.splits), b.dx, of, static_cast<T*>(dx), lddx);
     HIP_TRY(hipGetLastError());
   }
   return SGNN_OK;
@@ -1126,13 +935,13 @@ extern "C" int sgnn_class_xent_forward(int dtype, int64_t B, int64_t D, int64_t 
   float2* s = reinterpret_cast<float2*>(stats);
   if (const Few f = make_few(dtype, B, D, V, sd); f.rows) {
     const Buffers b = carve_few(f, B, D, V, false, workspace);
-    if (dtype == SGNN_F32) return few_forward<float, 3>(c, f, b, s, row_loss, loss, share, st);
-    return few_forward<Bf16, 1>(c, f, b, s, row_loss, loss, share, st);
+    if (dtype == SGNN_F32) return few_forward<float>(c, f, b, s, row_loss, loss, share, st);
+    return few_forward<Bf16>(c, f, b, s, row_loss, loss, share, st);
   }
   const Plan p = make_plan(dtype, B, D, V);
   const Buffers b = carve(p, B, V, false, workspace);
-  if (dtype == SGNN_F32) return forward<float, 3>(c, p, b, s, row_loss, loss, share, st);
-  return forward<Bf16, 1>(c, p, b, s, row_loss, loss, share, st);
+  if (dtype == SGNN_F32) return forward<float>(c, p, b, s, row_loss, loss, share, st);
+  return forward<Bf16>(c, p, b, s, row_loss, loss, share, st);
 }
 
 extern "C" int sgnn_class_xent_backward(int dtype, int64_t B, int64_t D, int64_t V, const void* x, int64_t ldx,
@@ -1154,11 +963,11 @@ extern "C" int sgnn_class_xent_backward(int dtype, int64_t B, int64_t D, int64_t
   const float2* s = reinterpret_cast<const float2*>(stats);
   if (const Few f = make_few(dtype, B, D, V, sd); f.rows) {
     const Buffers b = carve_few(f, B, D, V, true, workspace);
-    if (dtype == SGNN_F32) return few_backward<float, 3>(c, f, b, s, grad, share, dx, lddx, dweight, dsv, dsd, st);
-    return few_backward<Bf16, 1>(c, f, b, s, grad, share, dx, lddx, dweight, dsv, dsd, st);
+    if (dtype == SGNN_F32) return few_backward<float>(c, f, b, s, grad, share, dx, lddx, dweight, dsv, dsd, st);
+    return few_backward<Bf16>(c, f, b, s, grad, share, dx, lddx, dweight, dsv, dsd, st);
   }
   const Plan p = make_plan(dtype, B, D, V);
   const Buffers b = carve(p, B, V, true, workspace);
-  if (dtype == SGNN_F32) return backward<float, 3>(c, p, b, s, grad, share, dx, lddx, dweight, dsv, dsd, st);
-  return backward<Bf16, 1>(c, p, b, s, grad, share, dx, lddx, dweight, dsv, dsd, st);
+  if (dtype == SGNN_F32) return backward<float>(c, p, b, s, grad, share, dx, lddx, dweight, dsv, dsd, st);
+  return backward<Bf16>(c, p, b, s, grad, share, dx, lddx, dweight, dsv, dsd, st);
 }

@@ -1,0 +1,214 @@
+// Matrix products of fp32 or bf16 operands on the bf16 matrix instructions: element types, the
+// exact splitting of fp32 and the inner loop of a 128 x 128 tile.
+//
+// bf16 operands go in as they are: their products are exact and summed in 32 bits.  An fp32 number
+// is the sum of three bf16 numbers (8 + 8 + 8 bits of its mantissa, cut off, so the sum is exact),
+// taken apart in registers on the way from LDS to the matrix instruction; of the nine products of
+// two numbers the three smallest, below 3 * 2^-24 of the whole, are left out.
+#pragma once
+#include "common.h"
+
+namespace {
+
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+struct Bf16 { uint16_t bits; };
+
+__device__ __forceinline__ float widen(float v) { return v; }
+__device__ __forceinline__ float widen(Bf16 v) { return __uint_as_float(unsigned(v.bits) << 16); }
+__device__ __forceinline__ uint16_t to_bf16(float v) {                       // nearest even
+  const unsigned u = __float_as_uint(v);
+  if ((u & 0x7fffffffu) > 0x7f800000u) return 0x7fc0u;
+  return uint16_t((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+}
+template <typename T> __device__ __forceinline__ T narrow(float v);
+template <> __device__ __forceinline__ float narrow<float>(float v) { return v; }
+template <> __device__ __forceinline__ Bf16 narrow<Bf16>(float v) { return Bf16{to_bf16(v)}; }
+
+// v = a + b + c exactly, each a bf16 number; an infinity or NaN leaves a NaN behind
+__device__ __forceinline__ void split3(float v, float& a, float& b, float& c) {
+  a = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
+  const float r = v - a;
+  b = __uint_as_float(__float_as_uint(r) & 0xffff0000u);
+  c = r - b;
+}
+// the high halves of two floats as a bf16 pair
+__device__ __forceinline__ unsigned high_halves(float lo, float hi) {
+  return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+}
+
+// bf16 numbers an element of type T is made of
+template <typename T> struct Planes { static constexpr int kCount = sizeof(T) == 4 ? 3 : 1; };
+
+__device__ __forceinline__ void planes_of(const float (&v)[8], bf16x8 (&out)[3]) {
+  u32x4 pl[3];
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    float a0, b0, c0, a1, b1, c1;
+    split3(v[e], a0, b0, c0);
+    split3(v[e + 1], a1, b1, c1);
+    pl[0][e / 2] = high_halves(a0, a1);
+    pl[1][e / 2] = high_halves(b0, b1);
+    pl[2][e / 2] = high_halves(c0, c1);
+  }
+#pragma unroll
+  for (int q = 0; q < 3; ++q) __builtin_memcpy(&out[q], &pl[q], 16);
+}
+__device__ __forceinline__ void planes_of(const Bf16 (&v)[8], bf16x8 (&out)[1]) { __builtin_memcpy(&out[0], &v, 16); }
+
+// acc += a . b over the planes' products that count
+template <int P>
+__device__ __forceinline__ void multiply_planes(const bf16x8 (&a)[P], const bf16x8 (&b)[P], f32x16& acc) {
+#pragma unroll
+  for (int pa = 0; pa < P; ++pa)
+#pragma unroll
+    for (int pb = 0; pa + pb < P; ++pb) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[pa], b[pb], acc, 0, 0, 0);
+}
+
+// row of element e of a 32 x 32 block of results (its column is lane & 31)
+__device__ __forceinline__ int block_row(int e, int lane) { return 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3); }
+
+// ------------------------------------------------------------------ the 128 x 128 tile
+// Four wavefronts form a 128 x 128 tile, 64 x 64 each, in steps of 128 bytes of the reduction.
+// Operands travel from memory to LDS without passing registers, one step ahead.  An operand is
+// "deep" when its memory is contiguous along the reduction (LDS holds [128 rows][128 bytes], read
+// directly) and "flat" when it is contiguous along the tile ([reduction][128 columns]; bf16 is read
+// through the transposing LDS load, fp32 element by element).  16-byte chunks are permuted on the
+// way in so that no read meets bank conflicts.
+constexpr int kTile = 128;
+constexpr int kThreads = 256;
+constexpr int kStageBytes = kTile * 128;         // of one operand
+constexpr int kProductLds = 4 * kStageBytes;     // two operands, two stages
+
+template <typename T>
+struct Operand {
+  const T* base;           // 16-byte aligned, as every row is
+  int64_t ld;              // row stride in elements
+  int64_t rows;            // rows that exist: reads beyond repeat the last one
+  int64_t cols;            // columns that exist (flat operands; a multiple of 16 bytes): likewise
+};
+
+template <typename T> struct Step { static constexpr int kDepth = 128 / sizeof(T); };
+
+typedef __attribute__((address_space(3))) void lds_void;
+typedef const __attribute__((address_space(1))) void global_void;
+
+// deep: rows r0 .. r0 + 127 at reduction offset k0;  flat: reduction rows k0 .. at columns r0 ..
+template <typename T, bool DEEP>
+__device__ __forceinline__ void stage_operand(const Operand<T>& op, int64_t r0, int64_t k0, char* lds, int wave,
+                                              int lane) {
+  constexpr int V = 16 / sizeof(T);              // elements of a chunk
+#pragma unroll
+  for (int l = 0; l < kStageBytes / 16 / kThreads; ++l) {
+    const int first = (l * 4 + wave) * 64, q = first + lane;
+    const T* src;
+    if constexpr (DEEP) {
+      const int row = q >> 3, c = (q & 7) ^ (row & 7);
+      int64_t r = r0 + row;
+      r = r < op.rows ? r : op.rows - 1;
+      src = op.base + r * op.ld + k0 + c * V;
+    } else {
+      constexpr int cpr = kTile / V;
+      const int row = q / cpr;
+      const int c = (q % cpr) ^ (sizeof(T) == 2 ? (row & 3) << 2 : ((row >> 3) & 1) << 3);
+      int64_t r = k0 + row, col = r0 + c * V;
+      r = r < op.rows ? r : op.rows - 1;
+      col = col < op.cols ? col : op.cols - V;
+      src = op.base + r * op.ld + col;
+    }
+    __builtin_amdgcn_global_load_lds((global_void*)src, (lds_void*)(lds + first * 16), 16, 0, 0);
+  }
+}
+
+// the operand of one 32 x 32 x 16 instruction: element `lane & 31` of the block at m0, eight
+// reduction indexes from k0 + 8 * (lane / 32)
+template <typename T, bool DEEP>
+__device__ __forceinline__ void fragment(const char* lds, int m0, int k0, int lane,
+                                         bf16x8 (&out)[Planes<T>::kCount]) {
+  if constexpr (DEEP) {
+    const int row = m0 + (lane & 31);
+    const char* at = lds + row * 128;
+    if constexpr (sizeof(T) == 2) {
+      const int c = (k0 >> 3) + (lane >> 5);
+      out[0] = *reinterpret_cast<const bf16x8*>(at + ((c ^ (row & 7)) << 4));
+    } else {
+      const int c = (k0 >> 2) + 2 * (lane >> 5);
+      float v[8];
+      *reinterpret_cast<f32x4*>(&v[0]) = *reinterpret_cast<const f32x4*>(at + ((c ^ (row & 7)) << 4));
+      *reinterpret_cast<f32x4*>(&v[4]) = *reinterpret_cast<const f32x4*>(at + (((c + 1) ^ (row & 7)) << 4));
+      planes_of(v, out);
+    }
+  } else if constexpr (sizeof(T) == 2) {
+    const int k = k0 + 8 * (lane >> 5) + ((lane & 15) >> 2);
+    const int m = m0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    const int at = ((m >> 3) ^ ((k & 3) << 2)) * 16 + (m & 7) * 2;       // k and k + 4 share k & 3
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds + k * 256 + at));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds + (k + 4) * 256 + at));
+    __builtin_memcpy(&out[0], &lo, 8);
+    __builtin_memcpy(reinterpret_cast<char*>(&out[0]) + 8, &hi, 8);
+  } else {
+    const int k = k0 + 8 * (lane >> 5), m = m0 + (lane & 31);
+    const char* at = lds + k * 512 + (((m >> 5) ^ ((k >> 3) & 1)) << 7) + (m & 31) * 4;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = *reinterpret_cast<const float*>(at + j * 512);
+    planes_of(v, out);
+  }
+}
+
+typedef f32x16 Tile[2][2];
+
+__device__ __forceinline__ void clear(Tile& acc) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+}
+
+// acc += A[m0 .., k0 .. k1] . B[n0 .., k0 .. k1]; k1 - k0 a multiple of the step.  `lds` holds two
+// stages of both operands; every wavefront has left them when this returns.
+template <typename T, bool ADEEP, bool BDEEP>
+__device__ __forceinline__ void multiply(const Operand<T>& A, int64_t m0, const Operand<T>& B, int64_t n0, int64_t k0,
+                                         int64_t k1, char* lds, Tile& acc) {
+  constexpr int kDepth = Step<T>::kDepth, P = Planes<T>::kCount;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
+  stage_operand<T, ADEEP>(A, m0, k0, lds, wave, lane);
+  stage_operand<T, BDEEP>(B, n0, k0, lds + kStageBytes, wave, lane);
+  int cur = 0;
+  for (int64_t k = k0; k < k1; k += kDepth) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // this wavefront's part of the stage has landed
+    __syncthreads();                                         // everybody's has, and the other stage is free
+    const char* a = lds + cur * 2 * kStageBytes;
+    const char* b = a + kStageBytes;
+    if (k + kDepth < k1) {
+      char* next = lds + (cur ^ 1) * 2 * kStageBytes;
+      stage_operand<T, ADEEP>(A, m0, k + kDepth, next, wave, lane);
+      stage_operand<T, BDEEP>(B, n0, k + kDepth, next + kStageBytes, wave, lane);
+    }
+#pragma unroll
+    for (int kk = 0; kk < kDepth; kk += 16) {
+      bf16x8 fa[2][P], fb[2][P];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        fragment<T, ADEEP>(a, wm + 32 * i, kk, lane, fa[i]);
+        fragment<T, BDEEP>(b, wn + 32 * i, kk, lane, fb[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) multiply_planes<P>(fa[i], fb[j], acc[i][j]);
+    }
+    cur ^= 1;
+  }
+  __syncthreads();
+}
+
+}  // namespace
