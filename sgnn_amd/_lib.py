@@ -11,6 +11,8 @@ import ctypes
 import os
 from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_void_p
 
+import torch
+
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libsgnn_hip.so")
 
@@ -147,6 +149,8 @@ SIGNATURES = {
 
 _lib = None
 
+TYPES = {torch.float32: F32, torch.bfloat16: BF16}
+
 
 class SgnnHipError(RuntimeError):
     pass
@@ -189,6 +193,28 @@ def ptr(t):
     return None if t is None else c_void_p(t.data_ptr())
 
 
+def call_on(device, entry, *args):
+    """``entry(*args, stream)`` on the device's current stream, with the device made current;
+    raises on an error code.  Pointers may be plain addresses."""
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if torch.cuda.current_device() == device.index:
+        rc = entry(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = entry(*args, stream)
+    if rc != 0:
+        check(rc)
+
+
+def element_type(t, what):
+    """The library's code of a GPU tensor's element type."""
+    if not t.is_cuda:
+        raise ValueError(f"{what} must be on the GPU, got {t.device}")
+    code = TYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{what} must be float32 or bfloat16, got {t.dtype}")
+    return code
+
+
 def current_stream(device):
-    import torch
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)

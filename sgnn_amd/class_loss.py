@@ -10,7 +10,8 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .saved8 import element_type, unit_rows
+from ._lib import element_type
+from .saved8 import unit_rows
 
 
 def _weight_layout(w):
@@ -31,43 +32,42 @@ class _ClassXent(torch.autograd.Function):
     def forward(ctx, x, weight, labels, idx, mean):
         x, (w, sv, sd) = unit_rows(x.detach()), _weight_layout(weight.detach())
         (B, D), V, dev = x.shape, w.shape[0], x.device
-        lib, dtype = _lib.load(), element_type(x, "x")
-        stats = torch.empty(B, 2, dtype=torch.float32, device=dev)
-        rows = torch.empty(B, dtype=torch.float32, device=dev)
-        loss = torch.empty((), dtype=torch.float32, device=dev) if mean else None
-        share = torch.empty(1, dtype=torch.float32, device=dev) if mean else None
-        ws = torch.empty(lib.sgnn_class_xent_workspace_bytes(dtype, B, D, V, 0), dtype=torch.uint8, device=dev)
-        with torch.cuda.device(dev):
-            _lib.check(lib.sgnn_class_xent_forward(
-                dtype, B, D, V, _lib.ptr(x), max(x.stride(0), D), _lib.ptr(w), sv, sd, _lib.ptr(labels), labels.numel(),
-                _lib.ptr(idx), _lib.ptr(stats), _lib.ptr(rows), _lib.ptr(loss), _lib.ptr(share), _lib.ptr(ws),
-                ws.numel(), _lib.current_stream(dev)))
-        ctx.save_for_backward(x, w, labels, idx, stats, share)
-        ctx.strides = (sv, sd)
-        return loss if mean else rows
+        lib, dtype = _lib.load(), _lib.TYPES[x.dtype]
+        kept = torch.empty(3 * B + 1, dtype=torch.float32, device=dev)   # statistics, 1 / counted rows, row losses
+        out = torch.empty(() if mean else (B,), dtype=torch.float32, device=dev)
+        nbytes = lib.sgnn_class_xent_workspace_bytes(dtype, B, D, V, 0)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        at = kept.data_ptr()
+        rows, loss, share = (at + 8 * B + 4, out.data_ptr(), at + 8 * B) if mean else (out.data_ptr(), None, None)
+        _lib.call_on(dev, lib.sgnn_class_xent_forward, dtype, B, D, V, x.data_ptr(), max(x.stride(0), D), w.data_ptr(),
+                     sv, sd, labels.data_ptr(), labels.numel(), None if idx is None else idx.data_ptr(), at, rows, loss,
+                     share, ws.data_ptr(), nbytes)
+        ctx.save_for_backward(x, w, labels, idx, kept)
+        ctx.layout = (sv, sd, mean)
+        return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        x, w, labels, idx, stats, share = ctx.saved_tensors
+        x, w, labels, idx, kept = ctx.saved_tensors
         (B, D), V, dev = x.shape, w.shape[0], x.device
-        sv, sd = ctx.strides
-        lib, dtype = _lib.load(), element_type(x, "x")
+        sv, sd, mean = ctx.layout
+        lib, dtype = _lib.load(), _lib.TYPES[x.dtype]
         grad = grad.contiguous()
         dx = torch.empty(B, D, dtype=x.dtype, device=dev) if ctx.needs_input_grad[0] else None
         dw, dsv, dsd = None, D, 1
         if ctx.needs_input_grad[1]:                  # in the weight's own layout
-            by_class = sd == 1
-            dw = torch.empty((V, D) if by_class else (D, V), dtype=w.dtype, device=dev)
-            if not by_class:
-                dw = dw.t()
-                dsv, dsd = 1, V
-        ws = torch.empty(lib.sgnn_class_xent_workspace_bytes(dtype, B, D, V, 1), dtype=torch.uint8, device=dev)
-        with torch.cuda.device(dev):
-            _lib.check(lib.sgnn_class_xent_backward(
-                dtype, B, D, V, _lib.ptr(x), max(x.stride(0), D), _lib.ptr(w), sv, sd, _lib.ptr(labels), labels.numel(),
-                _lib.ptr(idx), _lib.ptr(stats), _lib.ptr(grad), _lib.ptr(share), _lib.ptr(dx), D, _lib.ptr(dw), dsv, dsd,
-                _lib.ptr(ws), ws.numel(), _lib.current_stream(dev)))
+            if sd == 1:
+                dw = torch.empty(V, D, dtype=w.dtype, device=dev)
+            else:
+                dw, dsv, dsd = torch.empty(D, V, dtype=w.dtype, device=dev).t(), 1, V
+        nbytes = lib.sgnn_class_xent_workspace_bytes(dtype, B, D, V, 1)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        at = kept.data_ptr()
+        _lib.call_on(dev, lib.sgnn_class_xent_backward, dtype, B, D, V, x.data_ptr(), max(x.stride(0), D), w.data_ptr(),
+                     sv, sd, labels.data_ptr(), labels.numel(), None if idx is None else idx.data_ptr(), at,
+                     grad.data_ptr(), at + 8 * B if mean else None, None if dx is None else dx.data_ptr(), D,
+                     None if dw is None else dw.data_ptr(), dsv, dsd, ws.data_ptr(), nbytes)
         return dx, dw, None, None, None
 
 

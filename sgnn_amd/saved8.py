@@ -12,23 +12,13 @@ the sign of ``x``, so the activation keeps nothing of its own (``SavedInt8.input
 """
 from __future__ import annotations
 
+import ctypes
 import math
 
 import torch
 
 from . import _lib
-
-_TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
-
-
-def element_type(t, what):
-    """The library's code of a GPU tensor's element type."""
-    if not t.is_cuda:
-        raise ValueError(f"{what} must be on the GPU, got {t.device}")
-    code = _TYPES.get(t.dtype)
-    if code is None:
-        raise TypeError(f"{what} must be float32 or bfloat16, got {t.dtype}")
-    return code
+from ._lib import TYPES, element_type
 
 
 def checked_slope(slope):
@@ -37,7 +27,7 @@ def checked_slope(slope):
     if not (math.isfinite(slope) and slope >= 0.0):
         raise ValueError(f"the activation's slope must be finite and not negative, got {slope}")
     # what the kernels compute with; a slope that 32 bits cannot hold is refused, not turned into another one
-    held = torch.tensor(slope, dtype=torch.float32).item()
+    held = ctypes.c_float(slope).value
     if math.isinf(held) or (held == 0.0) != (slope == 0.0) or (held == 1.0) != (slope == 1.0):
         raise ValueError(f"the activation's slope is not a 32-bit number: {slope}")
     return held
@@ -80,7 +70,7 @@ class SavedInt8:
             raise ValueError("codes and steps are on different devices")
         if codes.data_ptr() % 16:
             raise ValueError("codes must be 16-byte aligned")
-        if dtype not in _TYPES:
+        if dtype not in TYPES:
             raise TypeError(f"saved activations are float32 or bfloat16, got {dtype}")
 
     @property
@@ -94,13 +84,12 @@ class SavedInt8:
     def restore(self, dtype=None):
         """The values the codes stand for, ``n x F`` (exact in either type)."""
         dtype = self.dtype if dtype is None else dtype
-        if dtype not in _TYPES:
+        if dtype not in TYPES:
             raise TypeError(f"saved activations are restored as float32 or bfloat16, not {dtype}")
         n, F = self.shape
         out = torch.empty(n, F, dtype=dtype, device=self.device)
-        with torch.cuda.device(self.device):
-            _lib.check(_lib.load().sgnn_restore8(_TYPES[dtype], n, F, _lib.ptr(self.codes), _lib.ptr(self.steps),
-                                                 self.slope, _lib.ptr(out), F, _lib.current_stream(self.device)))
+        _lib.call_on(self.device, _lib.load().sgnn_restore8, TYPES[dtype], n, F, self.codes.data_ptr(),
+                     self.steps.data_ptr(), self.slope, out.data_ptr(), F)
         return out
 
     def _grad(self, grad, width, what):
@@ -121,12 +110,11 @@ class SavedInt8:
             return torch.zeros(H, F, dtype=grad.dtype, device=self.device)
         lib = _lib.load()
         dW = torch.empty(H, F, dtype=grad.dtype, device=self.device)
-        ws = torch.empty(lib.sgnn_saved8_weight_grad_workspace_bytes(n, F, H), dtype=torch.uint8, device=self.device)
-        with torch.cuda.device(self.device):
-            _lib.check(lib.sgnn_saved8_weight_grad(_TYPES[grad.dtype], n, F, H, _lib.ptr(self.codes),
-                                                   _lib.ptr(self.steps), self.slope, _lib.ptr(grad), _ld(grad),
-                                                   _lib.ptr(dW), F, _lib.ptr(ws), ws.numel(),
-                                                   _lib.current_stream(self.device)))
+        nbytes = lib.sgnn_saved8_weight_grad_workspace_bytes(n, F, H)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        _lib.call_on(self.device, lib.sgnn_saved8_weight_grad, TYPES[grad.dtype], n, F, H, self.codes.data_ptr(),
+                     self.steps.data_ptr(), self.slope, grad.data_ptr(), _ld(grad), dW.data_ptr(), F, ws.data_ptr(),
+                     nbytes)
         return dW
 
     def input_grad(self, grad):
@@ -138,10 +126,8 @@ class SavedInt8:
             return grad
         n, F = self.shape
         out = grad if in_place else torch.empty(n, F, dtype=grad.dtype, device=self.device)
-        with torch.cuda.device(self.device):
-            _lib.check(_lib.load().sgnn_saved8_input_grad(_TYPES[grad.dtype], n, F, _lib.ptr(self.codes), self.slope,
-                                                          _lib.ptr(grad), _ld(grad), _lib.ptr(out), _ld(out),
-                                                          _lib.current_stream(self.device)))
+        _lib.call_on(self.device, _lib.load().sgnn_saved8_input_grad, TYPES[grad.dtype], n, F, self.codes.data_ptr(),
+                     self.slope, grad.data_ptr(), _ld(grad), out.data_ptr(), _ld(out))
         return out
 
 
@@ -156,9 +142,8 @@ def _save(x, slope, with_act):
     codes = torch.empty(n, groups * _lib.SAVED8_GROUP, dtype=torch.int8, device=x.device)
     steps = torch.empty(n, groups, dtype=torch.uint8, device=x.device)
     act = torch.empty(n, F, dtype=x.dtype, device=x.device) if with_act and slope != 1.0 else None
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.load().sgnn_save8(code, n, F, _lib.ptr(x), _ld(x), slope, _lib.ptr(codes), _lib.ptr(steps),
-                                          _lib.ptr(act), F, _lib.current_stream(x.device)))
+    _lib.call_on(x.device, _lib.load().sgnn_save8, code, n, F, x.data_ptr(), _ld(x), slope, codes.data_ptr(),
+                 steps.data_ptr(), None if act is None else act.data_ptr(), F)
     return SavedInt8(codes, steps, (n, F), slope, x.dtype), (x if act is None else act)
 
 
