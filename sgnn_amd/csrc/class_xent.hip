@@ -332,16 +332,21 @@ __global__ __launch_bounds__(kThreads) void k_class_product(Operand<T> A, Operan
   Tile acc;
   clear(acc);
   if (k0 < k1) multiply<T, ADEEP, false>(A, m0, B, n0, k0, k1, lds, acc);
-  float* dst = out + split * plane;
+  float* dst = out + split * plane + (m0 + wm) * ldo + n0 + wn + (lane & 31);
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < 2; ++j) {
+      if (add) {                                 // all loads before the first sum waits
+        float old[16];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        float* at = dst + (m0 + wm + 32 * i + block_row(e, lane)) * ldo + n0 + wn + 32 * j + (lane & 31);
-        *at = add ? *at + acc[i][j][e] : acc[i][j][e];
+        for (int e = 0; e < 16; ++e) old[e] = dst[(32 * i + block_row(e, lane)) * ldo + 32 * j];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][j][e] += old[e];
       }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) dst[(32 * i + block_row(e, lane)) * ldo + 32 * j] = acc[i][j][e];
+    }
 }
 
 // out[r][d] = factor * (sum over the shares, in order, + rest[r] * weight[y(r)][d]), out at r * sr +

@@ -94,12 +94,23 @@ struct Operand {
 
 template <typename T> struct Step { static constexpr int kDepth = 128 / sizeof(T); };
 
-typedef __attribute__((address_space(3))) void lds_void;
-typedef const __attribute__((address_space(1))) void global_void;
+// 16 bytes a lane from `src` to LDS byte `dst` + 16 * lane (`dst` the same for the wavefront).
+// Written as an instruction, since behind the builtin the compiler makes every later transposing
+// LDS read wait for all loads in flight, which undoes the prefetch.  It has no result to wait for
+// in a register: `landed` and a barrier come before anybody reads the LDS.  m0 is reserved (the
+// compiler sets it right before the few instructions that take it, none of which is in these
+// kernels), so it is set here each time and needs no mention as a clobber.
+__device__ __forceinline__ void load_to_lds(const void* src, unsigned dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(src) : "memory");
+}
+__device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ unsigned lds_offset(const char* p) {
+  return unsigned(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) char*)p));
+}
 
 // deep: rows r0 .. r0 + 127 at reduction offset k0;  flat: reduction rows k0 .. at columns r0 ..
 template <typename T, bool DEEP>
-__device__ __forceinline__ void stage_operand(const Operand<T>& op, int64_t r0, int64_t k0, char* lds, int wave,
+__device__ __forceinline__ void stage_operand(const Operand<T>& op, int64_t r0, int64_t k0, unsigned lds, int wave,
                                               int lane) {
   constexpr int V = 16 / sizeof(T);              // elements of a chunk
 #pragma unroll
@@ -120,7 +131,7 @@ __device__ __forceinline__ void stage_operand(const Operand<T>& op, int64_t r0, 
       col = col < op.cols ? col : op.cols - V;
       src = op.base + r * op.ld + col;
     }
-    __builtin_amdgcn_global_load_lds((global_void*)src, (lds_void*)(lds + first * 16), 16, 0, 0);
+    load_to_lds(src, lds + first * 16);
   }
 }
 
@@ -180,16 +191,17 @@ __device__ __forceinline__ void multiply(const Operand<T>& A, int64_t m0, const 
   constexpr int kDepth = Step<T>::kDepth, P = Planes<T>::kCount;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
-  stage_operand<T, ADEEP>(A, m0, k0, lds, wave, lane);
-  stage_operand<T, BDEEP>(B, n0, k0, lds + kStageBytes, wave, lane);
+  const unsigned stages = lds_offset(lds);
+  stage_operand<T, ADEEP>(A, m0, k0, stages, wave, lane);
+  stage_operand<T, BDEEP>(B, n0, k0, stages + kStageBytes, wave, lane);
   int cur = 0;
   for (int64_t k = k0; k < k1; k += kDepth) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // this wavefront's part of the stage has landed
-    __syncthreads();                                         // everybody's has, and the other stage is free
+    landed();                                    // this wavefront's part of the stage
+    __syncthreads();                             // everybody's, and the other stage is free
     const char* a = lds + cur * 2 * kStageBytes;
     const char* b = a + kStageBytes;
     if (k + kDepth < k1) {
-      char* next = lds + (cur ^ 1) * 2 * kStageBytes;
+      const unsigned next = stages + (cur ^ 1) * 2 * kStageBytes;
       stage_operand<T, ADEEP>(A, m0, k + kDepth, next, wave, lane);
       stage_operand<T, BDEEP>(B, n0, k + kDepth, next + kStageBytes, wave, lane);
     }
