@@ -92,32 +92,42 @@ __global__ __launch_bounds__(256) void k_class_operands(int D, int Dp, Source fi
 }
 
 // ------------------------------------------------------------------ forward
-// (m, s) = (maximum, sum of exp relative to it).  While everything is -inf the sum stays 0; a NaN
-// never becomes the maximum but makes the sum NaN.
-__device__ __forceinline__ void join_stats(float& m, float& s, float om, float os) {
-  const float top = fmaxf(m, om), ref = top == -INFINITY ? 0.f : top;
-  s = s * exp2_raw((m - ref) * kLog2e) + os * exp2_raw((om - ref) * kLog2e);
-  m = top;
+// (r, s): s = sum of 2^(z log2 e - r), r the maximum of z log2 e as it came out rounded (any
+// reference does, as long as all use it).  While everything is -inf the sum stays 0; a NaN never
+// becomes the maximum but makes the sum NaN.
+struct RowStat { float r, s, picked; };          // what the backward pass needs of a row; picked = the label's logit
+
+__device__ __forceinline__ void join_stats(float& r, float& s, float orr, float os) {
+  const float top = fmaxf(r, orr), ref = top == -INFINITY ? 0.f : top;
+  s = s * exp2_raw(r - ref) + os * exp2_raw(orr - ref);
+  r = top;
 }
-__device__ __forceinline__ void accumulate(const f32x16& a, const f32x16& b, float& m, float& s) {
-  float top = m;
+template <int N>
+__device__ __forceinline__ void accumulate(const f32x16 (&z)[N], float& r, float& s) {
+  float top = z[0][0];
 #pragma unroll
-  for (int e = 0; e < 16; ++e) top = fmaxf(fmaxf(a[e], b[e]), top);
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; e += 2) top = fmaxf(fmaxf(z[i][e], z[i][e + 1]), top);
+  top = fmaxf(top * kLog2e, r);
   const float ref = top == -INFINITY ? 0.f : top;
-  s *= exp2_raw((m - ref) * kLog2e);
-  float s1 = 0.f;
+  float sum[N];
+  sum[0] = s * exp2_raw(r - ref);
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    s += exp2_raw((a[e] - ref) * kLog2e);
-    s1 += exp2_raw((b[e] - ref) * kLog2e);
-  }
-  s += s1;
-  m = top;
+  for (int i = 1; i < N; ++i) sum[i] = 0.f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e)
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum[i] += exp2_raw(fmaf(z[i][e], kLog2e, -ref));
+#pragma unroll
+  for (int i = 1; i < N; ++i) sum[0] += sum[i];
+  s = sum[0];
+  r = top;
 }
 
 // A workgroup takes 128 rows of x and a range of the classes, 128 at a time.  The tile is formed
 // as classes x rows, so that a lane holds 32 classes of each of two rows and its running maximum
-// and sum need no other lane until the end.  part[row][split][half] = (max, sum of exp relative to it).
+// and sum need no other lane until the end.  part[row][split][half] = (r, s).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_class_stats(int64_t B, int64_t V, int Dp, Operand<T> x, Operand<T> w,
                                                           const int64_t* __restrict__ labels,
@@ -160,7 +170,8 @@ __global__ __launch_bounds__(kThreads) void k_class_stats(int64_t B, int64_t V, 
           for (int e = 0; e < 16; ++e)
             if (vw + 32 * i + block_row(e, lane) >= V) acc[i][j][e] = -INFINITY;
       }
-      accumulate(acc[0][j], acc[1][j], top[j], sum[j]);
+      const f32x16 z[2] = {acc[0][j], acc[1][j]};
+      accumulate(z, top[j], sum[j]);
     }
   }
 #pragma unroll
@@ -172,12 +183,12 @@ __global__ __launch_bounds__(kThreads) void k_class_stats(int64_t B, int64_t V, 
   }
 }
 
-// A row's pieces joined by one wavefront: stats[b] = (max, sum), row_loss[b] (0 where the row has no class).
+// A row's pieces joined by one wavefront: stats[b], row_loss[b] (0 where the row has no class).
 __global__ __launch_bounds__(256) void k_class_rows(int64_t B, int64_t V, int parts, const float2* __restrict__ part,
                                                     const float* __restrict__ picked,
                                                     const int64_t* __restrict__ labels,
                                                     const int64_t* __restrict__ idx, int64_t n_labels,
-                                                    float2* __restrict__ stats, float* __restrict__ row_loss) {
+                                                    RowStat* __restrict__ stats, float* __restrict__ row_loss) {
   const int lane = threadIdx.x & 63;
   const int64_t b = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (b >= B) return;
@@ -192,8 +203,10 @@ __global__ __launch_bounds__(256) void k_class_rows(int64_t B, int64_t V, int pa
     join_stats(m, s, om, os);
   }
   if (lane == 0) {
-    stats[b] = make_float2(m, s);
-    row_loss[b] = label_of(b, labels, idx, n_labels, V) >= 0 ? (m - picked[b]) + log2f(s) * kLn2 : 0.f;
+    const bool live = label_of(b, labels, idx, n_labels, V) >= 0;
+    const float zy = live ? picked[b] : 0.f;
+    stats[b] = RowStat{m, s, zy};
+    row_loss[b] = live ? (fmaf(-zy, kLog2e, m) + log2f(s)) * kLn2 : 0.f;
   }
 }
 
@@ -239,7 +252,7 @@ template <typename T>
 __global__ __launch_bounds__(kThreads) void k_class_dz(int64_t B, int64_t V, int Dp, Operand<T> x, Operand<T> w,
                                                        const int64_t* __restrict__ labels,
                                                        const int64_t* __restrict__ idx, int64_t n_labels,
-                                                       const float2* __restrict__ stats,
+                                                       const RowStat* __restrict__ stats,
                                                        const float* __restrict__ grad, float* __restrict__ rest,
                                                        int64_t v0, int tiles, T* __restrict__ dz, int64_t ldz) {
   __shared__ __align__(128) char lds[kProductLds];
@@ -256,12 +269,12 @@ __global__ __launch_bounds__(kThreads) void k_class_dz(int64_t B, int64_t V, int
     const int64_t b = b0 + wb + 32 * j + (lane & 31);
     const int64_t y = b < B ? label_of(b, labels, idx, n_labels, V) : -1;
     const float g = y >= 0 ? (grad ? grad[b] : 1.f) : 0.f;
-    const float2 st = b < B ? stats[b] : make_float2(0.f, 1.f);
-    const float scale = g / st.y;
+    const RowStat st = b < B ? stats[b] : RowStat{0.f, 1.f, 0.f};
+    const float scale = g / st.s;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = exp2_raw((acc[i][j][e] - st.x) * kLog2e) * scale;
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = exp2_raw(fmaf(acc[i][j][e], kLog2e, -st.r)) * scale;
     if (__any(y >= vw && y < vw + 64)) {
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -350,7 +363,8 @@ __global__ __launch_bounds__(kThreads) void k_class_product(Operand<T> A, Operan
 }
 
 // out[r][d] = factor * (sum over the shares, in order, + rest[r] * weight[y(r)][d]), out at r * sr +
-// d * sd; factor = grad[0] * share[0] or 1; `rest` (dx in bf16) may be NULL.  With `of` rows without
+// d * sd; factor = grad[0] * share[0] with `share`, grad[r] with `grad` alone, else 1; `rest` (dx in
+// bf16) may be NULL.  With `of` rows without
 // a class are 0 whatever the weight holds.
 template <typename T>
 __global__ __launch_bounds__(256) void k_class_join(int64_t R, int D, int splits, const float* __restrict__ in,
@@ -361,13 +375,14 @@ __global__ __launch_bounds__(256) void k_class_join(int64_t R, int D, int splits
   __shared__ float tile[32][33];
   const int64_t r0 = int64_t(blockIdx.x) * 32;
   const int d0 = blockIdx.y * 32, t = threadIdx.x;
-  const float factor = share ? grad[0] * share[0] : 1.f;
+  const float common = share ? grad[0] * share[0] : 1.f;
 #pragma unroll
   for (int i = t; i < 32 * 32; i += 256) {
     const int lr = i >> 5, ld = i & 31;
     const int64_t r = r0 + lr;
     float s = 0.f;
     if (r < R && d0 + ld < D) {
+      const float factor = grad && !share ? grad[r] : common;
       const float* src = in + r * ldi + d0 + ld;
 #pragma unroll 4
       for (int q = 0; q < splits; ++q) s += src[q * plane];
@@ -486,14 +501,8 @@ __global__ __launch_bounds__(kThreads) void k_few_stats(int B, int D, int Dk, in
       for (int e = 0; e < 16; ++e)
         if (v0 + block_row(e, lane) >= V) z[e] = -INFINITY;
     }
-    float top = m;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) top = fmaxf(z[e], top);
-    const float ref = top == -INFINITY ? 0.f : top;
-    s *= exp2_raw((m - ref) * kLog2e);
-#pragma unroll
-    for (int e = 0; e < 16; ++e) s += exp2_raw((z[e] - ref) * kLog2e);
-    m = top;
+    const f32x16 one[1] = {z};
+    accumulate(one, m, s);
   }
   const float om = __shfl_xor(m, 32), os = __shfl_xor(s, 32);
   join_stats(m, s, om, os);
@@ -512,7 +521,7 @@ __global__ __launch_bounds__(kThreads) void k_few_stats(int B, int D, int Dk, in
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_few_dz(int B, int rows, int D, int Dk, int64_t V,
                                                      const T* __restrict__ x, int64_t ldx, const T* __restrict__ w,
-                                                     int64_t sv, Labels of, const float2* __restrict__ stats,
+                                                     int64_t sv, Labels of, const RowStat* __restrict__ stats,
                                                      const float* __restrict__ grad, const float* __restrict__ share,
                                                      float* __restrict__ dz) {
   extern __shared__ __align__(128) char few_lds[];
@@ -520,15 +529,15 @@ __global__ __launch_bounds__(kThreads) void k_few_dz(int B, int rows, int D, int
   few_stage<T>(of, B, D, Dk, x, ldx, few_lds);
   const int b = lane & 31;
   const int64_t y = b < B ? label_of(b, of.labels, of.idx, of.n_labels, of.V) : -1;
-  const float2 st = y >= 0 ? stats[b] : make_float2(0.f, 1.f);
+  const RowStat st = y >= 0 ? stats[b] : RowStat{0.f, 1.f, 0.f};
   const float g = y >= 0 ? (share ? grad[0] * share[0] : grad[b]) : 0.f;
-  const float scale = g / st.y;
+  const float scale = g / st.s;
   for (int64_t v0 = (int64_t(blockIdx.x) * 4 + wave) * 32; v0 < V; v0 += int64_t(gridDim.x) * 128) {
     const f32x16 z = few_logits<T>(D, Dk, v0, V, w, sv, few_lds, lane);
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       const int64_t v = v0 + block_row(e, lane);
-      const float d = exp2_raw((z[e] - st.x) * kLog2e) * scale - (v == y ? g : 0.f);
+      const float d = exp2_raw(fmaf(z[e], kLog2e, -st.r)) * scale - (v == y ? g : 0.f);
       if (b < rows && v < V) dz[v * rows + b] = y >= 0 ? d : 0.f;
     }
   }
@@ -638,6 +647,310 @@ __global__ __launch_bounds__(kThreads) void k_few_join(int D, int rows, int spli
   }
 }
 
+// ------------------------------------------------------------------ bf16, up to 256 features
+// Both operands of the logits are rows of up to 16 x 16 features, so one of them can stay in
+// registers: a wavefront owns 64 rows of it (the matrix instruction's columns) and the other
+// operand streams through LDS, 64 rows at a time, one step ahead.  The logits of a step come out
+// with a lane per owned row; turned into probabilities they already are the right operand of the
+// second product, streamed^T . p, which reads the same LDS tile through the transposing load.  So
+// logits and probabilities never leave the registers:
+//   owner x, stream weight:  statistics;  dx^T = weight^T . p
+//   owner weight, stream x:  dweight^T = x^T . dz
+// The step's rows are permuted within LDS so that neither way of reading meets bank conflicts.
+constexpr int kOwnRows = 256;                    // of a workgroup: 64 a wavefront
+constexpr int kStreamRows = 64;                  // of a step
+
+template <int KD> constexpr int stream_bytes() { return kStreamRows * KD * 32; }
+
+// position of a row's 16-byte chunk: eight neighbouring rows use eight different chunks (direct
+// reads), four rows from a multiple of four on use four different pairs (transposing reads)
+__device__ __forceinline__ int stream_chunk(int row, int chunk) {
+  return chunk ^ (((row & 3) << 1) | ((row >> 2) & 1));
+}
+
+template <int KD>
+__device__ __forceinline__ void stage_stream(const Operand<Bf16>& op, int64_t r0, unsigned lds, int wave, int lane) {
+  constexpr int cpr = KD * 2;                    // chunks of a row
+#pragma unroll
+  for (int l = 0; l < stream_bytes<KD>() / 16 / kThreads; ++l) {
+    const int first = (l * 4 + wave) * 64, q = first + lane;
+    const int row = q / cpr, c = stream_chunk(row, q % cpr);
+    int64_t r = r0 + row;
+    r = r < op.rows ? r : op.rows - 1;
+    load_to_lds(op.base + r * op.ld + c * 8, lds + first * 16);
+  }
+}
+
+template <int KD>
+__device__ __forceinline__ void load_owned(const Operand<Bf16>& op, int64_t r0, int lane, bf16x8 (&own)[2][KD]) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    int64_t r = r0 + 32 * j + (lane & 31);
+    r = r < op.rows ? r : op.rows - 1;
+    const Bf16* src = op.base + r * op.ld + 8 * (lane >> 5);
+#pragma unroll
+    for (int k = 0; k < KD; ++k) own[j][k] = *reinterpret_cast<const bf16x8*>(src + 16 * k);
+  }
+}
+
+// logits of the step's rows 32 * sub .. + 31 (rows of the block) and the owned rows (columns)
+template <int KD>
+__device__ __forceinline__ void stream_logits(const char* tile, int sub, int lane, const bf16x8 (&own)[2][KD],
+                                              f32x16 (&z)[2]) {
+  const int row = 32 * sub + (lane & 31);
+  const char* at = tile + row * (KD * 32);
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) z[j][e] = 0.f;
+#pragma unroll
+  for (int k = 0; k < KD; ++k) {
+    const bf16x8 a = *reinterpret_cast<const bf16x8*>(at + (stream_chunk(row, 2 * k + (lane >> 5)) << 4));
+#pragma unroll
+    for (int j = 0; j < 2; ++j) z[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, own[j][k], z[j], 0, 0, 0);
+  }
+}
+
+// streamed^T as an operand: features 32 * block .. + 31, and of rows 32 * sub .. the sixteen that
+// elements 8 * q .. of a logits block hold (in that order)
+template <int KD>
+__device__ __forceinline__ bf16x8 stream_across(const char* tile, int sub, int q, int block, int lane) {
+  const int row = 32 * sub + 16 * q + 4 * (lane >> 5) + ((lane & 15) >> 2);
+  const int d = 32 * block + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (lds_s16x4*)(tile + row * (KD * 32) + (stream_chunk(row, d >> 3) << 4) + (d & 7) * 2));
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (lds_s16x4*)(tile + (row + 8) * (KD * 32) + (stream_chunk(row + 8, d >> 3) << 4) + (d & 7) * 2));
+  bf16x8 r;
+  __builtin_memcpy(&r, &lo, 8);
+  __builtin_memcpy(reinterpret_cast<char*>(&r) + 8, &hi, 8);
+  return r;
+}
+
+template <int KD>
+__global__ __launch_bounds__(kThreads) void k_wide_stats(int64_t B, int64_t V, Operand<Bf16> x, Operand<Bf16> w,
+                                                         Labels of, int64_t steps, int splits,
+                                                         float2* __restrict__ part, float* __restrict__ picked) {
+  __shared__ __align__(128) char lds[2 * stream_bytes<KD>()];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int split = blockIdx.x % splits;
+  const int64_t b0 = int64_t(blockIdx.x / splits) * kOwnRows + 64 * wave;
+  const int64_t t0 = steps * split / splits, t1 = steps * (split + 1) / splits;
+  bf16x8 own[2][KD];
+  load_owned<KD>(x, b0, lane, own);
+  float top[2], sum[2];
+  int64_t y[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int64_t b = b0 + 32 * j + (lane & 31);
+    top[j] = -INFINITY;
+    sum[j] = 0.f;
+    y[j] = b < B ? label_of(b, of.labels, of.idx, of.n_labels, of.V) : -1;
+  }
+  const unsigned stages = lds_offset(lds);
+  if (t0 < t1) stage_stream<KD>(w, t0 * kStreamRows, stages, wave, lane);
+  for (int64_t t = t0; t < t1; ++t) {
+    landed();
+    __syncthreads();
+    const int cur = int(t - t0) & 1;
+    if (t + 1 < t1) stage_stream<KD>(w, (t + 1) * kStreamRows, stages + (cur ^ 1) * stream_bytes<KD>(), wave, lane);
+    const char* tile = lds + cur * stream_bytes<KD>();
+    const int64_t v0 = t * kStreamRows;
+    f32x16 z[2][2];                              // [owned block][sub]
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub) {
+      f32x16 s[2];
+      stream_logits<KD>(tile, sub, lane, own, s);
+      z[0][sub] = s[0];
+      z[1][sub] = s[1];
+    }
+    if (__any((y[0] >= v0 && y[0] < v0 + kStreamRows) || (y[1] >= v0 && y[1] < v0 + kStreamRows))) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (v0 + 32 * sub + block_row(e, lane) == y[j]) picked[b0 + 32 * j + (lane & 31)] = z[j][sub][e];
+    }
+    if (v0 + kStreamRows > V) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (v0 + 32 * sub + block_row(e, lane) >= V) z[j][sub][e] = -INFINITY;
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) accumulate(z[j], top[j], sum[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const float om = __shfl_xor(top[j], 32), os = __shfl_xor(sum[j], 32);
+    join_stats(top[j], sum[j], om, os);
+    const int64_t b = b0 + 32 * j + (lane & 31);
+    if (lane < 32 && b < B) part[b * splits + split] = make_float2(top[j], sum[j]);
+  }
+}
+
+// What the gradients need of a row: p = 2^(z log2 e - shift) (shift = infinity without a class), its
+// factor, its label, and what the label's element of dz adds in dx beyond its rounded probability.
+struct RowConst {
+  float *shift, *factor, *rest;
+  int* label;
+};
+
+__global__ __launch_bounds__(256) void k_wide_rows(int64_t B, int64_t padded, Labels of,
+                                                   const RowStat* __restrict__ stats, const float* __restrict__ grad,
+                                                   const float* __restrict__ share, RowConst out) {
+  const int64_t b = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (b >= padded) return;
+  const int64_t y = b < B ? label_of(b, of.labels, of.idx, of.n_labels, of.V) : -1;
+  const RowStat st = y >= 0 ? stats[b] : RowStat{INFINITY, 1.f, 0.f};
+  const float shift = st.r + log2f(st.s);
+  const float p = exp2_raw(fmaf(st.picked, kLog2e, -shift));
+  out.shift[b] = shift;
+  out.factor[b] = y < 0 ? 0.f : share ? grad[0] * share[0] : grad[b];
+  out.rest[b] = (p - widen(Bf16{to_bf16(p)})) - 1.f;
+  out.label[b] = int(y);
+}
+
+// BY_CLASS: owner weight, stream x, dz^T with the label's -1; else owner x, stream weight, p alone
+// (what the label takes off joins dx in its last step).  PER_ROW: every row has a factor of its own
+// (in dweight here; dx takes it in its last step).  part[split][owned row][KD * 16] in 32 bits.
+template <int KD, bool BY_CLASS, bool PER_ROW>
+__global__ __launch_bounds__(kThreads, 1) void k_wide_grads(int64_t owners, int64_t streams, Operand<Bf16> owned,
+                                                            Operand<Bf16> streamed, RowConst rows, int64_t steps,
+                                                            int splits, float* __restrict__ part, int64_t plane) {
+  __shared__ __align__(128) char lds[2 * stream_bytes<KD>()];
+  __shared__ __align__(16) float row_shift[4][kStreamRows], row_factor[4][kStreamRows];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int split = blockIdx.x % splits;
+  const int64_t o0 = int64_t(blockIdx.x / splits) * kOwnRows + 64 * wave;
+  const int64_t t0 = steps * split / splits, t1 = steps * (split + 1) / splits;
+  bf16x8 own[2][KD];
+  load_owned<KD>(owned, o0, lane, own);
+  f32x16 acc[KD / 2][2];
+#pragma unroll
+  for (int d = 0; d < KD / 2; ++d)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[d][j][e] = 0.f;
+  float shift[2] = {0.f, 0.f};
+  if constexpr (!BY_CLASS) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int64_t b = o0 + 32 * j + (lane & 31);
+      shift[j] = rows.shift[b < owners ? b : owners - 1];
+    }
+  }
+  float next_shift = 0.f, next_factor = 0.f;     // of row `lane` of the coming step
+  int next_label = -1;
+  const auto fetch_rows = [&](int64_t t) {
+    next_shift = rows.shift[t * kStreamRows + lane];
+    if constexpr (PER_ROW) next_factor = rows.factor[t * kStreamRows + lane];
+    next_label = rows.label[t * kStreamRows + lane];
+  };
+  const unsigned stages = lds_offset(lds);
+  if (t0 < t1) {
+    stage_stream<KD>(streamed, t0 * kStreamRows, stages, wave, lane);
+    if constexpr (BY_CLASS) fetch_rows(t0);
+  }
+  for (int64_t t = t0; t < t1; ++t) {
+    landed();
+    __syncthreads();
+    const int cur = int(t - t0) & 1;
+    int label = -1;
+    if constexpr (BY_CLASS) {                    // a wavefront's own copy: no barrier
+      row_shift[wave][lane] = next_shift;
+      if constexpr (PER_ROW) row_factor[wave][lane] = next_factor;
+      label = next_label;
+      __builtin_amdgcn_wave_barrier();
+    }
+    if (t + 1 < t1) {
+      stage_stream<KD>(streamed, (t + 1) * kStreamRows, stages + (cur ^ 1) * stream_bytes<KD>(), wave, lane);
+      if constexpr (BY_CLASS) fetch_rows(t + 1);
+    }
+    const char* tile = lds + cur * stream_bytes<KD>();
+    uint64_t hits = 0;                           // rows of the step whose label is among the owned classes
+    if constexpr (BY_CLASS) hits = __ballot(label >= o0 && label < o0 + 64);
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub) {
+      f32x16 z[2];
+      stream_logits<KD>(tile, sub, lane, own, z);
+      if constexpr (BY_CLASS) {
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const f32x4 c = *reinterpret_cast<const f32x4*>(&row_shift[wave][32 * sub + block_row(e, lane)]);
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) z[j][e + q] = exp2_raw(fmaf(z[j][e + q], kLog2e, -c[q]));
+        }
+        for (uint64_t h = (hits >> (32 * sub)) & 0xffffffffull; h != 0; h &= h - 1) {        // rare
+          const int r = __builtin_ctzll(h);
+          const int at = int(__shfl(label, 32 * sub + r) - o0);
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (block_row(e, lane) == r && 32 * j + (lane & 31) == at) z[j][e] -= 1.f;
+        }
+        if constexpr (PER_ROW) {
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) {
+            const f32x4 g = *reinterpret_cast<const f32x4*>(&row_factor[wave][32 * sub + block_row(e, lane)]);
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+              for (int j = 0; j < 2; ++j) z[j][e + q] *= g[q];
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) z[j][e] = exp2_raw(fmaf(z[j][e], kLog2e, -shift[j]));
+        if ((t + 1) * kStreamRows > streams) {   // classes beyond the last
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (t * kStreamRows + 32 * sub + block_row(e, lane) >= streams) z[j][e] = 0.f;
+        }
+      }
+      bf16x8 p[2][2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) p[j][e >> 3][e & 7] = static_cast<__bf16>(z[j][e]);
+#pragma unroll
+      for (int d = 0; d < KD / 2; ++d)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const bf16x8 a = stream_across<KD>(tile, sub, q, d, lane);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) acc[d][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, p[j][q], acc[d][j], 0, 0, 0);
+        }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int64_t r = o0 + 32 * j + (lane & 31);
+    if (r >= owners) continue;
+    float* dst = part + split * plane + r * (KD * 16);
+#pragma unroll
+    for (int d = 0; d < KD / 2; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4)
+        *reinterpret_cast<f32x4*>(dst + 32 * d + block_row(e, lane)) =
+            f32x4{acc[d][j][e], acc[d][j][e + 1], acc[d][j][e + 2], acc[d][j][e + 3]};
+  }
+}
+
 // ------------------------------------------------------------------ plans
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
@@ -705,10 +1018,36 @@ Few make_few(int dtype, int64_t B, int64_t D, int64_t V, int64_t sd) {
   return f;
 }
 
+// The kernels that keep rows in registers: sizes, KD 0 where they do not apply.
+struct Wide {
+  int KD;
+  int64_t own_b, own_v, steps_b, steps_v;        // owners' workgroups and stream steps of either operand
+  int stat_splits, dx_splits, dw_splits;
+};
+
+Wide make_wide(int dtype, int64_t B, int64_t D, int64_t V) {
+  Wide f{};
+  if (dtype != SGNN_BF16 || D > 256) return f;
+  f.KD = int(ceil_div(D, 64) * 4);
+  f.own_b = ceil_div(B, kOwnRows);
+  f.own_v = ceil_div(V, kOwnRows);
+  f.steps_b = ceil_div(B, kStreamRows);
+  f.steps_v = ceil_div(V, kStreamRows);
+  const auto spread = [](int64_t want, int64_t groups, int64_t steps) {
+    const int64_t s = ceil_div(want, groups);
+    return int(s < steps ? s : steps);
+  };
+  f.stat_splits = spread(512, f.own_b, f.steps_v);
+  f.dx_splits = spread(256, f.own_b, f.steps_v);
+  f.dw_splits = spread(256, f.own_v, f.steps_b);
+  return f;
+}
+
 struct Buffers {
   char *x, *w, *dz;
   float2* part;
   float *picked, *rest, *dx, *dw;
+  RowConst rows;
   size_t bytes;
 };
 
@@ -726,6 +1065,25 @@ Buffers carve(const Plan& p, int64_t B, int64_t V, bool backward, void* base) {
     b.rest = c.take<float>(size_t(B));
     b.dx = c.take<float>(size_t(p.dx_splits) * p.Bp * Np);
     b.dw = c.take<float>(size_t(p.dw_splits) * p.piece * Np);
+  }
+  b.bytes = c.off;
+  return b;
+}
+
+Buffers carve_wide(const Wide& f, const Plan& p, int64_t B, int64_t V, bool backward, void* base) {
+  sgnn::Carver c(base);
+  Buffers b{};
+  b.x = c.take<char>(p.elem * B * p.Dp);
+  b.w = c.take<char>(p.elem * V * p.Dp);
+  if (!backward) {
+    b.part = c.take<float2>(size_t(f.stat_splits) * B);
+    b.picked = c.take<float>(size_t(B));
+  } else {
+    const size_t padded = size_t(f.steps_b) * kStreamRows;
+    b.rows = RowConst{c.take<float>(padded), c.take<float>(padded), c.take<float>(padded), c.take<int>(padded)};
+    // the two gradients' shares take turns
+    const size_t dx = size_t(f.dx_splits) * B, dw = size_t(f.dw_splits) * V;
+    b.dx = c.take<float>((dx > dw ? dx : dw) * p.Dp);
   }
   b.bytes = c.off;
   return b;
@@ -797,7 +1155,7 @@ int operands(const Call& c, const Plan& p, const Buffers& b, Operand<T>* x, Oper
   return SGNN_OK;
 }
 
-int finish_forward(const Call& c, int parts, const Buffers& b, float2* stats, float* row_loss, float* loss,
+int finish_forward(const Call& c, int parts, const Buffers& b, RowStat* stats, float* row_loss, float* loss,
                    float* share, hipStream_t st) {
   hipLaunchKernelGGL(k_class_rows, dim3(unsigned(ceil_div(c.B, 4))), dim3(256), 0, st, c.B, c.V, parts, b.part, b.picked,
                      c.labels, c.idx, c.n_labels, stats, row_loss);
@@ -817,7 +1175,7 @@ int allow_lds(const void* kernel, size_t bytes) {
 }
 
 template <typename T>
-int forward(const Call& c, const Plan& p, const Buffers& b, float2* stats, float* row_loss, float* loss,
+int forward(const Call& c, const Plan& p, const Buffers& b, RowStat* stats, float* row_loss, float* loss,
             float* share, hipStream_t st) {
   Operand<T> x, w;
   if (int rc = operands<T>(c, p, b, &x, &w, st)) return rc;
@@ -829,7 +1187,7 @@ int forward(const Call& c, const Plan& p, const Buffers& b, float2* stats, float
 }
 
 template <typename T>
-int backward(const Call& c, const Plan& p, const Buffers& b, const float2* stats, const float* grad,
+int backward(const Call& c, const Plan& p, const Buffers& b, const RowStat* stats, const float* grad,
              const float* share, void* dx, int64_t lddx, void* dw, int64_t dsv, int64_t dsd, hipStream_t st) {
   Operand<T> x, w;
   if (int rc = operands<T>(c, p, b, &x, &w, st)) return rc;
@@ -858,14 +1216,14 @@ int backward(const Call& c, const Plan& p, const Buffers& b, const float2* stats
       HIP_TRY(hipGetLastError());
       const int64_t rows = c.V - v0 < width ? c.V - v0 : width;
       hipLaunchKernelGGL((k_class_join<T>), dim3(unsigned(ceil_div(rows, 32)), unsigned(ceil_div(c.D, 32))), dim3(256), 0,
-                         st, rows, int(c.D), p.dw_splits, b.dw, p.piece * Np, Np, grad, share, nullptr, Labels{}, nullptr,
+                         st, rows, int(c.D), p.dw_splits, b.dw, p.piece * Np, Np, share ? grad : nullptr, share, nullptr, Labels{}, nullptr,
                          0, 0, static_cast<T*>(dw) + v0 * dsv, dsv, dsd);
       HIP_TRY(hipGetLastError());
     }
   }
   if (dx) {
     hipLaunchKernelGGL((k_class_join<T>), dim3(unsigned(ceil_div(c.B, 32)), unsigned(ceil_div(c.D, 32))), dim3(256), 0, st,
-                       c.B, int(c.D), p.dx_splits, b.dx, p.Bp * Np, Np, grad, share, sizeof(T) == 2 ? b.rest : nullptr,
+                       c.B, int(c.D), p.dx_splits, b.dx, p.Bp * Np, Np, share ? grad : nullptr, share, sizeof(T) == 2 ? b.rest : nullptr,
                        Labels{c.labels, c.idx, c.n_labels, c.V}, static_cast<const T*>(c.w), c.sv, c.sd,
                        static_cast<T*>(dx), lddx, int64_t(1));
     HIP_TRY(hipGetLastError());
@@ -873,8 +1231,67 @@ int backward(const Call& c, const Plan& p, const Buffers& b, const float2* stats
   return SGNN_OK;
 }
 
+#define SGNN_WIDE(KDS, CALL)                 \
+  switch (KDS) {                             \
+    case 4: { constexpr int KD = 4; CALL; } break;   \
+    case 8: { constexpr int KD = 8; CALL; } break;   \
+    case 12: { constexpr int KD = 12; CALL; } break; \
+    default: { constexpr int KD = 16; CALL; } break; \
+  }
+
+int wide_forward(const Call& c, const Wide& f, const Plan& p, const Buffers& b, RowStat* stats, float* row_loss,
+                 float* loss, float* share, hipStream_t st) {
+  Operand<Bf16> x, w;
+  if (int rc = operands<Bf16>(c, p, b, &x, &w, st)) return rc;
+  const Labels of{c.labels, c.idx, c.n_labels, c.V};
+  SGNN_WIDE(f.KD, hipLaunchKernelGGL((k_wide_stats<KD>), dim3(unsigned(f.own_b * f.stat_splits)), dim3(kThreads), 0, st,
+                                     c.B, c.V, x, w, of, f.steps_v, f.stat_splits, b.part, b.picked));
+  HIP_TRY(hipGetLastError());
+  return finish_forward(c, f.stat_splits, b, stats, row_loss, loss, share, st);
+}
+
+int wide_backward(const Call& c, const Wide& f, const Plan& p, const Buffers& b, const RowStat* stats,
+                  const float* grad, const float* share, void* dx, int64_t lddx, void* dw, int64_t dsv, int64_t dsd,
+                  hipStream_t st) {
+  Operand<Bf16> x, w;
+  if (int rc = operands<Bf16>(c, p, b, &x, &w, st)) return rc;
+  const Labels of{c.labels, c.idx, c.n_labels, c.V};
+  const int64_t padded = f.steps_b * kStreamRows;
+  hipLaunchKernelGGL(k_wide_rows, dim3(unsigned(ceil_div(padded, 256))), dim3(256), 0, st, c.B, padded, of, stats, grad,
+                     share, b.rows);
+  HIP_TRY(hipGetLastError());
+  if (dx) {
+    SGNN_WIDE(f.KD, hipLaunchKernelGGL((k_wide_grads<KD, false, false>), dim3(unsigned(f.own_b * f.dx_splits)),
+                                       dim3(kThreads), 0, st, c.B, c.V, x, w, b.rows, f.steps_v, f.dx_splits, b.dx,
+                                       c.B * p.Dp));
+    HIP_TRY(hipGetLastError());
+    hipLaunchKernelGGL((k_class_join<Bf16>), dim3(unsigned(ceil_div(c.B, 32)), unsigned(ceil_div(c.D, 32))), dim3(256), 0,
+                       st, c.B, int(c.D), f.dx_splits, b.dx, c.B * p.Dp, int64_t(p.Dp), b.rows.factor, nullptr,
+                       b.rows.rest, of, static_cast<const Bf16*>(c.w), c.sv, c.sd, static_cast<Bf16*>(dx), lddx,
+                       int64_t(1));
+    HIP_TRY(hipGetLastError());
+  }
+  if (dw) {
+    if (share) {
+      SGNN_WIDE(f.KD, hipLaunchKernelGGL((k_wide_grads<KD, true, false>), dim3(unsigned(f.own_v * f.dw_splits)),
+                                         dim3(kThreads), 0, st, c.V, c.B, w, x, b.rows, f.steps_b, f.dw_splits, b.dx,
+                                         c.V * p.Dp));
+    } else {
+      SGNN_WIDE(f.KD, hipLaunchKernelGGL((k_wide_grads<KD, true, true>), dim3(unsigned(f.own_v * f.dw_splits)),
+                                         dim3(kThreads), 0, st, c.V, c.B, w, x, b.rows, f.steps_b, f.dw_splits, b.dx,
+                                         c.V * p.Dp));
+    }
+    HIP_TRY(hipGetLastError());
+    hipLaunchKernelGGL((k_class_join<Bf16>), dim3(unsigned(ceil_div(c.V, 32)), unsigned(ceil_div(c.D, 32))), dim3(256), 0,
+                       st, c.V, int(c.D), f.dw_splits, b.dx, c.V * p.Dp, int64_t(p.Dp), share ? grad : nullptr, share,
+                       nullptr, Labels{}, nullptr, 0, 0, static_cast<Bf16*>(dw), dsv, dsd);
+    HIP_TRY(hipGetLastError());
+  }
+  return SGNN_OK;
+}
+
 template <typename T>
-int few_forward(const Call& c, const Few& f, const Buffers& b, float2* stats, float* row_loss, float* loss,
+int few_forward(const Call& c, const Few& f, const Buffers& b, RowStat* stats, float* row_loss, float* loss,
                 float* share, hipStream_t st) {
   const Labels of{c.labels, c.idx, c.n_labels, c.V};
   if (int rc = allow_lds(reinterpret_cast<const void*>(&k_few_stats<T>), f.lds)) return rc;
@@ -885,7 +1302,7 @@ int few_forward(const Call& c, const Few& f, const Buffers& b, float2* stats, fl
 }
 
 template <typename T>
-int few_backward(const Call& c, const Few& f, const Buffers& b, const float2* stats, const float* grad,
+int few_backward(const Call& c, const Few& f, const Buffers& b, const RowStat* stats, const float* grad,
                  const float* share, void* dx, int64_t lddx, void* dw, int64_t dsv, int64_t dsd, hipStream_t st) {
   const Labels of{c.labels, c.idx, c.n_labels, c.V};
   const T* x = static_cast<const T*>(c.x);
@@ -922,7 +1339,9 @@ extern "C" size_t sgnn_class_xent_workspace_bytes(int dtype, int64_t B, int64_t 
   const size_t whole = carve(make_plan(dtype, B, D, V), B, V, backward != 0, nullptr).bytes;
   const Few f = make_few(dtype, B, D, V, 1);
   const size_t few = f.rows ? carve_few(f, B, D, V, backward != 0, nullptr).bytes : 0;
-  return whole > few ? whole : few;
+  const Wide wd = make_wide(dtype, B, D, V);
+  const size_t plain = wd.KD ? carve_wide(wd, make_plan(dtype, B, D, V), B, V, backward != 0, nullptr).bytes : whole;
+  return plain > few ? plain : few;
 }
 
 extern "C" int sgnn_class_xent_forward(int dtype, int64_t B, int64_t D, int64_t V, const void* x, int64_t ldx,
@@ -937,13 +1356,15 @@ extern "C" int sgnn_class_xent_forward(int dtype, int64_t B, int64_t D, int64_t 
   if (workspace_bytes < sgnn_class_xent_workspace_bytes(dtype, B, D, V, 0))
     return fail(SGNN_ERR_WORKSPACE, "class-loss workspace too small");
   hipStream_t st = static_cast<hipStream_t>(stream);
-  float2* s = reinterpret_cast<float2*>(stats);
+  RowStat* s = reinterpret_cast<RowStat*>(stats);
   if (const Few f = make_few(dtype, B, D, V, sd); f.rows) {
     const Buffers b = carve_few(f, B, D, V, false, workspace);
     if (dtype == SGNN_F32) return few_forward<float>(c, f, b, s, row_loss, loss, share, st);
     return few_forward<Bf16>(c, f, b, s, row_loss, loss, share, st);
   }
   const Plan p = make_plan(dtype, B, D, V);
+  if (const Wide f = make_wide(dtype, B, D, V); f.KD)
+    return wide_forward(c, f, p, carve_wide(f, p, B, V, false, workspace), s, row_loss, loss, share, st);
   const Buffers b = carve(p, B, V, false, workspace);
   if (dtype == SGNN_F32) return forward<float>(c, p, b, s, row_loss, loss, share, st);
   return forward<Bf16>(c, p, b, s, row_loss, loss, share, st);
@@ -965,13 +1386,15 @@ extern "C" int sgnn_class_xent_backward(int dtype, int64_t B, int64_t D, int64_t
   if (workspace_bytes < sgnn_class_xent_workspace_bytes(dtype, B, D, V, 1))
     return fail(SGNN_ERR_WORKSPACE, "class-loss workspace too small");
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const float2* s = reinterpret_cast<const float2*>(stats);
+  const RowStat* s = reinterpret_cast<const RowStat*>(stats);
   if (const Few f = make_few(dtype, B, D, V, sd); f.rows) {
     const Buffers b = carve_few(f, B, D, V, true, workspace);
     if (dtype == SGNN_F32) return few_backward<float>(c, f, b, s, grad, share, dx, lddx, dweight, dsv, dsd, st);
     return few_backward<Bf16>(c, f, b, s, grad, share, dx, lddx, dweight, dsv, dsd, st);
   }
   const Plan p = make_plan(dtype, B, D, V);
+  if (const Wide f = make_wide(dtype, B, D, V); f.KD)
+    return wide_backward(c, f, p, carve_wide(f, p, B, V, true, workspace), s, grad, share, dx, lddx, dweight, dsv, dsd, st);
   const Buffers b = carve(p, B, V, true, workspace);
   if (dtype == SGNN_F32) return backward<float>(c, p, b, s, grad, share, dx, lddx, dweight, dsv, dsd, st);
   return backward<Bf16>(c, p, b, s, grad, share, dx, lddx, dweight, dsv, dsd, st);

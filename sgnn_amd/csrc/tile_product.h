@@ -21,9 +21,10 @@ struct Bf16 { uint16_t bits; };
 __device__ __forceinline__ float widen(float v) { return v; }
 __device__ __forceinline__ float widen(Bf16 v) { return __uint_as_float(unsigned(v.bits) << 16); }
 __device__ __forceinline__ uint16_t to_bf16(float v) {                       // nearest even
-  const unsigned u = __float_as_uint(v);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return 0x7fc0u;
-  return uint16_t((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+  const __bf16 h = static_cast<__bf16>(v);
+  uint16_t bits;
+  __builtin_memcpy(&bits, &h, 2);
+  return bits;
 }
 template <typename T> __device__ __forceinline__ T narrow(float v);
 template <> __device__ __forceinline__ float narrow<float>(float v) { return v; }
