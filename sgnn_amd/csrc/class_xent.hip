@@ -693,19 +693,36 @@ __device__ __forceinline__ void load_owned(const Operand<Bf16>& op, int64_t r0, 
   }
 }
 
+// Where a lane reads: the permutation touches the low three bits of a chunk's number only and
+// depends on the lane alone, so everything else is a constant offset of the read.
+struct StreamLane {
+  int direct[4];           // logits: row lane & 31, chunks 0 .. 7 of it two by two
+  int across[2];           // second product: its row of the first four (second half: of the next), 64 features
+};
+template <int KD>
+__device__ __forceinline__ StreamLane stream_lane(int lane) {
+  StreamLane at;
+  const int row = lane & 31, half = lane >> 5;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) at.direct[i] = row * (KD * 32) + (stream_chunk(row, 2 * i + half) << 4);
+  const int r = 4 * half + ((lane & 15) >> 2), c = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) at.across[i] = r * (KD * 32) + (stream_chunk(r, 4 * i + c) << 4) + (lane & 1) * 8;
+  return at;
+}
+
 // logits of the step's rows 32 * sub .. + 31 (rows of the block) and the owned rows (columns)
 template <int KD>
-__device__ __forceinline__ void stream_logits(const char* tile, int sub, int lane, const bf16x8 (&own)[2][KD],
-                                              f32x16 (&z)[2]) {
-  const int row = 32 * sub + (lane & 31);
-  const char* at = tile + row * (KD * 32);
+__device__ __forceinline__ void stream_logits(const char* tile, int sub, const StreamLane& at,
+                                              const bf16x8 (&own)[2][KD], f32x16 (&z)[2]) {
 #pragma unroll
   for (int j = 0; j < 2; ++j)
 #pragma unroll
     for (int e = 0; e < 16; ++e) z[j][e] = 0.f;
 #pragma unroll
   for (int k = 0; k < KD; ++k) {
-    const bf16x8 a = *reinterpret_cast<const bf16x8*>(at + (stream_chunk(row, 2 * k + (lane >> 5)) << 4));
+    const bf16x8 a =
+        *reinterpret_cast<const bf16x8*>(tile + at.direct[k & 3] + (32 * sub * KD * 32 + (k >> 2) * 128));
 #pragma unroll
     for (int j = 0; j < 2; ++j) z[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, own[j][k], z[j], 0, 0, 0);
   }
@@ -714,14 +731,11 @@ __device__ __forceinline__ void stream_logits(const char* tile, int sub, int lan
 // streamed^T as an operand: features 32 * block .. + 31, and of rows 32 * sub .. the sixteen that
 // elements 8 * q .. of a logits block hold (in that order)
 template <int KD>
-__device__ __forceinline__ bf16x8 stream_across(const char* tile, int sub, int q, int block, int lane) {
-  const int row = 32 * sub + 16 * q + 4 * (lane >> 5) + ((lane & 15) >> 2);
-  const int d = 32 * block + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+__device__ __forceinline__ bf16x8 stream_across(const char* tile, int sub, int q, int block, const StreamLane& at) {
   typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-      (lds_s16x4*)(tile + row * (KD * 32) + (stream_chunk(row, d >> 3) << 4) + (d & 7) * 2));
-  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-      (lds_s16x4*)(tile + (row + 8) * (KD * 32) + (stream_chunk(row + 8, d >> 3) << 4) + (d & 7) * 2));
+  const char* src = tile + at.across[block & 1] + ((32 * sub + 16 * q) * KD * 32 + (block >> 1) * 128);
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)src);
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(src + 8 * KD * 32));
   bf16x8 r;
   __builtin_memcpy(&r, &lo, 8);
   __builtin_memcpy(reinterpret_cast<char*>(&r) + 8, &hi, 8);
@@ -737,6 +751,7 @@ __global__ __launch_bounds__(kThreads) void k_wide_stats(int64_t B, int64_t V, O
   const int split = blockIdx.x % splits;
   const int64_t b0 = int64_t(blockIdx.x / splits) * kOwnRows + 64 * wave;
   const int64_t t0 = steps * split / splits, t1 = steps * (split + 1) / splits;
+  const StreamLane at = stream_lane<KD>(lane);
   bf16x8 own[2][KD];
   load_owned<KD>(x, b0, lane, own);
   float top[2], sum[2];
@@ -761,7 +776,7 @@ __global__ __launch_bounds__(kThreads) void k_wide_stats(int64_t B, int64_t V, O
 #pragma unroll
     for (int sub = 0; sub < 2; ++sub) {
       f32x16 s[2];
-      stream_logits<KD>(tile, sub, lane, own, s);
+      stream_logits<KD>(tile, sub, at, own, s);
       z[0][sub] = s[0];
       z[1][sub] = s[1];
     }
@@ -830,6 +845,7 @@ __global__ __launch_bounds__(kThreads, 1) void k_wide_grads(int64_t owners, int6
   const int split = blockIdx.x % splits;
   const int64_t o0 = int64_t(blockIdx.x / splits) * kOwnRows + 64 * wave;
   const int64_t t0 = steps * split / splits, t1 = steps * (split + 1) / splits;
+  const StreamLane at = stream_lane<KD>(lane);
   bf16x8 own[2][KD];
   load_owned<KD>(owned, o0, lane, own);
   f32x16 acc[KD / 2][2];
@@ -877,10 +893,10 @@ __global__ __launch_bounds__(kThreads, 1) void k_wide_grads(int64_t owners, int6
     const char* tile = lds + cur * stream_bytes<KD>();
     uint64_t hits = 0;                           // rows of the step whose label is among the owned classes
     if constexpr (BY_CLASS) hits = __ballot(label >= o0 && label < o0 + 64);
-#pragma unroll
+#pragma unroll(KD > 8 ? 1 : 2)                   // two at a time would not fit the registers
     for (int sub = 0; sub < 2; ++sub) {
       f32x16 z[2];
-      stream_logits<KD>(tile, sub, lane, own, z);
+      stream_logits<KD>(tile, sub, at, own, z);
       if constexpr (BY_CLASS) {
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
@@ -892,12 +908,12 @@ __global__ __launch_bounds__(kThreads, 1) void k_wide_grads(int64_t owners, int6
         }
         for (uint64_t h = (hits >> (32 * sub)) & 0xffffffffull; h != 0; h &= h - 1) {        // rare
           const int r = __builtin_ctzll(h);
-          const int at = int(__shfl(label, 32 * sub + r) - o0);
+          const int col = int(__shfl(label, 32 * sub + r) - o0);
 #pragma unroll
           for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e)
-              if (block_row(e, lane) == r && 32 * j + (lane & 31) == at) z[j][e] -= 1.f;
+              if (block_row(e, lane) == r && 32 * j + (lane & 31) == col) z[j][e] -= 1.f;
         }
         if constexpr (PER_ROW) {
 #pragma unroll
@@ -931,7 +947,7 @@ __global__ __launch_bounds__(kThreads, 1) void k_wide_grads(int64_t owners, int6
       for (int d = 0; d < KD / 2; ++d)
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          const bf16x8 a = stream_across<KD>(tile, sub, q, d, lane);
+          const bf16x8 a = stream_across<KD>(tile, sub, q, d, at);
 #pragma unroll
           for (int j = 0; j < 2; ++j) acc[d][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, p[j][q], acc[d][j], 0, 0, 0);
         }
