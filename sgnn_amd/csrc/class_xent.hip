@@ -662,11 +662,13 @@ constexpr int kStreamRows = 64;                  // of a step
 
 template <int KD> constexpr int stream_bytes() { return kStreamRows * KD * 32; }
 
-// position of a row's 16-byte chunk: eight neighbouring rows use eight different chunks (direct
-// reads), four rows from a multiple of four on use four different pairs (transposing reads)
-__device__ __forceinline__ int stream_chunk(int row, int chunk) {
-  return chunk ^ (((row & 3) << 1) | ((row >> 2) & 1));
+// position of a row's 16-byte chunk; only the low bits of its number change, and how depends on
+// the row alone
+template <int KD>
+__device__ __forceinline__ int stream_spread(int row) {
+  return KD % 8 == 0 ? spread_256(row) : spread_128(row);
 }
+template <int KD> constexpr int stream_window() { return KD % 8 == 0 ? 256 : 128; }        // bytes it permutes
 
 template <int KD>
 __device__ __forceinline__ void stage_stream(const Operand<Bf16>& op, int64_t r0, unsigned lds, int wave, int lane) {
@@ -674,10 +676,9 @@ __device__ __forceinline__ void stage_stream(const Operand<Bf16>& op, int64_t r0
 #pragma unroll
   for (int l = 0; l < stream_bytes<KD>() / 16 / kThreads; ++l) {
     const int first = (l * 4 + wave) * 64, q = first + lane;
-    const int row = q / cpr, c = stream_chunk(row, q % cpr);
-    int64_t r = r0 + row;
-    r = r < op.rows ? r : op.rows - 1;
-    load_to_lds(op.base + r * op.ld + c * 8, lds + first * 16);
+    const int row = q / cpr, c = (q % cpr) ^ stream_spread<KD>(row);
+    const unsigned r = unsigned(r0) + row, last = unsigned(op.rows) - 1;   // at most 2^30 rows
+    load_to_lds(op.base + uint64_t(r < last ? r : last) * unsigned(op.ld) + c * 8, lds + first * 16);
   }
 }
 
@@ -693,22 +694,24 @@ __device__ __forceinline__ void load_owned(const Operand<Bf16>& op, int64_t r0, 
   }
 }
 
-// Where a lane reads: the permutation touches the low three bits of a chunk's number only and
-// depends on the lane alone, so everything else is a constant offset of the read.
+// Where a lane reads.  Rows are aligned to the permuted windows, so another chunk of the same window
+// is an exclusive-or away and everything else a constant offset of the read.
 struct StreamLane {
-  int direct[4];           // logits: row lane & 31, chunks 0 .. 7 of it two by two
-  int across[2];           // second product: its row of the first four (second half: of the next), 64 features
+  int direct;              // logits: row lane & 31, chunk lane / 32
+  int across;              // second product: its row of the first four (second half: of the next), first 64 features
 };
 template <int KD>
 __device__ __forceinline__ StreamLane stream_lane(int lane) {
-  StreamLane at;
   const int row = lane & 31, half = lane >> 5;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) at.direct[i] = row * (KD * 32) + (stream_chunk(row, 2 * i + half) << 4);
   const int r = 4 * half + ((lane & 15) >> 2), c = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) at.across[i] = r * (KD * 32) + (stream_chunk(r, 4 * i + c) << 4) + (lane & 1) * 8;
-  return at;
+  return {row * (KD * 32) + ((half ^ stream_spread<KD>(row)) << 4),
+          r * (KD * 32) + ((c ^ stream_spread<KD>(r)) << 4) + (lane & 1) * 8};
+}
+template <int KD>
+__device__ __forceinline__ bf16x8 stream_row(const char* tile, int sub, int k, const StreamLane& at) {
+  constexpr int kWindow = stream_window<KD>();
+  const int place = (at.direct ^ ((32 * k) % kWindow)) + (32 * sub * KD * 32 + 32 * k / kWindow * kWindow);
+  return *reinterpret_cast<const bf16x8*>(tile + place);
 }
 
 // logits of the step's rows 32 * sub .. + 31 (rows of the block) and the owned rows (columns)
@@ -721,8 +724,7 @@ __device__ __forceinline__ void stream_logits(const char* tile, int sub, const S
     for (int e = 0; e < 16; ++e) z[j][e] = 0.f;
 #pragma unroll
   for (int k = 0; k < KD; ++k) {
-    const bf16x8 a =
-        *reinterpret_cast<const bf16x8*>(tile + at.direct[k & 3] + (32 * sub * KD * 32 + (k >> 2) * 128));
+    const bf16x8 a = stream_row<KD>(tile, sub, k, at);
 #pragma unroll
     for (int j = 0; j < 2; ++j) z[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, own[j][k], z[j], 0, 0, 0);
   }
@@ -733,13 +735,42 @@ __device__ __forceinline__ void stream_logits(const char* tile, int sub, const S
 template <int KD>
 __device__ __forceinline__ bf16x8 stream_across(const char* tile, int sub, int q, int block, const StreamLane& at) {
   typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-  const char* src = tile + at.across[block & 1] + ((32 * sub + 16 * q) * KD * 32 + (block >> 1) * 128);
-  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)src);
-  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(src + 8 * KD * 32));
+  constexpr int kWindow = stream_window<KD>();
+  const int place = at.across ^ ((64 * block) % kWindow);
+  const char* src = tile + ((32 * sub + 16 * q) * KD * 32 + 64 * block / kWindow * kWindow);
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(src + place));
+  // eight rows on the permutation differs by two chunks
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(src + (place ^ 32) + 8 * KD * 32));
   bf16x8 r;
   __builtin_memcpy(&r, &lo, 8);
   __builtin_memcpy(reinterpret_cast<char*>(&r) + 8, &hi, 8);
   return r;
+}
+
+// stream_logits with other work between its matrix instructions: between(i) is called for
+// i = 0 .. 31, a few after each of them, and stays there.  The matrix unit works on while the
+// vector unit does; left to itself the compiler puts one after the other.
+template <int KD, typename Between>
+__device__ __forceinline__ void stream_logits_between(const char* tile, int sub, const StreamLane& at,
+                                                      const bf16x8 (&own)[2][KD], f32x16 (&z)[2], Between&& between) {
+  const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  constexpr int kAhead = KD < 16 ? 3 : 2;        // reads under way
+  bf16x8 a[kAhead];
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k) a[k] = stream_row<KD>(tile, sub, k, at);
+#pragma unroll
+  for (int k = 0; k < KD; ++k) {
+    const bf16x8 cur = a[k % kAhead];
+    if (k + kAhead < KD) a[k % kAhead] = stream_row<KD>(tile, sub, k + kAhead, at);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      z[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(cur, own[j][k], k ? z[j] : zero, 0, 0, 0);
+      const int step = 2 * k + j;
+#pragma unroll
+      for (int i = 32 * step / (2 * KD); i < 32 * (step + 1) / (2 * KD); ++i) between(i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
 }
 
 template <int KD>
@@ -755,51 +786,79 @@ __global__ __launch_bounds__(kThreads) void k_wide_stats(int64_t B, int64_t V, O
   bf16x8 own[2][KD];
   load_owned<KD>(x, b0, lane, own);
   float top[2], sum[2];
-  int64_t y[2];
+  int y[2];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const int64_t b = b0 + 32 * j + (lane & 31);
     top[j] = -INFINITY;
     sum[j] = 0.f;
-    y[j] = b < B ? label_of(b, of.labels, of.idx, of.n_labels, of.V) : -1;
+    y[j] = b < B ? int(label_of(b, of.labels, of.idx, of.n_labels, of.V)) : -1;
   }
+  // the label's logit and the classes beyond the last, both rare
+  const auto settle = [&](f32x16 (&z)[2], int64_t v0) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int at = y[j] - int(v0);
+      int mine = at - 4 * (lane >> 5);           // compared with constants
+      asm("" : "+v"(mine));                      // and not taken apart into sixteen registers
+      if (__any(at >= 0 && at < 32)) {
+        float hit = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) hit = block_row(e, 0) == mine ? z[j][e] : hit;
+        if (at >= 0 && at < 32 && ((at >> 2) & 1) == lane >> 5) picked[b0 + 32 * j + (lane & 31)] = hit;
+      }
+    }
+    if (v0 + 32 > V) {
+      int left = int(V - v0) - 4 * (lane >> 5);
+      asm("" : "+v"(left));
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) z[j][e] = block_row(e, 0) < left ? z[j][e] : -INFINITY;
+    }
+  };
+  // the logits of one half step while the other's are summed
+  const auto turn = [&](const char* tile, int sub, f32x16 (&next)[2], const f32x16 (&z)[2]) {
+    float ref[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float m = z[j][0];
+#pragma unroll
+      for (int e = 1; e < 15; e += 2) m = fmaxf(fmaxf(z[j][e], z[j][e + 1]), m);
+      m = fmaxf(fmaxf(m, z[j][15]) * kLog2e, top[j]);
+      ref[j] = m == -INFINITY ? 0.f : m;
+      sum[j] *= exp2_raw(top[j] - ref[j]);
+      top[j] = m;
+    }
+    stream_logits_between<KD>(tile, sub, at, own, next, [&](int i) {
+      sum[i >> 4] += exp2_raw(fmaf(z[i >> 4][i & 15], kLog2e, -ref[i >> 4]));
+      asm volatile("" : "+v"(sum[i >> 4]));      // now, not where the sum is used
+    });
+  };
   const unsigned stages = lds_offset(lds);
-  if (t0 < t1) stage_stream<KD>(w, t0 * kStreamRows, stages, wave, lane);
-  for (int64_t t = t0; t < t1; ++t) {
-    landed();
-    __syncthreads();
-    const int cur = int(t - t0) & 1;
-    if (t + 1 < t1) stage_stream<KD>(w, (t + 1) * kStreamRows, stages + (cur ^ 1) * stream_bytes<KD>(), wave, lane);
-    const char* tile = lds + cur * stream_bytes<KD>();
-    const int64_t v0 = t * kStreamRows;
-    f32x16 z[2][2];                              // [owned block][sub]
+  if (t0 < t1) {
+    stage_stream<KD>(w, t0 * kStreamRows, stages, wave, lane);
+    f32x16 first[2], second[2];
 #pragma unroll
-    for (int sub = 0; sub < 2; ++sub) {
-      f32x16 s[2];
-      stream_logits<KD>(tile, sub, at, own, s);
-      z[0][sub] = s[0];
-      z[1][sub] = s[1];
-    }
-    if (__any((y[0] >= v0 && y[0] < v0 + kStreamRows) || (y[1] >= v0 && y[1] < v0 + kStreamRows))) {
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (v0 + 32 * sub + block_row(e, lane) == y[j]) picked[b0 + 32 * j + (lane & 31)] = z[j][sub][e];
-    }
-    if (v0 + kStreamRows > V) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (v0 + 32 * sub + block_row(e, lane) >= V) z[j][sub][e] = -INFINITY;
+      for (int e = 0; e < 16; ++e) second[j][e] = -INFINITY;               // adds nothing
+    for (int64_t t = t0; t < t1; ++t) {
+      landed();
+      __syncthreads();
+      const int cur = int(t - t0) & 1;
+      if (t + 1 < t1) stage_stream<KD>(w, (t + 1) * kStreamRows, stages + (cur ^ 1) * stream_bytes<KD>(), wave, lane);
+      const char* tile = lds + cur * stream_bytes<KD>();
+      turn(tile, 0, first, second);
+      settle(first, t * kStreamRows);
+      turn(tile, 1, second, first);
+      settle(second, t * kStreamRows + 32);
     }
 #pragma unroll
-    for (int j = 0; j < 2; ++j) accumulate(z[j], top[j], sum[j]);
+    for (int j = 0; j < 2; ++j) {
+      const f32x16 one[1] = {second[j]};
+      accumulate(one, top[j], sum[j]);
+    }
   }
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
@@ -893,7 +952,7 @@ __global__ __launch_bounds__(kThreads, 1) void k_wide_grads(int64_t owners, int6
     const char* tile = lds + cur * stream_bytes<KD>();
     uint64_t hits = 0;                           // rows of the step whose label is among the owned classes
     if constexpr (BY_CLASS) hits = __ballot(label >= o0 && label < o0 + 64);
-#pragma unroll(KD > 8 ? 1 : 2)                   // two at a time would not fit the registers
+#pragma unroll KD > 8 ? 1 : 2                    // two at a time would not fit the registers
     for (int sub = 0; sub < 2; ++sub) {
       f32x16 z[2];
       stream_logits<KD>(tile, sub, at, own, z);

@@ -109,6 +109,14 @@ __device__ __forceinline__ unsigned lds_offset(const char* p) {
   return unsigned(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) char*)p));
 }
 
+// A 16-byte LDS read is served sixteen lanes at a time, not all of them neighbours (0-3, 12-15,
+// 20-23, 24-27, and so on); its chunks have to lie in sixteen different places of 256 bytes.
+// Rows of 128 bytes alternate between the halves; this moves the chunks of the others apart, and
+// the four rows that a transposing read touches together to different 64-byte blocks.
+__device__ __forceinline__ int spread_128(int row) { return ((row & 2) << 1) | ((row >> 2) & 3); }
+// the same for rows of 256 bytes (or a multiple): sixteen chunks
+__device__ __forceinline__ int spread_256(int row) { return ((row & 3) << 2) | ((row >> 2) & 3); }
+
 // deep: rows r0 .. r0 + 127 at reduction offset k0;  flat: reduction rows k0 .. at columns r0 ..
 template <typename T, bool DEEP>
 __device__ __forceinline__ void stage_operand(const Operand<T>& op, int64_t r0, int64_t k0, unsigned lds, int wave,
@@ -119,7 +127,7 @@ __device__ __forceinline__ void stage_operand(const Operand<T>& op, int64_t r0, 
     const int first = (l * 4 + wave) * 64, q = first + lane;
     const T* src;
     if constexpr (DEEP) {
-      const int row = q >> 3, c = (q & 7) ^ (row & 7);
+      const int row = q >> 3, c = (q & 7) ^ spread_128(row);
       int64_t r = r0 + row;
       r = r < op.rows ? r : op.rows - 1;
       src = op.base + r * op.ld + k0 + c * V;
@@ -146,12 +154,12 @@ __device__ __forceinline__ void fragment(const char* lds, int m0, int k0, int la
     const char* at = lds + row * 128;
     if constexpr (sizeof(T) == 2) {
       const int c = (k0 >> 3) + (lane >> 5);
-      out[0] = *reinterpret_cast<const bf16x8*>(at + ((c ^ (row & 7)) << 4));
+      out[0] = *reinterpret_cast<const bf16x8*>(at + ((c ^ spread_128(row)) << 4));
     } else {
       const int c = (k0 >> 2) + 2 * (lane >> 5);
       float v[8];
-      *reinterpret_cast<f32x4*>(&v[0]) = *reinterpret_cast<const f32x4*>(at + ((c ^ (row & 7)) << 4));
-      *reinterpret_cast<f32x4*>(&v[4]) = *reinterpret_cast<const f32x4*>(at + (((c + 1) ^ (row & 7)) << 4));
+      *reinterpret_cast<f32x4*>(&v[0]) = *reinterpret_cast<const f32x4*>(at + ((c ^ spread_128(row)) << 4));
+      *reinterpret_cast<f32x4*>(&v[4]) = *reinterpret_cast<const f32x4*>(at + (((c + 1) ^ spread_128(row)) << 4));
       planes_of(v, out);
     }
   } else if constexpr (sizeof(T) == 2) {
