@@ -649,7 +649,7 @@ __global__ __launch_bounds__(kThreads) void k_few_join(int D, int rows, int spli
 
 // ------------------------------------------------------------------ bf16, up to 256 features
 // Both operands of the logits are rows of up to 16 x 16 features, so one of them can stay in
-// registers: a wavefront owns 64 rows of it (the matrix instruction's columns) and the other
+// registers: a wavefront owns 64 rows of it (or 32; the matrix instruction's columns) and the other
 // operand streams through LDS, 64 rows at a time, one step ahead.  The logits of a step come out
 // with a lane per owned row; turned into probabilities they already are the right operand of the
 // second product, streamed^T . p, which reads the same LDS tile through the transposing load.  So
@@ -657,7 +657,7 @@ __global__ __launch_bounds__(kThreads) void k_few_join(int D, int rows, int spli
 //   owner x, stream weight:  statistics;  dx^T = weight^T . p
 //   owner weight, stream x:  dweight^T = x^T . dz
 // The step's rows are permuted within LDS so that neither way of reading meets bank conflicts.
-constexpr int kOwnRows = 256;                    // of a workgroup: 64 a wavefront
+constexpr int kOwnRows = 256;                    // of a workgroup: NB blocks of 32 a wavefront
 constexpr int kStreamRows = 64;                  // of a step
 
 template <int KD> constexpr int stream_bytes() { return kStreamRows * KD * 32; }
@@ -670,22 +670,24 @@ __device__ __forceinline__ int stream_spread(int row) {
 }
 template <int KD> constexpr int stream_window() { return KD % 8 == 0 ? 256 : 128; }        // bytes it permutes
 
-template <int KD>
+template <int KD, int WAVES>
 __device__ __forceinline__ void stage_stream(const Operand<Bf16>& op, int64_t r0, unsigned lds, int wave, int lane) {
   constexpr int cpr = KD * 2;                    // chunks of a row
+  const char* base = reinterpret_cast<const char*>(op.base + r0 * op.ld);              // uniform
+  const int left = op.rows - r0 < kStreamRows ? int(op.rows - r0) : kStreamRows;       // at least 1
+  const unsigned pitch = unsigned(op.ld) * 2;
 #pragma unroll
-  for (int l = 0; l < stream_bytes<KD>() / 16 / kThreads; ++l) {
-    const int first = (l * 4 + wave) * 64, q = first + lane;
+  for (int l = 0; l < stream_bytes<KD>() / 16 / (64 * WAVES); ++l) {
+    const int first = (l * WAVES + wave) * 64, q = first + lane;
     const int row = q / cpr, c = (q % cpr) ^ stream_spread<KD>(row);
-    const unsigned r = unsigned(r0) + row, last = unsigned(op.rows) - 1;   // at most 2^30 rows
-    load_to_lds(op.base + uint64_t(r < last ? r : last) * unsigned(op.ld) + c * 8, lds + first * 16);
+    load_to_lds(base, unsigned(row < left ? row : left - 1) * pitch + c * 16, lds + first * 16);
   }
 }
 
-template <int KD>
-__device__ __forceinline__ void load_owned(const Operand<Bf16>& op, int64_t r0, int lane, bf16x8 (&own)[2][KD]) {
+template <int KD, int NB>
+__device__ __forceinline__ void load_owned(const Operand<Bf16>& op, int64_t r0, int lane, bf16x8 (&own)[NB][KD]) {
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
+  for (int j = 0; j < NB; ++j) {
     int64_t r = r0 + 32 * j + (lane & 31);
     r = r < op.rows ? r : op.rows - 1;
     const Bf16* src = op.base + r * op.ld + 8 * (lane >> 5);
@@ -714,22 +716,6 @@ __device__ __forceinline__ bf16x8 stream_row(const char* tile, int sub, int k, c
   return *reinterpret_cast<const bf16x8*>(tile + place);
 }
 
-// logits of the step's rows 32 * sub .. + 31 (rows of the block) and the owned rows (columns)
-template <int KD>
-__device__ __forceinline__ void stream_logits(const char* tile, int sub, const StreamLane& at,
-                                              const bf16x8 (&own)[2][KD], f32x16 (&z)[2]) {
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) z[j][e] = 0.f;
-#pragma unroll
-  for (int k = 0; k < KD; ++k) {
-    const bf16x8 a = stream_row<KD>(tile, sub, k, at);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) z[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, own[j][k], z[j], 0, 0, 0);
-  }
-}
-
 // streamed^T as an operand: features 32 * block .. + 31, and of rows 32 * sub .. the sixteen that
 // elements 8 * q .. of a logits block hold (in that order)
 template <int KD>
@@ -747,12 +733,14 @@ __device__ __forceinline__ bf16x8 stream_across(const char* tile, int sub, int q
   return r;
 }
 
-// stream_logits with other work between its matrix instructions: between(i) is called for
-// i = 0 .. 31, a few after each of them, and stays there.  The matrix unit works on while the
+// Logits of the step's rows 32 * sub .. + 31 (rows of a block) and the owned rows (columns), with
+// other work between the matrix instructions: between(i) is called for i = 0 .. 16 * NB - 1, a few
+// after each of them, and stays there.  The matrix unit works on while the
 // vector unit does; left to itself the compiler puts one after the other.
-template <int KD, typename Between>
+template <int KD, int NB, typename Between>
 __device__ __forceinline__ void stream_logits_between(const char* tile, int sub, const StreamLane& at,
-                                                      const bf16x8 (&own)[2][KD], f32x16 (&z)[2], Between&& between) {
+                                                      const bf16x8 (&own)[NB][KD], f32x16 (&z)[NB],
+                                                      Between&& between) {
   const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   constexpr int kAhead = KD < 16 ? 3 : 2;        // reads under way
   bf16x8 a[kAhead];
@@ -763,11 +751,11 @@ __device__ __forceinline__ void stream_logits_between(const char* tile, int sub,
     const bf16x8 cur = a[k % kAhead];
     if (k + kAhead < KD) a[k % kAhead] = stream_row<KD>(tile, sub, k + kAhead, at);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < NB; ++j) {
       z[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(cur, own[j][k], k ? z[j] : zero, 0, 0, 0);
-      const int step = 2 * k + j;
+      const int step = NB * k + j;
 #pragma unroll
-      for (int i = 32 * step / (2 * KD); i < 32 * (step + 1) / (2 * KD); ++i) between(i);
+      for (int i = 16 * step / KD; i < 16 * (step + 1) / KD; ++i) between(i);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -784,7 +772,7 @@ __global__ __launch_bounds__(kThreads) void k_wide_stats(int64_t B, int64_t V, O
   const int64_t t0 = steps * split / splits, t1 = steps * (split + 1) / splits;
   const StreamLane at = stream_lane<KD>(lane);
   bf16x8 own[2][KD];
-  load_owned<KD>(x, b0, lane, own);
+  load_owned(x, b0, lane, own);
   float top[2], sum[2];
   int y[2];
 #pragma unroll
@@ -830,14 +818,14 @@ __global__ __launch_bounds__(kThreads) void k_wide_stats(int64_t B, int64_t V, O
       sum[j] *= exp2_raw(top[j] - ref[j]);
       top[j] = m;
     }
-    stream_logits_between<KD>(tile, sub, at, own, next, [&](int i) {
+    stream_logits_between(tile, sub, at, own, next, [&](int i) {
       sum[i >> 4] += exp2_raw(fmaf(z[i >> 4][i & 15], kLog2e, -ref[i >> 4]));
       asm volatile("" : "+v"(sum[i >> 4]));      // now, not where the sum is used
     });
   };
   const unsigned stages = lds_offset(lds);
   if (t0 < t1) {
-    stage_stream<KD>(w, t0 * kStreamRows, stages, wave, lane);
+    stage_stream<KD, 4>(w, t0 * kStreamRows, stages, wave, lane);
     f32x16 first[2], second[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j)
@@ -847,7 +835,7 @@ __global__ __launch_bounds__(kThreads) void k_wide_stats(int64_t B, int64_t V, O
       landed();
       __syncthreads();
       const int cur = int(t - t0) & 1;
-      if (t + 1 < t1) stage_stream<KD>(w, (t + 1) * kStreamRows, stages + (cur ^ 1) * stream_bytes<KD>(), wave, lane);
+      if (t + 1 < t1) stage_stream<KD, 4>(w, (t + 1) * kStreamRows, stages + (cur ^ 1) * stream_bytes<KD>(), wave, lane);
       const char* tile = lds + cur * stream_bytes<KD>();
       turn(tile, 0, first, second);
       settle(first, t * kStreamRows);
@@ -891,33 +879,58 @@ __global__ __launch_bounds__(256) void k_wide_rows(int64_t B, int64_t padded, La
   out.label[b] = int(y);
 }
 
+// acc += streamed^T . p over a half step, with other work between as above
+template <int KD, int NB, typename Between>
+__device__ __forceinline__ void stream_gather_between(const char* tile, int sub, const StreamLane& at,
+                                                      const bf16x8 (&p)[NB][2], f32x16 (&acc)[KD / 2][NB],
+                                                      Between&& between) {
+  constexpr int kAhead = 2;                      // reads under way
+  bf16x8 a[kAhead];
+#pragma unroll
+  for (int n = 0; n < kAhead; ++n) a[n] = stream_across<KD>(tile, sub, n & 1, n >> 1, at);
+#pragma unroll
+  for (int n = 0; n < KD; ++n) {                 // features 32 * (n / 2), rows 16 * (n & 1)
+    const bf16x8 cur = a[n % kAhead];
+    if (n + kAhead < KD) a[n % kAhead] = stream_across<KD>(tile, sub, (n + kAhead) & 1, (n + kAhead) >> 1, at);
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      acc[n >> 1][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(cur, p[j][n & 1], acc[n >> 1][j], 0, 0, 0);
+      const int step = NB * n + j;
+#pragma unroll
+      for (int i = 16 * step / KD; i < 16 * (step + 1) / KD; ++i) between(i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+}
+
 // BY_CLASS: owner weight, stream x, dz^T with the label's -1; else owner x, stream weight, p alone
 // (what the label takes off joins dx in its last step).  PER_ROW: every row has a factor of its own
 // (in dweight here; dx takes it in its last step).  part[split][owned row][KD * 16] in 32 bits.
-template <int KD, bool BY_CLASS, bool PER_ROW>
-__global__ __launch_bounds__(kThreads, 1) void k_wide_grads(int64_t owners, int64_t streams, Operand<Bf16> owned,
+template <int KD, int NB, bool BY_CLASS, bool PER_ROW>
+__global__ __launch_bounds__(512 / NB, NB == 1 ? 2 : 1) void k_wide_grads(int64_t owners, int64_t streams, Operand<Bf16> owned,
                                                             Operand<Bf16> streamed, RowConst rows, int64_t steps,
                                                             int splits, float* __restrict__ part, int64_t plane) {
   __shared__ __align__(128) char lds[2 * stream_bytes<KD>()];
-  __shared__ __align__(16) float row_shift[4][kStreamRows], row_factor[4][kStreamRows];
+  constexpr int kWaves = 8 / NB;
+  __shared__ __align__(16) float row_shift[kWaves][kStreamRows], row_factor[kWaves][kStreamRows];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int split = blockIdx.x % splits;
-  const int64_t o0 = int64_t(blockIdx.x / splits) * kOwnRows + 64 * wave;
+  const int64_t o0 = int64_t(blockIdx.x / splits) * kOwnRows + 32 * NB * wave;
   const int64_t t0 = steps * split / splits, t1 = steps * (split + 1) / splits;
   const StreamLane at = stream_lane<KD>(lane);
-  bf16x8 own[2][KD];
-  load_owned<KD>(owned, o0, lane, own);
-  f32x16 acc[KD / 2][2];
+  bf16x8 own[NB][KD];
+  load_owned(owned, o0, lane, own);
+  f32x16 acc[KD / 2][NB];
 #pragma unroll
   for (int d = 0; d < KD / 2; ++d)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < NB; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[d][j][e] = 0.f;
-  float shift[2] = {0.f, 0.f};
+  float shift[NB] = {};
   if constexpr (!BY_CLASS) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < NB; ++j) {
       const int64_t b = o0 + 32 * j + (lane & 31);
       shift[j] = rows.shift[b < owners ? b : owners - 1];
     }
@@ -925,95 +938,99 @@ __global__ __launch_bounds__(kThreads, 1) void k_wide_grads(int64_t owners, int6
   float next_shift = 0.f, next_factor = 0.f;     // of row `lane` of the coming step
   int next_label = -1;
   const auto fetch_rows = [&](int64_t t) {
-    next_shift = rows.shift[t * kStreamRows + lane];
-    if constexpr (PER_ROW) next_factor = rows.factor[t * kStreamRows + lane];
-    next_label = rows.label[t * kStreamRows + lane];
+    // a 32-bit offset from a uniform base: no address registers (at most 2^30 rows)
+    const int64_t first = t * kStreamRows;
+    next_shift = (rows.shift + first)[unsigned(lane)];
+    if constexpr (PER_ROW) next_factor = (rows.factor + first)[unsigned(lane)];
+    next_label = (rows.label + first)[unsigned(lane)];
   };
   const unsigned stages = lds_offset(lds);
   if (t0 < t1) {
-    stage_stream<KD>(streamed, t0 * kStreamRows, stages, wave, lane);
+    stage_stream<KD, kWaves>(streamed, t0 * kStreamRows, stages, wave, lane);
     if constexpr (BY_CLASS) fetch_rows(t0);
   }
+  // A half step's logits become p while the half step before is multiplied: p of -1 is 0
+  bf16x8 p[NB][2];
+#pragma unroll
+  for (int j = 0; j < NB; ++j)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) p[j][e >> 3][e & 7] = static_cast<__bf16>(0.f);
+  int label = -1;
+  const auto half_step = [&](int64_t t, const char* tile, int sub, const char* before) {
+    f32x16 z[NB];
+    stream_logits_between(tile, sub, at, own, z, [](int) {});
+    f32x4 c[2];                                  // shifts of four rows, and of the next four
+    const auto shifts = [&](int e) {
+      return *reinterpret_cast<const f32x4*>(&row_shift[wave][32 * sub + block_row(e, lane)]);
+    };
+    if constexpr (BY_CLASS) c[0] = shifts(0);
+    stream_gather_between<KD, NB>(before, sub ^ 1, at, p, acc, [&](int i) {
+      const int j = i % NB, e = i / NB;
+      if (BY_CLASS && j == 0 && e % 4 == 0 && e < 12) c[(e / 4 + 1) & 1] = shifts(e + 4);
+      z[j][e] = exp2_raw(fmaf(z[j][e], kLog2e, -(BY_CLASS ? c[e / 4 & 1][e & 3] : shift[j])));
+      float here = z[j][e];
+      asm volatile("" : "+v"(here));             // now, not where it is used
+      z[j][e] = here;
+    });
+    if constexpr (BY_CLASS) {
+      // rows whose label is among the owned classes: rare
+      for (uint64_t h = __ballot(label >= o0 && label < o0 + 32 * NB) >> (32 * sub) & 0xffffffffull; h != 0; h &= h - 1) {
+        const int r = __builtin_ctzll(h);
+        const int col = int(__shfl(label, 32 * sub + r) - o0);
+        int mine = r - 4 * (lane >> 5);          // compared with constants
+        asm("" : "+v"(mine));
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) z[j][e] -= block_row(e, 0) == mine && 32 * j + (lane & 31) == col ? 1.f : 0.f;
+      }
+      if constexpr (PER_ROW) {
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const f32x4 g = *reinterpret_cast<const f32x4*>(&row_factor[wave][32 * sub + block_row(e, lane)]);
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) z[j][e + q] *= g[q];
+        }
+      }
+    } else if (t * kStreamRows + 32 * sub + 32 > streams) {                // classes beyond the last
+      int left = int(streams - t * kStreamRows) - 32 * sub - 4 * (lane >> 5);
+      asm("" : "+v"(left));
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) z[j][e] = block_row(e, 0) < left ? z[j][e] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) p[j][e >> 3][e & 7] = static_cast<__bf16>(z[j][e]);
+  };
+  const char* tile = lds;
   for (int64_t t = t0; t < t1; ++t) {
     landed();
     __syncthreads();
     const int cur = int(t - t0) & 1;
-    int label = -1;
+    tile = lds + cur * stream_bytes<KD>();
     if constexpr (BY_CLASS) {                    // a wavefront's own copy: no barrier
       row_shift[wave][lane] = next_shift;
       if constexpr (PER_ROW) row_factor[wave][lane] = next_factor;
       label = next_label;
       __builtin_amdgcn_wave_barrier();
     }
+    // the first step has nothing before it: p is 0 and any numbers will do, its own
+    half_step(t, tile, 0, t == t0 ? tile : lds + (cur ^ 1) * stream_bytes<KD>());
+    __syncthreads();                             // everybody has left the step before
     if (t + 1 < t1) {
-      stage_stream<KD>(streamed, (t + 1) * kStreamRows, stages + (cur ^ 1) * stream_bytes<KD>(), wave, lane);
+      stage_stream<KD, kWaves>(streamed, (t + 1) * kStreamRows, stages + (cur ^ 1) * stream_bytes<KD>(), wave, lane);
       if constexpr (BY_CLASS) fetch_rows(t + 1);
     }
-    const char* tile = lds + cur * stream_bytes<KD>();
-    uint64_t hits = 0;                           // rows of the step whose label is among the owned classes
-    if constexpr (BY_CLASS) hits = __ballot(label >= o0 && label < o0 + 64);
-#pragma unroll KD > 8 ? 1 : 2                    // two at a time would not fit the registers
-    for (int sub = 0; sub < 2; ++sub) {
-      f32x16 z[2];
-      stream_logits<KD>(tile, sub, at, own, z);
-      if constexpr (BY_CLASS) {
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-          const f32x4 c = *reinterpret_cast<const f32x4*>(&row_shift[wave][32 * sub + block_row(e, lane)]);
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) z[j][e + q] = exp2_raw(fmaf(z[j][e + q], kLog2e, -c[q]));
-        }
-        for (uint64_t h = (hits >> (32 * sub)) & 0xffffffffull; h != 0; h &= h - 1) {        // rare
-          const int r = __builtin_ctzll(h);
-          const int col = int(__shfl(label, 32 * sub + r) - o0);
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if (block_row(e, lane) == r && 32 * j + (lane & 31) == col) z[j][e] -= 1.f;
-        }
-        if constexpr (PER_ROW) {
-#pragma unroll
-          for (int e = 0; e < 16; e += 4) {
-            const f32x4 g = *reinterpret_cast<const f32x4*>(&row_factor[wave][32 * sub + block_row(e, lane)]);
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-#pragma unroll
-              for (int j = 0; j < 2; ++j) z[j][e + q] *= g[q];
-          }
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) z[j][e] = exp2_raw(fmaf(z[j][e], kLog2e, -shift[j]));
-        if ((t + 1) * kStreamRows > streams) {   // classes beyond the last
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if (t * kStreamRows + 32 * sub + block_row(e, lane) >= streams) z[j][e] = 0.f;
-        }
-      }
-      bf16x8 p[2][2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) p[j][e >> 3][e & 7] = static_cast<__bf16>(z[j][e]);
-#pragma unroll
-      for (int d = 0; d < KD / 2; ++d)
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const bf16x8 a = stream_across<KD>(tile, sub, q, d, at);
-#pragma unroll
-          for (int j = 0; j < 2; ++j) acc[d][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, p[j][q], acc[d][j], 0, 0, 0);
-        }
-    }
+    half_step(t, tile, 1, tile);
   }
+  stream_gather_between<KD, NB>(tile, 1, at, p, acc, [](int) {});
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
+  for (int j = 0; j < NB; ++j) {
     const int64_t r = o0 + 32 * j + (lane & 31);
     if (r >= owners) continue;
     float* dst = part + split * plane + r * (KD * 16);
@@ -1306,12 +1323,13 @@ int backward(const Call& c, const Plan& p, const Buffers& b, const RowStat* stat
   return SGNN_OK;
 }
 
-#define SGNN_WIDE(KDS, CALL)                 \
-  switch (KDS) {                             \
-    case 4: { constexpr int KD = 4; CALL; } break;   \
-    case 8: { constexpr int KD = 8; CALL; } break;   \
-    case 12: { constexpr int KD = 12; CALL; } break; \
-    default: { constexpr int KD = 16; CALL; } break; \
+// NB: two blocks a wavefront where they fit the registers beside what they are multiplied into
+#define SGNN_WIDE(KDS, CALL)                                     \
+  switch (KDS) {                                                 \
+    case 4: { constexpr int KD = 4, NB = 2; (void)NB; CALL; } break;   \
+    case 8: { constexpr int KD = 8, NB = 2; (void)NB; CALL; } break;   \
+    case 12: { constexpr int KD = 12, NB = 1; (void)NB; CALL; } break; \
+    default: { constexpr int KD = 16, NB = 1; (void)NB; CALL; } break; \
   }
 
 int wide_forward(const Call& c, const Wide& f, const Plan& p, const Buffers& b, RowStat* stats, float* row_loss,
@@ -1336,8 +1354,8 @@ int wide_backward(const Call& c, const Wide& f, const Plan& p, const Buffers& b,
                      share, b.rows);
   HIP_TRY(hipGetLastError());
   if (dx) {
-    SGNN_WIDE(f.KD, hipLaunchKernelGGL((k_wide_grads<KD, false, false>), dim3(unsigned(f.own_b * f.dx_splits)),
-                                       dim3(kThreads), 0, st, c.B, c.V, x, w, b.rows, f.steps_v, f.dx_splits, b.dx,
+    SGNN_WIDE(f.KD, hipLaunchKernelGGL((k_wide_grads<KD, NB, false, false>), dim3(unsigned(f.own_b * f.dx_splits)),
+                                       dim3(512 / NB), 0, st, c.B, c.V, x, w, b.rows, f.steps_v, f.dx_splits, b.dx,
                                        c.B * p.Dp));
     HIP_TRY(hipGetLastError());
     hipLaunchKernelGGL((k_class_join<Bf16>), dim3(unsigned(ceil_div(c.B, 32)), unsigned(ceil_div(c.D, 32))), dim3(256), 0,
@@ -1348,12 +1366,12 @@ int wide_backward(const Call& c, const Wide& f, const Plan& p, const Buffers& b,
   }
   if (dw) {
     if (share) {
-      SGNN_WIDE(f.KD, hipLaunchKernelGGL((k_wide_grads<KD, true, false>), dim3(unsigned(f.own_v * f.dw_splits)),
-                                         dim3(kThreads), 0, st, c.V, c.B, w, x, b.rows, f.steps_b, f.dw_splits, b.dx,
+      SGNN_WIDE(f.KD, hipLaunchKernelGGL((k_wide_grads<KD, NB, true, false>), dim3(unsigned(f.own_v * f.dw_splits)),
+                                         dim3(512 / NB), 0, st, c.V, c.B, w, x, b.rows, f.steps_b, f.dw_splits, b.dx,
                                          c.V * p.Dp));
     } else {
-      SGNN_WIDE(f.KD, hipLaunchKernelGGL((k_wide_grads<KD, true, true>), dim3(unsigned(f.own_v * f.dw_splits)),
-                                         dim3(kThreads), 0, st, c.V, c.B, w, x, b.rows, f.steps_b, f.dw_splits, b.dx,
+      SGNN_WIDE(f.KD, hipLaunchKernelGGL((k_wide_grads<KD, NB, true, true>), dim3(unsigned(f.own_v * f.dw_splits)),
+                                         dim3(512 / NB), 0, st, c.V, c.B, w, x, b.rows, f.steps_b, f.dw_splits, b.dx,
                                          c.V * p.Dp));
     }
     HIP_TRY(hipGetLastError());

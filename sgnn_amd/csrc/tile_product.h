@@ -104,6 +104,11 @@ template <typename T> struct Step { static constexpr int kDepth = 128 / sizeof(T
 __device__ __forceinline__ void load_to_lds(const void* src, unsigned dst) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"(src) : "memory");
 }
+// the same from a uniform base and a 32-bit offset of the lane's own
+__device__ __forceinline__ void load_to_lds(const char* base, unsigned offset, unsigned dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(offset), "s"(base)
+               : "memory");
+}
 __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ unsigned lds_offset(const char* p) {
   return unsigned(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) char*)p));
