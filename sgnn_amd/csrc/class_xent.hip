@@ -912,6 +912,7 @@ __global__ __launch_bounds__(512 / NB, NB == 1 ? 2 : 1) void k_wide_grads(int64_
                                                             int splits, float* __restrict__ part, int64_t plane) {
   __shared__ __align__(128) char lds[2 * stream_bytes<KD>()];
   constexpr int kWaves = 8 / NB;
+  constexpr bool kTurns = KD < 16;               // p across half steps would not fit the registers at 256 features
   __shared__ __align__(16) float row_shift[kWaves][kStreamRows], row_factor[kWaves][kStreamRows];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int split = blockIdx.x % splits;
@@ -958,20 +959,28 @@ __global__ __launch_bounds__(512 / NB, NB == 1 ? 2 : 1) void k_wide_grads(int64_
   int label = -1;
   const auto half_step = [&](int64_t t, const char* tile, int sub, const char* before) {
     f32x16 z[NB];
-    stream_logits_between(tile, sub, at, own, z, [](int) {});
+    StreamLane here = at;                        // its variants are made where they are used, not kept
+    asm volatile("" : "+v"(here.direct), "+v"(here.across));
+    stream_logits_between(tile, sub, here, own, z, [](int) {});
     f32x4 c[2];                                  // shifts of four rows, and of the next four
     const auto shifts = [&](int e) {
       return *reinterpret_cast<const f32x4*>(&row_shift[wave][32 * sub + block_row(e, lane)]);
     };
     if constexpr (BY_CLASS) c[0] = shifts(0);
-    stream_gather_between<KD, NB>(before, sub ^ 1, at, p, acc, [&](int i) {
+    const auto weigh = [&](int i) {
       const int j = i % NB, e = i / NB;
       if (BY_CLASS && j == 0 && e % 4 == 0 && e < 12) c[(e / 4 + 1) & 1] = shifts(e + 4);
       z[j][e] = exp2_raw(fmaf(z[j][e], kLog2e, -(BY_CLASS ? c[e / 4 & 1][e & 3] : shift[j])));
-      float here = z[j][e];
-      asm volatile("" : "+v"(here));             // now, not where it is used
-      z[j][e] = here;
-    });
+      float now = z[j][e];
+      asm volatile("" : "+v"(now));              // now, not where it is used
+      z[j][e] = now;
+    };
+    if constexpr (kTurns) {
+      stream_gather_between<KD, NB>(before, sub ^ 1, here, p, acc, weigh);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16 * NB; ++i) weigh(i);
+    }
     if constexpr (BY_CLASS) {
       // rows whose label is among the owned classes: rare
       for (uint64_t h = __ballot(label >= o0 && label < o0 + 32 * NB) >> (32 * sub) & 0xffffffffull; h != 0; h &= h - 1) {
@@ -1006,6 +1015,7 @@ __global__ __launch_bounds__(512 / NB, NB == 1 ? 2 : 1) void k_wide_grads(int64_
     for (int j = 0; j < NB; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) p[j][e >> 3][e & 7] = static_cast<__bf16>(z[j][e]);
+    if constexpr (!kTurns) stream_gather_between<KD, NB>(tile, sub, here, p, acc, [](int) {});
   };
   const char* tile = lds;
   for (int64_t t = t0; t < t1; ++t) {
@@ -1021,14 +1031,14 @@ __global__ __launch_bounds__(512 / NB, NB == 1 ? 2 : 1) void k_wide_grads(int64_
     }
     // the first step has nothing before it: p is 0 and any numbers will do, its own
     half_step(t, tile, 0, t == t0 ? tile : lds + (cur ^ 1) * stream_bytes<KD>());
-    __syncthreads();                             // everybody has left the step before
+    if constexpr (kTurns) __syncthreads();       // everybody has left the step before
     if (t + 1 < t1) {
       stage_stream<KD, kWaves>(streamed, (t + 1) * kStreamRows, stages + (cur ^ 1) * stream_bytes<KD>(), wave, lane);
       if constexpr (BY_CLASS) fetch_rows(t + 1);
     }
     half_step(t, tile, 1, tile);
   }
-  stream_gather_between<KD, NB>(tile, 1, at, p, acc, [](int) {});
+  if constexpr (kTurns) stream_gather_between<KD, NB>(tile, 1, at, p, acc, [](int) {});
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
     const int64_t r = o0 + 32 * j + (lane & 31);
