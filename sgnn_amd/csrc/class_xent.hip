@@ -374,36 +374,41 @@ __global__ __launch_bounds__(256) void k_class_join(int64_t R, int D, int splits
                                                     T* __restrict__ out, int64_t sr, int64_t sd) {
   __shared__ float tile[32][33];
   const int64_t r0 = int64_t(blockIdx.x) * 32;
-  const int d0 = blockIdx.y * 32, t = threadIdx.x;
-  const float common = share ? grad[0] * share[0] : 1.f;
+  const int t = threadIdx.x, lr = t >> 3, ld = (t & 7) * 4, d = int(blockIdx.y) * 32 + ld;
+  const int64_t r = r0 + lr;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  if (r < R && d < D) {
+    const float factor = share ? grad[0] * share[0] : grad ? grad[r] : 1.f;
+    const float* src = in + r * ldi + d;         // ldi is a multiple of 4 and covers d .. d + 3
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int q = 0; q < splits; ++q) sum += *reinterpret_cast<const f32x4*>(src + q * plane);
 #pragma unroll
-  for (int i = t; i < 32 * 32; i += 256) {
-    const int lr = i >> 5, ld = i & 31;
-    const int64_t r = r0 + lr;
-    float s = 0.f;
-    if (r < R && d0 + ld < D) {
-      const float factor = grad && !share ? grad[r] : common;
-      const float* src = in + r * ldi + d0 + ld;
-#pragma unroll 4
-      for (int q = 0; q < splits; ++q) s += src[q * plane];
-      if (of.V) {
-        const int64_t y = label_of(r, of.labels, of.idx, of.n_labels, of.V);
-        if (y < 0) s = 0.f;
-        else if (rest) s += rest[r] * widen(weight[y * sv + (d0 + ld) * sdw]);
+    for (int e = 0; e < 4; ++e) v[e] = sum[e];
+    if (of.V) {
+      const int64_t y = label_of(r, of.labels, of.idx, of.n_labels, of.V);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (y < 0) v[e] = 0.f;
+        else if (rest && d + e < D) v[e] += rest[r] * widen(weight[y * sv + (d + e) * sdw]);
       }
-      s *= factor;
     }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] *= factor;
     if (sd == 1) {
-      if (r < R && d0 + ld < D) out[r * sr + d0 + ld] = narrow<T>(s);
-    } else {
-      tile[lr][ld] = s;
+      T* dst = out + r * sr + d;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (d + e < D) dst[e] = narrow<T>(v[e]);
     }
   }
-  if (sd == 1) return;
+  if (sd == 1) return;                           // the whole launch
+#pragma unroll
+  for (int e = 0; e < 4; ++e) tile[lr][ld + e] = v[e];
   __syncthreads();
   for (int i = t; i < 32 * 32; i += 256) {
-    const int lr = i & 31, ld = i >> 5;
-    if (r0 + lr < R && d0 + ld < D) out[(r0 + lr) * sr + (d0 + ld) * sd] = narrow<T>(tile[lr][ld]);
+    const int fr = i & 31, fd = i >> 5, at = int(blockIdx.y) * 32 + fd;
+    if (r0 + fr < R && at < D) out[(r0 + fr) * sr + at * sd] = narrow<T>(tile[fr][fd]);
   }
 }
 
@@ -905,14 +910,24 @@ __device__ __forceinline__ void stream_gather_between(const char* tile, int sub,
 
 // BY_CLASS: owner weight, stream x, dz^T with the label's -1; else owner x, stream weight, p alone
 // (what the label takes off joins dx in its last step).  PER_ROW: every row has a factor of its own
-// (in dweight here; dx takes it in its last step).  part[split][owned row][KD * 16] in 32 bits.
-template <int KD, int NB, bool BY_CLASS, bool PER_ROW>
-__global__ __launch_bounds__(512 / NB, NB == 1 ? 2 : 1) void k_wide_grads(int64_t owners, int64_t streams, Operand<Bf16> owned,
+// (in dweight here; dx takes it in its last step).  The sums go to part[split][owned row][KD * 16] in
+// 32 bits or, with `out` (dweight from one split), times the mean's factor to where they belong.
+// A wavefront owns 32 rows: 64 (half the LDS reads, but one wavefront a SIMD instead of two) took
+// 58 + 58 us instead of 56 + 52 us at 1777 x 100 x 30011, and spilled at 256 features.
+constexpr int kGradThreads = 512;
+
+template <int KD, bool BY_CLASS, bool PER_ROW>
+__global__ __launch_bounds__(kGradThreads, 2) void k_wide_grads(int64_t owners, int64_t streams, Operand<Bf16> owned,
                                                             Operand<Bf16> streamed, RowConst rows, int64_t steps,
-                                                            int splits, float* __restrict__ part, int64_t plane) {
+                                                            int splits, float* __restrict__ part, int64_t plane,
+                                                            int D, Bf16* __restrict__ out, int64_t sr, int64_t sd,
+                                                            const float* __restrict__ grad,
+                                                            const float* __restrict__ share) {
   __shared__ __align__(128) char lds[2 * stream_bytes<KD>()];
-  constexpr int kWaves = 8 / NB;
-  constexpr bool kTurns = KD < 16;               // p across half steps would not fit the registers at 256 features
+  constexpr int NB = 1, kWaves = kGradThreads / 64;
+  // Taking turns keeps p across half steps; at 256 features that spills where the rows' shifts are
+  // held, too (dweight of 4096 x 256 x 50000: 306 us with, 241 us without; dx 176 and 186 us).
+  constexpr bool kTurns = KD < 16 || !BY_CLASS;
   __shared__ __align__(16) float row_shift[kWaves][kStreamRows], row_factor[kWaves][kStreamRows];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int split = blockIdx.x % splits;
@@ -1043,6 +1058,30 @@ __global__ __launch_bounds__(512 / NB, NB == 1 ? 2 : 1) void k_wide_grads(int64_
   for (int j = 0; j < NB; ++j) {
     const int64_t r = o0 + 32 * j + (lane & 31);
     if (r >= owners) continue;
+    if (out != nullptr) {
+      const float factor = share ? grad[0] * share[0] : 1.f;
+      Bf16* dst = out + r * sr;
+      const bool whole = sd == 1 && sr % 4 == 0 && reinterpret_cast<uintptr_t>(out) % 8 == 0;
+#pragma unroll
+      for (int d = 0; d < KD / 2; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const int at = 32 * d + block_row(e, lane);
+          Bf16 four[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) four[q] = narrow<Bf16>(factor * acc[d][j][e + q]);
+          if (whole && at + 4 <= D) {
+            u32x2 w;
+            __builtin_memcpy(&w, &four, 8);
+            *reinterpret_cast<u32x2*>(dst + at) = w;
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (at + q < D) dst[(at + q) * sd] = four[q];
+          }
+        }
+      continue;
+    }
     float* dst = part + split * plane + r * (KD * 16);
 #pragma unroll
     for (int d = 0; d < KD / 2; ++d)
@@ -1135,8 +1174,19 @@ Wide make_wide(int dtype, int64_t B, int64_t D, int64_t V) {
   f.own_v = ceil_div(V, kOwnRows);
   f.steps_b = ceil_div(B, kStreamRows);
   f.steps_v = ceil_div(V, kStreamRows);
-  const auto spread = [](int64_t want, int64_t groups, int64_t steps) {
-    const int64_t s = ceil_div(want, groups);
+  // `slots` workgroups run at once: as many splits as fill them, or, where the owners alone are
+  // more, the number up to four whose last round is fullest (a fifth better than none, or none)
+  const auto spread = [](int64_t slots, int64_t groups, int64_t steps) {
+    int64_t s = slots / groups;
+    if (s < 1) {
+      s = 1;
+      double best = 0.8 * double(ceil_div(groups, slots));
+      for (int64_t q = 2; q <= 4; ++q)
+        if (const double rounds = double(ceil_div(groups * q, slots)) / double(q); rounds <= best) {
+          best = rounds;
+          s = q;
+        }
+    }
     return int(s < steps ? s : steps);
   };
   f.stat_splits = spread(512, f.own_b, f.steps_v);
@@ -1333,13 +1383,12 @@ int backward(const Call& c, const Plan& p, const Buffers& b, const RowStat* stat
   return SGNN_OK;
 }
 
-// NB: two blocks a wavefront where they fit the registers beside what they are multiplied into
-#define SGNN_WIDE(KDS, CALL)                                     \
-  switch (KDS) {                                                 \
-    case 4: { constexpr int KD = 4, NB = 2; (void)NB; CALL; } break;   \
-    case 8: { constexpr int KD = 8, NB = 2; (void)NB; CALL; } break;   \
-    case 12: { constexpr int KD = 12, NB = 1; (void)NB; CALL; } break; \
-    default: { constexpr int KD = 16, NB = 1; (void)NB; CALL; } break; \
+#define SGNN_WIDE(KDS, CALL)                         \
+  switch (KDS) {                                     \
+    case 4: { constexpr int KD = 4; CALL; } break;   \
+    case 8: { constexpr int KD = 8; CALL; } break;   \
+    case 12: { constexpr int KD = 12; CALL; } break; \
+    default: { constexpr int KD = 16; CALL; } break; \
   }
 
 int wide_forward(const Call& c, const Wide& f, const Plan& p, const Buffers& b, RowStat* stats, float* row_loss,
@@ -1364,9 +1413,9 @@ int wide_backward(const Call& c, const Wide& f, const Plan& p, const Buffers& b,
                      share, b.rows);
   HIP_TRY(hipGetLastError());
   if (dx) {
-    SGNN_WIDE(f.KD, hipLaunchKernelGGL((k_wide_grads<KD, NB, false, false>), dim3(unsigned(f.own_b * f.dx_splits)),
-                                       dim3(512 / NB), 0, st, c.B, c.V, x, w, b.rows, f.steps_v, f.dx_splits, b.dx,
-                                       c.B * p.Dp));
+    SGNN_WIDE(f.KD, hipLaunchKernelGGL((k_wide_grads<KD, false, false>), dim3(unsigned(f.own_b * f.dx_splits)),
+                                       dim3(kGradThreads), 0, st, c.B, c.V, x, w, b.rows, f.steps_v, f.dx_splits, b.dx,
+                                       c.B * p.Dp, int(c.D), nullptr, 0, 0, nullptr, nullptr));
     HIP_TRY(hipGetLastError());
     hipLaunchKernelGGL((k_class_join<Bf16>), dim3(unsigned(ceil_div(c.B, 32)), unsigned(ceil_div(c.D, 32))), dim3(256), 0,
                        st, c.B, int(c.D), f.dx_splits, b.dx, c.B * p.Dp, int64_t(p.Dp), b.rows.factor, nullptr,
@@ -1375,20 +1424,24 @@ int wide_backward(const Call& c, const Wide& f, const Plan& p, const Buffers& b,
     HIP_TRY(hipGetLastError());
   }
   if (dw) {
+    Bf16* const direct = f.dw_splits == 1 ? static_cast<Bf16*>(dw) : nullptr;
+#define SGNN_DWEIGHT(PER_ROW)                                                                                           \
+  SGNN_WIDE(f.KD, hipLaunchKernelGGL((k_wide_grads<KD, true, PER_ROW>), dim3(unsigned(f.own_v * f.dw_splits)),          \
+                                     dim3(kGradThreads), 0, st, c.V, c.B, w, x, b.rows, f.steps_b, f.dw_splits, b.dx,   \
+                                     c.V * p.Dp, int(c.D), direct, dsv, dsd, grad, share))
     if (share) {
-      SGNN_WIDE(f.KD, hipLaunchKernelGGL((k_wide_grads<KD, NB, true, false>), dim3(unsigned(f.own_v * f.dw_splits)),
-                                         dim3(512 / NB), 0, st, c.V, c.B, w, x, b.rows, f.steps_b, f.dw_splits, b.dx,
-                                         c.V * p.Dp));
+      SGNN_DWEIGHT(false);
     } else {
-      SGNN_WIDE(f.KD, hipLaunchKernelGGL((k_wide_grads<KD, NB, true, true>), dim3(unsigned(f.own_v * f.dw_splits)),
-                                         dim3(512 / NB), 0, st, c.V, c.B, w, x, b.rows, f.steps_b, f.dw_splits, b.dx,
-                                         c.V * p.Dp));
+      SGNN_DWEIGHT(true);
     }
+#undef SGNN_DWEIGHT
     HIP_TRY(hipGetLastError());
-    hipLaunchKernelGGL((k_class_join<Bf16>), dim3(unsigned(ceil_div(c.V, 32)), unsigned(ceil_div(c.D, 32))), dim3(256), 0,
-                       st, c.V, int(c.D), f.dw_splits, b.dx, c.V * p.Dp, int64_t(p.Dp), share ? grad : nullptr, share,
-                       nullptr, Labels{}, nullptr, 0, 0, static_cast<Bf16*>(dw), dsv, dsd);
-    HIP_TRY(hipGetLastError());
+    if (!direct) {
+      hipLaunchKernelGGL((k_class_join<Bf16>), dim3(unsigned(ceil_div(c.V, 32)), unsigned(ceil_div(c.D, 32))), dim3(256),
+                         0, st, c.V, int(c.D), f.dw_splits, b.dx, c.V * p.Dp, int64_t(p.Dp), share ? grad : nullptr,
+                         share, nullptr, Labels{}, nullptr, 0, 0, static_cast<Bf16*>(dw), dsv, dsd);
+      HIP_TRY(hipGetLastError());
+    }
   }
   return SGNN_OK;
 }
