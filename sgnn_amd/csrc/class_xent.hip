@@ -823,7 +823,9 @@ __global__ __launch_bounds__(kThreads) void k_wide_stats(int64_t B, int64_t V, O
       sum[j] *= exp2_raw(top[j] - ref[j]);
       top[j] = m;
     }
-    stream_logits_between(tile, sub, at, own, next, [&](int i) {
+    StreamLane here = at;                        // its variants are made where they are used, not kept
+    asm volatile("" : "+v"(here.direct));
+    stream_logits_between(tile, sub, here, own, next, [&](int i) {
       sum[i >> 4] += exp2_raw(fmaf(z[i >> 4][i & 15], kLog2e, -ref[i >> 4]));
       asm volatile("" : "+v"(sum[i >> 4]));      // now, not where the sum is used
     });
@@ -1189,9 +1191,10 @@ Wide make_wide(int dtype, int64_t B, int64_t D, int64_t V) {
     }
     return int(s < steps ? s : steps);
   };
-  f.stat_splits = spread(512, f.own_b, f.steps_v);
-  f.dx_splits = spread(256, f.own_b, f.steps_v);
-  f.dw_splits = spread(256, f.own_v, f.steps_b);
+  // by what a CU's registers hold: two workgroups of four wavefronts up to 192 features; of eight, one, up to 64 two
+  f.stat_splits = spread(f.KD < 16 ? 512 : 256, f.own_b, f.steps_v);
+  f.dx_splits = spread(f.KD > 4 ? 256 : 512, f.own_b, f.steps_v);
+  f.dw_splits = spread(f.KD > 4 ? 256 : 512, f.own_v, f.steps_b);
   return f;
 }
 
