@@ -8,8 +8,9 @@
 // in bf16 and multiplies it from either side.  A piece is sized to stay in the last-level cache
 // between the launch that writes it and the two that read it.
 //
-// All four products run on the bf16 matrix instructions (tile_product.h): bf16 operands as they
-// are, fp32 ones as three bf16 numbers each.  dz of bf16 operands is rounded to bf16 there
+// All four products run on the 16-bit matrix instructions (tile_product.h): bf16 operands as they
+// are, fp32 ones as two fp16 numbers each or, where an operand's range is too wide for that, as
+// three bf16 numbers.  dz of bf16 operands is rounded to bf16 there
 // (relative 2^-9 per element, below the half step that each result is rounded by).
 #include "tile_product.h"
 
@@ -91,6 +92,120 @@ __global__ __launch_bounds__(256) void k_class_operands(int D, int Dp, Source fi
   }
 }
 
+// Whether fp32 operands can go as halves, and their powers of two.  They can when every number is
+// finite and the largest is at most 2^12 times the average magnitude: an element is then off by
+// 2^-28 of that average at most, 2^-4 of what rounding numbers of that size to 32 bits costs.
+struct Range {
+  float x, w, back;        // scales of x and the weight; back = 1 / (x * w)
+  uint32_t halves;
+};
+constexpr float kDzScale = 16384.f;              // of dz without the rows' factors, at most 1
+constexpr int kRangeBlocks = 512;
+
+// part[block] = (largest magnitude as bits, sum of magnitudes) of the block's rows of x, then of the weight
+__global__ __launch_bounds__(256) void k_class_range(int64_t B, int64_t V, int D, const float* __restrict__ x,
+                                                     int64_t ldx, const float* __restrict__ w, int64_t sv, int64_t sd,
+                                                     Labels of, float4* __restrict__ part) {
+  __shared__ float4 joined[4];
+  unsigned top[2] = {0, 0};
+  float sum[2] = {0.f, 0.f};
+  const auto take = [&](int which, float v) {
+    const unsigned m = __float_as_uint(v) & 0x7fffffffu;
+    top[which] = m > top[which] ? m : top[which];
+    sum[which] += __uint_as_float(m);
+  };
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t first = int64_t(blockIdx.x) * 4 + wave, stride = int64_t(gridDim.x) * 4;
+  for (int64_t b = first; b < B; b += stride) {  // a wavefront takes a row
+    if (label_of(b, of.labels, of.idx, of.n_labels, of.V) < 0) continue;
+    for (int d = lane; d < D; d += 64) take(0, x[b * ldx + d]);
+  }
+  // the weight's contiguous direction along the lanes, four elements in flight
+  const int64_t outer = sd == 1 ? V : D, inner = sd == 1 ? D : V, so = sd == 1 ? sv : sd;
+  const int64_t pieces = (inner + 1023) / 1024;  // of a row
+  for (int64_t i = first; i < outer * pieces; i += stride) {
+    const int64_t row = i / pieces, c0 = (i - row * pieces) * 1024 + lane;
+    const float* src = w + row * so;
+#pragma unroll 4
+    for (int q = 0; q < 16; ++q)
+      if (c0 + 64 * q < inner) take(1, src[c0 + 64 * q]);
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1)
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const unsigned o = unsigned(__shfl_xor(int(top[q]), off));
+      top[q] = o > top[q] ? o : top[q];
+      sum[q] += __shfl_xor(sum[q], off);
+    }
+  if (lane == 0) joined[wave] = make_float4(__uint_as_float(top[0]), sum[0], __uint_as_float(top[1]), sum[1]);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    float4 r = joined[0];
+    for (int q = 1; q < 4; ++q) {
+      r.x = __uint_as_float(max(__float_as_uint(r.x), __float_as_uint(joined[q].x)));
+      r.y += joined[q].y;
+      r.z = __uint_as_float(max(__float_as_uint(r.z), __float_as_uint(joined[q].z)));
+      r.w += joined[q].w;
+    }
+    part[blockIdx.x] = r;
+  }
+}
+
+__global__ __launch_bounds__(64) void k_class_scales(int blocks, int64_t B, int64_t V, int D,
+                                                     const float4* __restrict__ part, Range* __restrict__ out) {
+  unsigned top[2] = {0, 0};
+  double sum[2] = {0.0, 0.0};
+  for (int i = threadIdx.x; i < blocks; i += 64) {
+    const float4 r = part[i];
+    top[0] = max(top[0], __float_as_uint(r.x));
+    top[1] = max(top[1], __float_as_uint(r.z));
+    sum[0] += double(r.y);
+    sum[1] += double(r.w);
+  }
+  for (int off = 32; off >= 1; off >>= 1)
+    for (int q = 0; q < 2; ++q) {
+      top[q] = max(top[q], unsigned(__shfl_xor(int(top[q]), off)));
+      sum[q] += __shfl_xor(sum[q], off);
+    }
+  if (threadIdx.x == 0) {
+    bool fits = true;
+    int exponent[2];
+    const double count[2] = {double(B) * D, double(V) * D};
+    for (int q = 0; q < 2; ++q) {
+      const double largest = double(__uint_as_float(top[q]));
+      exponent[q] = int(top[q] >> 23) - 127;     // of the largest; also excludes infinities and NaN
+      // an operand of zeros fits any scale; dead rows of x count as zeros
+      if (top[q] == 0) exponent[q] = 14;
+      else fits = fits && exponent[q] > -45 && exponent[q] < 60 && largest * count[q] <= 4096.0 * sum[q];
+    }
+    const float sx = __uint_as_float(unsigned(127 + 14 - exponent[0]) << 23);
+    const float sw = __uint_as_float(unsigned(127 + 14 - exponent[1]) << 23);
+    *out = fits ? Range{sx, sw, __uint_as_float(unsigned(127 + exponent[0] + exponent[1] - 28) << 23), 1u}
+                : Range{1.f, 1.f, 1.f, 0u};
+  }
+}
+
+// acc = A . B either way; `back` undoes both scales
+template <typename T, bool ADEEP, bool BDEEP>
+__device__ __forceinline__ void product(const Operand<T>& A, int64_t m0, const Operand<T>& B, int64_t n0, int64_t k0,
+                                        int64_t k1, char* lds, bool halves, float sa, float sb, float back, Tile& acc) {
+  clear(acc);
+  if constexpr (sizeof(T) == 4) {
+    if (halves) {
+      multiply<T, true, ADEEP, BDEEP>(A, m0, B, n0, k0, k1, lds, acc, sa, sb);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[i][j][e] *= back;
+      return;
+    }
+  }
+  multiply<T, false, ADEEP, BDEEP>(A, m0, B, n0, k0, k1, lds, acc);
+}
+
 // ------------------------------------------------------------------ forward
 // (r, s): s = sum of 2^(z log2 e - r), r the maximum of z log2 e as it came out rounded (any
 // reference does, as long as all use it).  While everything is -inf the sum stays 0; a NaN never
@@ -132,9 +247,11 @@ template <typename T>
 __global__ __launch_bounds__(kThreads) void k_class_stats(int64_t B, int64_t V, int Dp, Operand<T> x, Operand<T> w,
                                                           const int64_t* __restrict__ labels,
                                                           const int64_t* __restrict__ idx, int64_t n_labels,
-                                                          int64_t tiles_v, int splits, float2* __restrict__ part,
-                                                          float* __restrict__ picked) {
+                                                          int64_t tiles_v, int splits,
+                                                          const Range* __restrict__ range,
+                                                          float2* __restrict__ part, float* __restrict__ picked) {
   __shared__ __align__(128) char lds[kProductLds];
+  const Range rg = sizeof(T) == 4 ? *range : Range{};
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wv = (wave >> 1) * 64, wb = (wave & 1) * 64;
   const int split = blockIdx.x % splits;
@@ -151,8 +268,7 @@ __global__ __launch_bounds__(kThreads) void k_class_stats(int64_t B, int64_t V, 
   }
   for (int64_t t = t0; t < t1; ++t) {
     Tile acc;
-    clear(acc);
-    multiply<T, true, true>(w, t * kTile, x, b0, 0, Dp, lds, acc);
+    product<T, true, true>(w, t * kTile, x, b0, 0, Dp, lds, rg.halves, rg.w, rg.x, rg.back, acc);
     const int64_t vw = t * kTile + wv;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -254,15 +370,16 @@ __global__ __launch_bounds__(kThreads) void k_class_dz(int64_t B, int64_t V, int
                                                        const int64_t* __restrict__ idx, int64_t n_labels,
                                                        const RowStat* __restrict__ stats,
                                                        const float* __restrict__ grad, float* __restrict__ rest,
-                                                       int64_t v0, int tiles, T* __restrict__ dz, int64_t ldz) {
+                                                       int64_t v0, int tiles, const Range* __restrict__ range,
+                                                       T* __restrict__ dz, int64_t ldz) {
   __shared__ __align__(128) char lds[kProductLds];
+  const Range rg = sizeof(T) == 4 ? *range : Range{};
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wv = (wave >> 1) * 64, wb = (wave & 1) * 64;
   const int64_t vt = v0 + int64_t(blockIdx.x % tiles) * kTile;
   const int64_t b0 = int64_t(blockIdx.x / tiles) * kTile;
   Tile acc;
-  clear(acc);
-  multiply<T, true, true>(w, vt, x, b0, 0, Dp, lds, acc);
+  product<T, true, true>(w, vt, x, b0, 0, Dp, lds, rg.halves, rg.w, rg.x, rg.back, acc);
   const int64_t vw = vt + wv;
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
@@ -332,9 +449,13 @@ __global__ __launch_bounds__(kThreads) void k_class_dz(int64_t B, int64_t V, int
 // out[split][Mp][Np].
 template <typename T, bool ADEEP>
 __global__ __launch_bounds__(kThreads) void k_class_product(Operand<T> A, Operand<T> B, int tiles_m, int tiles_n,
-                                                            int64_t K, int splits, int add, float* __restrict__ out,
-                                                            int64_t plane, int64_t ldo) {
+                                                            int64_t K, int splits, int add,
+                                                            const Range* __restrict__ range, int by_class,
+                                                            float* __restrict__ out, int64_t plane, int64_t ldo) {
   __shared__ __align__(128) char lds[kProductLds];
+  // `range` NULL: dz holds the rows' factors and can be of any size
+  const Range rg = sizeof(T) == 4 && range ? *range : Range{};
+  const float sb = by_class ? rg.x : rg.w;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
   const int tn = blockIdx.x % tiles_n, rest = blockIdx.x / tiles_n;
@@ -343,8 +464,8 @@ __global__ __launch_bounds__(kThreads) void k_class_product(Operand<T> A, Operan
   const int64_t steps = K / Step<T>::kDepth;
   const int64_t k0 = steps * split / splits * Step<T>::kDepth, k1 = steps * (split + 1) / splits * Step<T>::kDepth;
   Tile acc;
-  clear(acc);
-  if (k0 < k1) multiply<T, ADEEP, false>(A, m0, B, n0, k0, k1, lds, acc);
+  if (k0 < k1) product<T, ADEEP, false>(A, m0, B, n0, k0, k1, lds, rg.halves, kDzScale, sb, 1.f / (kDzScale * sb), acc);
+  else clear(acc);
   float* dst = out + split * plane + (m0 + wm) * ldo + n0 + wn + (lane & 31);
 #pragma unroll
   for (int i = 0; i < 2; ++i)
@@ -477,7 +598,7 @@ __device__ __forceinline__ f32x16 few_logits(int D, int Dk, int64_t v0, int64_t 
 #pragma unroll
       for (int q = 0; q < P; ++q)
         b[q] = *reinterpret_cast<const bf16x8*>(lds + few_at<P>(q, lane & 31, (k + 16 * u) / 8 + half, Dk));
-      multiply_planes<P>(a, b, acc);
+      multiply_planes(a, b, acc);
     }
   }
   return acc;
@@ -1202,6 +1323,7 @@ struct Buffers {
   char *x, *w, *dz;
   float2* part;
   float *picked, *rest, *dx, *dw;
+  float4* range;
   RowConst rows;
   size_t bytes;
 };
@@ -1214,6 +1336,7 @@ Buffers carve(const Plan& p, int64_t B, int64_t V, bool backward, void* base) {
   if (!backward) {
     b.part = c.take<float2>(size_t(p.stat_splits) * 2 * B);
     b.picked = c.take<float>(size_t(B));
+    b.range = c.take<float4>(kRangeBlocks);
   } else {
     const size_t Np = size_t(p.tiles_d) * kTile;
     b.dz = c.take<char>(p.elem * p.Bp * p.piece);
@@ -1293,6 +1416,10 @@ bool weight_as_is(const Call& c, const Plan& p) {
          reinterpret_cast<uintptr_t>(c.w) % 16 == 0;
 }
 
+// the range is kept behind the rows' statistics
+Range* range_of(RowStat* stats, int64_t B) { return reinterpret_cast<Range*>(stats + B); }
+const Range* range_of(const RowStat* stats, int64_t B) { return reinterpret_cast<const Range*>(stats + B); }
+
 template <typename T>
 int operands(const Call& c, const Plan& p, const Buffers& b, Operand<T>* x, Operand<T>* w, hipStream_t st) {
   const int across = p.Dp / 64;
@@ -1335,8 +1462,17 @@ int forward(const Call& c, const Plan& p, const Buffers& b, RowStat* stats, floa
   Operand<T> x, w;
   if (int rc = operands<T>(c, p, b, &x, &w, st)) return rc;
   const int depth = int(ceil_div(c.D, p.depth) * p.depth);
+  Range* const range = range_of(stats, c.B);
+  if constexpr (sizeof(T) == 4) {
+    hipLaunchKernelGGL(k_class_range, dim3(kRangeBlocks), dim3(256), 0, st, c.B, c.V, int(c.D),
+                       static_cast<const float*>(c.x), c.ldx, static_cast<const float*>(c.w), c.sv, c.sd,
+                       Labels{c.labels, c.idx, c.n_labels, c.V}, b.range);
+    HIP_TRY(hipGetLastError());
+    hipLaunchKernelGGL(k_class_scales, dim3(1), dim3(64), 0, st, kRangeBlocks, c.B, c.V, int(c.D), b.range, range);
+    HIP_TRY(hipGetLastError());
+  }
   hipLaunchKernelGGL((k_class_stats<T>), dim3(unsigned(p.tiles_b * p.stat_splits)), dim3(kThreads), 0, st, c.B, c.V,
-                     p.Dp, x, w, c.labels, c.idx, c.n_labels, p.tiles_v, p.stat_splits, b.part, b.picked);
+                     depth, x, w, c.labels, c.idx, c.n_labels, p.tiles_v, p.stat_splits, range, b.part, b.picked);
   HIP_TRY(hipGetLastError());
   return finish_forward(c, 2 * p.stat_splits, b, stats, row_loss, loss, share, st);
 }
@@ -1348,26 +1484,29 @@ int backward(const Call& c, const Plan& p, const Buffers& b, const RowStat* stat
   if (int rc = operands<T>(c, p, b, &x, &w, st)) return rc;
   const int64_t Np = int64_t(p.tiles_d) * kTile;
   T* const dz = reinterpret_cast<T*>(b.dz);
+  const Range* const range = range_of(stats, c.B);
   const int depth = int(ceil_div(c.D, p.depth) * p.depth);
   for (int64_t v0 = 0; v0 < c.V; v0 += p.piece) {
     const int64_t left = ceil_div(c.V - v0, kTile);
     const int tiles = int(left < p.piece / kTile ? left : p.piece / kTile);
     const int64_t width = int64_t(tiles) * kTile;
     hipLaunchKernelGGL((k_class_dz<T>), dim3(unsigned(p.tiles_b * tiles)), dim3(kThreads), 0, st, c.B, c.V, depth, x, w,
-                       c.labels, c.idx, c.n_labels, stats, share ? nullptr : grad, b.rest, v0, tiles, dz, p.piece);
+                       c.labels, c.idx, c.n_labels, stats, share ? nullptr : grad, b.rest, v0, tiles, range, dz,
+                       p.piece);
     HIP_TRY(hipGetLastError());
     if (dx) {                                    // dx[b][d] += dz[b][v] . w[v][d]
       const Operand<T> a{dz, p.piece, p.Bp, p.piece};
       const Operand<T> wv{w.base + v0 * w.ld, w.ld, c.V - v0, w.cols};
       hipLaunchKernelGGL((k_class_product<T, true>), dim3(unsigned(p.tiles_b * p.dx_splits * p.tiles_d)),
                          dim3(kThreads), 0, st, a, wv, int(p.tiles_b), p.tiles_d, width, p.dx_splits, v0 > 0 ? 1 : 0,
-                         b.dx, p.Bp * Np, Np);
+                         share ? range : nullptr, 0, b.dx, p.Bp * Np, Np);
       HIP_TRY(hipGetLastError());
     }
     if (dw) {                                    // dw[v][d] = dz[b][v] . x[b][d]
       const Operand<T> a{dz, p.piece, p.Bp, p.piece};
       hipLaunchKernelGGL((k_class_product<T, false>), dim3(unsigned(tiles * p.dw_splits * p.tiles_d)), dim3(kThreads),
-                         0, st, a, x, tiles, p.tiles_d, p.Bp, p.dw_splits, 0, b.dw, p.piece * Np, Np);
+                         0, st, a, x, tiles, p.tiles_d, p.Bp, p.dw_splits, 0,
+                         share ? range : nullptr, 1, b.dw, p.piece * Np, Np);
       HIP_TRY(hipGetLastError());
       const int64_t rows = c.V - v0 < width ? c.V - v0 : width;
       hipLaunchKernelGGL((k_class_join<T>), dim3(unsigned(ceil_div(rows, 32)), unsigned(ceil_div(c.D, 32))), dim3(256), 0,

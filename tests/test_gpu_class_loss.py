@@ -2,8 +2,10 @@
 
 Tolerances, from the arithmetic.  u = 2^-23 bounds an addition or a product in 32 bits (2^-24 for
 a rounding, twice that where the matrix unit cuts off).
-* a logit is a sum of at most 6 D + 16 products (six for each pair of 32-bit numbers; the three
-  left out are below 3 * 2^-24 of the pair): off by ez = (6 D + 20) u |x| |w|^T;
+* a logit is a sum of at most 6 D + 16 products (six for each pair of 32-bit numbers; what is left
+  out or rounded off is below 3 u of the pair): off by ez = (6 D + 20) u |x| |w|^T; where 32-bit
+  numbers go as two fp16 numbers each, scaled so that the largest is 2^14 or more, an element is
+  also off by half a step of fp16's smallest, 2^-25, that is by 2^-39 of the largest at most;
 * relative to the row's maximum its exponential is off by 2 ez plus 4 u (1 + z_max - z) for the
   subtraction, the scaling and the function, and a row's sum of them by another (V / 4 + 1100) u
   (a lane adds every fourth class at most, then the lanes, wavefronts and up to 512 splits); so p
@@ -31,7 +33,7 @@ def make(B, D, V, dtype, device, seed=0, scale=1.5, nodes=None):
     return x.to(device, dtype), w.to(device, dtype), labels.to(device)
 
 
-def reference(x, w, labels, idx=None, g=None):
+def reference(x, w, labels, idx=None, g=None, halves=True):
     """Row losses, gradients for row weights g (the mean's if None), and the bounds above."""
     dtype = x.dtype
     xd, wd = x.double(), w.double()
@@ -47,7 +49,9 @@ def reference(x, w, labels, idx=None, g=None):
     at = torch.where(live, y, torch.zeros_like(y))[:, None]
     z = xd @ wd.t()
     size = xd.abs() @ wd.abs().t()
-    ez = (6 * D + 20) * U * size
+    tiny = 2.0 ** -39 if dtype == torch.float32 and halves else 0.0
+    tx, tw = tiny * xd.abs().nan_to_num(0, 0, 0).amax(), tiny * wd.abs().nan_to_num(0, 0, 0).amax()
+    ez = (6 * D + 20) * U * size + tx * wd.abs().sum(1) + tw * xd.abs().sum(1, keepdim=True)
     top = z.amax(1, keepdim=True)
     lse = torch.logsumexp(z, 1, keepdim=True)
     delta = 2 * ez.amax(1, keepdim=True) + 4 * U * (1 + top - z) + (V / 4 + 1100) * U
@@ -62,11 +66,11 @@ def reference(x, w, labels, idx=None, g=None):
     one = torch.zeros_like(z).scatter_(1, at, 1.0) * g
     dz = torch.exp(z - lse) * g - one
     plane = HALF_STEP[dtype] if dtype == torch.bfloat16 else U
-    edz = p * torch.expm1(delta) + 4 * U * (p + one.abs()) + plane * dz.abs()
+    edz = p * torch.expm1(delta) + 4 * U * (p + one.abs()) + plane * dz.abs() + tiny * g.abs()
     adz = dz.abs() + edz
     dx, dw = dz @ wd, dz.t() @ xd
-    edx = edz @ wd.abs() + (6 * V + 600) * U * (adz @ wd.abs())
-    edw = edz.t() @ xd.abs() + (6 * B + 600) * U * (adz.t() @ xd.abs())
+    edx = edz @ wd.abs() + (6 * V + 600) * U * (adz @ wd.abs()) + tw * adz.sum(1, keepdim=True)
+    edw = edz.t() @ xd.abs() + (6 * B + 600) * U * (adz.t() @ xd.abs()) + tx * adz.sum(0)[:, None]
     half = HALF_STEP[dtype]
     return dict(loss=loss, loss_bound=loss_bound, count=count, dx=dx, dw=dw,
                 dx_bound=edx + half * (dx.abs() + edx) + 1e-38, dw_bound=edw + half * (dw.abs() + edw) + 1e-38)
@@ -115,6 +119,21 @@ def test_several_pieces(gpu_device, dtype):
 @pytest.mark.parametrize("D,V", [(256, 3001), (101, 999)])
 def test_few_rows(gpu_device, dtype, B, D, V):
     check(*make(B, D, V, DTYPES[dtype], gpu_device, seed=B))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B", [20, 100])
+@pytest.mark.parametrize("D", [8, 32, 33, 64, 96, 160, 224, 256, 288, 320])
+def test_nothing_beside_the_operands_is_read(gpu_device, dtype, B, D):
+    """Operands in the middle of NaN, at every alignment of rows that takes a path of its own."""
+    t = DTYPES[dtype]
+    x, w, labels = make(B, D, 256, t, gpu_device, seed=D)
+    around = []
+    for m in (x, w):
+        nan = torch.full((m.numel() + 2048,), float("nan"), device=gpu_device, dtype=t)
+        nan[1024:1024 + m.numel()] = m.flatten()
+        around.append(nan[1024:1024 + m.numel()].view(m.shape))
+    check(around[0], around[1], labels)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -211,6 +230,35 @@ def test_peaked_and_far_logits(gpu_device, dtype):
     rows = snn.class_cross_entropy(masked_x, masked_w, keep, reduction="none")
     want = reference(masked_x, masked_w[:200], keep)
     close(rows, want["loss"], want["loss_bound"], "masked classes")
+
+
+def test_operands_of_wide_range(gpu_device):
+    """fp32 numbers too far apart for two fp16 numbers each (a row, a class or a feature far larger than
+    the rest): exact to 32 bits all the same, in the small rows too."""
+    x, w, labels = make(150, 40, 260, torch.float32, gpu_device, seed=13)
+    for scale in (2.0 ** 20, 2.0 ** 40, 2.0 ** -30):
+        far = x.clone()
+        far[3] *= scale
+        check_range(far, w, labels)
+        far = w.clone()
+        far[7] *= scale
+        check_range(x * 0.01, far, labels)
+    far, other = x.clone(), w.clone()
+    far[:, 5] *= 2.0 ** 30
+    other[:, 5] *= 2.0 ** -30
+    check_range(far, other, labels)
+
+
+def check_range(x, w, labels):
+    ref = reference(x, w, labels, halves=False)
+    rows = snn.class_cross_entropy(x, w, labels, reduction="none")
+    finite = torch.isfinite(ref["loss_bound"])
+    close(rows[finite], ref["loss"][finite], ref["loss_bound"][finite], "row losses")
+    xs, ws = x.clone().requires_grad_(), w.clone().requires_grad_()
+    snn.class_cross_entropy(xs, ws, labels).backward()
+    assert bool(torch.isfinite(xs.grad).all()) and bool(torch.isfinite(ws.grad).all())
+    keep = torch.isfinite(ref["dx_bound"]) & torch.isfinite(ref["dx"])
+    close(xs.grad[keep], ref["dx"][keep], ref["dx_bound"][keep], "dx")
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
