@@ -654,8 +654,8 @@ int sgnn_saved8_weight_grad(int dtype, int64_t n, int64_t F, int64_t H, const vo
  * when idx is given, else labels[b]; a row whose index or label is out of range has no class: its
  * loss is 0, it adds nothing to either gradient and does not count in the mean.
  *
- * forward: stats (3 B + 4 floats, what the backward pass goes by: r = max_v z log2(e), sum_v
- *   2^(z log2(e) - r) and the label's z of each row, then the operands' ranges), row_loss; with `loss` also
+ * forward: stats (3 floats a row, what the backward pass goes by: the largest z, the sum of
+ *   exp(z - that), the label's z), row_loss; with `loss` also
  *   loss[0] = mean of the counted rows (0 if there are none) and share[0] = 1 / their number (0).
  * backward: from the same operands and the forward's stats.  share given: g_b = grad[0] * share[0]
  *   (the mean's gradient); share NULL: g_b = grad[b].  dx or dweight may be NULL.

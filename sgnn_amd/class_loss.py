@@ -33,12 +33,12 @@ class _ClassXent(torch.autograd.Function):
         x, (w, sv, sd) = unit_rows(x.detach()), _weight_layout(weight.detach())
         (B, D), V, dev = x.shape, w.shape[0], x.device
         lib, dtype = _lib.load(), _lib.TYPES[x.dtype]
-        kept = torch.empty(4 * B + 5, dtype=torch.float32, device=dev)   # statistics and ranges, 1 / counted rows, row losses
+        kept = torch.empty(4 * B + 1, dtype=torch.float32, device=dev)   # statistics, 1 / counted rows, row losses
         out = torch.empty(() if mean else (B,), dtype=torch.float32, device=dev)
         nbytes = lib.sgnn_class_xent_workspace_bytes(dtype, B, D, V, 0)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         at = kept.data_ptr()
-        rows, loss, share = (at + 12 * B + 20, out.data_ptr(), at + 12 * B + 16) if mean else (out.data_ptr(), None, None)
+        rows, loss, share = (at + 12 * B + 4, out.data_ptr(), at + 12 * B) if mean else (out.data_ptr(), None, None)
         _lib.call_on(dev, lib.sgnn_class_xent_forward, dtype, B, D, V, x.data_ptr(), max(x.stride(0), D), w.data_ptr(),
                      sv, sd, labels.data_ptr(), labels.numel(), None if idx is None else idx.data_ptr(), at, rows, loss,
                      share, ws.data_ptr(), nbytes)
@@ -66,7 +66,7 @@ class _ClassXent(torch.autograd.Function):
         at = kept.data_ptr()
         _lib.call_on(dev, lib.sgnn_class_xent_backward, dtype, B, D, V, x.data_ptr(), max(x.stride(0), D), w.data_ptr(),
                      sv, sd, labels.data_ptr(), labels.numel(), None if idx is None else idx.data_ptr(), at,
-                     grad.data_ptr(), at + 12 * B + 16 if mean else None, None if dx is None else dx.data_ptr(), D,
+                     grad.data_ptr(), at + 12 * B if mean else None, None if dx is None else dx.data_ptr(), D,
                      None if dw is None else dw.data_ptr(), dsv, dsd, ws.data_ptr(), nbytes)
         return dx, dw, None, None, None
 

@@ -8,9 +8,8 @@
 // in bf16 and multiplies it from either side.  A piece is sized to stay in the last-level cache
 // between the launch that writes it and the two that read it.
 //
-// All four products run on the 16-bit matrix instructions (tile_product.h): bf16 operands as they
-// are, fp32 ones as two fp16 numbers each or, where an operand's range is too wide for that, as
-// three bf16 numbers.  dz of bf16 operands is rounded to bf16 there
+// All four products run on the bf16 matrix instructions (tile_product.h): bf16 operands as they
+// are, fp32 ones as three bf16 numbers each.  dz of bf16 operands is rounded to bf16 there
 // (relative 2^-9 per element, below the half step that each result is rounded by).
 #include "tile_product.h"
 
@@ -92,166 +91,71 @@ __global__ __launch_bounds__(256) void k_class_operands(int D, int Dp, Source fi
   }
 }
 
-// Whether fp32 operands can go as halves, and their powers of two.  They can when every number is
-// finite and the largest is at most 2^12 times the average magnitude: an element is then off by
-// 2^-28 of that average at most, 2^-4 of what rounding numbers of that size to 32 bits costs.
-struct Range {
-  float x, w, back;        // scales of x and the weight; back = 1 / (x * w)
-  uint32_t halves;
-};
-constexpr float kDzScale = 16384.f;              // of dz without the rows' factors, at most 1
-constexpr int kRangeBlocks = 512;
-
-// part[block] = (largest magnitude as bits, sum of magnitudes) of the block's rows of x, then of the weight
-__global__ __launch_bounds__(256) void k_class_range(int64_t B, int64_t V, int D, const float* __restrict__ x,
-                                                     int64_t ldx, const float* __restrict__ w, int64_t sv, int64_t sd,
-                                                     Labels of, float4* __restrict__ part) {
-  __shared__ float4 joined[4];
-  unsigned top[2] = {0, 0};
-  float sum[2] = {0.f, 0.f};
-  const auto take = [&](int which, float v) {
-    const unsigned m = __float_as_uint(v) & 0x7fffffffu;
-    top[which] = m > top[which] ? m : top[which];
-    sum[which] += __uint_as_float(m);
-  };
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t first = int64_t(blockIdx.x) * 4 + wave, stride = int64_t(gridDim.x) * 4;
-  for (int64_t b = first; b < B; b += stride) {  // a wavefront takes a row
-    if (label_of(b, of.labels, of.idx, of.n_labels, of.V) < 0) continue;
-    for (int d = lane; d < D; d += 64) take(0, x[b * ldx + d]);
-  }
-  // the weight's contiguous direction along the lanes, four elements in flight
-  const int64_t outer = sd == 1 ? V : D, inner = sd == 1 ? D : V, so = sd == 1 ? sv : sd;
-  const int64_t pieces = (inner + 1023) / 1024;  // of a row
-  for (int64_t i = first; i < outer * pieces; i += stride) {
-    const int64_t row = i / pieces, c0 = (i - row * pieces) * 1024 + lane;
-    const float* src = w + row * so;
-#pragma unroll 4
-    for (int q = 0; q < 16; ++q)
-      if (c0 + 64 * q < inner) take(1, src[c0 + 64 * q]);
-  }
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1)
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const unsigned o = unsigned(__shfl_xor(int(top[q]), off));
-      top[q] = o > top[q] ? o : top[q];
-      sum[q] += __shfl_xor(sum[q], off);
-    }
-  if (lane == 0) joined[wave] = make_float4(__uint_as_float(top[0]), sum[0], __uint_as_float(top[1]), sum[1]);
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    float4 r = joined[0];
-    for (int q = 1; q < 4; ++q) {
-      r.x = __uint_as_float(max(__float_as_uint(r.x), __float_as_uint(joined[q].x)));
-      r.y += joined[q].y;
-      r.z = __uint_as_float(max(__float_as_uint(r.z), __float_as_uint(joined[q].z)));
-      r.w += joined[q].w;
-    }
-    part[blockIdx.x] = r;
-  }
-}
-
-__global__ __launch_bounds__(64) void k_class_scales(int blocks, int64_t B, int64_t V, int D,
-                                                     const float4* __restrict__ part, Range* __restrict__ out) {
-  unsigned top[2] = {0, 0};
-  double sum[2] = {0.0, 0.0};
-  for (int i = threadIdx.x; i < blocks; i += 64) {
-    const float4 r = part[i];
-    top[0] = max(top[0], __float_as_uint(r.x));
-    top[1] = max(top[1], __float_as_uint(r.z));
-    sum[0] += double(r.y);
-    sum[1] += double(r.w);
-  }
-  for (int off = 32; off >= 1; off >>= 1)
-    for (int q = 0; q < 2; ++q) {
-      top[q] = max(top[q], unsigned(__shfl_xor(int(top[q]), off)));
-      sum[q] += __shfl_xor(sum[q], off);
-    }
-  if (threadIdx.x == 0) {
-    bool fits = true;
-    int exponent[2];
-    const double count[2] = {double(B) * D, double(V) * D};
-    for (int q = 0; q < 2; ++q) {
-      const double largest = double(__uint_as_float(top[q]));
-      exponent[q] = int(top[q] >> 23) - 127;     // of the largest; also excludes infinities and NaN
-      // an operand of zeros fits any scale; dead rows of x count as zeros
-      if (top[q] == 0) exponent[q] = 14;
-      else fits = fits && exponent[q] > -45 && exponent[q] < 60 && largest * count[q] <= 4096.0 * sum[q];
-    }
-    const float sx = __uint_as_float(unsigned(127 + 14 - exponent[0]) << 23);
-    const float sw = __uint_as_float(unsigned(127 + 14 - exponent[1]) << 23);
-    *out = fits ? Range{sx, sw, __uint_as_float(unsigned(127 + exponent[0] + exponent[1] - 28) << 23), 1u}
-                : Range{1.f, 1.f, 1.f, 0u};
-  }
-}
-
-// acc = A . B either way; `back` undoes both scales
-template <typename T, bool ADEEP, bool BDEEP>
-__device__ __forceinline__ void product(const Operand<T>& A, int64_t m0, const Operand<T>& B, int64_t n0, int64_t k0,
-                                        int64_t k1, char* lds, bool halves, float sa, float sb, float back, Tile& acc) {
-  clear(acc);
-  if constexpr (sizeof(T) == 4) {
-    if (halves) {
-      multiply<T, true, ADEEP, BDEEP>(A, m0, B, n0, k0, k1, lds, acc, sa, sb);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) acc[i][j][e] *= back;
-      return;
-    }
-  }
-  multiply<T, false, ADEEP, BDEEP>(A, m0, B, n0, k0, k1, lds, acc);
-}
-
 // ------------------------------------------------------------------ forward
-// (r, s): s = sum of 2^(z log2 e - r), r the maximum of z log2 e as it came out rounded (any
-// reference does, as long as all use it).  While everything is -inf the sum stays 0; a NaN never
-// becomes the maximum but makes the sum NaN.
-struct RowStat { float r, s, picked; };          // what the backward pass needs of a row; picked = the label's logit
+// (m, s): m = the largest logit, s = sum of 2^((z - m) log2 e).  While everything is -inf the sum
+// stays 0; a NaN never becomes the maximum but makes the sum NaN.
+struct RowStat { float m, s, picked; };          // what the backward pass needs of a row; picked = the label's logit
 
-__device__ __forceinline__ void join_stats(float& r, float& s, float orr, float os) {
-  const float top = fmaxf(r, orr), ref = top == -INFINITY ? 0.f : top;
-  s = s * exp2_raw(r - ref) + os * exp2_raw(orr - ref);
-  r = top;
+__device__ __forceinline__ void join_stats(float& m, float& s, float om, float os) {
+  const float top = fmaxf(m, om), ref = top == -INFINITY ? 0.f : top;
+  s = s * exp2_raw((m - ref) * kLog2e) + os * exp2_raw((om - ref) * kLog2e);
+  m = top;
+}
+
+// One multiply-add per logit: 2^(z log2 e - c) with c = ref * log2 e rounded, and what the rounding
+// took put right in the sum.  Where that could leave the exponent's range (logits of millions) the
+// reference is taken off the logits first.
+struct Reference { float c, fix; };
+constexpr float kFarLogit = 1048576.f;
+template <int N>
+__device__ __forceinline__ Reference reference_of(f32x16 (&z)[N], float ref) {
+  const bool far = !(fabsf(ref) < kFarLogit);
+  if (__any(far)) {
+    const float off = far ? ref : 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) z[i][e] -= off;
+  }
+  const float c = far ? 0.f : ref * kLog2e;
+  return {c, far ? 1.f : exp2_raw(-fmaf(ref, kLog2e, -c))};
 }
 template <int N>
-__device__ __forceinline__ void accumulate(const f32x16 (&z)[N], float& r, float& s) {
+__device__ __forceinline__ float largest(const f32x16 (&z)[N]) {
   float top = z[0][0];
 #pragma unroll
   for (int i = 0; i < N; ++i)
 #pragma unroll
     for (int e = 0; e < 16; e += 2) top = fmaxf(fmaxf(z[i][e], z[i][e + 1]), top);
-  top = fmaxf(top * kLog2e, r);
-  const float ref = top == -INFINITY ? 0.f : top;
+  return top;
+}
+template <int N>
+__device__ __forceinline__ void accumulate(f32x16 (&z)[N], float& m, float& s) {
+  const float top = fmaxf(largest(z), m), ref = top == -INFINITY ? 0.f : top;
+  const Reference at = reference_of(z, ref);
   float sum[N];
-  sum[0] = s * exp2_raw(r - ref);
 #pragma unroll
-  for (int i = 1; i < N; ++i) sum[i] = 0.f;
+  for (int i = 0; i < N; ++i) sum[i] = 0.f;
 #pragma unroll
   for (int e = 0; e < 16; ++e)
 #pragma unroll
-    for (int i = 0; i < N; ++i) sum[i] += exp2_raw(fmaf(z[i][e], kLog2e, -ref));
+    for (int i = 0; i < N; ++i) sum[i] += exp2_raw(fmaf(z[i][e], kLog2e, -at.c));
 #pragma unroll
   for (int i = 1; i < N; ++i) sum[0] += sum[i];
-  s = sum[0];
-  r = top;
+  s = s * exp2_raw((m - ref) * kLog2e) + sum[0] * at.fix;
+  m = top;
 }
 
 // A workgroup takes 128 rows of x and a range of the classes, 128 at a time.  The tile is formed
 // as classes x rows, so that a lane holds 32 classes of each of two rows and its running maximum
-// and sum need no other lane until the end.  part[row][split][half] = (r, s).
+// and sum need no other lane until the end.  part[row][split][half] = (m, s).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_class_stats(int64_t B, int64_t V, int Dp, Operand<T> x, Operand<T> w,
                                                           const int64_t* __restrict__ labels,
                                                           const int64_t* __restrict__ idx, int64_t n_labels,
-                                                          int64_t tiles_v, int splits,
-                                                          const Range* __restrict__ range,
-                                                          float2* __restrict__ part, float* __restrict__ picked) {
+                                                          int64_t tiles_v, int splits, float2* __restrict__ part,
+                                                          float* __restrict__ picked) {
   __shared__ __align__(128) char lds[kProductLds];
-  const Range rg = sizeof(T) == 4 ? *range : Range{};
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wv = (wave >> 1) * 64, wb = (wave & 1) * 64;
   const int split = blockIdx.x % splits;
@@ -268,7 +172,8 @@ __global__ __launch_bounds__(kThreads) void k_class_stats(int64_t B, int64_t V, 
   }
   for (int64_t t = t0; t < t1; ++t) {
     Tile acc;
-    product<T, true, true>(w, t * kTile, x, b0, 0, Dp, lds, rg.halves, rg.w, rg.x, rg.back, acc);
+    clear(acc);
+    multiply<T, true, true>(w, t * kTile, x, b0, 0, Dp, lds, acc);
     const int64_t vw = t * kTile + wv;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -286,7 +191,7 @@ __global__ __launch_bounds__(kThreads) void k_class_stats(int64_t B, int64_t V, 
           for (int e = 0; e < 16; ++e)
             if (vw + 32 * i + block_row(e, lane) >= V) acc[i][j][e] = -INFINITY;
       }
-      const f32x16 z[2] = {acc[0][j], acc[1][j]};
+      f32x16 z[2] = {acc[0][j], acc[1][j]};
       accumulate(z, top[j], sum[j]);
     }
   }
@@ -322,7 +227,7 @@ __global__ __launch_bounds__(256) void k_class_rows(int64_t B, int64_t V, int pa
     const bool live = label_of(b, labels, idx, n_labels, V) >= 0;
     const float zy = live ? picked[b] : 0.f;
     stats[b] = RowStat{m, s, zy};
-    row_loss[b] = live ? (fmaf(-zy, kLog2e, m) + log2f(s)) * kLn2 : 0.f;
+    row_loss[b] = live ? (m - zy) + log2f(s) * kLn2 : 0.f;
   }
 }
 
@@ -370,16 +275,15 @@ __global__ __launch_bounds__(kThreads) void k_class_dz(int64_t B, int64_t V, int
                                                        const int64_t* __restrict__ idx, int64_t n_labels,
                                                        const RowStat* __restrict__ stats,
                                                        const float* __restrict__ grad, float* __restrict__ rest,
-                                                       int64_t v0, int tiles, const Range* __restrict__ range,
-                                                       T* __restrict__ dz, int64_t ldz) {
+                                                       int64_t v0, int tiles, T* __restrict__ dz, int64_t ldz) {
   __shared__ __align__(128) char lds[kProductLds];
-  const Range rg = sizeof(T) == 4 ? *range : Range{};
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wv = (wave >> 1) * 64, wb = (wave & 1) * 64;
   const int64_t vt = v0 + int64_t(blockIdx.x % tiles) * kTile;
   const int64_t b0 = int64_t(blockIdx.x / tiles) * kTile;
   Tile acc;
-  product<T, true, true>(w, vt, x, b0, 0, Dp, lds, rg.halves, rg.w, rg.x, rg.back, acc);
+  clear(acc);
+  multiply<T, true, true>(w, vt, x, b0, 0, Dp, lds, acc);
   const int64_t vw = vt + wv;
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
@@ -391,7 +295,7 @@ __global__ __launch_bounds__(kThreads) void k_class_dz(int64_t B, int64_t V, int
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = exp2_raw(fmaf(acc[i][j][e], kLog2e, -st.r)) * scale;
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = exp2_raw((acc[i][j][e] - st.m) * kLog2e) * scale;
     if (__any(y >= vw && y < vw + 64)) {
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -449,13 +353,9 @@ __global__ __launch_bounds__(kThreads) void k_class_dz(int64_t B, int64_t V, int
 // out[split][Mp][Np].
 template <typename T, bool ADEEP>
 __global__ __launch_bounds__(kThreads) void k_class_product(Operand<T> A, Operand<T> B, int tiles_m, int tiles_n,
-                                                            int64_t K, int splits, int add,
-                                                            const Range* __restrict__ range, int by_class,
-                                                            float* __restrict__ out, int64_t plane, int64_t ldo) {
+                                                            int64_t K, int splits, int add, float* __restrict__ out,
+                                                            int64_t plane, int64_t ldo) {
   __shared__ __align__(128) char lds[kProductLds];
-  // `range` NULL: dz holds the rows' factors and can be of any size
-  const Range rg = sizeof(T) == 4 && range ? *range : Range{};
-  const float sb = by_class ? rg.x : rg.w;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
   const int tn = blockIdx.x % tiles_n, rest = blockIdx.x / tiles_n;
@@ -464,8 +364,8 @@ __global__ __launch_bounds__(kThreads) void k_class_product(Operand<T> A, Operan
   const int64_t steps = K / Step<T>::kDepth;
   const int64_t k0 = steps * split / splits * Step<T>::kDepth, k1 = steps * (split + 1) / splits * Step<T>::kDepth;
   Tile acc;
-  if (k0 < k1) product<T, ADEEP, false>(A, m0, B, n0, k0, k1, lds, rg.halves, kDzScale, sb, 1.f / (kDzScale * sb), acc);
-  else clear(acc);
+  clear(acc);
+  if (k0 < k1) multiply<T, ADEEP, false>(A, m0, B, n0, k0, k1, lds, acc);
   float* dst = out + split * plane + (m0 + wm) * ldo + n0 + wn + (lane & 31);
 #pragma unroll
   for (int i = 0; i < 2; ++i)
@@ -627,7 +527,7 @@ __global__ __launch_bounds__(kThreads) void k_few_stats(int B, int D, int Dk, in
       for (int e = 0; e < 16; ++e)
         if (v0 + block_row(e, lane) >= V) z[e] = -INFINITY;
     }
-    const f32x16 one[1] = {z};
+    f32x16 one[1] = {z};
     accumulate(one, m, s);
   }
   const float om = __shfl_xor(m, 32), os = __shfl_xor(s, 32);
@@ -663,7 +563,7 @@ __global__ __launch_bounds__(kThreads) void k_few_dz(int B, int rows, int D, int
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       const int64_t v = v0 + block_row(e, lane);
-      const float d = exp2_raw(fmaf(z[e], kLog2e, -st.r)) * scale - (v == y ? g : 0.f);
+      const float d = exp2_raw((z[e] - st.m) * kLog2e) * scale - (v == y ? g : 0.f);
       if (b < rows && v < V) dz[v * rows + b] = y >= 0 ? d : 0.f;
     }
   }
@@ -932,24 +832,26 @@ __global__ __launch_bounds__(kThreads) void k_wide_stats(int64_t B, int64_t V, O
     }
   };
   // the logits of one half step while the other's are summed
-  const auto turn = [&](const char* tile, int sub, f32x16 (&next)[2], const f32x16 (&z)[2]) {
-    float ref[2];
+  const auto turn = [&](const char* tile, int sub, f32x16 (&next)[2], f32x16 (&z)[2]) {
+    Reference ref[2];
+    float part[2] = {0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      float m = z[j][0];
-#pragma unroll
-      for (int e = 1; e < 15; e += 2) m = fmaxf(fmaxf(z[j][e], z[j][e + 1]), m);
-      m = fmaxf(fmaxf(m, z[j][15]) * kLog2e, top[j]);
-      ref[j] = m == -INFINITY ? 0.f : m;
-      sum[j] *= exp2_raw(top[j] - ref[j]);
+      f32x16 one[1] = {z[j]};
+      const float m = fmaxf(largest(one), top[j]), r = m == -INFINITY ? 0.f : m;
+      ref[j] = reference_of(one, r);
+      z[j] = one[0];
+      sum[j] *= exp2_raw((top[j] - r) * kLog2e);
       top[j] = m;
     }
     StreamLane here = at;                        // its variants are made where they are used, not kept
     asm volatile("" : "+v"(here.direct));
     stream_logits_between(tile, sub, here, own, next, [&](int i) {
-      sum[i >> 4] += exp2_raw(fmaf(z[i >> 4][i & 15], kLog2e, -ref[i >> 4]));
-      asm volatile("" : "+v"(sum[i >> 4]));      // now, not where the sum is used
+      part[i >> 4] += exp2_raw(fmaf(z[i >> 4][i & 15], kLog2e, -ref[i >> 4].c));
+      asm volatile("" : "+v"(part[i >> 4]));     // now, not where the sum is used
     });
+#pragma unroll
+    for (int j = 0; j < 2; ++j) sum[j] = fmaf(part[j], ref[j].fix, sum[j]);
   };
   const unsigned stages = lds_offset(lds);
   if (t0 < t1) {
@@ -972,7 +874,7 @@ __global__ __launch_bounds__(kThreads) void k_wide_stats(int64_t B, int64_t V, O
     }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const f32x16 one[1] = {second[j]};
+      f32x16 one[1] = {second[j]};
       accumulate(one, top[j], sum[j]);
     }
   }
@@ -985,10 +887,13 @@ __global__ __launch_bounds__(kThreads) void k_wide_stats(int64_t B, int64_t V, O
   }
 }
 
-// What the gradients need of a row: p = 2^(z log2 e - shift) (shift = infinity without a class), its
-// factor, its label, and what the label's element of dz adds in dx beyond its rounded probability.
+// What the gradients need of a row: p = 2^((z - top) log2 e - shift) with top = 0 but for rows whose
+// logits are so large that the rounding of shift would be felt (2^12: by 2^-12, a bf16 half step
+// being 2^-9); shift = infinity without a class; its factor, its label, and what the label's element
+// of dz adds in dx beyond its rounded probability.
+constexpr float kLargeLogit = 4096.f;
 struct RowConst {
-  float *shift, *factor, *rest;
+  float *shift, *top, *factor, *rest;
   int* label;
 };
 
@@ -999,9 +904,11 @@ __global__ __launch_bounds__(256) void k_wide_rows(int64_t B, int64_t padded, La
   if (b >= padded) return;
   const int64_t y = b < B ? label_of(b, of.labels, of.idx, of.n_labels, of.V) : -1;
   const RowStat st = y >= 0 ? stats[b] : RowStat{INFINITY, 1.f, 0.f};
-  const float shift = st.r + log2f(st.s);
-  const float p = exp2_raw(fmaf(st.picked, kLog2e, -shift));
+  const bool large = y >= 0 && !(fabsf(st.m) <= kLargeLogit);
+  const float top = large ? st.m : 0.f, shift = large ? log2f(st.s) : fmaf(st.m, kLog2e, log2f(st.s));
+  const float p = exp2_raw(fmaf(st.picked - top, kLog2e, -shift));
   out.shift[b] = shift;
+  out.top[b] = top;
   out.factor[b] = y < 0 ? 0.f : share ? grad[0] * share[0] : grad[b];
   out.rest[b] = (p - widen(Bf16{to_bf16(p)})) - 1.f;
   out.label[b] = int(y);
@@ -1051,7 +958,8 @@ __global__ __launch_bounds__(kGradThreads, 2) void k_wide_grads(int64_t owners, 
   // Taking turns keeps p across half steps; at 256 features that spills where the rows' shifts are
   // held, too (dweight of 4096 x 256 x 50000: 306 us with, 241 us without; dx 176 and 186 us).
   constexpr bool kTurns = KD < 16 || !BY_CLASS;
-  __shared__ __align__(16) float row_shift[kWaves][kStreamRows], row_factor[kWaves][kStreamRows];
+  __shared__ __align__(16) float row_shift[kWaves][kStreamRows], row_top[kWaves][kStreamRows],
+      row_factor[kWaves][kStreamRows];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int split = blockIdx.x % splits;
   const int64_t o0 = int64_t(blockIdx.x / splits) * kOwnRows + 32 * NB * wave;
@@ -1067,19 +975,22 @@ __global__ __launch_bounds__(kGradThreads, 2) void k_wide_grads(int64_t owners, 
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[d][j][e] = 0.f;
   float shift[NB] = {};
+  bool any_large = false;
   if constexpr (!BY_CLASS) {
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
       const int64_t b = o0 + 32 * j + (lane & 31);
       shift[j] = rows.shift[b < owners ? b : owners - 1];
+      any_large = any_large || __any(rows.top[b < owners ? b : owners - 1] != 0.f);
     }
   }
-  float next_shift = 0.f, next_factor = 0.f;     // of row `lane` of the coming step
+  float next_shift = 0.f, next_top = 0.f, next_factor = 0.f;               // of row `lane` of the coming step
   int next_label = -1;
   const auto fetch_rows = [&](int64_t t) {
     // a 32-bit offset from a uniform base: no address registers (at most 2^30 rows)
     const int64_t first = t * kStreamRows;
     next_shift = (rows.shift + first)[unsigned(lane)];
+    next_top = (rows.top + first)[unsigned(lane)];
     if constexpr (PER_ROW) next_factor = (rows.factor + first)[unsigned(lane)];
     next_label = (rows.label + first)[unsigned(lane)];
   };
@@ -1100,6 +1011,15 @@ __global__ __launch_bounds__(kGradThreads, 2) void k_wide_grads(int64_t owners, 
     StreamLane here = at;                        // its variants are made where they are used, not kept
     asm volatile("" : "+v"(here.direct), "+v"(here.across));
     stream_logits_between(tile, sub, here, own, z, [](int) {});
+    if (any_large) {                             // rare
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        const int64_t b = o0 + 32 * j + (lane & 31);
+        const float top = BY_CLASS ? 0.f : rows.top[b < owners ? b : owners - 1];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) z[j][e] -= BY_CLASS ? row_top[wave][32 * sub + block_row(e, lane)] : top;
+      }
+    }
     f32x4 c[2];                                  // shifts of four rows, and of the next four
     const auto shifts = [&](int e) {
       return *reinterpret_cast<const f32x4*>(&row_shift[wave][32 * sub + block_row(e, lane)]);
@@ -1163,6 +1083,8 @@ __global__ __launch_bounds__(kGradThreads, 2) void k_wide_grads(int64_t owners, 
     tile = lds + cur * stream_bytes<KD>();
     if constexpr (BY_CLASS) {                    // a wavefront's own copy: no barrier
       row_shift[wave][lane] = next_shift;
+      row_top[wave][lane] = next_top;
+      any_large = __any(next_top != 0.f);
       if constexpr (PER_ROW) row_factor[wave][lane] = next_factor;
       label = next_label;
       __builtin_amdgcn_wave_barrier();
@@ -1323,7 +1245,6 @@ struct Buffers {
   char *x, *w, *dz;
   float2* part;
   float *picked, *rest, *dx, *dw;
-  float4* range;
   RowConst rows;
   size_t bytes;
 };
@@ -1336,7 +1257,6 @@ Buffers carve(const Plan& p, int64_t B, int64_t V, bool backward, void* base) {
   if (!backward) {
     b.part = c.take<float2>(size_t(p.stat_splits) * 2 * B);
     b.picked = c.take<float>(size_t(B));
-    b.range = c.take<float4>(kRangeBlocks);
   } else {
     const size_t Np = size_t(p.tiles_d) * kTile;
     b.dz = c.take<char>(p.elem * p.Bp * p.piece);
@@ -1358,7 +1278,8 @@ Buffers carve_wide(const Wide& f, const Plan& p, int64_t B, int64_t V, bool back
     b.picked = c.take<float>(size_t(B));
   } else {
     const size_t padded = size_t(f.steps_b) * kStreamRows;
-    b.rows = RowConst{c.take<float>(padded), c.take<float>(padded), c.take<float>(padded), c.take<int>(padded)};
+    b.rows = RowConst{c.take<float>(padded), c.take<float>(padded), c.take<float>(padded), c.take<float>(padded),
+                      c.take<int>(padded)};
     // the two gradients' shares take turns
     const size_t dx = size_t(f.dx_splits) * B, dw = size_t(f.dw_splits) * V;
     b.dx = c.take<float>((dx > dw ? dx : dw) * p.Dp);
@@ -1416,10 +1337,6 @@ bool weight_as_is(const Call& c, const Plan& p) {
          reinterpret_cast<uintptr_t>(c.w) % 16 == 0;
 }
 
-// the range is kept behind the rows' statistics
-Range* range_of(RowStat* stats, int64_t B) { return reinterpret_cast<Range*>(stats + B); }
-const Range* range_of(const RowStat* stats, int64_t B) { return reinterpret_cast<const Range*>(stats + B); }
-
 template <typename T>
 int operands(const Call& c, const Plan& p, const Buffers& b, Operand<T>* x, Operand<T>* w, hipStream_t st) {
   const int across = p.Dp / 64;
@@ -1462,17 +1379,8 @@ int forward(const Call& c, const Plan& p, const Buffers& b, RowStat* stats, floa
   Operand<T> x, w;
   if (int rc = operands<T>(c, p, b, &x, &w, st)) return rc;
   const int depth = int(ceil_div(c.D, p.depth) * p.depth);
-  Range* const range = range_of(stats, c.B);
-  if constexpr (sizeof(T) == 4) {
-    hipLaunchKernelGGL(k_class_range, dim3(kRangeBlocks), dim3(256), 0, st, c.B, c.V, int(c.D),
-                       static_cast<const float*>(c.x), c.ldx, static_cast<const float*>(c.w), c.sv, c.sd,
-                       Labels{c.labels, c.idx, c.n_labels, c.V}, b.range);
-    HIP_TRY(hipGetLastError());
-    hipLaunchKernelGGL(k_class_scales, dim3(1), dim3(64), 0, st, kRangeBlocks, c.B, c.V, int(c.D), b.range, range);
-    HIP_TRY(hipGetLastError());
-  }
   hipLaunchKernelGGL((k_class_stats<T>), dim3(unsigned(p.tiles_b * p.stat_splits)), dim3(kThreads), 0, st, c.B, c.V,
-                     depth, x, w, c.labels, c.idx, c.n_labels, p.tiles_v, p.stat_splits, range, b.part, b.picked);
+                     depth, x, w, c.labels, c.idx, c.n_labels, p.tiles_v, p.stat_splits, b.part, b.picked);
   HIP_TRY(hipGetLastError());
   return finish_forward(c, 2 * p.stat_splits, b, stats, row_loss, loss, share, st);
 }
@@ -1484,29 +1392,26 @@ int backward(const Call& c, const Plan& p, const Buffers& b, const RowStat* stat
   if (int rc = operands<T>(c, p, b, &x, &w, st)) return rc;
   const int64_t Np = int64_t(p.tiles_d) * kTile;
   T* const dz = reinterpret_cast<T*>(b.dz);
-  const Range* const range = range_of(stats, c.B);
   const int depth = int(ceil_div(c.D, p.depth) * p.depth);
   for (int64_t v0 = 0; v0 < c.V; v0 += p.piece) {
     const int64_t left = ceil_div(c.V - v0, kTile);
     const int tiles = int(left < p.piece / kTile ? left : p.piece / kTile);
     const int64_t width = int64_t(tiles) * kTile;
     hipLaunchKernelGGL((k_class_dz<T>), dim3(unsigned(p.tiles_b * tiles)), dim3(kThreads), 0, st, c.B, c.V, depth, x, w,
-                       c.labels, c.idx, c.n_labels, stats, share ? nullptr : grad, b.rest, v0, tiles, range, dz,
-                       p.piece);
+                       c.labels, c.idx, c.n_labels, stats, share ? nullptr : grad, b.rest, v0, tiles, dz, p.piece);
     HIP_TRY(hipGetLastError());
     if (dx) {                                    // dx[b][d] += dz[b][v] . w[v][d]
       const Operand<T> a{dz, p.piece, p.Bp, p.piece};
       const Operand<T> wv{w.base + v0 * w.ld, w.ld, c.V - v0, w.cols};
       hipLaunchKernelGGL((k_class_product<T, true>), dim3(unsigned(p.tiles_b * p.dx_splits * p.tiles_d)),
                          dim3(kThreads), 0, st, a, wv, int(p.tiles_b), p.tiles_d, width, p.dx_splits, v0 > 0 ? 1 : 0,
-                         share ? range : nullptr, 0, b.dx, p.Bp * Np, Np);
+                         b.dx, p.Bp * Np, Np);
       HIP_TRY(hipGetLastError());
     }
     if (dw) {                                    // dw[v][d] = dz[b][v] . x[b][d]
       const Operand<T> a{dz, p.piece, p.Bp, p.piece};
       hipLaunchKernelGGL((k_class_product<T, false>), dim3(unsigned(tiles * p.dw_splits * p.tiles_d)), dim3(kThreads),
-                         0, st, a, x, tiles, p.tiles_d, p.Bp, p.dw_splits, 0,
-                         share ? range : nullptr, 1, b.dw, p.piece * Np, Np);
+                         0, st, a, x, tiles, p.tiles_d, p.Bp, p.dw_splits, 0, b.dw, p.piece * Np, Np);
       HIP_TRY(hipGetLastError());
       const int64_t rows = c.V - v0 < width ? c.V - v0 : width;
       hipLaunchKernelGGL((k_class_join<T>), dim3(unsigned(ceil_div(rows, 32)), unsigned(ceil_div(c.D, 32))), dim3(256), 0,

@@ -2,15 +2,9 @@
 // exact splitting of fp32 and the inner loop of a 128 x 128 tile.
 //
 // bf16 operands go in as they are: their products are exact and summed in 32 bits.  An fp32 number
-// is taken apart in registers on the way from LDS to the matrix instruction, one way or the other:
-// * thirds: the sum of three bf16 numbers (8 + 8 + 8 bits of its mantissa, cut off, so the sum is
-//   exact); of the nine products of two numbers the three smallest, below 3 * 2^-24 of the whole,
-//   are left out.  Takes any number.
-// * halves: the sum of two fp16 numbers (11 + 11 bits, each to nearest: off by 2^-23 of it at most),
-//   after a multiplication by a power of two that brings the operand's largest number to
-//   2^14 .. 2^15; of the four products the smallest, below 2^-24, is left out.  Half the matrix
-//   instructions and half the splitting, but what lies 2^14 below the largest number loses bits
-//   (an element is off by 2^-40 of the largest at most), so the operand's range has to be known.
+// is the sum of three bf16 numbers (8 + 8 + 8 bits of its mantissa, cut off, so the sum is exact),
+// taken apart in registers on the way from LDS to the matrix instruction; of the nine products of
+// two numbers the three smallest, below 3 * 2^-24 of the whole, are left out.
 #pragma once
 #include "common.h"
 
@@ -20,7 +14,6 @@ typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 struct Bf16 { uint16_t bits; };
@@ -49,15 +42,8 @@ __device__ __forceinline__ unsigned high_halves(float lo, float hi) {
   return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
 }
 
-// what an element of type T is made of
-template <typename T, bool HALVES = false> struct Planes {
-  static constexpr int kCount = sizeof(T) == 4 ? 3 : 1;
-  typedef bf16x8 Part;
-};
-template <> struct Planes<float, true> {
-  static constexpr int kCount = 2;
-  typedef f16x8 Part;
-};
+// bf16 numbers an element of type T is made of
+template <typename T> struct Planes { static constexpr int kCount = sizeof(T) == 4 ? 3 : 1; };
 
 __device__ __forceinline__ void planes_of(const float (&v)[8], bf16x8 (&out)[3]) {
   u32x4 pl[3];
@@ -74,28 +60,14 @@ __device__ __forceinline__ void planes_of(const float (&v)[8], bf16x8 (&out)[3])
   for (int q = 0; q < 3; ++q) __builtin_memcpy(&out[q], &pl[q], 16);
 }
 __device__ __forceinline__ void planes_of(const Bf16 (&v)[8], bf16x8 (&out)[1]) { __builtin_memcpy(&out[0], &v, 16); }
-__device__ __forceinline__ void planes_of(const float (&v)[8], float scale, f16x8 (&out)[2]) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const _Float16 high = static_cast<_Float16>(fmaf(v[e], scale, 0.f));
-    out[0][e] = high;
-    out[1][e] = static_cast<_Float16>(fmaf(v[e], scale, -static_cast<float>(high)));
-  }
-}
 
-__device__ __forceinline__ f32x16 mfma(const bf16x8& a, const bf16x8& b, const f32x16& c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-}
-__device__ __forceinline__ f32x16 mfma(const f16x8& a, const f16x8& b, const f32x16& c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-}
 // acc += a . b over the planes' products that count
-template <typename Part, int P>
-__device__ __forceinline__ void multiply_planes(const Part (&a)[P], const Part (&b)[P], f32x16& acc) {
+template <int P>
+__device__ __forceinline__ void multiply_planes(const bf16x8 (&a)[P], const bf16x8 (&b)[P], f32x16& acc) {
 #pragma unroll
   for (int pa = 0; pa < P; ++pa)
 #pragma unroll
-    for (int pb = 0; pa + pb < P; ++pb) acc = mfma(a[pa], b[pb], acc);
+    for (int pb = 0; pa + pb < P; ++pb) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[pa], b[pb], acc, 0, 0, 0);
 }
 
 // row of element e of a 32 x 32 block of results (its column is lane & 31)
@@ -179,13 +151,9 @@ __device__ __forceinline__ void stage_operand(const Operand<T>& op, int64_t r0, 
 
 // the operand of one 32 x 32 x 16 instruction: element `lane & 31` of the block at m0, eight
 // reduction indexes from k0 + 8 * (lane / 32)
-template <typename T, bool HALVES, bool DEEP>
-__device__ __forceinline__ void fragment(const char* lds, int m0, int k0, int lane, float scale,
-                                         typename Planes<T, HALVES>::Part (&out)[Planes<T, HALVES>::kCount]) {
-  const auto split = [&](const float (&v)[8]) {
-    if constexpr (HALVES) planes_of(v, scale, out);
-    else if constexpr (sizeof(T) == 4) planes_of(v, out);
-  };
+template <typename T, bool DEEP>
+__device__ __forceinline__ void fragment(const char* lds, int m0, int k0, int lane,
+                                         bf16x8 (&out)[Planes<T>::kCount]) {
   if constexpr (DEEP) {
     const int row = m0 + (lane & 31);
     const char* at = lds + row * 128;
@@ -197,7 +165,7 @@ __device__ __forceinline__ void fragment(const char* lds, int m0, int k0, int la
       float v[8];
       *reinterpret_cast<f32x4*>(&v[0]) = *reinterpret_cast<const f32x4*>(at + ((c ^ spread_128(row)) << 4));
       *reinterpret_cast<f32x4*>(&v[4]) = *reinterpret_cast<const f32x4*>(at + (((c + 1) ^ spread_128(row)) << 4));
-      split(v);
+      planes_of(v, out);
     }
   } else if constexpr (sizeof(T) == 2) {
     const int k = k0 + 8 * (lane >> 5) + ((lane & 15) >> 2);
@@ -214,7 +182,7 @@ __device__ __forceinline__ void fragment(const char* lds, int m0, int k0, int la
     float v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = *reinterpret_cast<const float*>(at + j * 512);
-    split(v);
+    planes_of(v, out);
   }
 }
 
@@ -230,13 +198,11 @@ __device__ __forceinline__ void clear(Tile& acc) {
 }
 
 // acc += A[m0 .., k0 .. k1] . B[n0 .., k0 .. k1]; k1 - k0 a multiple of the step.  `lds` holds two
-// stages of both operands; every wavefront has left them when this returns.  With HALVES the
-// operands are multiplied by `sa` and `sb`, powers of two, and the result with them.
-template <typename T, bool HALVES, bool ADEEP, bool BDEEP>
+// stages of both operands; every wavefront has left them when this returns.
+template <typename T, bool ADEEP, bool BDEEP>
 __device__ __forceinline__ void multiply(const Operand<T>& A, int64_t m0, const Operand<T>& B, int64_t n0, int64_t k0,
-                                         int64_t k1, char* lds, Tile& acc, float sa = 1.f, float sb = 1.f) {
-  typedef Planes<T, HALVES> Pl;
-  constexpr int kDepth = Step<T>::kDepth, P = Pl::kCount;
+                                         int64_t k1, char* lds, Tile& acc) {
+  constexpr int kDepth = Step<T>::kDepth, P = Planes<T>::kCount;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
   const unsigned stages = lds_offset(lds);
@@ -255,16 +221,16 @@ __device__ __forceinline__ void multiply(const Operand<T>& A, int64_t m0, const 
     }
 #pragma unroll
     for (int kk = 0; kk < kDepth; kk += 16) {
-      typename Pl::Part fa[2][P], fb[2][P];
+      bf16x8 fa[2][P], fb[2][P];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        fragment<T, HALVES, ADEEP>(a, wm + 32 * i, kk, lane, sa, fa[i]);
-        fragment<T, HALVES, BDEEP>(b, wn + 32 * i, kk, lane, sb, fb[i]);
+        fragment<T, ADEEP>(a, wm + 32 * i, kk, lane, fa[i]);
+        fragment<T, BDEEP>(b, wn + 32 * i, kk, lane, fb[i]);
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) multiply_planes(fa[i], fb[j], acc[i][j]);
+        for (int j = 0; j < 2; ++j) multiply_planes<P>(fa[i], fb[j], acc[i][j]);
     }
     cur ^= 1;
   }
