@@ -799,12 +799,22 @@ __global__ __launch_bounds__(kThreads) void k_wide_stats(int64_t B, int64_t V, O
   const StreamLane at = stream_lane<KD>(lane);
   bf16x8 own[2][KD];
   load_owned(x, b0, lane, own);
-  float top[2], sum[2];
+  // The sums are relative to a reference logit that follows the largest one only when that gets
+  // kSlack ahead (2^60), so that most half steps are a multiply-add, an exponential and an addition
+  // per logit: 2^(z log2 e - c), c = ref * log2 e rounded, `back` = what the rounding has to be put
+  // right by.  Where the rounding alone could leave the exponent's range (logits of millions) c is 0
+  // and the reference is taken off the logits first.
+  constexpr float kSlack = 41.f;
+  float top[2], sum[2], ref[2], limit[2], c[2], back[2];
+  bool any_far = false;
   int y[2];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const int64_t b = b0 + 32 * j + (lane & 31);
     top[j] = -INFINITY;
+    ref[j] = limit[j] = -INFINITY;
+    c[j] = 0.f;
+    back[j] = 1.f;
     sum[j] = 0.f;
     y[j] = b < B ? int(label_of(b, of.labels, of.idx, of.n_labels, of.V)) : -1;
   }
@@ -833,25 +843,43 @@ __global__ __launch_bounds__(kThreads) void k_wide_stats(int64_t B, int64_t V, O
   };
   // the logits of one half step while the other's are summed
   const auto turn = [&](const char* tile, int sub, f32x16 (&next)[2], f32x16 (&z)[2]) {
-    Reference ref[2];
-    float part[2] = {0.f, 0.f};
+    float m[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      f32x16 one[1] = {z[j]};
-      const float m = fmaxf(largest(one), top[j]), r = m == -INFINITY ? 0.f : m;
-      ref[j] = reference_of(one, r);
-      z[j] = one[0];
-      sum[j] *= exp2_raw((top[j] - r) * kLog2e);
-      top[j] = m;
+      const f32x16 one[1] = {z[j]};
+      m[j] = largest(one);
+      top[j] = fmaxf(top[j], m[j]);
+    }
+    if (__any(m[0] > limit[0] || m[1] > limit[1])) {                       // rare after the first few
+      any_far = false;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (m[j] > limit[j]) {
+          sum[j] *= exp2_raw((ref[j] - m[j]) * kLog2e) * back[j];
+          ref[j] = m[j];
+          limit[j] = m[j] + kSlack;
+          const bool far = !(fabsf(m[j]) < kFarLogit);
+          c[j] = far ? 0.f : m[j] * kLog2e;
+          back[j] = far ? 1.f : exp2_raw(-fmaf(m[j], kLog2e, -c[j]));
+          sum[j] *= far ? 1.f : exp2_raw(fmaf(m[j], kLog2e, -c[j]));
+        }
+        any_far = any_far || __any(!(fabsf(ref[j]) < kFarLogit) && ref[j] != -INFINITY);
+      }
+    }
+    if (any_far) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float off = !(fabsf(ref[j]) < kFarLogit) && ref[j] != -INFINITY ? ref[j] : 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) z[j][e] -= off;
+      }
     }
     StreamLane here = at;                        // its variants are made where they are used, not kept
     asm volatile("" : "+v"(here.direct));
     stream_logits_between(tile, sub, here, own, next, [&](int i) {
-      part[i >> 4] += exp2_raw(fmaf(z[i >> 4][i & 15], kLog2e, -ref[i >> 4].c));
-      asm volatile("" : "+v"(part[i >> 4]));     // now, not where the sum is used
+      sum[i >> 4] += exp2_raw(fmaf(z[i >> 4][i & 15], kLog2e, -c[i >> 4]));
+      asm volatile("" : "+v"(sum[i >> 4]));      // now, not where the sum is used
     });
-#pragma unroll
-    for (int j = 0; j < 2; ++j) sum[j] = fmaf(part[j], ref[j].fix, sum[j]);
   };
   const unsigned stages = lds_offset(lds);
   if (t0 < t1) {
@@ -870,11 +898,16 @@ __global__ __launch_bounds__(kThreads) void k_wide_stats(int64_t B, int64_t V, O
       turn(tile, 0, first, second);
       settle(first, t * kStreamRows);
       turn(tile, 1, second, first);
-      settle(second, t * kStreamRows + 32);
+        settle(second, t * kStreamRows + 32);
     }
+    // to the largest logit, and the last half step's share
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
+      float m = ref[j];
+      sum[j] *= back[j];
+      join_stats(m, sum[j], top[j], 0.f);
       f32x16 one[1] = {second[j]};
+      top[j] = m;
       accumulate(one, top[j], sum[j]);
     }
   }
@@ -957,7 +990,7 @@ __global__ __launch_bounds__(kGradThreads, 2) void k_wide_grads(int64_t owners, 
   constexpr int NB = 1, kWaves = kGradThreads / 64;
   // Taking turns keeps p across half steps; at 256 features that spills where the rows' shifts are
   // held, too (dweight of 4096 x 256 x 50000: 306 us with, 241 us without; dx 176 and 186 us).
-  constexpr bool kTurns = KD < 16 || !BY_CLASS;
+  constexpr bool kTurns = KD < 16;
   __shared__ __align__(16) float row_shift[kWaves][kStreamRows], row_top[kWaves][kStreamRows],
       row_factor[kWaves][kStreamRows];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
