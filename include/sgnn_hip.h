@@ -622,9 +622,14 @@ int sgnn_head_xent_f32(int64_t B, int64_t D, int64_t C, const float* E, int64_t 
  *                |a| <= 128 * 2^s; code < 0 exactly where x > 0 is false (NaN groups too); with
  *                slope 0 negative codes stand for 0.
  * An element is off by at most half its group's step.  `dtype` is SGNN_F32 or SGNN_BF16 and holds
- * for x, act, out, grad, dx and dW alike; each result is rounded once, to nearest even.
+ * for x, y, weight, out, grad, dx and dW alike (bf16 activations that the slope moved are
+ * rounded before the product); each result is rounded once, to nearest even.
  *
- * sgnn_save8            x -> codes, steps and, when act is given, a itself.
+ * sgnn_save8            x -> codes and steps.
+ * sgnn_saved8_linear    y = a . weight^T (weight H x F, row stride ldw) and, with codes and steps, those
+ *                       of x on the way (both NULL: nothing is kept).
+ * sgnn_saved8_linear_grad  dx = (grad . weight) * act'(x), the derivative read off the codes (codes may
+ *                       be NULL with slope 1).
  * sgnn_restore8         the values, exact in either type.
  * sgnn_saved8_input_grad  dx = code < 0 ? slope * grad : grad (slope 0: 0 there, whatever grad
  *                       holds); dx may be grad itself; slope 1 is refused (nothing to do).
@@ -633,7 +638,12 @@ int sgnn_head_xent_f32(int64_t B, int64_t D, int64_t C, const float* E, int64_t 
  *                       contents irrelevant.  Any row strides; 16-byte aligned rows are faster.
  */
 int sgnn_save8(int dtype, int64_t n, int64_t F, const void* x, int64_t ldx, float slope, void* codes, void* steps,
-               void* act, int64_t ldact, void* stream);
+               void* stream);
+int sgnn_saved8_linear(int dtype, int64_t n, int64_t F, int64_t H, const void* x, int64_t ldx, const void* weight,
+                       int64_t ldw, float slope, void* codes, void* steps, void* y, int64_t ldy, void* stream);
+int sgnn_saved8_linear_grad(int dtype, int64_t n, int64_t F, int64_t H, const void* codes, float slope,
+                            const void* grad, int64_t ldg, const void* weight, int64_t ldw, void* dx, int64_t lddx,
+                            void* stream);
 int sgnn_restore8(int dtype, int64_t n, int64_t F, const void* codes, const void* steps, float slope, void* out,
                   int64_t ldo, void* stream);
 int sgnn_saved8_input_grad(int dtype, int64_t n, int64_t F, const void* codes, float slope, const void* grad,

@@ -128,8 +128,11 @@ SIGNATURES = {
                                       c_void_p, c_int64, c_void_p, c_size_t, c_void_p]),
     "sgnn_sq_err_f32": (c_int, [c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_float,
                                 c_void_p, c_void_p, c_int64, c_void_p, c_size_t, c_void_p]),
-    "sgnn_save8": (c_int, [c_int, c_int64, c_int64, c_void_p, c_int64, c_float, c_void_p, c_void_p, c_void_p, c_int64,
-                           c_void_p]),
+    "sgnn_save8": (c_int, [c_int, c_int64, c_int64, c_void_p, c_int64, c_float, c_void_p, c_void_p, c_void_p]),
+    "sgnn_saved8_linear": (c_int, [c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_float,
+                                   c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    "sgnn_saved8_linear_grad": (c_int, [c_int, c_int64, c_int64, c_int64, c_void_p, c_float, c_void_p, c_int64, c_void_p,
+                                        c_int64, c_void_p, c_int64, c_void_p]),
     "sgnn_restore8": (c_int, [c_int, c_int64, c_int64, c_void_p, c_void_p, c_float, c_void_p, c_int64, c_void_p]),
     "sgnn_saved8_input_grad": (c_int, [c_int, c_int64, c_int64, c_void_p, c_float, c_void_p, c_int64, c_void_p, c_int64,
                                        c_void_p]),

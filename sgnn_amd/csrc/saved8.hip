@@ -14,7 +14,7 @@
 // without any rounding: the weight gradient dW = grad^T . value runs on the bf16 matrix
 // instructions with an exact left operand, and coding is exact in 32 bits, too (a multiplication
 // by a power of two, one rounding to a whole number).
-#include "common.h"
+#include "tile_product.h"
 
 namespace {
 
@@ -22,24 +22,6 @@ constexpr int kGroup = 32;
 constexpr int kMinBiased = 2;                     // s >= -125: half a step is still a normal number
 constexpr int kMaxBiased = 248;                   // s <= 121: 127.5 steps are still finite
 constexpr int kBadGroup = 255;
-
-typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-
-struct Bf16 { uint16_t bits; };
-
-__device__ __forceinline__ float widen(float v) { return v; }
-__device__ __forceinline__ float widen(Bf16 v) { return __uint_as_float(unsigned(v.bits) << 16); }
-template <typename T> __device__ __forceinline__ T narrow(float v);
-template <> __device__ __forceinline__ float narrow<float>(float v) { return v; }
-template <> __device__ __forceinline__ Bf16 narrow<Bf16>(float v) {          // nearest even, the only rounding of a result
-  unsigned u = __float_as_uint(v);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return Bf16{uint16_t(0x7fc0u)};
-  return Bf16{uint16_t((u + 0x7fffu + ((u >> 16) & 1u)) >> 16)};
-}
 
 // slope 0 is a selection, not a product: -inf becomes 0 there, NaN stays NaN
 __device__ __forceinline__ float activate(float x, float slope) {
@@ -58,6 +40,21 @@ __device__ __forceinline__ int step_of(unsigned peak_bits, bool plain) {      //
 }
 __device__ __forceinline__ float step_value(int biased) {      // NaN for a bad group
   return biased == kBadGroup ? __uint_as_float(0x7fc00000u) : __uint_as_float(unsigned(biased) << 23);
+}
+
+// the code of `a` (from `x`) at 1 / step = inv; inv 0 in a bad group
+__device__ __forceinline__ int code_of(float a, bool positive, float inv, bool plain) {
+  const float s = inv == 0.f ? 0.f : a * inv;
+  if (plain) {
+    const int q = int(rintf(s));
+    return q > 127 ? 127 : q < -127 ? -127 : q;  // beyond 127.5 * 2^121 only
+  }
+  const int q = int(ceilf(s)) - 1;
+  if (positive) return q < 0 ? 0 : (q > 127 ? 127 : q);
+  return q > -1 ? -1 : (q < -128 ? -128 : q);
+}
+__device__ __forceinline__ float inverse_step(int biased) {
+  return biased == kBadGroup ? 0.f : __uint_as_float(unsigned(254 - biased) << 23);
 }
 
 // `u` = code + 128 as a number: value = (u - (plain ? 128 : 127.5)) * step, exact.  With slope 0
@@ -99,8 +96,7 @@ constexpr int kEltThreads = 256;
 template <typename T>
 __global__ __launch_bounds__(kEltThreads) void k_save8(int64_t n, int F, const T* __restrict__ x, int64_t ldx,
                                                        bool wide, float slope, int rows, int per_row,
-                                                       uint8_t* __restrict__ codes, uint8_t* __restrict__ steps,
-                                                       T* __restrict__ act, int64_t ldact, bool act_wide) {
+                                                       uint8_t* __restrict__ codes, uint8_t* __restrict__ steps) {
   constexpr int V = Lane<T>::kElems, kPer = kGroup / V;
   const bool plain = slope == 1.f;
   const int groups = (F + kGroup - 1) / kGroup;
@@ -120,37 +116,20 @@ __global__ __launch_bounds__(kEltThreads) void k_save8(int64_t n, int F, const T
       const unsigned m = __float_as_uint(a[e]) & 0x7fffffffu;                 // a NaN is larger than any number here
       peak = m > peak ? m : peak;
     }
-    if (act != nullptr) {
-      T out[V];
-#pragma unroll
-      for (int e = 0; e < V; ++e) out[e] = narrow<T>(a[e]);
-      store_row<T, V>(act + r * ldact + f, left, act_wide, out);
-    }
 #pragma unroll
     for (int off = 1; off < kPer; off <<= 1) {
       const unsigned o = unsigned(__shfl_xor(int(peak), off));
       peak = o > peak ? o : peak;
     }
     const int biased = step_of(peak, plain);
-    const float inv = biased == kBadGroup ? 0.f : __uint_as_float(unsigned(254 - biased) << 23);
+    const float inv = inverse_step(biased);
     unsigned packed[V / 4];
 #pragma unroll
     for (int w = 0; w < V / 4; ++w) {
       packed[w] = 0;
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const float s = biased == kBadGroup ? 0.f : a[4 * w + b] * inv;
-        int q;
-        if (plain) {
-          q = int(rintf(s));
-          q = q > 127 ? 127 : q < -127 ? -127 : q;             // beyond 127.5 * 2^121 only
-        } else {
-          q = int(ceilf(s)) - 1;
-          if (widen(raw[4 * w + b]) > 0.f) q = q < 0 ? 0 : (q > 127 ? 127 : q);
-          else q = q > -1 ? -1 : (q < -128 ? -128 : q);
-        }
-        packed[w] |= (unsigned(q) & 0xffu) << (8 * b);
-      }
+      for (int e = 0; e < 4; ++e)
+        packed[w] |= (unsigned(code_of(a[4 * w + e], widen(raw[4 * w + e]) > 0.f, inv, plain)) & 0xffu) << (8 * e);
     }
     unsigned* dst = reinterpret_cast<unsigned*>(codes + r * (int64_t(groups) * kGroup) + f);
     if constexpr (V == 4) dst[0] = packed[0];
@@ -244,23 +223,6 @@ __device__ __forceinline__ bf16x8 slab_frag(const char* slab, int k0, int c0, in
   __builtin_memcpy(&r, &lo, 8);
   __builtin_memcpy(reinterpret_cast<char*>(&r) + 8, &hi, 8);
   return r;
-}
-
-// the high halves of two floats as a bf16 pair
-__device__ __forceinline__ unsigned high_halves(float lo, float hi) {
-  return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
-}
-
-__device__ __forceinline__ void split3(float v, float& a, float& b, float& c) {
-  const unsigned u = __float_as_uint(v);
-  a = __uint_as_float(u & 0xffff0000u);
-  const float r = v - a;
-  b = __uint_as_float(__float_as_uint(r) & 0xffff0000u);
-  c = r - b;
-  if ((u & 0x7f800000u) == 0x7f800000u) {         // infinities and NaN live in the first plane only
-    a = (u & 0x7fffffu) ? __uint_as_float(0x7fc00000u) : v;
-    b = c = 0.f;
-  }
 }
 
 template <typename T, int BH, int BF, int WH, int WF>
@@ -440,6 +402,318 @@ __global__ __launch_bounds__(256) void k_weight_grad_sum8(int F, int64_t total, 
     dW[(e / F) * lddw + e % F] = narrow<T>((part[0][c] + part[1][c]) + (part[2][c] + part[3][c]));
 }
 
+// ---------------------------------------------------------------------------------
+// The layer around the codes: y = a . weight^T from x itself, its codes written on the way, and
+// dx = (grad . weight) * act'(x) with the activation's derivative read off the codes.  Both are
+// bound by the rows they stream (x and y, grad and dx): a wavefront takes 32 * RB of them straight
+// from memory into the matrix instructions' operand, a lane holding eight features of one row;
+// features 0-3 and 8-11 of sixteen in the first half of the wavefront, the others in the second, so
+// that a load takes whole 32-byte pieces of a row.  The weight is split into bf16 planes on its way
+// to LDS, 64 features (of x, or units of grad) at a time, and serves the workgroup's rows.
+constexpr int kLinStep = 64;
+
+// eight elements of a row from `k`: k .. k + 3 and k + 8 .. k + 11, zeros from `left` on
+template <typename T>
+__device__ __forceinline__ void load_eight(const T* src, int left, T (&v)[8]) {
+  if (left >= 12) {
+    __builtin_memcpy(&v[0], src, 4 * sizeof(T));
+    __builtin_memcpy(&v[4], src + 8, 4 * sizeof(T));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (e & 3) + (e >> 2) * 8 < left ? src[(e & 3) + (e >> 2) * 8] : T{};
+  }
+}
+
+// one group's codes from a lane's sixteen of its 32 elements; lanes l and l + 32 share a row
+__device__ __forceinline__ void save_group(const float (&a)[2][8], const bool (&positive)[2][8], bool plain, bool store,
+                                           int half, uint8_t* code_row, uint8_t* step_at) {
+  unsigned peak = 0;
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const unsigned m = __float_as_uint(a[s][e]) & 0x7fffffffu;
+      peak = m > peak ? m : peak;
+    }
+  const unsigned other = unsigned(__shfl_xor(int(peak), 32));
+  const int biased = step_of(other > peak ? other : peak, plain);
+  const float inv = inverse_step(biased);
+  unsigned word[2][2];                           // features 16 s + 8 w + 4 half ..
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      word[s][w] = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        word[s][w] |= (unsigned(code_of(a[s][4 * w + e], positive[s][4 * w + e], inv, plain)) & 0xffu) << (8 * e);
+    }
+  // the first half keeps features 0 .. 15, the second 16 .. 31
+  const unsigned g0 = unsigned(__shfl_xor(int(half ? word[0][0] : word[1][0]), 32));
+  const unsigned g1 = unsigned(__shfl_xor(int(half ? word[0][1] : word[1][1]), 32));
+  const u32x4 out = half ? u32x4{g0, word[1][0], g1, word[1][1]} : u32x4{word[0][0], g0, word[0][1], g1};
+  if (store) {
+    *reinterpret_cast<u32x4*>(code_row + 16 * half) = out;
+    if (half == 0) *step_at = uint8_t(biased);
+  }
+}
+
+__device__ __forceinline__ void lin_planes(const float (&v)[8], bf16x8 (&out)[3]) { planes_of(v, out); }
+__device__ __forceinline__ void lin_planes(const float (&v)[8], bf16x8 (&out)[1]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) out[0][e] = static_cast<__bf16>(v[e]);
+}
+
+// y[r][h] for 128 * RB rows and 32 * NB units a workgroup; `codes` NULL: nothing is kept
+template <typename T, int NB, int RB>
+__global__ __launch_bounds__(256) void k_linear8(int64_t n, int F, int H, const T* __restrict__ x, int64_t ldx,
+                                                 const T* __restrict__ w, int64_t ldw, float slope,
+                                                 uint8_t* __restrict__ codes, uint8_t* __restrict__ steps,
+                                                 T* __restrict__ y, int64_t ldy) {
+  constexpr int P = Planes<T>::kCount, kUnits = 32 * NB;
+  constexpr int kChunks = kUnits * (kLinStep / 8) / 256;        // of 8 features, a thread's share of a weight step
+  __shared__ __align__(128) char lds[P * kUnits * kLinStep * 2];
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), half = lane >> 5;
+  const int h0 = int(blockIdx.y) * kUnits, groups = (F + kGroup - 1) / kGroup;
+  const int64_t first = (int64_t(blockIdx.x) * 4 + wave) * (32 * RB) + (lane & 31);
+  const bool plain = slope == 1.f, save = codes != nullptr && blockIdx.y == 0;
+  const T* rows[RB];
+#pragma unroll
+  for (int i = 0; i < RB; ++i) {
+    const int64_t r = first + 32 * i;
+    rows[i] = x + (r < n ? r : n - 1) * ldx + 4 * half;
+  }
+  T wreg[kChunks][8];
+  const auto fetch_weight = [&](int f0) {
+#pragma unroll
+    for (int l = 0; l < kChunks; ++l) {
+      const int c = t + 256 * l, h = h0 + (c >> 3), f = f0 + 16 * ((c & 7) >> 1) + 4 * (c & 1);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) wreg[l][e] = T{};
+      if (h < H) load_eight(w + int64_t(h) * ldw + f, F - f, wreg[l]);
+    }
+  };
+  T xreg[RB][2][8];
+  const auto fetch_rows = [&](int f0) {
+#pragma unroll
+    for (int i = 0; i < RB; ++i)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) load_eight(rows[i] + f0 + 16 * s, F - f0 - 16 * s - 4 * half, xreg[i][s]);
+  };
+  f32x16 acc[RB][NB];
+#pragma unroll
+  for (int i = 0; i < RB; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  fetch_weight(0);
+  fetch_rows(0);
+  for (int f0 = 0; f0 < F; f0 += kLinStep) {
+    __syncthreads();
+#pragma unroll
+    for (int l = 0; l < kChunks; ++l) {
+      const int c = t + 256 * l, row = c >> 3;
+      bf16x8 pl[P];
+      planes_of(wreg[l], pl);
+#pragma unroll
+      for (int q = 0; q < P; ++q)
+        *reinterpret_cast<bf16x8*>(lds + (q * kUnits + row) * (kLinStep * 2) + (((c & 7) ^ spread_128(row)) << 4)) = pl[q];
+    }
+    __syncthreads();
+    if (f0 + kLinStep < F) fetch_weight(f0 + kLinStep);
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {                // groups of 32 features
+      const int f = f0 + 32 * g;
+      if (f >= F) break;
+      float a[RB][2][8];
+      bool positive[RB][2][8];
+#pragma unroll
+      for (int i = 0; i < RB; ++i)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float v = widen(xreg[i][s][e]);
+            positive[i][s][e] = v > 0.f;
+            a[i][s][e] = activate(v, slope);
+          }
+      if (f + 32 < F) fetch_rows(f + 32);
+      if (save) {
+#pragma unroll
+        for (int i = 0; i < RB; ++i) {
+          const int64_t r = first + 32 * i;
+          save_group(a[i], positive[i], plain, r < n, half, codes + r * (int64_t(groups) * kGroup) + f,
+                     steps + r * groups + (f >> 5));
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        bf16x8 fa[RB][P];
+#pragma unroll
+        for (int i = 0; i < RB; ++i) lin_planes(a[i][s], fa[i]);
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          const int row = 32 * j + (lane & 31), c = 4 * g + 2 * s + half;
+          bf16x8 fb[P];
+#pragma unroll
+          for (int q = 0; q < P; ++q)
+            fb[q] = *reinterpret_cast<const bf16x8*>(lds + (q * kUnits + row) * (kLinStep * 2) +
+                                                     ((c ^ spread_128(row)) << 4));
+#pragma unroll
+          for (int i = 0; i < RB; ++i) multiply_planes<P>(fa[i], fb, acc[i][j]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < RB; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const int h = h0 + 32 * j + (lane & 31);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int64_t r = (int64_t(blockIdx.x) * 4 + wave) * (32 * RB) + 32 * i + block_row(e, lane);
+        if (r < n && h < H) y[r * ldy + h] = narrow<T>(acc[i][j][e]);
+      }
+    }
+}
+
+// dx[r][f] for 128 * RB rows and the features of blockIdx.y, 64 at a time, a workgroup.  The product
+// comes out features x rows, so that a lane holds four neighbouring features of one row: their codes
+// are one word and their results one store.
+template <typename T, int RB>
+__global__ __launch_bounds__(256) void k_linear_grad8(int64_t n, int F, int H, const T* __restrict__ g, int64_t ldg,
+                                                      const T* __restrict__ w, int64_t ldw, float slope,
+                                                      const uint8_t* __restrict__ codes, T* __restrict__ dx,
+                                                      int64_t lddx, bool dx_wide) {
+  constexpr int P = Planes<T>::kCount;
+  constexpr int kChunks = kLinStep * 8 / 256;    // of 8 features, a thread's share of a weight step (64 x 64)
+  constexpr int kKept = 4;                       // sixteens of units whose grad stays in registers
+  __shared__ __align__(128) char lds[P * kLinStep * 128];
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), half = lane >> 5;
+  const int64_t first = (int64_t(blockIdx.x) * 4 + wave) * (32 * RB) + (lane & 31);
+  const int ldq = (F + kGroup - 1) / kGroup * kGroup;
+  const T* rows[RB];
+#pragma unroll
+  for (int i = 0; i < RB; ++i) {
+    const int64_t r = first + 32 * i;
+    rows[i] = g + (r < n ? r : n - 1) * ldg + 4 * half;
+  }
+  bf16x8 fb[RB][kKept][P];
+  const auto fetch_grad = [&](int k0) {
+#pragma unroll
+    for (int i = 0; i < RB; ++i)
+#pragma unroll
+      for (int s = 0; s < kKept; ++s) {
+        T v[8];
+        load_eight(rows[i] + k0 + 16 * s, H - k0 - 16 * s - 4 * half, v);
+        planes_of(v, fb[i][s]);
+      }
+  };
+  T wreg[kChunks][8];
+  const auto fetch_weight = [&](int k0, int f0) {
+#pragma unroll
+    for (int l = 0; l < kChunks; ++l) {
+      const int c = t + 256 * l, h = k0 + (c >> 3), f = f0 + 8 * (c & 7);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) wreg[l][e] = T{};
+      if (h < H) {
+        const T* src = w + int64_t(h) * ldw + f;
+        if (f + 8 <= F) {
+          __builtin_memcpy(&wreg[l], src, sizeof(wreg[l]));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (f + e < F) wreg[l][e] = src[e];
+        }
+      }
+    }
+  };
+  const int tiles = (F + kLinStep - 1) / kLinStep;
+  const int tile0 = int(int64_t(tiles) * blockIdx.y / gridDim.y), tile1 = int(int64_t(tiles) * (blockIdx.y + 1) / gridDim.y);
+  if (tile0 >= tile1) return;                    // the whole workgroup
+  fetch_grad(0);
+  fetch_weight(0, tile0 * kLinStep);
+  for (int tile = tile0; tile < tile1; ++tile) {
+    const int f0 = tile * kLinStep;
+    f32x16 acc[RB][2];
+#pragma unroll
+    for (int i = 0; i < RB; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+    for (int k0 = 0; k0 < H; k0 += kLinStep) {
+      if (H > kLinStep) fetch_grad(k0);
+      __syncthreads();
+#pragma unroll
+      for (int l = 0; l < kChunks; ++l) {
+        const int c = t + 256 * l, row = c >> 3;
+        bf16x8 pl[P];
+        planes_of(wreg[l], pl);
+#pragma unroll
+        for (int q = 0; q < P; ++q)
+          *reinterpret_cast<bf16x8*>(lds + (q * kLinStep + row) * 128 + (((c & 7) ^ spread_128(row)) << 4)) = pl[q];
+      }
+      __syncthreads();
+      if (k0 + kLinStep < H) fetch_weight(k0 + kLinStep, f0);
+      else if (tile + 1 < tile1) fetch_weight(0, f0 + kLinStep);
+#pragma unroll
+      for (int s = 0; s < kKept; ++s) {
+        if (k0 + 16 * s >= H) break;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          // units 16 s + 4 half .. and eight further on, features 32 j ..
+          const int row = 16 * s + 4 * half + ((lane & 15) >> 2);
+          const int c = 4 * j + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), inner = (lane & 1) * 8;
+          typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+          bf16x8 fa[P];
+#pragma unroll
+          for (int q = 0; q < P; ++q) {
+            const char* at = lds + (q * kLinStep + row) * 128;
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + ((c ^ spread_128(row)) << 4) + inner));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (lds_s16x4*)(at + 8 * 128 + ((c ^ spread_128(row + 8)) << 4) + inner));
+            __builtin_memcpy(&fa[q], &lo, 8);
+            __builtin_memcpy(reinterpret_cast<char*>(&fa[q]) + 8, &hi, 8);
+          }
+#pragma unroll
+          for (int i = 0; i < RB; ++i) multiply_planes<P>(fa, fb[i][s], acc[i][j]);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < RB; ++i) {
+      const int64_t r = first + 32 * i;
+      if (r >= n) continue;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const int f = f0 + 32 * j + block_row(e, lane), left = F - f;
+          if (left <= 0) continue;
+          const unsigned q = slope == 1.f ? 0u : *reinterpret_cast<const unsigned*>(codes + r * ldq + f);
+          T v[4];
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            const float d = acc[i][j][e + b];
+            // x > 0 is false where the code's sign bit is set
+            v[b] = narrow<T>((q >> (8 * b + 7)) & 1u ? (slope == 0.f ? 0.f : slope * d) : d);
+          }
+          T* dst = dx + r * lddx + f;
+          if (dx_wide && left >= 4) {
+            __builtin_memcpy(__builtin_assume_aligned(dst, 4 * sizeof(T)), &v, 4 * sizeof(T));
+          } else {
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+              if (b < left) dst[b] = v[b];
+          }
+        }
+    }
+  }
+}
+
 struct GradPlan {
   int bh, bf, tiles_h, tiles_f, chunks;
   int64_t chunk_rows;
@@ -518,10 +792,10 @@ int launch_weight_grad(const GradPlan& p, int64_t n, int64_t F, int64_t H, const
 }  // namespace
 
 extern "C" int sgnn_save8(int dtype, int64_t n, int64_t F, const void* x, int64_t ldx, float slope, void* codes,
-                          void* steps, void* act, int64_t ldact, void* stream) {
+                          void* steps, void* stream) {
   using sgnn::fail;
   if (int rc = check_saved(dtype, n, F, slope)) return rc;
-  if (ldx < F || (act && ldact < F)) return fail(SGNN_ERR_INVALID, "row stride smaller than the width");
+  if (ldx < F) return fail(SGNN_ERR_INVALID, "row stride smaller than the width");
   if (n == 0) return SGNN_OK;
   if (!x || !codes || !steps) return fail(SGNN_ERR_INVALID, "null pointer");
   if (reinterpret_cast<uintptr_t>(codes) % 16) return fail(SGNN_ERR_INVALID, "codes must be 16-byte aligned");
@@ -532,16 +806,97 @@ extern "C" int sgnn_save8(int dtype, int64_t n, int64_t F, const void* x, int64_
   if (dtype == SGNN_F32) {
     if (int rc = elt_grid(n, F, Lane<float>::kElems, &g)) return rc;
     hipLaunchKernelGGL((k_save8<float>), dim3(g.blocks), dim3(kEltThreads), 0, st, n, int(F),
-                       static_cast<const float*>(x), ldx, wide_ok(x, ldx, 4), slope, g.rows, g.per_row, q, s,
-                       static_cast<float*>(act), ldact, wide_ok(act, ldact, 4));
+                       static_cast<const float*>(x), ldx, wide_ok(x, ldx, 4), slope, g.rows, g.per_row, q, s);
   } else {
     if (int rc = elt_grid(n, F, Lane<Bf16>::kElems, &g)) return rc;
     hipLaunchKernelGGL((k_save8<Bf16>), dim3(g.blocks), dim3(kEltThreads), 0, st, n, int(F),
-                       static_cast<const Bf16*>(x), ldx, wide_ok(x, ldx, 2), slope, g.rows, g.per_row, q, s,
-                       static_cast<Bf16*>(act), ldact, wide_ok(act, ldact, 2));
+                       static_cast<const Bf16*>(x), ldx, wide_ok(x, ldx, 2), slope, g.rows, g.per_row, q, s);
   }
   HIP_TRY(hipGetLastError());
   return SGNN_OK;
+}
+
+namespace {
+int check_linear(int dtype, int64_t n, int64_t F, int64_t H, float slope, const void* weight, int64_t ldw) {
+  using sgnn::fail;
+  if (int rc = check_saved(dtype, n, F, slope)) return rc;
+  if (H <= 0) return fail(SGNN_ERR_INVALID, "need H > 0");
+  if (H > (int64_t(1) << 20)) return fail(SGNN_ERR_UNSUPPORTED, "more than 2^20 units");
+  if ((n + 127) / 128 > 0xffffff) return fail(SGNN_ERR_UNSUPPORTED, "too many rows for one launch");
+  if (ldw < F) return fail(SGNN_ERR_INVALID, "row stride smaller than the width");
+  if (n > 0 && !weight) return fail(SGNN_ERR_INVALID, "null pointer");
+  return SGNN_OK;
+}
+
+// 64 rows a wavefront halve the weight's share of the work; 32 keep more of the card busy on few rows
+constexpr int64_t kManyRows = 256 * 256;
+
+template <typename T>
+int launch_linear(int64_t n, int64_t F, int64_t H, const void* x, int64_t ldx, const void* w, int64_t ldw, float slope,
+                  uint8_t* codes, uint8_t* steps, void* y, int64_t ldy, hipStream_t st) {
+#define SGNN_LIN8(NB, RB)                                                                                          \
+  hipLaunchKernelGGL((k_linear8<T, NB, RB>), dim3(unsigned((n + 128 * RB - 1) / (128 * RB)),                       \
+                                                  unsigned((H + 32 * NB - 1) / (32 * NB))),                        \
+                     dim3(256), 0, st, n, int(F), int(H), static_cast<const T*>(x), ldx, static_cast<const T*>(w), \
+                     ldw, slope, codes, steps, static_cast<T*>(y), ldy)
+  const bool many = n >= kManyRows;
+  if (H <= 32) { if (many) SGNN_LIN8(1, 2); else SGNN_LIN8(1, 1); }
+  else if (H <= 64) { if (many) SGNN_LIN8(2, 2); else SGNN_LIN8(2, 1); }
+  else { if (many) SGNN_LIN8(4, 2); else SGNN_LIN8(4, 1); }
+#undef SGNN_LIN8
+  HIP_TRY(hipGetLastError());
+  return SGNN_OK;
+}
+
+template <typename T>
+int launch_linear_grad(int64_t n, int64_t F, int64_t H, const void* g, int64_t ldg, const void* w, int64_t ldw,
+                       float slope, const uint8_t* codes, void* dx, int64_t lddx, hipStream_t st) {
+  const int rb = n >= kManyRows ? 2 : 1;
+  const int64_t blocks = (n + 128 * rb - 1) / (128 * rb), tiles = (F + kLinStep - 1) / kLinStep;
+  int64_t across = (1024 + blocks - 1) / blocks;
+  if (across > tiles) across = tiles;
+  const dim3 grid{unsigned(blocks), unsigned(across), 1};
+  const bool wide = wide_ok(dx, lddx, sizeof(T));
+  if (rb == 2)
+    hipLaunchKernelGGL((k_linear_grad8<T, 2>), grid, dim3(256), 0, st, n, int(F), int(H), static_cast<const T*>(g), ldg,
+                       static_cast<const T*>(w), ldw, slope, codes, static_cast<T*>(dx), lddx, wide);
+  else
+    hipLaunchKernelGGL((k_linear_grad8<T, 1>), grid, dim3(256), 0, st, n, int(F), int(H), static_cast<const T*>(g), ldg,
+                       static_cast<const T*>(w), ldw, slope, codes, static_cast<T*>(dx), lddx, wide);
+  HIP_TRY(hipGetLastError());
+  return SGNN_OK;
+}
+}  // namespace
+
+extern "C" int sgnn_saved8_linear(int dtype, int64_t n, int64_t F, int64_t H, const void* x, int64_t ldx,
+                                  const void* weight, int64_t ldw, float slope, void* codes, void* steps, void* y,
+                                  int64_t ldy, void* stream) {
+  using sgnn::fail;
+  if (int rc = check_linear(dtype, n, F, H, slope, weight, ldw)) return rc;
+  if (ldx < F || ldy < H) return fail(SGNN_ERR_INVALID, "row stride smaller than the width");
+  if (n == 0) return SGNN_OK;
+  if (!x || !y || (codes == nullptr) != (steps == nullptr)) return fail(SGNN_ERR_INVALID, "null pointer");
+  if (reinterpret_cast<uintptr_t>(codes) % 16) return fail(SGNN_ERR_INVALID, "codes must be 16-byte aligned");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  uint8_t* q = static_cast<uint8_t*>(codes);
+  uint8_t* s = static_cast<uint8_t*>(steps);
+  if (dtype == SGNN_F32) return launch_linear<float>(n, F, H, x, ldx, weight, ldw, slope, q, s, y, ldy, st);
+  return launch_linear<Bf16>(n, F, H, x, ldx, weight, ldw, slope, q, s, y, ldy, st);
+}
+
+extern "C" int sgnn_saved8_linear_grad(int dtype, int64_t n, int64_t F, int64_t H, const void* codes, float slope,
+                                       const void* grad, int64_t ldg, const void* weight, int64_t ldw, void* dx,
+                                       int64_t lddx, void* stream) {
+  using sgnn::fail;
+  if (int rc = check_linear(dtype, n, F, H, slope, weight, ldw)) return rc;
+  if (ldg < H || lddx < F) return fail(SGNN_ERR_INVALID, "row stride smaller than the width");
+  if (n == 0) return SGNN_OK;
+  if (!grad || !dx || (!codes && slope != 1.f)) return fail(SGNN_ERR_INVALID, "null pointer");
+  if (reinterpret_cast<uintptr_t>(codes) % 16) return fail(SGNN_ERR_INVALID, "codes must be 16-byte aligned");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const uint8_t* q = static_cast<const uint8_t*>(codes);
+  if (dtype == SGNN_F32) return launch_linear_grad<float>(n, F, H, grad, ldg, weight, ldw, slope, q, dx, lddx, st);
+  return launch_linear_grad<Bf16>(n, F, H, grad, ldg, weight, ldw, slope, q, dx, lddx, st);
 }
 
 extern "C" int sgnn_restore8(int dtype, int64_t n, int64_t F, const void* codes, const void* steps, float slope,

@@ -119,58 +119,68 @@ class SavedInt8:
 
     def input_grad(self, grad):
         """``grad * act'(x)``: the gradient of the activation's input from that of its output."""
-        return self._input_grad(self._grad(grad, self.shape[1], "the activation's gradient"), in_place=False)
-
-    def _input_grad(self, grad, in_place):
+        grad = self._grad(grad, self.shape[1], "the activation's gradient")
         if self.slope == 1.0:
             return grad
         n, F = self.shape
-        out = grad if in_place else torch.empty(n, F, dtype=grad.dtype, device=self.device)
+        out = torch.empty(n, F, dtype=grad.dtype, device=self.device)
         _lib.call_on(self.device, _lib.load().sgnn_saved8_input_grad, TYPES[grad.dtype], n, F, self.codes.data_ptr(),
-                     self.slope, grad.data_ptr(), _ld(grad), out.data_ptr(), _ld(out))
+                     self.slope, grad.data_ptr(), _ld(grad), out.data_ptr(), F)
         return out
 
 
-def _save(x, slope, with_act):
+def _empty(n, F, device):
+    groups = -(-F // _lib.SAVED8_GROUP)
+    return (torch.empty(n, groups * _lib.SAVED8_GROUP, dtype=torch.int8, device=device),
+            torch.empty(n, groups, dtype=torch.uint8, device=device))
+
+
+def save_int8(x, slope=1.0):
+    """``x if x > 0 else slope * x`` in 8 bits (``slope`` 1: no activation, 0: ReLU)."""
     code = element_type(x, "the activation")
     if x.dim() != 2 or x.shape[1] == 0:
         raise ValueError(f"the activation must be a matrix with at least one column, got {tuple(x.shape)}")
     slope = checked_slope(slope)
     x = unit_rows(x.detach())
     n, F = x.shape
-    groups = -(-F // _lib.SAVED8_GROUP)
-    codes = torch.empty(n, groups * _lib.SAVED8_GROUP, dtype=torch.int8, device=x.device)
-    steps = torch.empty(n, groups, dtype=torch.uint8, device=x.device)
-    act = torch.empty(n, F, dtype=x.dtype, device=x.device) if with_act and slope != 1.0 else None
+    codes, steps = _empty(n, F, x.device)
     _lib.call_on(x.device, _lib.load().sgnn_save8, code, n, F, x.data_ptr(), _ld(x), slope, codes.data_ptr(),
-                 steps.data_ptr(), None if act is None else act.data_ptr(), F)
-    return SavedInt8(codes, steps, (n, F), slope, x.dtype), (x if act is None else act)
+                 steps.data_ptr())
+    return SavedInt8(codes, steps, (n, F), slope, x.dtype)
 
 
-def save_int8(x, slope=1.0):
-    """``x if x > 0 else slope * x`` in 8 bits (``slope`` 1: no activation, 0: ReLU)."""
-    return _save(x, slope, with_act=False)[0]
+def _linear(x, weight, slope, codes=None, steps=None):
+    x, w = unit_rows(x.detach()), unit_rows(weight.detach())
+    (n, F), H = x.shape, w.shape[0]
+    y = torch.empty(n, H, dtype=x.dtype, device=x.device)
+    _lib.call_on(x.device, _lib.load().sgnn_saved8_linear, TYPES[x.dtype], n, F, H, x.data_ptr(), _ld(x), w.data_ptr(),
+                 _ld(w), slope, None if codes is None else codes.data_ptr(), None if steps is None else steps.data_ptr(),
+                 y.data_ptr(), H)
+    return y
 
 
 class _LinearSaved(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, slope):
-        saved, act = _save(x, slope, with_act=True)
-        ctx.save_for_backward(saved.codes, saved.steps, weight)
-        ctx.meta = (saved.shape, saved.slope, saved.dtype)
-        with torch.autocast("cuda", enabled=False):          # in the operands' own type
-            return torch.nn.functional.linear(act, weight.detach())
+        codes, steps = _empty(*x.shape, x.device)
+        ctx.save_for_backward(codes, steps, weight)
+        ctx.meta = (tuple(x.shape), slope, x.dtype)
+        return _linear(x, weight, slope, codes, steps)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         codes, steps, weight = ctx.saved_tensors
-        saved = SavedInt8(codes, steps, *ctx.meta)
+        (n, F), slope, dtype = ctx.meta
         dx = dw = None
+        grad = unit_rows(grad)
         if ctx.needs_input_grad[0]:
-            dx = saved._input_grad(grad.matmul(weight), in_place=True)
+            w, H = unit_rows(weight), weight.shape[0]
+            dx = torch.empty(n, F, dtype=dtype, device=grad.device)
+            _lib.call_on(grad.device, _lib.load().sgnn_saved8_linear_grad, TYPES[dtype], n, F, H, codes.data_ptr(), slope,
+                         grad.data_ptr(), _ld(grad), w.data_ptr(), _ld(w), dx.data_ptr(), F)
         if ctx.needs_input_grad[1]:
-            dw = saved.weight_grad(grad)
+            dw = SavedInt8(codes, steps, (n, F), slope, dtype).weight_grad(grad)
         return dx, dw, None
 
 
@@ -178,16 +188,16 @@ def linear_saved_int8(x, weight, slope=1.0):
     """``act(x) @ weight.T`` with ``act(x) = x if x > 0 else slope * x``, keeping nothing of its
     input but the 8-bit codes for the backward pass.  The output and ``x``'s gradient are those of
     the full activation; the weight's gradient is formed from the codes (off by half a step of
-    their group at most, element by element)."""
+    their group at most, element by element).  An infinite or NaN element makes its row's outputs
+    NaN."""
     code = element_type(x, "the input")
     if element_type(weight, "the weight") != code:
         raise TypeError(f"the input is {x.dtype}, the weight {weight.dtype}")
-    if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1]:
+    if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1] or 0 in weight.shape:
         raise ValueError(f"need an (n, F) input and an (H, F) weight, got {tuple(x.shape)} and {tuple(weight.shape)}")
     if weight.device != x.device:
         raise ValueError(f"the input is on {x.device}, the weight on {weight.device}")
+    slope = checked_slope(slope)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         return _LinearSaved.apply(x, weight, slope)
-    act = activated(x, checked_slope(slope))
-    with torch.autocast("cuda", enabled=False):
-        return torch.nn.functional.linear(act, weight)
+    return _linear(x, weight, slope)

@@ -210,21 +210,68 @@ def test_linear_layer(gpu_device, dtype, slope):
     grad = torch.randn(400, 24, device=gpu_device).to(t)
     y = snn.linear_saved_int8(x, w, slope=slope)
     y.backward(grad)
+    check_layer(x, w, grad, y, slope)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("slope", [0.0, 1.0, 0.2])
+@pytest.mark.parametrize("n,F,H", [(1, 1, 1), (3, 7, 33), (130, 31, 64), (129, 33, 65), (200, 65, 128), (64, 602, 130),
+                                   (257, 96, 200), (500, 300, 16), (66000, 40, 20), (65537, 33, 70)])
+def test_linear_layer_sizes(gpu_device, dtype, slope, n, F, H):
+    t = DTYPES[dtype]
+    g = torch.Generator().manual_seed(n + F + H)
+    x = inputs(n, F, t, gpu_device, seed=n, spread=0.5).requires_grad_()
+    w = (torch.randn(H, F, generator=g) / F ** 0.5).to(gpu_device, t).requires_grad_()
+    grad = torch.randn(n, H, generator=g).to(gpu_device, t)
+    y = snn.linear_saved_int8(x, w, slope=slope)
+    y.backward(grad)
+    check_layer(x, w, grad, y, slope)
+
+
+def check_layer(x, w, grad, y, slope):
+    t = x.dtype
+    F, H = x.shape[1], w.shape[0]
     xd, wd, gd = x.detach().double(), w.detach().double(), grad.double()
     s = float(np.float32(slope))
     act = torch.where(xd > 0, xd, s * xd)
     half = HALF_STEP[t]
-    # a rounded activation, a 32-bit sum of 90 terms and a rounded result
-    bound = (half + 92 * 2.0 ** -23) * (act.abs() @ wd.abs().t()) + half * (act @ wd.t()).abs()
+    # a rounded activation, a 32-bit sum of up to six products a feature and a rounded result
+    bound = (half + (6 * F + 20) * 2.0 ** -23) * (act.abs() @ wd.abs().t()) + half * (act @ wd.t()).abs() + LEAST[t]
     assert bool(((y.detach().double() - act @ wd.t()).abs() <= bound).all())
     dact = gd @ wd
     want = torch.where(xd > 0, dact, s * dact)
-    # a 32-bit sum of 24 terms, rounded, times the slope, rounded
-    bound = 26 * 2.0 ** -23 * (gd.abs() @ wd.abs()) + 2.1 * half * dact.abs()
+    # the same over the units, times the slope and rounded
+    bound = (6 * H + 20) * 2.0 ** -23 * (gd.abs() @ wd.abs()) + 1.01 * half * dact.abs() + LEAST[t]
     assert bool(((x.grad.double() - want).abs() <= bound).all())
     assert torch.equal(w.grad, snn.save_int8(x.detach(), slope).weight_grad(grad))
     with torch.no_grad():
         assert torch.equal(snn.linear_saved_int8(x, w, slope=slope), y)
+        frozen = snn.linear_saved_int8(x.detach(), w.detach(), slope=slope)
+    assert torch.equal(frozen, y)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_layer_layouts(gpu_device, dtype):
+    """Strided, transposed, offset and expanded operands in the middle of NaN: the results of their copies."""
+    t = DTYPES[dtype]
+    n, F, H = 150, 45, 37
+    xs, ws, gs = (torch.full((r, c), float("nan"), device=gpu_device, dtype=t) for r, c in ((160, 64), (50, 60), (160, 50)))
+    x, w, g = xs[3:153, 5:50], ws[2:39, 7:52], gs[1:151, 3:40]
+    x.copy_(inputs(n, F, t, gpu_device, seed=1, spread=0.5))
+    w.copy_(torch.randn(H, F, device=gpu_device) / 7)
+    g.copy_(torch.randn(n, H, device=gpu_device))
+
+    def run(x, w, g):
+        xi, wi = x.detach().requires_grad_(), w.detach().requires_grad_()
+        y = snn.linear_saved_int8(xi, wi, slope=0.2)
+        return (y.detach(), *torch.autograd.grad(y, (xi, wi), g))
+    want = run(x.contiguous(), w.contiguous(), g.contiguous())
+    for args in ((x, w, g), (x.t().contiguous().t(), w.t().contiguous().t(), g.t().contiguous().t())):
+        for a, b in zip(run(*args), want):
+            assert torch.equal(a, b)
+    one = g[:1].expand(n, H)
+    for a, b in zip(run(x, w, one), run(x.contiguous(), w.contiguous(), one.contiguous())):
+        assert torch.equal(a, b)
 
 
 def test_linear_layer_gradient_against_differences(gpu_device):

@@ -22,7 +22,7 @@ P = ctypes.c_void_p(4096)                            # never followed: every cal
 ])
 def test_save_refuses(dtype, n, F, ldx, slope, x, codes, word):
     mod, lib = _lib()
-    rc = lib.sgnn_save8(dtype, n, F, x, ldx, slope, codes, P, None, 0, None)
+    rc = lib.sgnn_save8(dtype, n, F, x, ldx, slope, codes, P, None)
     assert rc < 0 and word in lib.sgnn_last_error()
     with pytest.raises(mod.SgnnHipError):
         mod.check(rc)
@@ -30,7 +30,16 @@ def test_save_refuses(dtype, n, F, ldx, slope, x, codes, word):
 
 def test_the_other_entry_points_refuse():
     _, lib = _lib()
-    assert lib.sgnn_save8(0, 4, 8, P, 8, 0.0, P, P, P, 7, None) == -1
+    assert lib.sgnn_saved8_linear(0, 4, 8, 0, P, 8, P, 8, 0.0, P, P, P, 4, None) == -1
+    assert lib.sgnn_saved8_linear(0, 4, 8, 4, P, 7, P, 8, 0.0, P, P, P, 4, None) == -1
+    assert lib.sgnn_saved8_linear(0, 4, 8, 4, P, 8, P, 7, 0.0, P, P, P, 4, None) == -1
+    assert lib.sgnn_saved8_linear(0, 4, 8, 4, P, 8, P, 8, 0.0, P, P, P, 3, None) == -1
+    assert lib.sgnn_saved8_linear(0, 4, 8, 4, P, 8, P, 8, 0.0, P, None, P, 4, None) == -1
+    assert lib.sgnn_saved8_linear(0, 4, 8, 4, P, 8, None, 8, 0.0, P, P, P, 4, None) == -1
+    assert lib.sgnn_saved8_linear(3, 4, 8, 4, P, 8, P, 8, 0.0, P, P, P, 4, None) == -1
+    assert lib.sgnn_saved8_linear_grad(0, 4, 8, 4, None, 0.0, P, 4, P, 8, P, 8, None) == -1
+    assert lib.sgnn_saved8_linear_grad(0, 4, 8, 4, P, 0.0, P, 3, P, 8, P, 8, None) == -1
+    assert lib.sgnn_saved8_linear_grad(0, 4, 8, 4, P, 0.0, P, 4, P, 8, P, 7, None) == -1
     assert lib.sgnn_restore8(0, 4, 8, P, P, 0.0, P, 7, None) == -1
     assert lib.sgnn_restore8(0, 4, 8, P, None, 0.0, P, 8, None) == -1
     assert lib.sgnn_saved8_input_grad(0, 4, 8, P, 1.0, P, 8, P, 8, None) == -1
@@ -48,7 +57,9 @@ def test_the_other_entry_points_refuse():
 
 def test_nothing_to_do_is_not_an_error():
     _, lib = _lib()
-    assert lib.sgnn_save8(0, 0, 8, None, 8, 0.0, None, None, None, 0, None) == 0
+    assert lib.sgnn_save8(0, 0, 8, None, 8, 0.0, None, None, None) == 0
+    assert lib.sgnn_saved8_linear(0, 0, 8, 4, None, 8, None, 8, 0.0, None, None, None, 4, None) == 0
+    assert lib.sgnn_saved8_linear_grad(0, 0, 8, 4, None, 0.0, None, 4, None, 8, None, 8, None) == 0
     assert lib.sgnn_restore8(1, 0, 8, None, None, 0.0, None, 8, None) == 0
     assert lib.sgnn_saved8_input_grad(1, 0, 8, None, 0.0, None, 8, None, 8, None) == 0
 
