@@ -24,10 +24,26 @@ constexpr int kMaxBiased = 248;                   // s <= 121: 127.5 steps are s
 constexpr int kBadGroup = 255;
 
 // slope 0 is a selection, not a product: -inf becomes 0 there, NaN stays NaN
-__device__ __forceinline__ float activate(float x, float slope) {
-  if (x > 0.f) return x;
-  if (slope == 0.f) return x != x ? x : 0.f;
-  return slope * x;
+template <int N>
+__device__ __forceinline__ void activate(float (&x)[N], float slope) {
+  if (slope == 1.f) return;
+  if (slope == 0.f) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = x[e] <= 0.f ? 0.f : x[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = x[e] > 0.f ? x[e] : slope * x[e];
+  }
+}
+// the largest magnitude, as bits: a NaN is larger than any number there
+template <int N>
+__device__ __forceinline__ unsigned peak_of(const float (&a)[N], unsigned peak = 0) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const unsigned m = __float_as_uint(a[e]) & 0x7fffffffu;
+    peak = m > peak ? m : peak;
+  }
+  return peak;
 }
 
 __device__ __forceinline__ int step_of(unsigned peak_bits, bool plain) {      // peak = max |a|, as bits
@@ -42,16 +58,19 @@ __device__ __forceinline__ float step_value(int biased) {      // NaN for a bad 
   return biased == kBadGroup ? __uint_as_float(0x7fc00000u) : __uint_as_float(unsigned(biased) << 23);
 }
 
-// the code of `a` (from `x`) at 1 / step = inv; inv 0 in a bad group
-__device__ __forceinline__ int code_of(float a, bool positive, float inv, bool plain) {
-  const float s = inv == 0.f ? 0.f : a * inv;
-  if (plain) {
-    const int q = int(rintf(s));
-    return q > 127 ? 127 : q < -127 ? -127 : q;  // beyond 127.5 * 2^121 only
+// four codes at 1 / step = inv (0 in a bad group), as a word.  They are formed as code + 128, which
+// the conversion to a byte holds within 0 .. 255 by itself: -129 becomes -128 and 128 becomes 127.
+// A positive element whose quotient fell to 0 keeps its sign by the maximum with `floor`, which also
+// drops the NaN of a bad group.
+__device__ __forceinline__ unsigned pack_codes(const float* a, float inv, bool plain) {
+  unsigned word = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float s = a[e] * inv;
+    const float u = plain ? fmaxf(rintf(s) + 128.f, 1.f) : fmaxf(ceilf(s) + 127.f, a[e] > 0.f ? 128.f : 0.f);
+    word = __builtin_amdgcn_cvt_pk_u8_f32(u, e, word);
   }
-  const int q = int(ceilf(s)) - 1;
-  if (positive) return q < 0 ? 0 : (q > 127 ? 127 : q);
-  return q > -1 ? -1 : (q < -128 ? -128 : q);
+  return word ^ 0x80808080u;
 }
 __device__ __forceinline__ float inverse_step(int biased) {
   return biased == kBadGroup ? 0.f : __uint_as_float(unsigned(254 - biased) << 23);
@@ -109,13 +128,10 @@ __global__ __launch_bounds__(kEltThreads) void k_save8(int64_t n, int F, const T
     T raw[V];
     load_row<T, V>(x + r * ldx + f, left, wide, raw);
     float a[V];
-    unsigned peak = 0;
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      a[e] = activate(widen(raw[e]), slope);
-      const unsigned m = __float_as_uint(a[e]) & 0x7fffffffu;                 // a NaN is larger than any number here
-      peak = m > peak ? m : peak;
-    }
+    for (int e = 0; e < V; ++e) a[e] = widen(raw[e]);
+    activate(a, slope);
+    unsigned peak = peak_of(a);
 #pragma unroll
     for (int off = 1; off < kPer; off <<= 1) {
       const unsigned o = unsigned(__shfl_xor(int(peak), off));
@@ -125,12 +141,7 @@ __global__ __launch_bounds__(kEltThreads) void k_save8(int64_t n, int F, const T
     const float inv = inverse_step(biased);
     unsigned packed[V / 4];
 #pragma unroll
-    for (int w = 0; w < V / 4; ++w) {
-      packed[w] = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        packed[w] |= (unsigned(code_of(a[4 * w + e], widen(raw[4 * w + e]) > 0.f, inv, plain)) & 0xffu) << (8 * e);
-    }
+    for (int w = 0; w < V / 4; ++w) packed[w] = pack_codes(a + 4 * w, inv, plain);
     unsigned* dst = reinterpret_cast<unsigned*>(codes + r * (int64_t(groups) * kGroup) + f);
     if constexpr (V == 4) dst[0] = packed[0];
     else *reinterpret_cast<u32x2*>(dst) = u32x2{packed[0], packed[1]};
@@ -425,29 +436,16 @@ __device__ __forceinline__ void load_eight(const T* src, int left, T (&v)[8]) {
 }
 
 // one group's codes from a lane's sixteen of its 32 elements; lanes l and l + 32 share a row
-__device__ __forceinline__ void save_group(const float (&a)[2][8], const bool (&positive)[2][8], bool plain, bool store,
-                                           int half, uint8_t* code_row, uint8_t* step_at) {
-  unsigned peak = 0;
-#pragma unroll
-  for (int s = 0; s < 2; ++s)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const unsigned m = __float_as_uint(a[s][e]) & 0x7fffffffu;
-      peak = m > peak ? m : peak;
-    }
-  const unsigned other = unsigned(__shfl_xor(int(peak), 32));
+__device__ __forceinline__ void save_group(const float (&a)[2][8], bool plain, bool store, int half, uint8_t* code_row,
+                                           uint8_t* step_at) {
+  const unsigned peak = peak_of(a[1], peak_of(a[0])), other = unsigned(__shfl_xor(int(peak), 32));
   const int biased = step_of(other > peak ? other : peak, plain);
   const float inv = inverse_step(biased);
   unsigned word[2][2];                           // features 16 s + 8 w + 4 half ..
 #pragma unroll
   for (int s = 0; s < 2; ++s)
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      word[s][w] = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        word[s][w] |= (unsigned(code_of(a[s][4 * w + e], positive[s][4 * w + e], inv, plain)) & 0xffu) << (8 * e);
-    }
+    for (int w = 0; w < 2; ++w) word[s][w] = pack_codes(a[s] + 4 * w, inv, plain);
   // the first half keeps features 0 .. 15, the second 16 .. 31
   const unsigned g0 = unsigned(__shfl_xor(int(half ? word[0][0] : word[1][0]), 32));
   const unsigned g1 = unsigned(__shfl_xor(int(half ? word[0][1] : word[1][1]), 32));
@@ -527,23 +525,20 @@ __global__ __launch_bounds__(256) void k_linear8(int64_t n, int F, int H, const 
       const int f = f0 + 32 * g;
       if (f >= F) break;
       float a[RB][2][8];
-      bool positive[RB][2][8];
 #pragma unroll
       for (int i = 0; i < RB; ++i)
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+        for (int s = 0; s < 2; ++s) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float v = widen(xreg[i][s][e]);
-            positive[i][s][e] = v > 0.f;
-            a[i][s][e] = activate(v, slope);
-          }
+          for (int e = 0; e < 8; ++e) a[i][s][e] = widen(xreg[i][s][e]);
+          activate(a[i][s], slope);
+        }
       if (f + 32 < F) fetch_rows(f + 32);
       if (save) {
 #pragma unroll
         for (int i = 0; i < RB; ++i) {
           const int64_t r = first + 32 * i;
-          save_group(a[i], positive[i], plain, r < n, half, codes + r * (int64_t(groups) * kGroup) + f,
+          save_group(a[i], plain, r < n, half, codes + r * (int64_t(groups) * kGroup) + f,
                      steps + r * groups + (f >> 5));
         }
       }
@@ -637,6 +632,17 @@ __global__ __launch_bounds__(256) void k_linear_grad8(int64_t n, int F, int H, c
   fetch_weight(0, tile0 * kLinStep);
   for (int tile = tile0; tile < tile1; ++tile) {
     const int f0 = tile * kLinStep;
+    unsigned signs[RB][2][4];                    // four features each, under way while the product forms
+#pragma unroll
+    for (int i = 0; i < RB; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int64_t r = first + 32 * i;
+          const int f = f0 + 32 * j + block_row(4 * e, lane);
+          signs[i][j][e] = slope != 1.f && r < n && f < F ? *reinterpret_cast<const unsigned*>(codes + r * ldq + f) : 0u;
+        }
     f32x16 acc[RB][2];
 #pragma unroll
     for (int i = 0; i < RB; ++i)
@@ -693,7 +699,7 @@ __global__ __launch_bounds__(256) void k_linear_grad8(int64_t n, int F, int H, c
         for (int e = 0; e < 16; e += 4) {
           const int f = f0 + 32 * j + block_row(e, lane), left = F - f;
           if (left <= 0) continue;
-          const unsigned q = slope == 1.f ? 0u : *reinterpret_cast<const unsigned*>(codes + r * ldq + f);
+          const unsigned q = signs[i][j][e >> 2];
           T v[4];
 #pragma unroll
           for (int b = 0; b < 4; ++b) {
