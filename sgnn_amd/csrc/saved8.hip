@@ -416,11 +416,14 @@ __global__ __launch_bounds__(256) void k_weight_grad_sum8(int F, int64_t total, 
 // ---------------------------------------------------------------------------------
 // The layer around the codes: y = a . weight^T from x itself, its codes written on the way, and
 // dx = (grad . weight) * act'(x) with the activation's derivative read off the codes.  Both are
-// bound by the rows they stream (x and y, grad and dx): a wavefront takes 32 * RB of them straight
-// from memory into the matrix instructions' operand, a lane holding eight features of one row;
-// features 0-3 and 8-11 of sixteen in the first half of the wavefront, the others in the second, so
-// that a load takes whole 32-byte pieces of a row.  The weight is split into bf16 planes on its way
-// to LDS, 64 features (of x, or units of grad) at a time, and serves the workgroup's rows.
+// bound by the rows they stream (x and y, grad and dx): a wavefront takes 32 of them straight from
+// memory into the matrix instructions' operand, a lane holding eight features of one row; features
+// 0-3 and 8-11 of sixteen in the first half of the wavefront, the others in the second, so that a
+// load takes whole 32-byte pieces of a row.  The weight is split into bf16 planes on its way to LDS,
+// 64 features (of x, or units of grad) at a time, and serves the workgroup's rows.  Measured on
+// 232965 x 256 fp32 with 64 units: y and the codes 103 us (3.5 TB/s of the 360 MB it moves), dx 116 us;
+// with 64 rows a wavefront, so that a piece of the weight read from LDS serves two products, 114 and
+// 129 us: half the wavefronts wait for the same loads.
 constexpr int kLinStep = 64;
 
 // eight elements of a row from `k`: k .. k + 3 and k + 8 .. k + 11, zeros from `left` on
@@ -462,8 +465,8 @@ __device__ __forceinline__ void lin_planes(const float (&v)[8], bf16x8 (&out)[1]
   for (int e = 0; e < 8; ++e) out[0][e] = static_cast<__bf16>(v[e]);
 }
 
-// y[r][h] for 128 * RB rows and 32 * NB units a workgroup; `codes` NULL: nothing is kept
-template <typename T, int NB, int RB>
+// y[r][h] for 128 rows and 32 * NB units a workgroup; `codes` NULL: nothing is kept
+template <typename T, int NB>
 __global__ __launch_bounds__(256) void k_linear8(int64_t n, int F, int H, const T* __restrict__ x, int64_t ldx,
                                                  const T* __restrict__ w, int64_t ldw, float slope,
                                                  uint8_t* __restrict__ codes, uint8_t* __restrict__ steps,
@@ -473,14 +476,9 @@ __global__ __launch_bounds__(256) void k_linear8(int64_t n, int F, int H, const 
   __shared__ __align__(128) char lds[P * kUnits * kLinStep * 2];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), half = lane >> 5;
   const int h0 = int(blockIdx.y) * kUnits, groups = (F + kGroup - 1) / kGroup;
-  const int64_t first = (int64_t(blockIdx.x) * 4 + wave) * (32 * RB) + (lane & 31);
+  const int64_t r = (int64_t(blockIdx.x) * 4 + wave) * 32 + (lane & 31);
   const bool plain = slope == 1.f, save = codes != nullptr && blockIdx.y == 0;
-  const T* rows[RB];
-#pragma unroll
-  for (int i = 0; i < RB; ++i) {
-    const int64_t r = first + 32 * i;
-    rows[i] = x + (r < n ? r : n - 1) * ldx + 4 * half;
-  }
+  const T* row_at = x + (r < n ? r : n - 1) * ldx + 4 * half;
   T wreg[kChunks][8];
   const auto fetch_weight = [&](int f0) {
 #pragma unroll
@@ -491,20 +489,16 @@ __global__ __launch_bounds__(256) void k_linear8(int64_t n, int F, int H, const 
       if (h < H) load_eight(w + int64_t(h) * ldw + f, F - f, wreg[l]);
     }
   };
-  T xreg[RB][2][8];
+  T xreg[2][8];
   const auto fetch_rows = [&](int f0) {
 #pragma unroll
-    for (int i = 0; i < RB; ++i)
-#pragma unroll
-      for (int s = 0; s < 2; ++s) load_eight(rows[i] + f0 + 16 * s, F - f0 - 16 * s - 4 * half, xreg[i][s]);
+    for (int s = 0; s < 2; ++s) load_eight(row_at + f0 + 16 * s, F - f0 - 16 * s - 4 * half, xreg[s]);
   };
-  f32x16 acc[RB][NB];
+  f32x16 acc[NB];
 #pragma unroll
-  for (int i = 0; i < RB; ++i)
+  for (int j = 0; j < NB; ++j)
 #pragma unroll
-    for (int j = 0; j < NB; ++j)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+    for (int e = 0; e < 16; ++e) acc[j][e] = 0.f;
   fetch_weight(0);
   fetch_rows(0);
   for (int f0 = 0; f0 < F; f0 += kLinStep) {
@@ -524,29 +518,20 @@ __global__ __launch_bounds__(256) void k_linear8(int64_t n, int F, int H, const 
     for (int g = 0; g < 2; ++g) {                // groups of 32 features
       const int f = f0 + 32 * g;
       if (f >= F) break;
-      float a[RB][2][8];
-#pragma unroll
-      for (int i = 0; i < RB; ++i)
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) a[i][s][e] = widen(xreg[i][s][e]);
-          activate(a[i][s], slope);
-        }
-      if (f + 32 < F) fetch_rows(f + 32);
-      if (save) {
-#pragma unroll
-        for (int i = 0; i < RB; ++i) {
-          const int64_t r = first + 32 * i;
-          save_group(a[i], plain, r < n, half, codes + r * (int64_t(groups) * kGroup) + f,
-                     steps + r * groups + (f >> 5));
-        }
-      }
+      float a[2][8];
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        bf16x8 fa[RB][P];
 #pragma unroll
-        for (int i = 0; i < RB; ++i) lin_planes(a[i][s], fa[i]);
+        for (int e = 0; e < 8; ++e) a[s][e] = widen(xreg[s][e]);
+        activate(a[s], slope);
+      }
+      if (f + 32 < F) fetch_rows(f + 32);
+      if (save)
+        save_group(a, plain, r < n, half, codes + r * (int64_t(groups) * kGroup) + f, steps + r * groups + (f >> 5));
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        bf16x8 fa[P];
+        lin_planes(a[s], fa);
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
           const int row = 32 * j + (lane & 31), c = 4 * g + 2 * s + half;
@@ -555,29 +540,26 @@ __global__ __launch_bounds__(256) void k_linear8(int64_t n, int F, int H, const 
           for (int q = 0; q < P; ++q)
             fb[q] = *reinterpret_cast<const bf16x8*>(lds + (q * kUnits + row) * (kLinStep * 2) +
                                                      ((c ^ spread_128(row)) << 4));
-#pragma unroll
-          for (int i = 0; i < RB; ++i) multiply_planes<P>(fa[i], fb, acc[i][j]);
+          multiply_planes<P>(fa, fb, acc[j]);
         }
       }
     }
   }
 #pragma unroll
-  for (int i = 0; i < RB; ++i)
+  for (int j = 0; j < NB; ++j) {
+    const int h = h0 + 32 * j + (lane & 31);
 #pragma unroll
-    for (int j = 0; j < NB; ++j) {
-      const int h = h0 + 32 * j + (lane & 31);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int64_t r = (int64_t(blockIdx.x) * 4 + wave) * (32 * RB) + 32 * i + block_row(e, lane);
-        if (r < n && h < H) y[r * ldy + h] = narrow<T>(acc[i][j][e]);
-      }
+    for (int e = 0; e < 16; ++e) {
+      const int64_t out = (int64_t(blockIdx.x) * 4 + wave) * 32 + block_row(e, lane);
+      if (out < n && h < H) y[out * ldy + h] = narrow<T>(acc[j][e]);
     }
+  }
 }
 
-// dx[r][f] for 128 * RB rows and the features of blockIdx.y, 64 at a time, a workgroup.  The product
+// dx[r][f] for 128 rows and the features of blockIdx.y, 64 at a time, a workgroup.  The product
 // comes out features x rows, so that a lane holds four neighbouring features of one row: their codes
 // are one word and their results one store.
-template <typename T, int RB>
+template <typename T>
 __global__ __launch_bounds__(256) void k_linear_grad8(int64_t n, int F, int H, const T* __restrict__ g, int64_t ldg,
                                                       const T* __restrict__ w, int64_t ldw, float slope,
                                                       const uint8_t* __restrict__ codes, T* __restrict__ dx,
@@ -587,24 +569,17 @@ __global__ __launch_bounds__(256) void k_linear_grad8(int64_t n, int F, int H, c
   constexpr int kKept = 4;                       // sixteens of units whose grad stays in registers
   __shared__ __align__(128) char lds[P * kLinStep * 128];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), half = lane >> 5;
-  const int64_t first = (int64_t(blockIdx.x) * 4 + wave) * (32 * RB) + (lane & 31);
+  const int64_t r = (int64_t(blockIdx.x) * 4 + wave) * 32 + (lane & 31);
   const int ldq = (F + kGroup - 1) / kGroup * kGroup;
-  const T* rows[RB];
-#pragma unroll
-  for (int i = 0; i < RB; ++i) {
-    const int64_t r = first + 32 * i;
-    rows[i] = g + (r < n ? r : n - 1) * ldg + 4 * half;
-  }
-  bf16x8 fb[RB][kKept][P];
+  const T* row_at = g + (r < n ? r : n - 1) * ldg + 4 * half;
+  bf16x8 fb[kKept][P];
   const auto fetch_grad = [&](int k0) {
 #pragma unroll
-    for (int i = 0; i < RB; ++i)
-#pragma unroll
-      for (int s = 0; s < kKept; ++s) {
-        T v[8];
-        load_eight(rows[i] + k0 + 16 * s, H - k0 - 16 * s - 4 * half, v);
-        planes_of(v, fb[i][s]);
-      }
+    for (int s = 0; s < kKept; ++s) {
+      T v[8];
+      load_eight(row_at + k0 + 16 * s, H - k0 - 16 * s - 4 * half, v);
+      planes_of(v, fb[s]);
+    }
   };
   T wreg[kChunks][8];
   const auto fetch_weight = [&](int k0, int f0) {
@@ -632,24 +607,19 @@ __global__ __launch_bounds__(256) void k_linear_grad8(int64_t n, int F, int H, c
   fetch_weight(0, tile0 * kLinStep);
   for (int tile = tile0; tile < tile1; ++tile) {
     const int f0 = tile * kLinStep;
-    unsigned signs[RB][2][4];                    // four features each, under way while the product forms
+    unsigned signs[2][4];                        // four features each, under way while the product forms
 #pragma unroll
-    for (int i = 0; i < RB; ++i)
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int e = 0; e < 4; ++e) {
+        const int f = f0 + 32 * j + block_row(4 * e, lane);
+        signs[j][e] = slope != 1.f && r < n && f < F ? *reinterpret_cast<const unsigned*>(codes + r * ldq + f) : 0u;
+      }
+    f32x16 acc[2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int64_t r = first + 32 * i;
-          const int f = f0 + 32 * j + block_row(4 * e, lane);
-          signs[i][j][e] = slope != 1.f && r < n && f < F ? *reinterpret_cast<const unsigned*>(codes + r * ldq + f) : 0u;
-        }
-    f32x16 acc[RB][2];
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
-    for (int i = 0; i < RB; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+      for (int e = 0; e < 16; ++e) acc[j][e] = 0.f;
     for (int k0 = 0; k0 < H; k0 += kLinStep) {
       if (H > kLinStep) fetch_grad(k0);
       __syncthreads();
@@ -684,37 +654,34 @@ __global__ __launch_bounds__(256) void k_linear_grad8(int64_t n, int F, int H, c
             __builtin_memcpy(&fa[q], &lo, 8);
             __builtin_memcpy(reinterpret_cast<char*>(&fa[q]) + 8, &hi, 8);
           }
-#pragma unroll
-          for (int i = 0; i < RB; ++i) multiply_planes<P>(fa, fb[i][s], acc[i][j]);
+          multiply_planes<P>(fa, fb[s], acc[j]);
         }
       }
     }
-#pragma unroll
-    for (int i = 0; i < RB; ++i) {
-      const int64_t r = first + 32 * i;
-      if (r >= n) continue;
+    // x > 0 is false where the code's sign bit is set
+    const auto result = [&](int j, int e) {
+      const float d = acc[j][e];
+      return narrow<T>((signs[j][e >> 2] >> (8 * (e & 3) + 7)) & 1u ? (slope == 0.f ? 0.f : slope * d) : d);
+    };
+    if (r >= n) continue;
+    if (dx_wide && f0 + kLinStep <= F) {         // whole words, and no other way of storing in sight of the compiler
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
-          const int f = f0 + 32 * j + block_row(e, lane), left = F - f;
-          if (left <= 0) continue;
-          const unsigned q = signs[i][j][e >> 2];
-          T v[4];
+          const T v[4] = {result(j, e), result(j, e + 1), result(j, e + 2), result(j, e + 3)};
+          typedef unsigned Word __attribute__((ext_vector_type(sizeof(T))));
+          Word word;
+          __builtin_memcpy(&word, &v, sizeof(word));
+          *reinterpret_cast<Word*>(dx + r * lddx + f0 + 32 * j + block_row(e, lane)) = word;
+        }
+    } else {
 #pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            const float d = acc[i][j][e + b];
-            // x > 0 is false where the code's sign bit is set
-            v[b] = narrow<T>((q >> (8 * b + 7)) & 1u ? (slope == 0.f ? 0.f : slope * d) : d);
-          }
-          T* dst = dx + r * lddx + f;
-          if (dx_wide && left >= 4) {
-            __builtin_memcpy(__builtin_assume_aligned(dst, 4 * sizeof(T)), &v, 4 * sizeof(T));
-          } else {
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int b = 0; b < 4; ++b)
-              if (b < left) dst[b] = v[b];
-          }
+        for (int e = 0; e < 16; ++e) {
+          const int f = f0 + 32 * j + block_row(e, lane);
+          if (f < F) dx[r * lddx + f] = result(j, e);
         }
     }
   }
@@ -834,21 +801,16 @@ int check_linear(int dtype, int64_t n, int64_t F, int64_t H, float slope, const 
   return SGNN_OK;
 }
 
-// 64 rows a wavefront halve the weight's share of the work; 32 keep more of the card busy on few rows
-constexpr int64_t kManyRows = 256 * 256;
-
 template <typename T>
 int launch_linear(int64_t n, int64_t F, int64_t H, const void* x, int64_t ldx, const void* w, int64_t ldw, float slope,
                   uint8_t* codes, uint8_t* steps, void* y, int64_t ldy, hipStream_t st) {
-#define SGNN_LIN8(NB, RB)                                                                                          \
-  hipLaunchKernelGGL((k_linear8<T, NB, RB>), dim3(unsigned((n + 128 * RB - 1) / (128 * RB)),                       \
-                                                  unsigned((H + 32 * NB - 1) / (32 * NB))),                        \
+#define SGNN_LIN8(NB)                                                                                              \
+  hipLaunchKernelGGL((k_linear8<T, NB>), dim3(unsigned((n + 127) / 128), unsigned((H + 32 * NB - 1) / (32 * NB))), \
                      dim3(256), 0, st, n, int(F), int(H), static_cast<const T*>(x), ldx, static_cast<const T*>(w), \
                      ldw, slope, codes, steps, static_cast<T*>(y), ldy)
-  const bool many = n >= kManyRows;
-  if (H <= 32) { if (many) SGNN_LIN8(1, 2); else SGNN_LIN8(1, 1); }
-  else if (H <= 64) { if (many) SGNN_LIN8(2, 2); else SGNN_LIN8(2, 1); }
-  else { if (many) SGNN_LIN8(4, 2); else SGNN_LIN8(4, 1); }
+  if (H <= 32) SGNN_LIN8(1);
+  else if (H <= 64) SGNN_LIN8(2);
+  else SGNN_LIN8(4);
 #undef SGNN_LIN8
   HIP_TRY(hipGetLastError());
   return SGNN_OK;
@@ -857,18 +819,14 @@ int launch_linear(int64_t n, int64_t F, int64_t H, const void* x, int64_t ldx, c
 template <typename T>
 int launch_linear_grad(int64_t n, int64_t F, int64_t H, const void* g, int64_t ldg, const void* w, int64_t ldw,
                        float slope, const uint8_t* codes, void* dx, int64_t lddx, hipStream_t st) {
-  const int rb = n >= kManyRows ? 2 : 1;
-  const int64_t blocks = (n + 128 * rb - 1) / (128 * rb), tiles = (F + kLinStep - 1) / kLinStep;
+  const int64_t blocks = (n + 127) / 128, tiles = (F + kLinStep - 1) / kLinStep;
+  // Few rows: features over several workgroups, each of which reads its rows of grad again.  Aimed at
+  // 1024 workgroups; at 2048 the 232965 rows (1821 workgroups by themselves) take 127 us, not 116.
   int64_t across = (1024 + blocks - 1) / blocks;
   if (across > tiles) across = tiles;
-  const dim3 grid{unsigned(blocks), unsigned(across), 1};
-  const bool wide = wide_ok(dx, lddx, sizeof(T));
-  if (rb == 2)
-    hipLaunchKernelGGL((k_linear_grad8<T, 2>), grid, dim3(256), 0, st, n, int(F), int(H), static_cast<const T*>(g), ldg,
-                       static_cast<const T*>(w), ldw, slope, codes, static_cast<T*>(dx), lddx, wide);
-  else
-    hipLaunchKernelGGL((k_linear_grad8<T, 1>), grid, dim3(256), 0, st, n, int(F), int(H), static_cast<const T*>(g), ldg,
-                       static_cast<const T*>(w), ldw, slope, codes, static_cast<T*>(dx), lddx, wide);
+  hipLaunchKernelGGL((k_linear_grad8<T>), dim3(unsigned(blocks), unsigned(across)), dim3(256), 0, st, n, int(F), int(H),
+                     static_cast<const T*>(g), ldg, static_cast<const T*>(w), ldw, slope, codes, static_cast<T*>(dx),
+                     lddx, wide_ok(dx, lddx, sizeof(T)));
   HIP_TRY(hipGetLastError());
   return SGNN_OK;
 }
