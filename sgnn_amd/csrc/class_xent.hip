@@ -988,8 +988,8 @@ __global__ __launch_bounds__(kGradThreads, 2) void k_wide_grads(int64_t owners, 
                                                             const float* __restrict__ share) {
   __shared__ __align__(128) char lds[2 * stream_bytes<KD>()];
   constexpr int NB = 1, kWaves = kGradThreads / 64;
-  // Taking turns keeps p across half steps; at 256 features that spills where the rows' shifts are
-  // held, too (dweight of 4096 x 256 x 50000: 306 us with, 241 us without; dx 176 and 186 us).
+  // Taking turns keeps p across half steps; at 256 features that no longer fits the registers
+  // (4096 x 256 x 50000: dweight 306 us with turns, 253 us without; dx 218 and 193 us).
   constexpr bool kTurns = KD < 16;
   __shared__ __align__(16) float row_shift[kWaves][kStreamRows], row_top[kWaves][kStreamRows],
       row_factor[kWaves][kStreamRows];

@@ -45,7 +45,7 @@ CUDA are not comparable with the ones produced here.
 An optimiser iteration itself runs on the library's own kernels where its shape allows:
 the batch projection with the row gather and the inner activation folded in
 (``_BatchProject``, ``_DenseProject``), the label head with its loss and gradients
-(``_HeadXent``), the target error (``_SqErr``), the reconstruction loss
+(``_HeadXent``; ``class_cross_entropy`` for thousands of classes), the target error (``_SqErr``), the reconstruction loss
 (``_FusedReconstruction``) and Adam with the ridge / LASSO penalty applied through the
 gradient (``_FusedAdam``); each has the stock torch operators as the route for shapes or
 dtypes it does not cover, and ``tests/test_gpu_train_step.py`` holds them to those
@@ -61,6 +61,7 @@ import torch.nn.functional as Fn
 
 from . import _lib
 from . import utils as prop
+from .class_loss import class_cross_entropy
 
 
 class Func(torch.nn.Module):
@@ -301,6 +302,14 @@ class _HeadXent(torch.autograd.Function):
         return dE * grad_loss, dWt * grad_loss, None, None, None
 
 
+# From this many classes on the loss runs over the classes in pieces instead of forming the batch's
+# logits and their gradient.  Loss and both gradients, replayed from a graph, logits formed / in
+# pieces: 64 rows of 64 features 32 / 53 us at 1024 classes, 62 / 58 at 4096, 190 / 82 at 16384;
+# 4096 rows of 128, 95 / 98, 251 / 177 and 927 / 591 us; 16384 rows of 256, 344 / 305, 1045 / 1046
+# and 4159 / 3933 us, with two arrays of rows x classes fewer in memory.
+_PIECEWISE_CLASSES = 4096
+
+
 def _head_cross_entropy(E, Wt, labels, idx, unit=False):
     """``cross_entropy(E @ Wt, labels[idx])``."""
     if (E.is_cuda and E.dtype == torch.float32 and E.dim() == 2 and Wt.dtype == torch.float32 and Wt.stride(1) == 1
@@ -308,6 +317,10 @@ def _head_cross_entropy(E, Wt, labels, idx, unit=False):
             and E.shape[1] <= 256 and Wt.shape[1] <= 64
             and 4 * (E.shape[1] * Wt.shape[1] + 8 * E.shape[1] + 8 * Wt.shape[1]) <= 65536):
         return _HeadXent.apply(E, Wt, labels, idx, unit)
+    if (E.is_cuda and E.dtype == torch.float32 and E.dim() == 2 and Wt.dtype == torch.float32
+            and labels.dtype == torch.int64 and labels.dim() == 1 and E.shape[0] > 0
+            and Wt.shape[1] >= _PIECEWISE_CLASSES):
+        return class_cross_entropy(E, Wt.t(), labels, idx)
     return _cross_entropy(E.matmul(Wt), labels, idx, unit)
 
 

@@ -463,3 +463,47 @@ def test_head_over_a_checkpointed_stack(gpu_device):
         assert (a - b).norm() <= 1e-4 * a.norm()
     for a, b in zip(full[2:4], kept[2:4]):
         assert (a - b).norm() <= 0.03 * a.norm()
+
+
+@pytest.mark.parametrize("indexed", [False, True])
+@pytest.mark.parametrize("B,D,V", [(64, 128, 4096), (300, 33, 5001)])
+def test_label_head_of_a_stacked_layer(gpu_device, B, D, V, indexed):
+    """The label head of the stacked training with thousands of classes runs through the same loss."""
+    from sgnn_amd.stacked import _head_cross_entropy
+    x, w, labels = make(B, D, V, torch.float32, gpu_device, seed=B, nodes=3 * B if indexed else B)
+    idx = torch.randperm(3 * B, generator=torch.Generator().manual_seed(3)).to(gpu_device)[:B] if indexed else None
+    ref = reference(x, w, labels, idx)
+    E, Wt = x.requires_grad_(), w.t().contiguous().requires_grad_()
+    loss = _head_cross_entropy(E, Wt, labels, idx, unit=True)
+    assert "ClassXent" in loss.grad_fn.name()
+    loss.backward()
+    assert Wt.grad.is_contiguous()
+    close(loss.detach(), ref["loss"].mean(), ref["loss_bound"].mean() + 1e-30, "mean loss")
+    close(E.grad, ref["dx"], ref["dx_bound"], "dE")
+    close(Wt.grad, ref["dw"].t(), ref["dw_bound"].t(), "dWt")
+
+
+def test_stacked_layer_with_thousands_of_classes(gpu_device):
+    """Its captured training steps give what the same steps give one by one, bit for bit."""
+    from sgnn_amd.norm_adj import NormAdj
+    from sgnn_amd.stacked import EmbeddingLayer, LayerParam, get_activation
+    n, F, V = 500, 40, 4500
+    g = torch.Generator().manual_seed(0)
+    edges = torch.randint(0, n, (2, 3000), generator=g).numpy()
+    adj = NormAdj.from_coo(edges[0], edges[1], None, n, gpu_device)
+    X = torch.randn(n, F, generator=g).to(gpu_device)
+    labels = torch.randint(0, V, (n,), generator=g).to(gpu_device)
+    results = []
+    for graph in (True, False):
+        torch.manual_seed(5)
+        p = LayerParam(16, inner_act=get_activation("leaky_relu=0.2"), act=get_activation("linear"), max_iter=12,
+                       batch_size=64, learning_rate=0.01, lam=1e-4)
+        layer = EmbeddingLayer(adj, labels, torch.ones(n, dtype=torch.bool, device=gpu_device), F, 16, V, p, gpu_device)
+        before = layer.Wt.detach().clone()
+        layer.use_graph = graph
+        layer.run(X)
+        assert layer.use_graph is graph                              # the capture did not fall back
+        assert not torch.equal(before, layer.Wt)
+        results.append((layer.W.detach().clone(), layer.Wt.detach().clone()))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
