@@ -212,6 +212,11 @@ __global__ __launch_bounds__(kEltThreads) void k_input_grad8(int64_t n, int F, c
 // bf16 numbers (8 + 8 + 8 bits of its mantissa, cut off, not rounded, so the sum is exact), which
 // makes every product exact and the sums those of 32-bit arithmetic; bf16 grad takes one plane.
 // Chunks go to the workspace and are added in chunk order by a second launch.
+// Measured with its sum on 232965 x 602 fp32, 128 units: 147 us (codes and grad are 260 MB, 51 us; the
+// matrix instructions of three planes 65 us, decoding and splitting as much again).  Two workgroups
+// of eight wavefronts on a compute unit take turns at these; at one, 227 us.  Staging one step
+// ahead into a second buffer saves a barrier a step and gains nothing (140 us instead of 137 without
+// the sum).  169343 x 256 bf16, 256 units after a ReLU: 53 us, for 130 MB and as much of partial sums.
 constexpr int kRowsStep = 32;
 
 template <int COLS>                               // byte offset of (row, col) in a row-major bf16 slab of COLS columns
@@ -237,7 +242,7 @@ __device__ __forceinline__ bf16x8 slab_frag(const char* slab, int k0, int c0, in
 }
 
 template <typename T, int BH, int BF, int WH, int WF>
-__global__ __launch_bounds__(64 * WH * WF) void k_weight_grad8(
+__global__ __launch_bounds__(64 * WH * WF, BH >= 128 ? 4 : 2) void k_weight_grad8(
     int64_t n, int F, int H, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ steps, float slope,
     const T* __restrict__ g, int64_t ldg, bool wide, int64_t chunk_rows, int chunks, int tiles_f, int tiles_h,
     T* __restrict__ dW, int64_t lddw, float* __restrict__ partial) {
@@ -255,7 +260,9 @@ __global__ __launch_bounds__(64 * WH * WF) void k_weight_grad8(
   // the tiles of one chunk of rows go to one XCD, one after the other: they share grad and codes through its L2
   const int tiles = tiles_f * tiles_h;
   const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
-  const int tile = slot % tiles, chunk = (slot / tiles) * 8 + xcd;
+  const bool spread = chunks < 8;                 // too few chunks for that: over all of them
+  const int tile = (spread ? int(blockIdx.x) : slot) % tiles;
+  const int chunk = spread ? int(blockIdx.x) / tiles : (slot / tiles) * 8 + xcd;
   if (chunk >= chunks) return;                    // the whole workgroup
   const int f0 = (tile % tiles_f) * BF, h0 = (tile / tiles_f) * BH;
   const int groups = (F + kGroup - 1) / kGroup, ldq = groups * kGroup;
@@ -692,6 +699,11 @@ struct GradPlan {
   int64_t chunk_rows;
 };
 
+// Workgroups that run at once on an XCD: two on each of its 32 compute units.  A workgroup more than
+// that starts when the others end: 232965 x 602 x 128 units (3 tiles) with 66 on two of the XCDs 180 us,
+// with 63 on each 137 us; with 32 165 us, with 96 147 us.
+constexpr int kSlots = 64;
+
 GradPlan grad_plan(int64_t n, int64_t F, int64_t H) {
   GradPlan p;
   p.bh = H <= 32 ? 32 : H <= 64 ? 64 : 128;
@@ -699,8 +711,18 @@ GradPlan grad_plan(int64_t n, int64_t F, int64_t H) {
   p.tiles_h = int((H + p.bh - 1) / p.bh);
   p.tiles_f = int((F + p.bf - 1) / p.bf);
   const int64_t steps = (n + kRowsStep - 1) / kRowsStep;
-  int64_t want = 512 / (int64_t(p.tiles_h) * p.tiles_f);
-  if (want < 1) want = 1;
+  const int64_t tiles = int64_t(p.tiles_h) * p.tiles_f;
+  int64_t want = tiles < 512 ? 512 / tiles : 1;
+  if (tiles <= kSlots) {                         // whole chunks for every XCD, filling its slots 1 to 4 times over
+    int per_xcd = 1;
+    double best = 0.;
+    for (int rounds = 1; rounds <= 4; ++rounds) {
+      const int c = int(rounds * kSlots / tiles);
+      const double used = double(c * tiles) / (rounds * kSlots);
+      if (used > best + 0.02) best = used, per_xcd = c;
+    }
+    want = 8 * int64_t(per_xcd);
+  }
   if (want > steps) want = steps;
   int64_t per = (steps + want - 1) / want;
   if (per < 1) per = 1;
@@ -743,7 +765,7 @@ int launch_weight_grad(const GradPlan& p, int64_t n, int64_t F, int64_t H, const
   const T* g = static_cast<const T*>(grad);
   T* out = static_cast<T*>(dW);
   const bool wide = wide_ok(grad, ldg, sizeof(T));
-  const unsigned blocks = unsigned((p.chunks + 7) / 8 * 8) * unsigned(p.tiles_f * p.tiles_h);
+  const unsigned blocks = unsigned((p.chunks < 8 ? p.chunks : (p.chunks + 7) / 8 * 8) * p.tiles_f * p.tiles_h);
 #define SGNN_WG8(BH, BF, WH, WF)                                                                                  \
   hipLaunchKernelGGL((k_weight_grad8<T, BH, BF, WH, WF>), dim3(blocks), dim3(64 * WH * WF), 0, st, n, int(F),     \
                      int(H), codes, steps, slope, g, ldg, wide, p.chunk_rows, p.chunks, p.tiles_f, p.tiles_h, out, \

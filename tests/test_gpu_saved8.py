@@ -151,7 +151,8 @@ def check_weight_grad(saved, grad):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("slope", [0.0, 1.0, 0.2])
 @pytest.mark.parametrize("n,F,H", [(1, 1, 1), (2, 33, 5), (31, 32, 32), (32, 256, 33), (33, 257, 64), (100, 602, 65),
-                                   (777, 40, 130), (5000, 100, 128), (4096, 300, 16), (20000, 64, 300)])
+                                   (777, 40, 130), (5000, 100, 128), (4096, 300, 16), (20000, 64, 300),
+                                   (300, 2100, 1100), (3000, 700, 1000), (2000, 1300, 900)])
 def test_weight_grad(gpu_device, dtype, slope, n, F, H):
     x = inputs(n, F, DTYPES[dtype], gpu_device, seed=n, spread=0.5)
     grad = torch.randn(n, H, generator=torch.Generator().manual_seed(H)).to(gpu_device, DTYPES[dtype])
@@ -310,7 +311,9 @@ def test_layer_keeps_only_the_codes(gpu_device):
     y = snn.linear_saved_int8(hidden, w, slope=0.0)
     del hidden
     kept = torch.cuda.memory_allocated(gpu_device) - before - y.numel() * 4
-    assert kept <= n * F + n * F // 32 + 4096
+    # codes, steps and y (subtracted at its size): the allocator hands out a block it has whole when
+    # less than 1 MiB of it would be left, so each may count for up to 1 MiB more.  x would be 97 MiB.
+    assert kept <= n * F + n * F // 32 + 4096 + 3 * 2 ** 20
     y.sum().backward()
 
 
