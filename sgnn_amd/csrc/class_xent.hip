@@ -1185,7 +1185,25 @@ struct Plan {
 };
 
 constexpr int64_t kPieceBytes = int64_t(96) << 20;      // of dz: stays in the 256 MB last-level cache with its operands
-constexpr int kWant = 512;                              // workgroups a launch should have: two per CU
+constexpr int kSlots = 512;                             // workgroups that run at once: two on a CU, by their LDS
+
+// Shares of a reduction of `most` steps for `groups` workgroups a share, where `slots` workgroups
+// run at once: as many as fill the slots, or, where the groups alone are more, the number up to
+// four whose last round is fullest (a fifth better than none, or none).
+int spread(int64_t slots, int64_t groups, int64_t most) {
+  int64_t s = slots / groups;
+  if (s < 1) {
+    s = 1;
+    double best = 0.8 * double(ceil_div(groups, slots));
+    for (int64_t q = 2; q <= 4; ++q)
+      if (const double rounds = double(ceil_div(groups * q, slots)) / double(q); rounds <= best) {
+        best = rounds;
+        s = q;
+      }
+  }
+  if (s > most) s = most;
+  return s < 1 ? 1 : int(s);
+}
 
 Plan make_plan(int dtype, int64_t B, int64_t D, int64_t V) {
   Plan p;
@@ -1195,21 +1213,14 @@ Plan make_plan(int dtype, int64_t B, int64_t D, int64_t V) {
   p.tiles_b = ceil_div(B, kTile);
   p.tiles_v = ceil_div(V, kTile);
   p.Bp = p.tiles_b * kTile;
-  int64_t s = ceil_div(kWant, p.tiles_b);
-  p.stat_splits = int(s < p.tiles_v ? s : p.tiles_v);
+  p.stat_splits = spread(kSlots, p.tiles_b, p.tiles_v);
   int64_t tiles = kPieceBytes / (p.Bp * int64_t(p.elem) * kTile);
   if (tiles < 1) tiles = 1;
   if (tiles > p.tiles_v) tiles = p.tiles_v;
   p.piece = tiles * kTile;
   p.tiles_d = int(ceil_div(D, kTile));
-  s = ceil_div(kWant, p.tiles_b * p.tiles_d);
-  int64_t most = p.piece / p.depth / 2;
-  p.dx_splits = int(s < most ? s : most);
-  s = ceil_div(kWant, tiles * p.tiles_d);
-  most = p.Bp / p.depth / 2;
-  p.dw_splits = int(s < most ? s : most);
-  if (p.dx_splits < 1) p.dx_splits = 1;
-  if (p.dw_splits < 1) p.dw_splits = 1;
+  p.dx_splits = spread(kSlots, p.tiles_b * p.tiles_d, p.piece / p.depth / 2);
+  p.dw_splits = spread(kSlots, tiles * p.tiles_d, p.Bp / p.depth / 2);
   return p;
 }
 
@@ -1252,21 +1263,6 @@ Wide make_wide(int dtype, int64_t B, int64_t D, int64_t V) {
   f.own_v = ceil_div(V, kOwnRows);
   f.steps_b = ceil_div(B, kStreamRows);
   f.steps_v = ceil_div(V, kStreamRows);
-  // `slots` workgroups run at once: as many splits as fill them, or, where the owners alone are
-  // more, the number up to four whose last round is fullest (a fifth better than none, or none)
-  const auto spread = [](int64_t slots, int64_t groups, int64_t steps) {
-    int64_t s = slots / groups;
-    if (s < 1) {
-      s = 1;
-      double best = 0.8 * double(ceil_div(groups, slots));
-      for (int64_t q = 2; q <= 4; ++q)
-        if (const double rounds = double(ceil_div(groups * q, slots)) / double(q); rounds <= best) {
-          best = rounds;
-          s = q;
-        }
-    }
-    return int(s < steps ? s : steps);
-  };
   // by what a CU's registers hold: two workgroups of four wavefronts up to 192 features; of eight, one, up to 64 two
   f.stat_splits = spread(f.KD < 16 ? 512 : 256, f.own_b, f.steps_v);
   f.dx_splits = spread(f.KD > 4 ? 256 : 512, f.own_b, f.steps_v);

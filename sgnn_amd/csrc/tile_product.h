@@ -151,38 +151,34 @@ __device__ __forceinline__ void stage_operand(const Operand<T>& op, int64_t r0, 
 
 // the operand of one 32 x 32 x 16 instruction: element `lane & 31` of the block at m0, eight
 // reduction indexes from k0 + 8 * (lane / 32)
-template <typename T, bool DEEP>
-__device__ __forceinline__ void fragment(const char* lds, int m0, int k0, int lane,
-                                         bf16x8 (&out)[Planes<T>::kCount]) {
+template <bool DEEP>
+__device__ __forceinline__ void read_fragment(const char* lds, int m0, int k0, int lane, bf16x8& out) {
   if constexpr (DEEP) {
-    const int row = m0 + (lane & 31);
-    const char* at = lds + row * 128;
-    if constexpr (sizeof(T) == 2) {
-      const int c = (k0 >> 3) + (lane >> 5);
-      out[0] = *reinterpret_cast<const bf16x8*>(at + ((c ^ spread_128(row)) << 4));
-    } else {
-      const int c = (k0 >> 2) + 2 * (lane >> 5);
-      float v[8];
-      *reinterpret_cast<f32x4*>(&v[0]) = *reinterpret_cast<const f32x4*>(at + ((c ^ spread_128(row)) << 4));
-      *reinterpret_cast<f32x4*>(&v[4]) = *reinterpret_cast<const f32x4*>(at + (((c + 1) ^ spread_128(row)) << 4));
-      planes_of(v, out);
-    }
-  } else if constexpr (sizeof(T) == 2) {
+    const int row = m0 + (lane & 31), c = (k0 >> 3) + (lane >> 5);
+    out = *reinterpret_cast<const bf16x8*>(lds + row * 128 + ((c ^ spread_128(row)) << 4));
+  } else {
     const int k = k0 + 8 * (lane >> 5) + ((lane & 15) >> 2);
     const int m = m0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
     const int at = ((m >> 3) ^ ((k & 3) << 2)) * 16 + (m & 7) * 2;       // k and k + 4 share k & 3
     typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds + k * 256 + at));
     const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds + (k + 4) * 256 + at));
-    __builtin_memcpy(&out[0], &lo, 8);
-    __builtin_memcpy(reinterpret_cast<char*>(&out[0]) + 8, &hi, 8);
+    __builtin_memcpy(&out, &lo, 8);
+    __builtin_memcpy(reinterpret_cast<char*>(&out) + 8, &hi, 8);
+  }
+}
+template <bool DEEP>
+__device__ __forceinline__ void read_fragment(const char* lds, int m0, int k0, int lane, float (&out)[8]) {
+  if constexpr (DEEP) {
+    const int row = m0 + (lane & 31), c = (k0 >> 2) + 2 * (lane >> 5);
+    const char* at = lds + row * 128;
+    *reinterpret_cast<f32x4*>(&out[0]) = *reinterpret_cast<const f32x4*>(at + ((c ^ spread_128(row)) << 4));
+    *reinterpret_cast<f32x4*>(&out[4]) = *reinterpret_cast<const f32x4*>(at + (((c + 1) ^ spread_128(row)) << 4));
   } else {
     const int k = k0 + 8 * (lane >> 5), m = m0 + (lane & 31);
     const char* at = lds + k * 512 + (((m >> 5) ^ ((k >> 3) & 1)) << 7) + (m & 31) * 4;
-    float v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = *reinterpret_cast<const float*>(at + j * 512);
-    planes_of(v, out);
+    for (int j = 0; j < 8; ++j) out[j] = *reinterpret_cast<const float*>(at + j * 512);
   }
 }
 
@@ -197,40 +193,104 @@ __device__ __forceinline__ void clear(Tile& acc) {
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 }
 
+// What a wavefront's 64 x 64 needs for sixteen of the reduction: A's two blocks, then B's
+typedef float Sixteen[4][8];
+typedef u32x4 SixteenPlanes[4][3];
+
+template <bool ADEEP, bool BDEEP>
+__device__ __forceinline__ void read_sixteen(const char* stage, int kk, int wm, int wn, int lane, Sixteen& v) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    read_fragment<ADEEP>(stage, wm + 32 * i, kk, lane, v[i]);
+    read_fragment<BDEEP>(stage + kStageBytes, wn + 32 * i, kk, lane, v[2 + i]);
+  }
+}
+// two neighbours of the 32 numbers a lane holds, to their planes
+__device__ __forceinline__ void take_apart(const Sixteen& v, int pair, SixteenPlanes& out) {
+  const int x = pair >> 2, e = 2 * (pair & 3);
+  float a0, b0, c0, a1, b1, c1;
+  split3(v[x][e], a0, b0, c0);
+  split3(v[x][e + 1], a1, b1, c1);
+  unsigned a = high_halves(a0, a1), b = high_halves(b0, b1), c = high_halves(c0, c1);
+  asm volatile("" : "+v"(a), "+v"(b), "+v"(c));  // now, not where it is used
+  out[x][0][e / 2] = a;
+  out[x][1][e / 2] = b;
+  out[x][2][e / 2] = c;
+}
+// the products of `now`, and between them `next` taken apart: a wavefront's arithmetic fills the 32
+// cycles of each matrix instruction (with all of a step's numbers taken apart before its products
+// 2048 x 602 against 10007 classes in fp32 takes 190 + 173 us for statistics and dz, so 177 + 166 us)
+__device__ __forceinline__ void multiply_sixteen(const SixteenPlanes& now, Tile& acc, const Sixteen& next,
+                                                 SixteenPlanes& then) {
+  constexpr int kPa[6] = {0, 0, 0, 1, 1, 2}, kPb[6] = {0, 1, 2, 0, 1, 0};
+  int pair = 0;
+#pragma unroll
+  for (int s = 0; s < 24; ++s) {
+    const int i = s / 12, j = s / 6 % 2, q = s % 6;
+    bf16x8 a, b;
+    __builtin_memcpy(&a, &now[i][kPa[q]], 16);
+    __builtin_memcpy(&b, &now[2 + j][kPb[q]], 16);
+    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc[i][j], 0, 0, 0);
+    if (s >= 4 && s % 5 != 3) take_apart(next, pair++, then);
+  }
+}
+
 // acc += A[m0 .., k0 .. k1] . B[n0 .., k0 .. k1]; k1 - k0 a multiple of the step.  `lds` holds two
 // stages of both operands; every wavefront has left them when this returns.
 template <typename T, bool ADEEP, bool BDEEP>
 __device__ __forceinline__ void multiply(const Operand<T>& A, int64_t m0, const Operand<T>& B, int64_t n0, int64_t k0,
                                          int64_t k1, char* lds, Tile& acc) {
-  constexpr int kDepth = Step<T>::kDepth, P = Planes<T>::kCount;
+  constexpr int kDepth = Step<T>::kDepth;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
   const unsigned stages = lds_offset(lds);
-  stage_operand<T, ADEEP>(A, m0, k0, stages, wave, lane);
-  stage_operand<T, BDEEP>(B, n0, k0, stages + kStageBytes, wave, lane);
+  const auto stage = [&](int64_t k, int at) {
+    stage_operand<T, ADEEP>(A, m0, k, stages + at * 2 * kStageBytes, wave, lane);
+    stage_operand<T, BDEEP>(B, n0, k, stages + (at * 2 + 1) * kStageBytes, wave, lane);
+  };
+  stage(k0, 0);
   int cur = 0;
+  if constexpr (sizeof(T) == 4) {
+    static_assert(kDepth == 32, "two sixteens a step");
+    Sixteen raw;
+    SixteenPlanes first, second;
+    landed();
+    __syncthreads();
+    if (k0 + kDepth < k1) stage(k0 + kDepth, 1);
+    read_sixteen<ADEEP, BDEEP>(lds, 0, wm, wn, lane, raw);
+#pragma unroll
+    for (int pair = 0; pair < 16; ++pair) take_apart(raw, pair, first);
+    for (int64_t k = k0; k < k1; k += kDepth) {
+      read_sixteen<ADEEP, BDEEP>(lds + cur * 2 * kStageBytes, 16, wm, wn, lane, raw);
+      multiply_sixteen(first, acc, raw, second);
+      landed();                                  // this wavefront's part of the next stage
+      __syncthreads();                           // everybody's, and this one has been read
+      cur ^= 1;
+      if (k + 2 * kDepth < k1) stage(k + 2 * kDepth, cur ^ 1);
+      read_sixteen<ADEEP, BDEEP>(lds + cur * 2 * kStageBytes, 0, wm, wn, lane, raw);    // behind the last: not used
+      multiply_sixteen(second, acc, raw, first);
+    }
+    __syncthreads();
+    return;
+  }
   for (int64_t k = k0; k < k1; k += kDepth) {
     landed();                                    // this wavefront's part of the stage
     __syncthreads();                             // everybody's, and the other stage is free
+    if (k + kDepth < k1) stage(k + kDepth, cur ^ 1);
     const char* a = lds + cur * 2 * kStageBytes;
-    const char* b = a + kStageBytes;
-    if (k + kDepth < k1) {
-      const unsigned next = stages + (cur ^ 1) * 2 * kStageBytes;
-      stage_operand<T, ADEEP>(A, m0, k + kDepth, next, wave, lane);
-      stage_operand<T, BDEEP>(B, n0, k + kDepth, next + kStageBytes, wave, lane);
-    }
 #pragma unroll
     for (int kk = 0; kk < kDepth; kk += 16) {
-      bf16x8 fa[2][P], fb[2][P];
+      bf16x8 fa[2], fb[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        fragment<T, ADEEP>(a, wm + 32 * i, kk, lane, fa[i]);
-        fragment<T, BDEEP>(b, wn + 32 * i, kk, lane, fb[i]);
+        read_fragment<ADEEP>(a, wm + 32 * i, kk, lane, fa[i]);
+        read_fragment<BDEEP>(a + kStageBytes, wn + 32 * i, kk, lane, fb[i]);
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) multiply_planes<P>(fa[i], fb[j], acc[i][j]);
+        for (int j = 0; j < 2; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[i], fb[j], acc[i][j], 0, 0, 0);
     }
     cur ^= 1;
   }
