@@ -62,15 +62,27 @@ __device__ __forceinline__ float step_value(int biased) {      // NaN for a bad 
 // the conversion to a byte holds within 0 .. 255 by itself: -129 becomes -128 and 128 becomes 127.
 // A positive element whose quotient fell to 0 keeps its sign by the maximum with `floor`, which also
 // drops the NaN of a bad group.
-__device__ __forceinline__ unsigned pack_codes(const float* a, float inv, bool plain) {
+template <bool PLAIN>
+__device__ __forceinline__ unsigned pack_four(const float* a, float inv) {
   unsigned word = 0;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const float s = a[e] * inv;
-    const float u = plain ? fmaxf(rintf(s) + 128.f, 1.f) : fmaxf(ceilf(s) + 127.f, a[e] > 0.f ? 128.f : 0.f);
+    const float u = PLAIN ? fmaxf(rintf(s) + 128.f, 1.f) : fmaxf(ceilf(s) + 127.f, a[e] > 0.f ? 128.f : 0.f);
     word = __builtin_amdgcn_cvt_pk_u8_f32(u, e, word);
   }
   return word ^ 0x80808080u;
+}
+// 4 * W elements: the choice is made once, not for every element
+template <int W>
+__device__ __forceinline__ void pack_codes(const float (&a)[4 * W], float inv, bool plain, unsigned (&word)[W]) {
+  if (plain) {
+#pragma unroll
+    for (int w = 0; w < W; ++w) word[w] = pack_four<true>(a + 4 * w, inv);
+  } else {
+#pragma unroll
+    for (int w = 0; w < W; ++w) word[w] = pack_four<false>(a + 4 * w, inv);
+  }
 }
 __device__ __forceinline__ float inverse_step(int biased) {
   return biased == kBadGroup ? 0.f : __uint_as_float(unsigned(254 - biased) << 23);
@@ -140,8 +152,7 @@ __global__ __launch_bounds__(kEltThreads) void k_save8(int64_t n, int F, const T
     const int biased = step_of(peak, plain);
     const float inv = inverse_step(biased);
     unsigned packed[V / 4];
-#pragma unroll
-    for (int w = 0; w < V / 4; ++w) packed[w] = pack_codes(a + 4 * w, inv, plain);
+    pack_codes(a, inv, plain, packed);
     unsigned* dst = reinterpret_cast<unsigned*>(codes + r * (int64_t(groups) * kGroup) + f);
     if constexpr (V == 4) dst[0] = packed[0];
     else *reinterpret_cast<u32x2*>(dst) = u32x2{packed[0], packed[1]};
@@ -428,18 +439,21 @@ __global__ __launch_bounds__(256) void k_weight_grad_sum8(int F, int64_t total, 
 // 0-3 and 8-11 of sixteen in the first half of the wavefront, the others in the second, so that a
 // load takes whole 32-byte pieces of a row.  The weight is split into bf16 planes on its way to LDS,
 // 64 features (of x, or units of grad) at a time, and serves the workgroup's rows.  Measured on
-// 232965 x 256 fp32 with 64 units: y and the codes 103 us (3.5 TB/s of the 360 MB it moves), dx 116 us;
+// 232965 x 256 fp32 with 64 units: y and the codes 103 us (3.5 TB/s of the 360 MB it moves), dx 113 us
+// (in pieces of 32 bytes, without the way through LDS, 118 us);
 // with 64 rows a wavefront, so that a piece of the weight read from LDS serves two products, 114 and
 // 129 us: half the wavefronts wait for the same loads.
 constexpr int kLinStep = 64;
 
-// eight elements of a row from `k`: k .. k + 3 and k + 8 .. k + 11, zeros from `left` on
+// eight elements of a row from `k`: k .. k + 3 and k + 8 .. k + 11; unless `whole`, which is the same
+// for the wavefront, zeros from `left` on
 template <typename T>
-__device__ __forceinline__ void load_eight(const T* src, int left, T (&v)[8]) {
-  if (left >= 12) {
+__device__ __forceinline__ void load_eight(const T* src, bool whole, int left, T (&v)[8]) {
+  if (whole) {
     __builtin_memcpy(&v[0], src, 4 * sizeof(T));
     __builtin_memcpy(&v[4], src + 8, 4 * sizeof(T));
   } else {
+    asm("" : "+v"(src));                         // or the last of these is merged with the last of those
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = (e & 3) + (e >> 2) * 8 < left ? src[(e & 3) + (e >> 2) * 8] : T{};
   }
@@ -452,10 +466,8 @@ __device__ __forceinline__ void save_group(const float (&a)[2][8], bool plain, b
   const int biased = step_of(other > peak ? other : peak, plain);
   const float inv = inverse_step(biased);
   unsigned word[2][2];                           // features 16 s + 8 w + 4 half ..
-#pragma unroll
-  for (int s = 0; s < 2; ++s)
-#pragma unroll
-    for (int w = 0; w < 2; ++w) word[s][w] = pack_codes(a[s] + 4 * w, inv, plain);
+  pack_codes(a[0], inv, plain, word[0]);
+  pack_codes(a[1], inv, plain, word[1]);
   // the first half keeps features 0 .. 15, the second 16 .. 31
   const unsigned g0 = unsigned(__shfl_xor(int(half ? word[0][0] : word[1][0]), 32));
   const unsigned g1 = unsigned(__shfl_xor(int(half ? word[0][1] : word[1][1]), 32));
@@ -493,13 +505,13 @@ __global__ __launch_bounds__(256) void k_linear8(int64_t n, int F, int H, const 
       const int c = t + 256 * l, h = h0 + (c >> 3), f = f0 + 16 * ((c & 7) >> 1) + 4 * (c & 1);
 #pragma unroll
       for (int e = 0; e < 8; ++e) wreg[l][e] = T{};
-      if (h < H) load_eight(w + int64_t(h) * ldw + f, F - f, wreg[l]);
+      if (h < H) load_eight(w + int64_t(h) * ldw + f, F - f0 >= kLinStep, F - f, wreg[l]);
     }
   };
   T xreg[2][8];
   const auto fetch_rows = [&](int f0) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s) load_eight(row_at + f0 + 16 * s, F - f0 - 16 * s - 4 * half, xreg[s]);
+    for (int s = 0; s < 2; ++s) load_eight(row_at + f0 + 16 * s, F - f0 >= kGroup, F - f0 - 16 * s - 4 * half, xreg[s]);
   };
   f32x16 acc[NB];
 #pragma unroll
@@ -574,9 +586,10 @@ __global__ __launch_bounds__(256) void k_linear_grad8(int64_t n, int F, int H, c
   constexpr int P = Planes<T>::kCount;
   constexpr int kChunks = kLinStep * 8 / 256;    // of 8 features, a thread's share of a weight step (64 x 64)
   constexpr int kKept = 4;                       // sixteens of units whose grad stays in registers
-  __shared__ __align__(128) char lds[P * kLinStep * 128];
+  constexpr int kJoined = sizeof(T) == 4 ? 1 : 2;        // blocks of 32 features in 128 bytes of a row
+  __shared__ __align__(128) char lds[P * kLinStep * 128], turned[4][32 * 128];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), half = lane >> 5;
-  const int64_t r = (int64_t(blockIdx.x) * 4 + wave) * 32 + (lane & 31);
+  const int64_t first = (int64_t(blockIdx.x) * 4 + wave) * 32, r = first + (lane & 31);
   const int ldq = (F + kGroup - 1) / kGroup * kGroup;
   const T* row_at = g + (r < n ? r : n - 1) * ldg + 4 * half;
   bf16x8 fb[kKept][P];
@@ -584,7 +597,7 @@ __global__ __launch_bounds__(256) void k_linear_grad8(int64_t n, int F, int H, c
 #pragma unroll
     for (int s = 0; s < kKept; ++s) {
       T v[8];
-      load_eight(row_at + k0 + 16 * s, H - k0 - 16 * s - 4 * half, v);
+      load_eight(row_at + k0 + 16 * s, H - k0 >= 16 * (s + 1), H - k0 - 16 * s - 4 * half, v);
       planes_of(v, fb[s]);
     }
   };
@@ -670,19 +683,34 @@ __global__ __launch_bounds__(256) void k_linear_grad8(int64_t n, int F, int H, c
       const float d = acc[j][e];
       return narrow<T>((signs[j][e >> 2] >> (8 * (e & 3) + 7)) & 1u ? (slope == 0.f ? 0.f : slope * d) : d);
     };
-    if (r >= n) continue;
-    if (dx_wide && f0 + kLinStep <= F) {         // whole words, and no other way of storing in sight of the compiler
+    if (dx_wide && f0 + kLinStep <= F) {
+      // whole 128-byte pieces of a row at a time, by way of LDS: as the lanes hold them, four features of
+      // a row each, dx leaves in pieces of 32 bytes
+      char* const mine = turned[wave];
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int jj = 0; jj < 2; jj += kJoined) {
 #pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-          const T v[4] = {result(j, e), result(j, e + 1), result(j, e + 2), result(j, e + 3)};
-          typedef unsigned Word __attribute__((ext_vector_type(sizeof(T))));
-          Word word;
-          __builtin_memcpy(&word, &v, sizeof(word));
-          *reinterpret_cast<Word*>(dx + r * lddx + f0 + 32 * j + block_row(e, lane)) = word;
+        for (int j = jj; j < jj + kJoined; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) {
+            const T v[4] = {result(j, e), result(j, e + 1), result(j, e + 2), result(j, e + 3)};
+            typedef unsigned Word __attribute__((ext_vector_type(sizeof(T))));
+            Word word;
+            __builtin_memcpy(&word, &v, sizeof(word));
+            const int row = lane & 31, byte = (32 * (j - jj) + block_row(e, lane)) * int(sizeof(T));
+            *reinterpret_cast<Word*>(mine + row * 128 + (((byte >> 4) ^ ((row >> 1) & 7)) << 4) + (byte & 15)) = word;
+          }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = 8 * i + (lane >> 3), c = lane & 7;
+          const u32x4 word = *reinterpret_cast<const u32x4*>(mine + row * 128 + ((c ^ ((row >> 1) & 7)) << 4));
+          const int64_t at = first + row;
+          if (at < n) *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(dx + at * lddx + f0 + 32 * jj) + 16 * c) = word;
         }
-    } else {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      }
+    } else if (r < n) {
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -843,7 +871,7 @@ int launch_linear_grad(int64_t n, int64_t F, int64_t H, const void* g, int64_t l
                        float slope, const uint8_t* codes, void* dx, int64_t lddx, hipStream_t st) {
   const int64_t blocks = (n + 127) / 128, tiles = (F + kLinStep - 1) / kLinStep;
   // Few rows: features over several workgroups, each of which reads its rows of grad again.  Aimed at
-  // 1024 workgroups; at 2048 the 232965 rows (1821 workgroups by themselves) take 127 us, not 116.
+  // 1024 workgroups; at 2048 the 232965 rows (1821 workgroups by themselves) take 10 us longer.
   int64_t across = (1024 + blocks - 1) / blocks;
   if (across > tiles) across = tiles;
   hipLaunchKernelGGL((k_linear_grad8<T>), dim3(unsigned(blocks), unsigned(across)), dim3(256), 0, st, n, int(F), int(H),
