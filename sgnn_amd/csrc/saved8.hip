@@ -484,25 +484,36 @@ __device__ __forceinline__ void lin_planes(const float (&v)[8], bf16x8 (&out)[1]
   for (int e = 0; e < 8; ++e) out[0][e] = static_cast<__bf16>(v[e]);
 }
 
-// y[r][h] for 128 rows and 32 * NB units a workgroup; `codes` NULL: nothing is kept
-template <typename T, int NB>
+// y[r][h] for 128 rows and 32 * NB units a workgroup; `codes` NULL: nothing is kept.  SPLIT, for few
+// rows: 32 rows a workgroup, whose wavefronts take turns at the steps of the features, each with a
+// piece of the weight of its own, and add their sums up in the end, in order.
+template <typename T, int NB, bool SPLIT>
 __global__ __launch_bounds__(256) void k_linear8(int64_t n, int F, int H, const T* __restrict__ x, int64_t ldx,
                                                  const T* __restrict__ w, int64_t ldw, float slope,
                                                  uint8_t* __restrict__ codes, uint8_t* __restrict__ steps,
                                                  T* __restrict__ y, int64_t ldy) {
   constexpr int P = Planes<T>::kCount, kUnits = 32 * NB;
-  constexpr int kChunks = kUnits * (kLinStep / 8) / 256;        // of 8 features, a thread's share of a weight step
-  __shared__ __align__(128) char lds[P * kUnits * kLinStep * 2];
-  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), half = lane >> 5;
+  constexpr int kLoaders = SPLIT ? 64 : 256;
+  constexpr int kChunks = kUnits * (kLinStep / 8) / kLoaders;   // of 8 features, a thread's share of a weight step
+  constexpr int kPiece = P * kUnits * kLinStep * 2, kStride = SPLIT ? 4 * kLinStep : kLinStep;
+  static_assert(!SPLIT || NB <= 2, "LDS");
+  __shared__ __align__(128) char all[SPLIT ? 4 * (kPiece > 128 * kUnits ? kPiece : 128 * kUnits) : kPiece];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+  const int t = SPLIT ? lane : threadIdx.x;
+  char* const lds = all + (SPLIT ? wave * kPiece : 0);
+  const auto sync = [&] {
+    if constexpr (SPLIT) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    else __syncthreads();
+  };
   const int h0 = int(blockIdx.y) * kUnits, groups = (F + kGroup - 1) / kGroup;
-  const int64_t r = (int64_t(blockIdx.x) * 4 + wave) * 32 + (lane & 31);
+  const int64_t first = (SPLIT ? int64_t(blockIdx.x) : int64_t(blockIdx.x) * 4 + wave) * 32, r = first + (lane & 31);
   const bool plain = slope == 1.f, save = codes != nullptr && blockIdx.y == 0;
   const T* row_at = x + (r < n ? r : n - 1) * ldx + 4 * half;
   T wreg[kChunks][8];
   const auto fetch_weight = [&](int f0) {
 #pragma unroll
     for (int l = 0; l < kChunks; ++l) {
-      const int c = t + 256 * l, h = h0 + (c >> 3), f = f0 + 16 * ((c & 7) >> 1) + 4 * (c & 1);
+      const int c = t + kLoaders * l, h = h0 + (c >> 3), f = f0 + 16 * ((c & 7) >> 1) + 4 * (c & 1);
 #pragma unroll
       for (int e = 0; e < 8; ++e) wreg[l][e] = T{};
       if (h < H) load_eight(w + int64_t(h) * ldw + f, F - f0 >= kLinStep, F - f, wreg[l]);
@@ -518,21 +529,22 @@ __global__ __launch_bounds__(256) void k_linear8(int64_t n, int F, int H, const 
   for (int j = 0; j < NB; ++j)
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[j][e] = 0.f;
-  fetch_weight(0);
-  fetch_rows(0);
-  for (int f0 = 0; f0 < F; f0 += kLinStep) {
-    __syncthreads();
+  const int begin = SPLIT ? wave * kLinStep : 0;
+  fetch_weight(begin);
+  fetch_rows(begin);
+  for (int f0 = begin; f0 < F; f0 += kStride) {
+    sync();
 #pragma unroll
     for (int l = 0; l < kChunks; ++l) {
-      const int c = t + 256 * l, row = c >> 3;
+      const int c = t + kLoaders * l, row = c >> 3;
       bf16x8 pl[P];
       planes_of(wreg[l], pl);
 #pragma unroll
       for (int q = 0; q < P; ++q)
         *reinterpret_cast<bf16x8*>(lds + (q * kUnits + row) * (kLinStep * 2) + (((c & 7) ^ spread_128(row)) << 4)) = pl[q];
     }
-    __syncthreads();
-    if (f0 + kLinStep < F) fetch_weight(f0 + kLinStep);
+    sync();
+    if (f0 + kStride < F) fetch_weight(f0 + kStride);
 #pragma unroll
     for (int g = 0; g < 2; ++g) {                // groups of 32 features
       const int f = f0 + 32 * g;
@@ -544,7 +556,8 @@ __global__ __launch_bounds__(256) void k_linear8(int64_t n, int F, int H, const 
         for (int e = 0; e < 8; ++e) a[s][e] = widen(xreg[s][e]);
         activate(a[s], slope);
       }
-      if (f + 32 < F) fetch_rows(f + 32);
+      const int next = g == 0 ? f + 32 : f0 + kStride;
+      if (next < F) fetch_rows(next);
       if (save)
         save_group(a, plain, r < n, half, codes + r * (int64_t(groups) * kGroup) + f, steps + r * groups + (f >> 5));
 #pragma unroll
@@ -564,12 +577,29 @@ __global__ __launch_bounds__(256) void k_linear8(int64_t n, int F, int H, const 
       }
     }
   }
+  if constexpr (SPLIT) {
+    __syncthreads();
+    float* const shares = reinterpret_cast<float*>(all);         // [wave][row][unit]
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        shares[(wave * 32 + block_row(e, lane)) * kUnits + 32 * j + (lane & 31)] = acc[j][e];
+    __syncthreads();
+    for (int c = threadIdx.x; c < 32 * kUnits; c += 256) {
+      const int64_t out = first + c / kUnits;
+      const int h = h0 + c % kUnits;
+      const float sum = (shares[c] + shares[c + 32 * kUnits]) + (shares[c + 64 * kUnits] + shares[c + 96 * kUnits]);
+      if (out < n && h < H) y[out * ldy + h] = narrow<T>(sum);
+    }
+    return;
+  }
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
     const int h = h0 + 32 * j + (lane & 31);
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      const int64_t out = (int64_t(blockIdx.x) * 4 + wave) * 32 + block_row(e, lane);
+      const int64_t out = first + block_row(e, lane);
       if (out < n && h < H) y[out * ldy + h] = narrow<T>(acc[j][e]);
     }
   }
@@ -854,13 +884,22 @@ int check_linear(int dtype, int64_t n, int64_t F, int64_t H, float slope, const 
 template <typename T>
 int launch_linear(int64_t n, int64_t F, int64_t H, const void* x, int64_t ldx, const void* w, int64_t ldw, float slope,
                   uint8_t* codes, uint8_t* steps, void* y, int64_t ldy, hipStream_t st) {
-#define SGNN_LIN8(NB)                                                                                              \
-  hipLaunchKernelGGL((k_linear8<T, NB>), dim3(unsigned((n + 127) / 128), unsigned((H + 32 * NB - 1) / (32 * NB))), \
-                     dim3(256), 0, st, n, int(F), int(H), static_cast<const T*>(x), ldx, static_cast<const T*>(w), \
+#define SGNN_LIN8(NB, SPLIT)                                                                                         \
+  hipLaunchKernelGGL((k_linear8<T, NB, SPLIT>), dim3(unsigned((n + (SPLIT ? 31 : 127)) / (SPLIT ? 32 : 128)),        \
+                                                     unsigned((H + 32 * NB - 1) / (32 * NB))),                       \
+                     dim3(256), 0, st, n, int(F), int(H), static_cast<const T*>(x), ldx, static_cast<const T*>(w),   \
                      ldw, slope, codes, steps, static_cast<T*>(y), ldy)
-  if (H <= 32) SGNN_LIN8(1);
-  else if (H <= 64) SGNN_LIN8(2);
-  else SGNN_LIN8(4);
+  // Few rows are bound by the wait for one load after the other along the features, which four
+  // wavefronts share; more rows than fill the card gain nothing by it.  fp32, together / split, at 8192,
+  // 16384 and 32768 rows: 1433 features, 16 units 64 / 24, 64 / 32, 67 / 62 us; 500, 64: 33 / 15, 35 / 27,
+  // 37 / 51 us; 602, 128 (two workgroups for the same rows): 51 / 30, 53 / 57, 55 / 108 us.  A single step
+  // has nothing to share.
+  const bool split = F > kLinStep && (n + 31) / 32 * ((H + 63) / 64) <= 512;
+  if (H <= 32) {
+    if (split) SGNN_LIN8(1, true); else SGNN_LIN8(1, false);
+  } else if (split) SGNN_LIN8(2, true);
+  else if (H <= 64) SGNN_LIN8(2, false);
+  else SGNN_LIN8(4, false);
 #undef SGNN_LIN8
   HIP_TRY(hipGetLastError());
   return SGNN_OK;

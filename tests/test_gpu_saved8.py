@@ -217,7 +217,8 @@ def test_linear_layer(gpu_device, dtype, slope):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("slope", [0.0, 1.0, 0.2])
 @pytest.mark.parametrize("n,F,H", [(1, 1, 1), (3, 7, 33), (130, 31, 64), (129, 33, 65), (200, 65, 128), (64, 602, 130),
-                                   (257, 96, 200), (500, 300, 16), (66000, 40, 20), (65537, 33, 70)])
+                                   (257, 96, 200), (500, 300, 16), (66000, 40, 20), (65537, 33, 70),
+                                   (20000, 100, 20), (17000, 130, 70), (9001, 70, 200), (4000, 200, 130)])
 def test_linear_layer_sizes(gpu_device, dtype, slope, n, F, H):
     t = DTYPES[dtype]
     g = torch.Generator().manual_seed(n + F + H)
