@@ -1343,15 +1343,21 @@ struct Call {
   const int64_t* idx;
 };
 
+// One launch takes fewer than 2^32 threads: a wavefront a row, a workgroup of 256 for 64 x 64 of either
+// operand and for 32 x 32 of a gradient.
+const char* too_large(int64_t B, int64_t D, int64_t V) {
+  if (B > (int64_t(1) << 25) || V > (int64_t(1) << 28) || D > (int64_t(1) << 16))
+    return "head larger than 2^25 rows, 2^28 classes or 65536 features";
+  const int64_t width = ceil_div(D, 64) * 64;
+  if (B * width > (int64_t(1) << 34) || V * width > (int64_t(1) << 34)) return "an operand of more than 2^34 elements";
+  return nullptr;
+}
+
 int check_call(const Call& c) {
   using sgnn::fail;
   if (c.dtype != SGNN_F32 && c.dtype != SGNN_BF16) return fail(SGNN_ERR_INVALID, "unknown element type");
   if (c.B <= 0 || c.D <= 0 || c.V <= 0) return fail(SGNN_ERR_INVALID, "need B > 0, D > 0, V > 0");
-  if (c.B > (int64_t(1) << 30) || c.V > (int64_t(1) << 30) || c.D > (int64_t(1) << 16))
-    return fail(SGNN_ERR_UNSUPPORTED, "head larger than 2^30 rows, 2^30 classes or 65536 features");
-  const int64_t width = ceil_div(c.D, 64) * 64;
-  if (c.B * width > (int64_t(1) << 35) || c.V * width > (int64_t(1) << 35))      // one launch lays either out
-    return fail(SGNN_ERR_UNSUPPORTED, "an operand of more than 2^35 elements");
+  if (const char* why = too_large(c.B, c.D, c.V)) return fail(SGNN_ERR_UNSUPPORTED, why);
   if (c.ldx < c.D) return fail(SGNN_ERR_INVALID, "row stride smaller than the width");
   if (!((c.sd == 1 && c.sv >= c.D) || (c.sv == 1 && c.sd >= c.V)))
     return fail(SGNN_ERR_INVALID, "the weight must have unit stride along its features or its classes");
@@ -1566,7 +1572,7 @@ int few_backward(const Call& c, const Few& f, const Buffers& b, const RowStat* s
 }  // namespace
 
 extern "C" size_t sgnn_class_xent_workspace_bytes(int dtype, int64_t B, int64_t D, int64_t V, int backward) {
-  if (B <= 0 || D <= 0 || V <= 0 || (dtype != SGNN_F32 && dtype != SGNN_BF16)) return 0;
+  if (B <= 0 || D <= 0 || V <= 0 || (dtype != SGNN_F32 && dtype != SGNN_BF16) || too_large(B, D, V)) return 0;
   // the weight's layout is not known here: enough for either way
   const size_t whole = carve(make_plan(dtype, B, D, V), B, V, backward != 0, nullptr).bytes;
   const Few f = make_few(dtype, B, D, V, 1);

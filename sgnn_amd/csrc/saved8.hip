@@ -811,7 +811,7 @@ int elt_grid(int64_t n, int64_t F, int elems, EltGrid* g) {
   int64_t rows = (4 * kEltThreads) / per_row;
   if (rows < 1) rows = 1;
   const int64_t blocks = (n + rows - 1) / rows;
-  if (blocks > 0x7fffffff) return sgnn::fail(SGNN_ERR_UNSUPPORTED, "too many rows for one launch");
+  if (blocks > 0xffffff) return sgnn::fail(SGNN_ERR_UNSUPPORTED, "too many rows for one launch");
   *g = {int(rows), int(per_row), unsigned(blocks)};
   return SGNN_OK;
 }

@@ -42,6 +42,8 @@ def propagate(x, adj, K=1):
 
 
 class _GraphConvBase(nn.Module):
+    checkpoint, input_slope = None, 1.0              # of modules stored before there were these
+
     def __init__(self, add_self_loops=True, cached=False, checkpoint=None):
         super().__init__()
         if checkpoint not in (None, "int8"):

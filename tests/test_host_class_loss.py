@@ -30,7 +30,8 @@ def backward(lib, dx=P, lddx=8, dw=P, dsv=8, dsd=1, grad=P, stats=P, ws=P, ws_by
     (dict(sv=1, sd=69), -1, b"unit stride"), (dict(n=9), -1, b"labels"), (dict(n=-1, idx=P), -1, b"labels"),
     (dict(x=None), -1, b"null"), (dict(w=None), -1, b"null"), (dict(labels=None), -1, b"null"),
     (dict(stats=None), -1, b"null"), (dict(rows=None), -1, b"null"), (dict(share=None), -1, b"null"),
-    (dict(ws=None), -1, b"null"), (dict(ws_bytes=16), -2, b"workspace"), (dict(V=1 << 31), -4, b"2^30"),
+    (dict(ws=None), -1, b"null"), (dict(ws_bytes=16), -2, b"workspace"), (dict(V=1 << 29), -4, b"2^28"),
+    (dict(B=1 << 26, n=1 << 26), -4, b"2^25"), (dict(V=1 << 28, D=65, ldx=65, sv=65), -4, b"2^34"),
     (dict(D=1 << 17, ldx=1 << 17, sv=1 << 17), -4, b"65536"),
 ])
 def test_forward_refuses(bad, rc, word):
@@ -50,6 +51,7 @@ def test_workspace_grows_with_rows_plus_classes():
     lib = _lib()
     need = lib.sgnn_class_xent_workspace_bytes
     assert need(0, 0, 8, 70, 0) == 0 and need(5, 10, 8, 70, 0) == 0
+    assert need(0, 10, 1 << 40, 70, 0) == 0 and need(1, 1 << 40, 8, 70, 1) == 0          # the call refuses them
     for dtype in (0, 1):
         for back in (0, 1):
             assert need(dtype, 10, 8, 70, back) > 0
