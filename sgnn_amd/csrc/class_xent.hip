@@ -1197,7 +1197,7 @@ int spread(int64_t slots, int64_t groups, int64_t most) {
     double best = 0.8 * double(ceil_div(groups, slots));
     for (int64_t q = 2; q <= 4; ++q)
       if (const double rounds = double(ceil_div(groups * q, slots)) / double(q); rounds <= best) {
-        best = rounds;
+        best = 0.95 * rounds;                    // each share more is one more to write and to join
         s = q;
       }
   }

@@ -439,7 +439,7 @@ __global__ __launch_bounds__(256) void k_weight_grad_sum8(int F, int64_t total, 
 // 0-3 and 8-11 of sixteen in the first half of the wavefront, the others in the second, so that a
 // load takes whole 32-byte pieces of a row.  The weight is split into bf16 planes on its way to LDS,
 // 64 features (of x, or units of grad) at a time, and serves the workgroup's rows.  Measured on
-// 232965 x 256 fp32 with 64 units: y and the codes 103 us (3.5 TB/s of the 360 MB it moves), dx 113 us
+// 232965 x 256 fp32 with 64 units: y and the codes 103 us (3.5 TB/s of the 360 MB it moves), dx 108 us
 // (in pieces of 32 bytes, without the way through LDS, 118 us);
 // with 64 rows a wavefront, so that a piece of the weight read from LDS serves two products, 114 and
 // 129 us: half the wavefronts wait for the same loads.
@@ -713,41 +713,41 @@ __global__ __launch_bounds__(256) void k_linear_grad8(int64_t n, int F, int H, c
       const float d = acc[j][e];
       return narrow<T>((signs[j][e >> 2] >> (8 * (e & 3) + 7)) & 1u ? (slope == 0.f ? 0.f : slope * d) : d);
     };
-    if (dx_wide && f0 + kLinStep <= F) {
-      // whole 128-byte pieces of a row at a time, by way of LDS: as the lanes hold them, four features of
-      // a row each, dx leaves in pieces of 32 bytes
-      char* const mine = turned[wave];
+    // whole 128-byte pieces of a row at a time, by way of LDS: as the lanes hold them, four features of
+    // a row each, dx would leave in pieces of 32 bytes, or 2 where rows are not aligned
+    char* const mine = turned[wave];
 #pragma unroll
-      for (int jj = 0; jj < 2; jj += kJoined) {
+    for (int jj = 0; jj < 2; jj += kJoined) {
 #pragma unroll
-        for (int j = jj; j < jj + kJoined; ++j)
+      for (int j = jj; j < jj + kJoined; ++j)
 #pragma unroll
-          for (int e = 0; e < 16; e += 4) {
-            const T v[4] = {result(j, e), result(j, e + 1), result(j, e + 2), result(j, e + 3)};
-            typedef unsigned Word __attribute__((ext_vector_type(sizeof(T))));
-            Word word;
-            __builtin_memcpy(&word, &v, sizeof(word));
-            const int row = lane & 31, byte = (32 * (j - jj) + block_row(e, lane)) * int(sizeof(T));
-            *reinterpret_cast<Word*>(mine + row * 128 + (((byte >> 4) ^ ((row >> 1) & 7)) << 4) + (byte & 15)) = word;
-          }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        for (int e = 0; e < 16; e += 4) {
+          const T v[4] = {result(j, e), result(j, e + 1), result(j, e + 2), result(j, e + 3)};
+          typedef unsigned Word __attribute__((ext_vector_type(sizeof(T))));
+          Word word;
+          __builtin_memcpy(&word, &v, sizeof(word));
+          const int row = lane & 31, byte = (32 * (j - jj) + block_row(e, lane)) * int(sizeof(T));
+          *reinterpret_cast<Word*>(mine + row * 128 + (((byte >> 4) ^ ((row >> 1) & 7)) << 4) + (byte & 15)) = word;
+        }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      T* const out = dx + first * lddx + f0 + 32 * jj;
+      if (dx_wide && f0 + kLinStep <= F) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int row = 8 * i + (lane >> 3), c = lane & 7;
           const u32x4 word = *reinterpret_cast<const u32x4*>(mine + row * 128 + ((c ^ ((row >> 1) & 7)) << 4));
-          const int64_t at = first + row;
-          if (at < n) *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(dx + at * lddx + f0 + 32 * jj) + 16 * c) = word;
+          if (first + row < n) __builtin_memcpy(reinterpret_cast<char*>(out + row * lddx) + 16 * c, &word, 16);
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      } else {
+        constexpr int kAcross = 128 / sizeof(T);               // lanes along a row
+#pragma unroll 8
+        for (int i = 0; i < 32 * kAcross / 64; ++i) {
+          const int row = i * (64 / kAcross) + lane / kAcross, f = lane % kAcross, byte = f * int(sizeof(T));
+          const T v = *reinterpret_cast<const T*>(mine + row * 128 + (((byte >> 4) ^ ((row >> 1) & 7)) << 4) + (byte & 15));
+          if (first + row < n && f0 + 32 * jj + f < F) out[row * lddx + f] = v;
+        }
       }
-    } else if (r < n) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int f = f0 + 32 * j + block_row(e, lane);
-          if (f < F) dx[r * lddx + f] = result(j, e);
-        }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
   }
 }
@@ -915,7 +915,7 @@ int launch_linear_grad(int64_t n, int64_t F, int64_t H, const void* g, int64_t l
   if (across > tiles) across = tiles;
   hipLaunchKernelGGL((k_linear_grad8<T>), dim3(unsigned(blocks), unsigned(across)), dim3(256), 0, st, n, int(F), int(H),
                      static_cast<const T*>(g), ldg, static_cast<const T*>(w), ldw, slope, codes, static_cast<T*>(dx),
-                     lddx, wide_ok(dx, lddx, sizeof(T)));
+                     lddx, sizeof(T) == 4 || wide_ok(dx, lddx, sizeof(T)));
   HIP_TRY(hipGetLastError());
   return SGNN_OK;
 }
