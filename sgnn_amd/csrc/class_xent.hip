@@ -349,12 +349,22 @@ __global__ __launch_bounds__(kThreads) void k_class_dz(int64_t B, int64_t V, int
   }
 }
 
+// Where a product that is one share goes at once: row m of the result to out + m * stride, times the
+// mean's factor if there is one.
+template <typename T>
+struct Direct {
+  T* out;                                        // NULL: to the shares
+  int64_t stride, rows;
+  int cols;
+  const float *grad, *share;
+};
+
 // C[m][n] += or = A . B over this workgroup's share of the reduction, 32 bits, one buffer per share:
-// out[split][Mp][Np].
+// out[split][Mp][Np]; or, where there is one share, the result itself.
 template <typename T, bool ADEEP>
 __global__ __launch_bounds__(kThreads) void k_class_product(Operand<T> A, Operand<T> B, int tiles_m, int tiles_n,
                                                             int64_t K, int splits, int add, float* __restrict__ out,
-                                                            int64_t plane, int64_t ldo) {
+                                                            int64_t plane, int64_t ldo, Direct<T> direct) {
   __shared__ __align__(128) char lds[kProductLds];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
@@ -366,6 +376,21 @@ __global__ __launch_bounds__(kThreads) void k_class_product(Operand<T> A, Operan
   Tile acc;
   clear(acc);
   if (k0 < k1) multiply<T, ADEEP, false>(A, m0, B, n0, k0, k1, lds, acc);
+  if (!ADEEP && direct.out) {
+    const float factor = direct.share ? direct.grad[0] * direct.share[0] : 1.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int64_t n = n0 + wn + 32 * j + (lane & 31);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int64_t m = m0 + wm + 32 * i + block_row(e, lane);
+          if (m < direct.rows && n < direct.cols) direct.out[m * direct.stride + n] = narrow<T>(factor * acc[i][j][e]);
+        }
+      }
+    return;
+  }
   float* dst = out + split * plane + (m0 + wm) * ldo + n0 + wn + (lane & 31);
 #pragma unroll
   for (int i = 0; i < 2; ++i)
@@ -1440,15 +1465,19 @@ int backward(const Call& c, const Plan& p, const Buffers& b, const RowStat* stat
       const Operand<T> wv{w.base + v0 * w.ld, w.ld, c.V - v0, w.cols};
       hipLaunchKernelGGL((k_class_product<T, true>), dim3(unsigned(p.tiles_b * p.dx_splits * p.tiles_d)),
                          dim3(kThreads), 0, st, a, wv, int(p.tiles_b), p.tiles_d, width, p.dx_splits, v0 > 0 ? 1 : 0,
-                         b.dx, p.Bp * Np, Np);
+                         b.dx, p.Bp * Np, Np, Direct<T>{});
       HIP_TRY(hipGetLastError());
     }
     if (dw) {                                    // dw[v][d] = dz[b][v] . x[b][d]
       const Operand<T> a{dz, p.piece, p.Bp, p.piece};
-      hipLaunchKernelGGL((k_class_product<T, false>), dim3(unsigned(tiles * p.dw_splits * p.tiles_d)), dim3(kThreads),
-                         0, st, a, x, tiles, p.tiles_d, p.Bp, p.dw_splits, 0, b.dw, p.piece * Np, Np);
-      HIP_TRY(hipGetLastError());
       const int64_t rows = c.V - v0 < width ? c.V - v0 : width;
+      Direct<T> direct{};
+      if (p.dw_splits == 1 && dsd == 1)
+        direct = Direct<T>{static_cast<T*>(dw) + v0 * dsv, dsv, rows, int(c.D), share ? grad : nullptr, share};
+      hipLaunchKernelGGL((k_class_product<T, false>), dim3(unsigned(tiles * p.dw_splits * p.tiles_d)), dim3(kThreads),
+                         0, st, a, x, tiles, p.tiles_d, p.Bp, p.dw_splits, 0, b.dw, p.piece * Np, Np, direct);
+      HIP_TRY(hipGetLastError());
+      if (direct.out) continue;
       hipLaunchKernelGGL((k_class_join<T>), dim3(unsigned(ceil_div(rows, 32)), unsigned(ceil_div(c.D, 32))), dim3(256), 0,
                          st, rows, int(c.D), p.dw_splits, b.dw, p.piece * Np, Np, share ? grad : nullptr, share, nullptr, Labels{}, nullptr,
                          0, 0, static_cast<T*>(dw) + v0 * dsv, dsv, dsd);
