@@ -5,12 +5,11 @@
 //
 // The forward pass runs over the classes once and keeps a running maximum and sum per row; the
 // backward pass forms the logits again, a piece of the classes at a time, writes that piece of dz
-// in bf16 and multiplies it from either side.  A piece is sized to stay in the last-level cache
-// between the launch that writes it and the two that read it.
+// and multiplies it from either side.
 //
 // All four products run on the bf16 matrix instructions (tile_product.h): bf16 operands as they
 // are, fp32 ones as three bf16 numbers each.  dz of bf16 operands is rounded to bf16 there
-// (relative 2^-9 per element, below the half step that each result is rounded by).
+// (relative 2^-8 per element at most, the half step that each result is rounded by, too).
 #include "tile_product.h"
 
 namespace {
@@ -947,7 +946,7 @@ __global__ __launch_bounds__(kThreads) void k_wide_stats(int64_t B, int64_t V, O
 
 // What the gradients need of a row: p = 2^((z - top) log2 e - shift) with top = 0 but for rows whose
 // logits are so large that the rounding of shift would be felt (2^12: by 2^-12, a bf16 half step
-// being 2^-9); shift = infinity without a class; its factor, its label, and what the label's element
+// being 2^-8); shift = infinity without a class; its factor, its label, and what the label's element
 // of dz adds in dx beyond its rounded probability.
 constexpr float kLargeLogit = 4096.f;
 struct RowConst {
@@ -1209,7 +1208,11 @@ struct Plan {
   int dx_splits, dw_splits;
 };
 
-constexpr int64_t kPieceBytes = int64_t(96) << 20;      // of dz: stays in the 256 MB last-level cache with its operands
+// Of dz at a time.  Larger pieces mean fewer and fuller launches; past the 256 MB of the last-level
+// cache there is nothing more to gain.  Loss and gradients in fp32 at 32 / 96 / 256 MB: 4096 rows of 128
+// features, 50000 classes 2025 / 1533 / 1459 us; 16384, 64, 20000: 2872 / 1970 / 1772; 512, 128, 100000:
+// 581 / 451 / 417.
+constexpr int64_t kPieceBytes = int64_t(256) << 20;
 constexpr int kSlots = 512;                             // workgroups that run at once: two on a CU, by their LDS
 
 // Shares of a reduction of `most` steps for `groups` workgroups a share, where `slots` workgroups
@@ -1249,30 +1252,6 @@ Plan make_plan(int dtype, int64_t B, int64_t D, int64_t V) {
   return p;
 }
 
-// The few-rows kernels: sizes that fit them, 0 rows where they do not apply.
-struct Few {
-  int rows, Dk, vec;
-  size_t lds;
-  unsigned blocks, slabs, splits;
-};
-
-Few make_few(int dtype, int64_t B, int64_t D, int64_t V, int64_t sd) {
-  Few f{};
-  const int P = dtype == SGNN_F32 ? 3 : 1;
-  if (B > kFewRows || sd != 1 || D > 65536) return f;
-  f.Dk = int(ceil_div(D, 64) * 64);
-  f.lds = size_t(P) * kFewRows * f.Dk * 2;
-  if (f.lds > 150 * 1024) return f;              // of 160 KB
-  f.rows = B <= 2 ? 2 : B <= 4 ? 4 : B <= 8 ? 8 : B <= 16 ? 16 : 32;
-  f.vec = f.rows > 16 ? 2 : 4;
-  const int64_t blocks = ceil_div(V, 128);
-  f.blocks = unsigned(blocks < kFewBlocks ? blocks : kFewBlocks);
-  f.slabs = unsigned(ceil_div(D, 64 * f.vec));
-  const int64_t want = ceil_div(f.rows > 8 ? 512 : 1024, f.slabs), most = ceil_div(V, 16);
-  f.splits = unsigned(want < most ? want : most);
-  return f;
-}
-
 // The kernels that keep rows in registers: sizes, KD 0 where they do not apply.
 struct Wide {
   int KD;
@@ -1292,6 +1271,32 @@ Wide make_wide(int dtype, int64_t B, int64_t D, int64_t V) {
   f.stat_splits = spread(f.KD < 16 ? 512 : 256, f.own_b, f.steps_v);
   f.dx_splits = spread(f.KD > 4 ? 256 : 512, f.own_b, f.steps_v);
   f.dw_splits = spread(f.KD > 4 ? 256 : 512, f.own_v, f.steps_b);
+  return f;
+}
+
+// The few-rows kernels: sizes that fit them, 0 rows where they do not apply.  Loss and gradients of 256
+// features and 100003 classes: fp32 32 rows 175 us (104 at one row), 33 rows by the tiles 228 us; bf16 16
+// rows 99 us, 32 rows 141 us, which the kernels with rows in registers take 114 us for.
+struct Few {
+  int rows, Dk, vec;
+  size_t lds;
+  unsigned blocks, slabs, splits;
+};
+
+Few make_few(int dtype, int64_t B, int64_t D, int64_t V, int64_t sd) {
+  Few f{};
+  const int P = dtype == SGNN_F32 ? 3 : 1;
+  if (B > (make_wide(dtype, B, D, V).KD ? 16 : kFewRows) || sd != 1 || D > 65536) return f;
+  f.Dk = int(ceil_div(D, 64) * 64);
+  f.lds = size_t(P) * kFewRows * f.Dk * 2;
+  if (f.lds > 150 * 1024) return f;              // of 160 KB
+  f.rows = B <= 2 ? 2 : B <= 4 ? 4 : B <= 8 ? 8 : B <= 16 ? 16 : 32;
+  f.vec = f.rows > 16 ? 2 : 4;
+  const int64_t blocks = ceil_div(V, 128);
+  f.blocks = unsigned(blocks < kFewBlocks ? blocks : kFewBlocks);
+  f.slabs = unsigned(ceil_div(D, 64 * f.vec));
+  const int64_t want = ceil_div(f.rows > 8 ? 512 : 1024, f.slabs), most = ceil_div(V, 16);
+  f.splits = unsigned(want < most ? want : most);
   return f;
 }
 

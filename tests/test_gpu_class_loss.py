@@ -106,8 +106,8 @@ def test_loss_and_gradients(gpu_device, dtype, B, D, V):
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_several_pieces(gpu_device, dtype):
     """More classes than one piece of the backward pass holds, the last piece ragged."""
-    B, V = (3000, 25000) if dtype == "bf16" else (3000, 9001)
-    check(*make(B, 40, V, DTYPES[dtype], gpu_device, seed=1))
+    B, D, V = (12000, 264, 23001) if dtype == "bf16" else (12000, 40, 12001)
+    check(*make(B, D, V, DTYPES[dtype], gpu_device, seed=1))
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
