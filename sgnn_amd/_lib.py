@@ -199,7 +199,9 @@ def ptr(t):
 def call_on(device, entry, *args):
     """``entry(*args, stream)`` on the device's current stream, with the device made current;
     raises on an error code.  Pointers may be plain addresses."""
-    stream = torch.cuda.current_stream(device).cuda_stream
+    # the stream's address as it is: torch.cuda.current_stream(device).cuda_stream is the same at 1.9 us a
+    # call instead of 0.1, of the 8 us that a whole call takes on the host
+    stream = torch._C._cuda_getCurrentRawStream(device.index)
     if torch.cuda.current_device() == device.index:
         rc = entry(*args, stream)
     else:

@@ -73,6 +73,13 @@ class SavedInt8:
         if dtype not in TYPES:
             raise TypeError(f"saved activations are float32 or bfloat16, got {dtype}")
 
+    @classmethod
+    def _of(cls, codes, steps, shape, slope, dtype):
+        """The same of parts that were just made to fit."""
+        saved = object.__new__(cls)
+        saved.codes, saved.steps, saved.shape, saved.slope, saved.dtype = codes, steps, shape, slope, dtype
+        return saved
+
     @property
     def nbytes(self):
         return self.codes.numel() + self.steps.numel()
@@ -146,7 +153,7 @@ def save_int8(x, slope=1.0):
     codes, steps = _empty(n, F, x.device)
     _lib.call_on(x.device, _lib.load().sgnn_save8, code, n, F, x.data_ptr(), _ld(x), slope, codes.data_ptr(),
                  steps.data_ptr())
-    return SavedInt8(codes, steps, (n, F), slope, x.dtype)
+    return SavedInt8._of(codes, steps, (n, F), slope, x.dtype)
 
 
 def _linear(x, weight, slope, codes=None, steps=None):
@@ -180,7 +187,7 @@ class _LinearSaved(torch.autograd.Function):
             _lib.call_on(grad.device, _lib.load().sgnn_saved8_linear_grad, TYPES[dtype], n, F, H, codes.data_ptr(), slope,
                          grad.data_ptr(), _ld(grad), w.data_ptr(), _ld(w), dx.data_ptr(), F)
         if ctx.needs_input_grad[1]:
-            dw = SavedInt8(codes, steps, (n, F), slope, dtype).weight_grad(grad)
+            dw = SavedInt8._of(codes, steps, (n, F), slope, dtype).weight_grad(grad)
         return dx, dw, None
 
 
