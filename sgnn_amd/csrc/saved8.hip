@@ -122,6 +122,8 @@ __device__ __forceinline__ void store_row(T* p, int left, bool wide, const T (&v
 
 // A workgroup owns `rows` whole rows; `per_row` = lanes a row takes (a multiple of a group's
 // lanes, so that a group never leaves its wavefront's aligned block of lanes).
+// Bound by memory: 232965 x 256 fp32 saved in 71 us (301 MB, 4.2 TB/s) and restored in 60 us (5.0; a
+// copy reaches 5.1).
 constexpr int kEltThreads = 256;
 
 template <typename T>
