@@ -670,8 +670,8 @@ int sgnn_saved8_weight_grad(int dtype, int64_t n, int64_t F, int64_t H, const vo
  * backward: from the same operands and the forward's stats.  share given: g_b = grad[0] * share[0]
  *   (the mean's gradient); share NULL: g_b = grad[b].  dx or dweight may be NULL.
  * Sums are formed in 32 bits in a fixed order.  `workspace`: sgnn_class_xent_workspace_bytes bytes
- * (backward = 0 or 1), contents irrelevant.  At most 2^25 rows, 2^28 classes, 65536 features and 2^34
- * elements (features rounded up to 64) an operand: more is refused, with a workspace of 0 bytes.
+ * (backward = 0 or 1), contents irrelevant.  At most 2^25 rows, 2^28 classes, 65536 features and 2^33
+ * elements of x and weight together (features rounded up to 64): more is refused, with a workspace of 0 bytes.
  */
 size_t sgnn_class_xent_workspace_bytes(int dtype, int64_t B, int64_t D, int64_t V, int backward);
 int sgnn_class_xent_forward(int dtype, int64_t B, int64_t D, int64_t V, const void* x, int64_t ldx,

@@ -362,24 +362,33 @@ struct Direct {
   const float *grad, *share;
 };
 
-// C[m][n] += or = A . B over this workgroup's share of the reduction, 32 bits, one buffer per share:
+// C[m][n] += or = A . B over a workgroup's share of the reduction, 32 bits, one buffer per share:
 // out[split][Mp][Np]; or, where there is one share, the result itself.
+template <typename T>
+struct Product {
+  Operand<T> a, b;
+  int64_t K;
+  int tiles_n, splits, add;
+  float* out;
+  int64_t plane, ldo;
+  Direct<T> direct;
+  unsigned blocks;                               // workgroups it takes: tiles_m * splits * tiles_n
+};
+
 template <typename T, bool ADEEP>
-__global__ __launch_bounds__(kThreads) void k_class_product(Operand<T> A, Operand<T> B, int tiles_m, int tiles_n,
-                                                            int64_t K, int splits, int add, float* __restrict__ out,
-                                                            int64_t plane, int64_t ldo, Direct<T> direct) {
-  __shared__ __align__(128) char lds[kProductLds];
+__device__ __forceinline__ void form_product(const Product<T>& p, unsigned block, char* lds) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
-  const int tn = blockIdx.x % tiles_n, rest = blockIdx.x / tiles_n;
-  const int split = rest % splits, tm = rest / splits;
+  const int tn = block % unsigned(p.tiles_n), rest = block / unsigned(p.tiles_n);
+  const int split = rest % p.splits, tm = rest / p.splits;
   const int64_t m0 = int64_t(tm) * kTile, n0 = int64_t(tn) * kTile;
-  const int64_t steps = K / Step<T>::kDepth;
-  const int64_t k0 = steps * split / splits * Step<T>::kDepth, k1 = steps * (split + 1) / splits * Step<T>::kDepth;
+  const int64_t steps = p.K / Step<T>::kDepth;
+  const int64_t k0 = steps * split / p.splits * Step<T>::kDepth, k1 = steps * (split + 1) / p.splits * Step<T>::kDepth;
   Tile acc;
   clear(acc);
-  if (k0 < k1) multiply<T, ADEEP, false>(A, m0, B, n0, k0, k1, lds, acc);
-  if (!ADEEP && direct.out) {
+  if (k0 < k1) multiply<T, ADEEP, false>(p.a, m0, p.b, n0, k0, k1, lds, acc);
+  if (!ADEEP && p.direct.out) {
+    const Direct<T>& direct = p.direct;
     const float factor = direct.share ? direct.grad[0] * direct.share[0] : 1.f;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -394,70 +403,92 @@ __global__ __launch_bounds__(kThreads) void k_class_product(Operand<T> A, Operan
       }
     return;
   }
-  float* dst = out + split * plane + (m0 + wm) * ldo + n0 + wn + (lane & 31);
+  float* dst = p.out + split * p.plane + (m0 + wm) * p.ldo + n0 + wn + (lane & 31);
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      if (add) {                                 // all loads before the first sum waits
+      if (p.add) {                               // all loads before the first sum waits
         float old[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) old[e] = dst[(32 * i + block_row(e, lane)) * ldo + 32 * j];
+        for (int e = 0; e < 16; ++e) old[e] = dst[(32 * i + block_row(e, lane)) * p.ldo + 32 * j];
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[i][j][e] += old[e];
       }
 #pragma unroll
-      for (int e = 0; e < 16; ++e) dst[(32 * i + block_row(e, lane)) * ldo + 32 * j] = acc[i][j][e];
+      for (int e = 0; e < 16; ++e) dst[(32 * i + block_row(e, lane)) * p.ldo + 32 * j] = acc[i][j][e];
     }
+}
+
+// Both gradients' products in one launch: 512 x 128 against 1000 classes in fp32 11 us, one after the
+// other 17 and a launch more; where either fills the card the same.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void k_class_products(Product<T> dx, Product<T> dw) {
+  __shared__ __align__(128) char lds[kProductLds];
+  if (blockIdx.x < dx.blocks) form_product<T, true>(dx, blockIdx.x, lds);
+  else form_product<T, false>(dw, blockIdx.x - dx.blocks, lds);
 }
 
 // out[r][d] = factor * (sum over the shares, in order, + rest[r] * weight[y(r)][d]), out at r * sr +
 // d * sd; factor = grad[0] * share[0] with `share`, grad[r] with `grad` alone, else 1; `rest` (dx in
-// bf16) may be NULL.  With `of` rows without
-// a class are 0 whatever the weight holds.
+// bf16) may be NULL.  With `of` rows without a class are 0 whatever the weight holds.
 template <typename T>
-__global__ __launch_bounds__(256) void k_class_join(int64_t R, int D, int splits, const float* __restrict__ in,
-                                                    int64_t plane, int64_t ldi, const float* __restrict__ grad,
-                                                    const float* __restrict__ share, const float* __restrict__ rest,
-                                                    Labels of, const T* __restrict__ weight, int64_t sv, int64_t sdw,
-                                                    T* __restrict__ out, int64_t sr, int64_t sd) {
+struct Join {
+  int64_t R;
+  int D, splits;
+  const float* in;
+  int64_t plane, ldi;
+  const float *grad, *share, *rest;
+  Labels of;
+  const T* weight;
+  int64_t sv, sdw;
+  T* out;
+  int64_t sr, sd;
+  unsigned blocks() const { return out ? unsigned((R + 31) / 32 * ((D + 31) / 32)) : 0u; }
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_class_join(Join<T> first, Join<T> second, unsigned of_first) {
+  const bool one = blockIdx.x < of_first;
+  const Join<T> j = one ? first : second;
+  const unsigned block = one ? blockIdx.x : blockIdx.x - of_first, across = unsigned(j.D + 31) / 32;
   __shared__ float tile[32][33];
-  const int64_t r0 = int64_t(blockIdx.x) * 32;
-  const int t = threadIdx.x, lr = t >> 3, ld = (t & 7) * 4, d = int(blockIdx.y) * 32 + ld;
+  const int64_t r0 = int64_t(block / across) * 32;
+  const int t = threadIdx.x, lr = t >> 3, ld = (t & 7) * 4, db = int(block % across) * 32, d = db + ld;
   const int64_t r = r0 + lr;
   float v[4] = {0.f, 0.f, 0.f, 0.f};
-  if (r < R && d < D) {
-    const float factor = share ? grad[0] * share[0] : grad ? grad[r] : 1.f;
-    const float* src = in + r * ldi + d;         // ldi is a multiple of 4 and covers d .. d + 3
+  if (r < j.R && d < j.D) {
+    const float factor = j.share ? j.grad[0] * j.share[0] : j.grad ? j.grad[r] : 1.f;
+    const float* src = j.in + r * j.ldi + d;         // j.ldi is a multiple of 4 and covers d .. d + 3
     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-    for (int q = 0; q < splits; ++q) sum += *reinterpret_cast<const f32x4*>(src + q * plane);
+    for (int q = 0; q < j.splits; ++q) sum += *reinterpret_cast<const f32x4*>(src + q * j.plane);
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = sum[e];
-    if (of.V) {
-      const int64_t y = label_of(r, of.labels, of.idx, of.n_labels, of.V);
+    if (j.of.V) {
+      const int64_t y = label_of(r, j.of.labels, j.of.idx, j.of.n_labels, j.of.V);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         if (y < 0) v[e] = 0.f;
-        else if (rest && d + e < D) v[e] += rest[r] * widen(weight[y * sv + (d + e) * sdw]);
+        else if (j.rest && d + e < j.D) v[e] += j.rest[r] * widen(j.weight[y * j.sv + (d + e) * j.sdw]);
       }
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] *= factor;
-    if (sd == 1) {
-      T* dst = out + r * sr + d;
+    if (j.sd == 1) {
+      T* dst = j.out + r * j.sr + d;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (d + e < D) dst[e] = narrow<T>(v[e]);
+        if (d + e < j.D) dst[e] = narrow<T>(v[e]);
     }
   }
-  if (sd == 1) return;                           // the whole launch
+  if (j.sd == 1) return;                         // the whole workgroup
 #pragma unroll
   for (int e = 0; e < 4; ++e) tile[lr][ld + e] = v[e];
   __syncthreads();
   for (int i = t; i < 32 * 32; i += 256) {
-    const int fr = i & 31, fd = i >> 5, at = int(blockIdx.y) * 32 + fd;
-    if (r0 + fr < R && at < D) out[(r0 + fr) * sr + at * sd] = narrow<T>(tile[fr][fd]);
+    const int fr = i & 31, fd = i >> 5, at = db + fd;
+    if (r0 + fr < j.R && at < j.D) j.out[(r0 + fr) * j.sr + at * j.sd] = narrow<T>(tile[fr][fd]);
   }
 }
 
@@ -1345,9 +1376,8 @@ Buffers carve_wide(const Wide& f, const Plan& p, int64_t B, int64_t V, bool back
     const size_t padded = size_t(f.steps_b) * kStreamRows;
     b.rows = RowConst{c.take<float>(padded), c.take<float>(padded), c.take<float>(padded), c.take<float>(padded),
                       c.take<int>(padded)};
-    // the two gradients' shares take turns
-    const size_t dx = size_t(f.dx_splits) * B, dw = size_t(f.dw_splits) * V;
-    b.dx = c.take<float>((dx > dw ? dx : dw) * p.Dp);
+    b.dx = c.take<float>(size_t(f.dx_splits) * B * p.Dp);
+    b.dw = c.take<float>(size_t(f.dw_splits) * V * p.Dp);
   }
   b.bytes = c.off;
   return b;
@@ -1379,13 +1409,13 @@ struct Call {
   const int64_t* idx;
 };
 
-// One launch takes fewer than 2^32 threads: a wavefront a row, a workgroup of 256 for 64 x 64 of either
-// operand and for 32 x 32 of a gradient.
+// One launch takes fewer than 2^32 threads: a wavefront a row, a workgroup of 256 for 64 x 64 of the
+// operands and for 32 x 32 of the gradients.
 const char* too_large(int64_t B, int64_t D, int64_t V) {
   if (B > (int64_t(1) << 25) || V > (int64_t(1) << 28) || D > (int64_t(1) << 16))
     return "head larger than 2^25 rows, 2^28 classes or 65536 features";
   const int64_t width = ceil_div(D, 64) * 64;
-  if (B * width > (int64_t(1) << 34) || V * width > (int64_t(1) << 34)) return "an operand of more than 2^34 elements";
+  if ((B + V) * width > (int64_t(1) << 33)) return "operands of more than 2^33 elements";
   return nullptr;
 }
 
@@ -1457,6 +1487,15 @@ int forward(const Call& c, const Plan& p, const Buffers& b, RowStat* stats, floa
 }
 
 template <typename T>
+int launch_joins(const Join<T>& first, const Join<T>& second, hipStream_t st) {
+  const unsigned blocks = first.blocks() + second.blocks();
+  if (blocks == 0) return SGNN_OK;
+  hipLaunchKernelGGL((k_class_join<T>), dim3(blocks), dim3(256), 0, st, first, second, first.blocks());
+  HIP_TRY(hipGetLastError());
+  return SGNN_OK;
+}
+
+template <typename T>
 int backward(const Call& c, const Plan& p, const Buffers& b, const RowStat* stats, const float* grad,
              const float* share, void* dx, int64_t lddx, void* dw, int64_t dsv, int64_t dsd, hipStream_t st) {
   Operand<T> x, w;
@@ -1471,36 +1510,31 @@ int backward(const Call& c, const Plan& p, const Buffers& b, const RowStat* stat
     hipLaunchKernelGGL((k_class_dz<T>), dim3(unsigned(p.tiles_b * tiles)), dim3(kThreads), 0, st, c.B, c.V, depth, x, w,
                        c.labels, c.idx, c.n_labels, stats, share ? nullptr : grad, b.rest, v0, tiles, dz, p.piece);
     HIP_TRY(hipGetLastError());
-    if (dx) {                                    // dx[b][d] += dz[b][v] . w[v][d]
-      const Operand<T> a{dz, p.piece, p.Bp, p.piece};
-      const Operand<T> wv{w.base + v0 * w.ld, w.ld, c.V - v0, w.cols};
-      hipLaunchKernelGGL((k_class_product<T, true>), dim3(unsigned(p.tiles_b * p.dx_splits * p.tiles_d)),
-                         dim3(kThreads), 0, st, a, wv, int(p.tiles_b), p.tiles_d, width, p.dx_splits, v0 > 0 ? 1 : 0,
-                         b.dx, p.Bp * Np, Np, Direct<T>{});
-      HIP_TRY(hipGetLastError());
-    }
+    const Operand<T> a{dz, p.piece, p.Bp, p.piece};
+    Product<T> to_dx{}, to_dw{};
+    if (dx)                                      // dx[b][d] += dz[b][v] . w[v][d]
+      to_dx = Product<T>{a, Operand<T>{w.base + v0 * w.ld, w.ld, c.V - v0, w.cols}, width, p.tiles_d, p.dx_splits,
+                         v0 > 0 ? 1 : 0, b.dx, p.Bp * Np, Np, Direct<T>{}, unsigned(p.tiles_b * p.dx_splits * p.tiles_d)};
+    Join<T> join_dw{};
     if (dw) {                                    // dw[v][d] = dz[b][v] . x[b][d]
-      const Operand<T> a{dz, p.piece, p.Bp, p.piece};
       const int64_t rows = c.V - v0 < width ? c.V - v0 : width;
-      Direct<T> direct{};
+      T* const out = static_cast<T*>(dw) + v0 * dsv;
+      to_dw = Product<T>{a, x, p.Bp, p.tiles_d, p.dw_splits, 0, b.dw, p.piece * Np, Np, Direct<T>{},
+                         unsigned(tiles * p.dw_splits * p.tiles_d)};
       if (p.dw_splits == 1 && dsd == 1)
-        direct = Direct<T>{static_cast<T*>(dw) + v0 * dsv, dsv, rows, int(c.D), share ? grad : nullptr, share};
-      hipLaunchKernelGGL((k_class_product<T, false>), dim3(unsigned(tiles * p.dw_splits * p.tiles_d)), dim3(kThreads),
-                         0, st, a, x, tiles, p.tiles_d, p.Bp, p.dw_splits, 0, b.dw, p.piece * Np, Np, direct);
-      HIP_TRY(hipGetLastError());
-      if (direct.out) continue;
-      hipLaunchKernelGGL((k_class_join<T>), dim3(unsigned(ceil_div(rows, 32)), unsigned(ceil_div(c.D, 32))), dim3(256), 0,
-                         st, rows, int(c.D), p.dw_splits, b.dw, p.piece * Np, Np, share ? grad : nullptr, share, nullptr, Labels{}, nullptr,
-                         0, 0, static_cast<T*>(dw) + v0 * dsv, dsv, dsd);
-      HIP_TRY(hipGetLastError());
+        to_dw.direct = Direct<T>{out, dsv, rows, int(c.D), share ? grad : nullptr, share};
+      else
+        join_dw = Join<T>{rows, int(c.D), p.dw_splits, b.dw, p.piece * Np, Np, share ? grad : nullptr, share, nullptr,
+                          Labels{}, nullptr, 0, 0, out, dsv, dsd};
     }
-  }
-  if (dx) {
-    hipLaunchKernelGGL((k_class_join<T>), dim3(unsigned(ceil_div(c.B, 32)), unsigned(ceil_div(c.D, 32))), dim3(256), 0, st,
-                       c.B, int(c.D), p.dx_splits, b.dx, p.Bp * Np, Np, share ? grad : nullptr, share, sizeof(T) == 2 ? b.rest : nullptr,
-                       Labels{c.labels, c.idx, c.n_labels, c.V}, static_cast<const T*>(c.w), c.sv, c.sd,
-                       static_cast<T*>(dx), lddx, int64_t(1));
+    hipLaunchKernelGGL((k_class_products<T>), dim3(to_dx.blocks + to_dw.blocks), dim3(kThreads), 0, st, to_dx, to_dw);
     HIP_TRY(hipGetLastError());
+    Join<T> join_dx{};
+    if (dx && v0 + p.piece >= c.V)               // all pieces are in
+      join_dx = Join<T>{c.B, int(c.D), p.dx_splits, b.dx, p.Bp * Np, Np, share ? grad : nullptr, share,
+                        sizeof(T) == 2 ? b.rest : nullptr, Labels{c.labels, c.idx, c.n_labels, c.V},
+                        static_cast<const T*>(c.w), c.sv, c.sd, static_cast<T*>(dx), lddx, int64_t(1)};
+    if (int rc = launch_joins(join_dx, join_dw, st)) return rc;
   }
   return SGNN_OK;
 }
@@ -1534,22 +1568,20 @@ int wide_backward(const Call& c, const Wide& f, const Plan& p, const Buffers& b,
   hipLaunchKernelGGL(k_wide_rows, dim3(unsigned(ceil_div(padded, 256))), dim3(256), 0, st, c.B, padded, of, stats, grad,
                      share, b.rows);
   HIP_TRY(hipGetLastError());
+  Join<Bf16> join_dx{}, join_dw{};
   if (dx) {
     SGNN_WIDE(f.KD, hipLaunchKernelGGL((k_wide_grads<KD, false, false>), dim3(unsigned(f.own_b * f.dx_splits)),
                                        dim3(kGradThreads), 0, st, c.B, c.V, x, w, b.rows, f.steps_v, f.dx_splits, b.dx,
                                        c.B * p.Dp, int(c.D), nullptr, 0, 0, nullptr, nullptr));
     HIP_TRY(hipGetLastError());
-    hipLaunchKernelGGL((k_class_join<Bf16>), dim3(unsigned(ceil_div(c.B, 32)), unsigned(ceil_div(c.D, 32))), dim3(256), 0,
-                       st, c.B, int(c.D), f.dx_splits, b.dx, c.B * p.Dp, int64_t(p.Dp), b.rows.factor, nullptr,
-                       b.rows.rest, of, static_cast<const Bf16*>(c.w), c.sv, c.sd, static_cast<Bf16*>(dx), lddx,
-                       int64_t(1));
-    HIP_TRY(hipGetLastError());
+    join_dx = Join<Bf16>{c.B, int(c.D), f.dx_splits, b.dx, c.B * p.Dp, int64_t(p.Dp), b.rows.factor, nullptr, b.rows.rest,
+                         of, static_cast<const Bf16*>(c.w), c.sv, c.sd, static_cast<Bf16*>(dx), lddx, int64_t(1)};
   }
   if (dw) {
     Bf16* const direct = f.dw_splits == 1 ? static_cast<Bf16*>(dw) : nullptr;
 #define SGNN_DWEIGHT(PER_ROW)                                                                                           \
   SGNN_WIDE(f.KD, hipLaunchKernelGGL((k_wide_grads<KD, true, PER_ROW>), dim3(unsigned(f.own_v * f.dw_splits)),          \
-                                     dim3(kGradThreads), 0, st, c.V, c.B, w, x, b.rows, f.steps_b, f.dw_splits, b.dx,   \
+                                     dim3(kGradThreads), 0, st, c.V, c.B, w, x, b.rows, f.steps_b, f.dw_splits, b.dw,   \
                                      c.V * p.Dp, int(c.D), direct, dsv, dsd, grad, share))
     if (share) {
       SGNN_DWEIGHT(false);
@@ -1558,14 +1590,11 @@ int wide_backward(const Call& c, const Wide& f, const Plan& p, const Buffers& b,
     }
 #undef SGNN_DWEIGHT
     HIP_TRY(hipGetLastError());
-    if (!direct) {
-      hipLaunchKernelGGL((k_class_join<Bf16>), dim3(unsigned(ceil_div(c.V, 32)), unsigned(ceil_div(c.D, 32))), dim3(256),
-                         0, st, c.V, int(c.D), f.dw_splits, b.dx, c.V * p.Dp, int64_t(p.Dp), share ? grad : nullptr,
-                         share, nullptr, Labels{}, nullptr, 0, 0, static_cast<Bf16*>(dw), dsv, dsd);
-      HIP_TRY(hipGetLastError());
-    }
+    if (!direct)
+      join_dw = Join<Bf16>{c.V, int(c.D), f.dw_splits, b.dw, c.V * p.Dp, int64_t(p.Dp), share ? grad : nullptr, share,
+                           nullptr, Labels{}, nullptr, 0, 0, static_cast<Bf16*>(dw), dsv, dsd};
   }
-  return SGNN_OK;
+  return launch_joins(join_dx, join_dw, st);
 }
 
 template <typename T>

@@ -31,7 +31,7 @@ def backward(lib, dx=P, lddx=8, dw=P, dsv=8, dsd=1, grad=P, stats=P, ws=P, ws_by
     (dict(x=None), -1, b"null"), (dict(w=None), -1, b"null"), (dict(labels=None), -1, b"null"),
     (dict(stats=None), -1, b"null"), (dict(rows=None), -1, b"null"), (dict(share=None), -1, b"null"),
     (dict(ws=None), -1, b"null"), (dict(ws_bytes=16), -2, b"workspace"), (dict(V=1 << 29), -4, b"2^28"),
-    (dict(B=1 << 26, n=1 << 26), -4, b"2^25"), (dict(V=1 << 28, D=65, ldx=65, sv=65), -4, b"2^34"),
+    (dict(B=1 << 26, n=1 << 26), -4, b"2^25"), (dict(V=1 << 28, D=65, ldx=65, sv=65), -4, b"2^33"),
     (dict(D=1 << 17, ldx=1 << 17, sv=1 << 17), -4, b"65536"),
 ])
 def test_forward_refuses(bad, rc, word):
