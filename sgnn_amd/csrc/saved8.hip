@@ -97,23 +97,25 @@ __device__ __forceinline__ float decode(float u, float step, float offset, float
 // Elements per thread of the element-wise passes: 16 bytes of the wide operand.
 template <typename T> struct Lane { static constexpr int kElems = 16 / sizeof(T); };
 
+// A lane's piece of a row: one access of 16 bytes wherever the row begins (memory takes any alignment;
+// element by element 19717 x 500 in bf16 takes 14 us to save and 17 to restore, so 10 and 8), single
+// elements at its end.
 template <typename T, int V>
-__device__ __forceinline__ void load_row(const T* p, int left, bool wide, T (&out)[V]) {
-  if (wide && left >= V) {
-    const u32x4 w = *reinterpret_cast<const u32x4*>(p);
-    __builtin_memcpy(&out, &w, 16);
+__device__ __forceinline__ void load_row(const T* p, int left, T (&out)[V]) {
+  if (left >= V) {
+    __builtin_memcpy(&out, p, sizeof(out));
   } else {
+    asm("" : "+v"(p));                           // or the last of these is merged with the last of those
 #pragma unroll
     for (int i = 0; i < V; ++i) out[i] = i < left ? p[i] : narrow<T>(0.f);
   }
 }
 template <typename T, int V>
-__device__ __forceinline__ void store_row(T* p, int left, bool wide, const T (&v)[V]) {
-  if (wide && left >= V) {
-    u32x4 w;
-    __builtin_memcpy(&w, &v, 16);
-    *reinterpret_cast<u32x4*>(p) = w;
+__device__ __forceinline__ void store_row(T* p, int left, const T (&v)[V]) {
+  if (left >= V) {
+    __builtin_memcpy(p, &v, sizeof(v));
   } else {
+    asm("" : "+v"(p));
 #pragma unroll
     for (int i = 0; i < V; ++i)
       if (i < left) p[i] = v[i];
@@ -128,8 +130,7 @@ constexpr int kEltThreads = 256;
 
 template <typename T>
 __global__ __launch_bounds__(kEltThreads) void k_save8(int64_t n, int F, const T* __restrict__ x, int64_t ldx,
-                                                       bool wide, float slope, int rows, int per_row,
-                                                       uint8_t* __restrict__ codes, uint8_t* __restrict__ steps) {
+                                                       float slope, int rows, int per_row, uint8_t* __restrict__ codes, uint8_t* __restrict__ steps) {
   constexpr int V = Lane<T>::kElems, kPer = kGroup / V;
   const bool plain = slope == 1.f;
   const int groups = (F + kGroup - 1) / kGroup;
@@ -140,7 +141,7 @@ __global__ __launch_bounds__(kEltThreads) void k_save8(int64_t n, int F, const T
     const int64_t r = row0 + lr;
     const int f = at * V, left = F - f;
     T raw[V];
-    load_row<T, V>(x + r * ldx + f, left, wide, raw);
+    load_row<T, V>(x + r * ldx + f, left, raw);
     float a[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) a[e] = widen(raw[e]);
@@ -165,7 +166,7 @@ __global__ __launch_bounds__(kEltThreads) void k_save8(int64_t n, int F, const T
 template <typename T>
 __global__ __launch_bounds__(kEltThreads) void k_restore8(int64_t n, int F, const uint8_t* __restrict__ codes,
                                                           const uint8_t* __restrict__ steps, float slope, int rows,
-                                                          int per_row, T* __restrict__ out, int64_t ldo, bool wide) {
+                                                          int per_row, T* __restrict__ out, int64_t ldo) {
   constexpr int V = Lane<T>::kElems, kPer = kGroup / V;
   const float offset = slope == 1.f ? -128.f : -127.5f, floor_u = slope == 0.f ? 127.5f : 0.f;
   const int groups = (F + kGroup - 1) / kGroup;
@@ -185,7 +186,7 @@ __global__ __launch_bounds__(kEltThreads) void k_restore8(int64_t n, int F, cons
       for (int b = 0; b < 4; ++b)
         v[4 * w + b] = narrow<T>(decode(float((u >> (8 * b)) & 0xffu), step, offset, floor_u));
     }
-    store_row<T, V>(out + r * ldo + f, F - f, wide, v);
+    store_row<T, V>(out + r * ldo + f, F - f, v);
   }
 }
 
@@ -193,8 +194,7 @@ __global__ __launch_bounds__(kEltThreads) void k_restore8(int64_t n, int F, cons
 template <typename T>
 __global__ __launch_bounds__(kEltThreads) void k_input_grad8(int64_t n, int F, const uint8_t* __restrict__ codes,
                                                              float slope, int rows, int per_row, const T* g,
-                                                             int64_t ldg, bool g_wide, T* dx, int64_t lddx,
-                                                             bool dx_wide) {
+                                                             int64_t ldg, T* dx, int64_t lddx) {
   constexpr int V = Lane<T>::kElems;
   const int groups = (F + kGroup - 1) / kGroup;
   const int64_t row0 = int64_t(blockIdx.x) * rows;
@@ -206,13 +206,13 @@ __global__ __launch_bounds__(kEltThreads) void k_input_grad8(int64_t n, int F, c
     if (left <= 0) continue;
     const unsigned* src = reinterpret_cast<const unsigned*>(codes + r * (int64_t(groups) * kGroup) + f);
     T v[V];
-    load_row<T, V>(g + r * ldg + f, left, g_wide, v);
+    load_row<T, V>(g + r * ldg + f, left, v);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       const bool negative = (src[e / 4] >> (8 * (e % 4) + 7)) & 1u;
       if (negative) v[e] = slope == 0.f ? narrow<T>(0.f) : narrow<T>(slope * widen(v[e]));
     }
-    store_row<T, V>(dx + r * lddx + f, left, dx_wide, v);
+    store_row<T, V>(dx + r * lddx + f, left, v);
   }
 }
 
@@ -257,7 +257,7 @@ __device__ __forceinline__ bf16x8 slab_frag(const char* slab, int k0, int c0, in
 template <typename T, int BH, int BF, int WH, int WF>
 __global__ __launch_bounds__(64 * WH * WF, BH >= 128 ? 4 : 2) void k_weight_grad8(
     int64_t n, int F, int H, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ steps, float slope,
-    const T* __restrict__ g, int64_t ldg, bool wide, int64_t chunk_rows, int chunks, int tiles_f, int tiles_h,
+    const T* __restrict__ g, int64_t ldg, int64_t chunk_rows, int chunks, int tiles_f, int tiles_h,
     T* __restrict__ dW, int64_t lddw, float* __restrict__ partial) {
   constexpr int kThreads = 64 * WH * WF;
   constexpr int P = sizeof(T) == 4 ? 3 : 1;
@@ -306,13 +306,10 @@ __global__ __launch_bounds__(64 * WH * WF, BH >= 128 ? 4 : 2) void k_weight_grad
       for (int e = 0; e < GV; ++e) rg[l][e] = narrow<T>(0.f);
       if (s < kGradSlots && r < last && h < H) {
         const T* p = g + r * ldg + h;
-        if (wide && h + GV <= H) {
-#pragma unroll
-          for (int q = 0; q < GV * int(sizeof(T)) / 16; ++q) {
-            const u32x4 w = reinterpret_cast<const u32x4*>(p)[q];
-            __builtin_memcpy(reinterpret_cast<char*>(&rg[l][0]) + 16 * q, &w, 16);
-          }
+        if (h + GV <= H) {
+          __builtin_memcpy(&rg[l], p, sizeof(rg[l]));
         } else {
+          asm("" : "+v"(p));
 #pragma unroll
           for (int e = 0; e < GV; ++e)
             if (h + e < H) rg[l][e] = p[e];
@@ -614,7 +611,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void k_linear_grad8(int64_t n, int F, int H, const T* __restrict__ g, int64_t ldg,
                                                       const T* __restrict__ w, int64_t ldw, float slope,
                                                       const uint8_t* __restrict__ codes, T* __restrict__ dx,
-                                                      int64_t lddx, bool dx_wide) {
+                                                      int64_t lddx) {
   constexpr int P = Planes<T>::kCount;
   constexpr int kChunks = kLinStep * 8 / 256;    // of 8 features, a thread's share of a weight step (64 x 64)
   constexpr int kKept = 4;                       // sixteens of units whose grad stays in registers
@@ -733,7 +730,7 @@ __global__ __launch_bounds__(256) void k_linear_grad8(int64_t n, int F, int H, c
         }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       T* const out = dx + first * lddx + f0 + 32 * jj;
-      if (dx_wide && f0 + kLinStep <= F) {
+      if (f0 + kLinStep <= F) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int row = 8 * i + (lane >> 3), c = lane & 7;
@@ -802,10 +799,6 @@ int check_saved(int dtype, int64_t n, int64_t F, float slope) {
   return SGNN_OK;
 }
 
-bool wide_ok(const void* p, int64_t ld, size_t elem) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (size_t(ld) * elem) % 16 == 0;
-}
-
 struct EltGrid { int rows, per_row; unsigned blocks; };
 int elt_grid(int64_t n, int64_t F, int elems, EltGrid* g) {
   const int64_t per_row = (F + kGroup - 1) / kGroup * (kGroup / elems);
@@ -824,11 +817,10 @@ int launch_weight_grad(const GradPlan& p, int64_t n, int64_t F, int64_t H, const
                        hipStream_t st) {
   const T* g = static_cast<const T*>(grad);
   T* out = static_cast<T*>(dW);
-  const bool wide = wide_ok(grad, ldg, sizeof(T));
   const unsigned blocks = unsigned((p.chunks < 8 ? p.chunks : (p.chunks + 7) / 8 * 8) * p.tiles_f * p.tiles_h);
 #define SGNN_WG8(BH, BF, WH, WF)                                                                                  \
   hipLaunchKernelGGL((k_weight_grad8<T, BH, BF, WH, WF>), dim3(blocks), dim3(64 * WH * WF), 0, st, n, int(F),     \
-                     int(H), codes, steps, slope, g, ldg, wide, p.chunk_rows, p.chunks, p.tiles_f, p.tiles_h, out, \
+                     int(H), codes, steps, slope, g, ldg, p.chunk_rows, p.chunks, p.tiles_f, p.tiles_h, out,       \
                      lddw, partial)
   if (p.bh == 32) SGNN_WG8(32, 256, 1, 4);
   else if (p.bh == 64) SGNN_WG8(64, 256, 1, 4);
@@ -861,11 +853,11 @@ extern "C" int sgnn_save8(int dtype, int64_t n, int64_t F, const void* x, int64_
   if (dtype == SGNN_F32) {
     if (int rc = elt_grid(n, F, Lane<float>::kElems, &g)) return rc;
     hipLaunchKernelGGL((k_save8<float>), dim3(g.blocks), dim3(kEltThreads), 0, st, n, int(F),
-                       static_cast<const float*>(x), ldx, wide_ok(x, ldx, 4), slope, g.rows, g.per_row, q, s);
+                       static_cast<const float*>(x), ldx, slope, g.rows, g.per_row, q, s);
   } else {
     if (int rc = elt_grid(n, F, Lane<Bf16>::kElems, &g)) return rc;
     hipLaunchKernelGGL((k_save8<Bf16>), dim3(g.blocks), dim3(kEltThreads), 0, st, n, int(F),
-                       static_cast<const Bf16*>(x), ldx, wide_ok(x, ldx, 2), slope, g.rows, g.per_row, q, s);
+                       static_cast<const Bf16*>(x), ldx, slope, g.rows, g.per_row, q, s);
   }
   HIP_TRY(hipGetLastError());
   return SGNN_OK;
@@ -917,7 +909,7 @@ int launch_linear_grad(int64_t n, int64_t F, int64_t H, const void* g, int64_t l
   if (across > tiles) across = tiles;
   hipLaunchKernelGGL((k_linear_grad8<T>), dim3(unsigned(blocks), unsigned(across)), dim3(256), 0, st, n, int(F), int(H),
                      static_cast<const T*>(g), ldg, static_cast<const T*>(w), ldw, slope, codes, static_cast<T*>(dx),
-                     lddx, sizeof(T) == 4 || wide_ok(dx, lddx, sizeof(T)));
+                     lddx);
   HIP_TRY(hipGetLastError());
   return SGNN_OK;
 }
@@ -969,11 +961,11 @@ extern "C" int sgnn_restore8(int dtype, int64_t n, int64_t F, const void* codes,
   if (dtype == SGNN_F32) {
     if (int rc = elt_grid(n, F, Lane<float>::kElems, &g)) return rc;
     hipLaunchKernelGGL((k_restore8<float>), dim3(g.blocks), dim3(kEltThreads), 0, st, n, int(F), q, s, slope, g.rows,
-                       g.per_row, static_cast<float*>(out), ldo, wide_ok(out, ldo, 4));
+                       g.per_row, static_cast<float*>(out), ldo);
   } else {
     if (int rc = elt_grid(n, F, Lane<Bf16>::kElems, &g)) return rc;
     hipLaunchKernelGGL((k_restore8<Bf16>), dim3(g.blocks), dim3(kEltThreads), 0, st, n, int(F), q, s, slope, g.rows,
-                       g.per_row, static_cast<Bf16*>(out), ldo, wide_ok(out, ldo, 2));
+                       g.per_row, static_cast<Bf16*>(out), ldo);
   }
   HIP_TRY(hipGetLastError());
   return SGNN_OK;
@@ -994,13 +986,13 @@ extern "C" int sgnn_saved8_input_grad(int dtype, int64_t n, int64_t F, const voi
   if (dtype == SGNN_F32) {
     if (int rc = elt_grid(n, F, Lane<float>::kElems, &g)) return rc;
     hipLaunchKernelGGL((k_input_grad8<float>), dim3(g.blocks), dim3(kEltThreads), 0, st, n, int(F), q, slope, g.rows,
-                       g.per_row, static_cast<const float*>(grad), ldg, wide_ok(grad, ldg, 4),
-                       static_cast<float*>(dx), lddx, wide_ok(dx, lddx, 4));
+                       g.per_row, static_cast<const float*>(grad), ldg,
+                       static_cast<float*>(dx), lddx);
   } else {
     if (int rc = elt_grid(n, F, Lane<Bf16>::kElems, &g)) return rc;
     hipLaunchKernelGGL((k_input_grad8<Bf16>), dim3(g.blocks), dim3(kEltThreads), 0, st, n, int(F), q, slope, g.rows,
-                       g.per_row, static_cast<const Bf16*>(grad), ldg, wide_ok(grad, ldg, 2),
-                       static_cast<Bf16*>(dx), lddx, wide_ok(dx, lddx, 2));
+                       g.per_row, static_cast<const Bf16*>(grad), ldg,
+                       static_cast<Bf16*>(dx), lddx);
   }
   HIP_TRY(hipGetLastError());
   return SGNN_OK;
