@@ -35,6 +35,37 @@ struct Labels {
   int64_t n_labels, V;
 };
 
+struct RowStat { float m, s, picked; };          // what the backward pass needs of a row; picked = the label's logit
+
+// What the gradients of the kernels with rows in registers need of a row: p = 2^((z - top) log2 e - shift)
+// with top = 0 but for rows whose logits are so large that the rounding of shift would be felt (2^12: by
+// 2^-12, a bf16 half step being 2^-8); shift = infinity without a class; its factor, its label, and what
+// the label's element of dz adds in dx beyond its rounded probability.
+constexpr float kLargeLogit = 4096.f;
+struct RowConst {
+  float *shift, *top, *factor, *rest;
+  int* label;
+};
+struct Rows {
+  int64_t B;
+  const RowStat* stats;                          // NULL: not wanted
+  const float *grad, *share;
+  RowConst out;
+};
+
+__device__ __forceinline__ void prepare_row(const Rows& rows, int64_t b, const Labels& of) {
+  const int64_t y = b < rows.B ? label_of(b, of.labels, of.idx, of.n_labels, of.V) : -1;
+  const RowStat st = y >= 0 ? rows.stats[b] : RowStat{INFINITY, 1.f, 0.f};
+  const bool large = y >= 0 && !(fabsf(st.m) <= kLargeLogit);
+  const float top = large ? st.m : 0.f, shift = large ? log2f(st.s) : fmaf(st.m, kLog2e, log2f(st.s));
+  const float p = exp2_raw(fmaf(st.picked - top, kLog2e, -shift));
+  rows.out.shift[b] = shift;
+  rows.out.top[b] = top;
+  rows.out.factor[b] = y < 0 ? 0.f : rows.share ? rows.grad[0] * rows.share[0] : rows.grad[b];
+  rows.out.rest[b] = (p - widen(Bf16{to_bf16(p)})) - 1.f;
+  rows.out.label[b] = int(y);
+}
+
 // in[r][d] at r * sr + d * sd  ->  out[r][Dp], columns D .. Dp zero.  Rows of x without a class
 // become zeros, so that whatever a padded row holds (NaN too) reaches no gradient.
 struct Source {
@@ -44,10 +75,11 @@ struct Source {
   int64_t blocks;          // workgroups it takes: one for 64 x 64 elements
 };
 
-// x and the weight in one launch.  Rows that are contiguous go straight through registers, eight
+// x and the weight in one launch, and with `rows` what the gradients need of each row, up to a whole
+// number of 64.  Rows that are contiguous go straight through registers, eight
 // elements a lane; a weight stored by feature goes through a tile in LDS.
 template <typename T>
-__global__ __launch_bounds__(256) void k_class_operands(int D, int Dp, Source first, Source second, Labels of) {
+__global__ __launch_bounds__(256) void k_class_operands(int D, int Dp, Source first, Source second, Labels of, Rows rows) {
   __shared__ T tile[64][sizeof(T) == 4 ? 65 : 66];
   const bool is_x = int64_t(blockIdx.x) < first.blocks;
   const Source src = is_x ? first : second;
@@ -56,6 +88,7 @@ __global__ __launch_bounds__(256) void k_class_operands(int D, int Dp, Source fi
   const int64_t r0 = block / across * 64;
   const int d0 = int(block % across) * 64, t = threadIdx.x;
   const T* in = static_cast<const T*>(src.in);
+  if (is_x && d0 == 0 && t < 64 && rows.stats) prepare_row(rows, r0 + t, of);
   const auto live = [&](int64_t r) {
     return r < src.rows && (!is_x || label_of(r, of.labels, of.idx, of.n_labels, of.V) >= 0);
   };
@@ -97,8 +130,6 @@ __global__ __launch_bounds__(256) void k_class_operands(int D, int Dp, Source fi
 // ------------------------------------------------------------------ forward
 // (m, s): m = the largest logit, s = sum of 2^((z - m) log2 e).  While everything is -inf the sum
 // stays 0; a NaN never becomes the maximum but makes the sum NaN.
-struct RowStat { float m, s, picked; };          // what the backward pass needs of a row; picked = the label's logit
-
 __device__ __forceinline__ void join_stats(float& m, float& s, float om, float os) {
   const float top = fmaxf(m, om), ref = top == -INFINITY ? 0.f : top;
   s = s * exp2_raw((m - ref) * kLog2e) + os * exp2_raw((om - ref) * kLog2e);
@@ -981,33 +1012,6 @@ __global__ __launch_bounds__(kThreads) void k_wide_stats(int64_t B, int64_t V, O
   }
 }
 
-// What the gradients need of a row: p = 2^((z - top) log2 e - shift) with top = 0 but for rows whose
-// logits are so large that the rounding of shift would be felt (2^12: by 2^-12, a bf16 half step
-// being 2^-8); shift = infinity without a class; its factor, its label, and what the label's element
-// of dz adds in dx beyond its rounded probability.
-constexpr float kLargeLogit = 4096.f;
-struct RowConst {
-  float *shift, *top, *factor, *rest;
-  int* label;
-};
-
-__global__ __launch_bounds__(256) void k_wide_rows(int64_t B, int64_t padded, Labels of,
-                                                   const RowStat* __restrict__ stats, const float* __restrict__ grad,
-                                                   const float* __restrict__ share, RowConst out) {
-  const int64_t b = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (b >= padded) return;
-  const int64_t y = b < B ? label_of(b, of.labels, of.idx, of.n_labels, of.V) : -1;
-  const RowStat st = y >= 0 ? stats[b] : RowStat{INFINITY, 1.f, 0.f};
-  const bool large = y >= 0 && !(fabsf(st.m) <= kLargeLogit);
-  const float top = large ? st.m : 0.f, shift = large ? log2f(st.s) : fmaf(st.m, kLog2e, log2f(st.s));
-  const float p = exp2_raw(fmaf(st.picked - top, kLog2e, -shift));
-  out.shift[b] = shift;
-  out.top[b] = top;
-  out.factor[b] = y < 0 ? 0.f : share ? grad[0] * share[0] : grad[b];
-  out.rest[b] = (p - widen(Bf16{to_bf16(p)})) - 1.f;
-  out.label[b] = int(y);
-}
-
 // acc += streamed^T . p over a half step, with other work between as above
 template <int KD, int NB, typename Between>
 __device__ __forceinline__ void stream_gather_between(const char* tile, int sub, const StreamLane& at,
@@ -1373,6 +1377,7 @@ Buffers carve_wide(const Wide& f, const Plan& p, int64_t B, int64_t V, bool back
     b.part = c.take<float2>(size_t(f.stat_splits) * B);
     b.picked = c.take<float>(size_t(B));
   } else {
+    static_assert(kStreamRows == 64, "rows are laid out and prepared 64 at a time");
     const size_t padded = size_t(f.steps_b) * kStreamRows;
     b.rows = RowConst{c.take<float>(padded), c.take<float>(padded), c.take<float>(padded), c.take<float>(padded),
                       c.take<int>(padded)};
@@ -1439,7 +1444,8 @@ bool weight_as_is(const Call& c, const Plan& p) {
 }
 
 template <typename T>
-int operands(const Call& c, const Plan& p, const Buffers& b, Operand<T>* x, Operand<T>* w, hipStream_t st) {
+int operands(const Call& c, const Plan& p, const Buffers& b, const Rows& rows, Operand<T>* x, Operand<T>* w,
+             hipStream_t st) {
   const int across = p.Dp / 64;
   const Source sx{c.x, c.B, c.ldx, 1, b.x, ceil_div(c.B, 64) * across};
   Source sw{c.w, c.V, c.sv, c.sd, b.w, ceil_div(c.V, 64) * across};
@@ -1450,7 +1456,7 @@ int operands(const Call& c, const Plan& p, const Buffers& b, Operand<T>* x, Oper
     *w = Operand<T>{static_cast<const T*>(c.w), c.sv, c.V, c.D};
   }
   hipLaunchKernelGGL((k_class_operands<T>), dim3(unsigned(sx.blocks + sw.blocks)), dim3(256), 0, st, int(c.D), p.Dp, sx,
-                     sw, Labels{c.labels, c.idx, c.n_labels, c.V});
+                     sw, Labels{c.labels, c.idx, c.n_labels, c.V}, rows);
   HIP_TRY(hipGetLastError());
   return SGNN_OK;
 }
@@ -1478,7 +1484,7 @@ template <typename T>
 int forward(const Call& c, const Plan& p, const Buffers& b, RowStat* stats, float* row_loss, float* loss,
             float* share, hipStream_t st) {
   Operand<T> x, w;
-  if (int rc = operands<T>(c, p, b, &x, &w, st)) return rc;
+  if (int rc = operands<T>(c, p, b, Rows{}, &x, &w, st)) return rc;
   const int depth = int(ceil_div(c.D, p.depth) * p.depth);
   hipLaunchKernelGGL((k_class_stats<T>), dim3(unsigned(p.tiles_b * p.stat_splits)), dim3(kThreads), 0, st, c.B, c.V,
                      depth, x, w, c.labels, c.idx, c.n_labels, p.tiles_v, p.stat_splits, b.part, b.picked);
@@ -1499,7 +1505,7 @@ template <typename T>
 int backward(const Call& c, const Plan& p, const Buffers& b, const RowStat* stats, const float* grad,
              const float* share, void* dx, int64_t lddx, void* dw, int64_t dsv, int64_t dsd, hipStream_t st) {
   Operand<T> x, w;
-  if (int rc = operands<T>(c, p, b, &x, &w, st)) return rc;
+  if (int rc = operands<T>(c, p, b, Rows{}, &x, &w, st)) return rc;
   const int64_t Np = int64_t(p.tiles_d) * kTile;
   T* const dz = reinterpret_cast<T*>(b.dz);
   const int depth = int(ceil_div(c.D, p.depth) * p.depth);
@@ -1550,7 +1556,7 @@ int backward(const Call& c, const Plan& p, const Buffers& b, const RowStat* stat
 int wide_forward(const Call& c, const Wide& f, const Plan& p, const Buffers& b, RowStat* stats, float* row_loss,
                  float* loss, float* share, hipStream_t st) {
   Operand<Bf16> x, w;
-  if (int rc = operands<Bf16>(c, p, b, &x, &w, st)) return rc;
+  if (int rc = operands<Bf16>(c, p, b, Rows{}, &x, &w, st)) return rc;
   const Labels of{c.labels, c.idx, c.n_labels, c.V};
   SGNN_WIDE(f.KD, hipLaunchKernelGGL((k_wide_stats<KD>), dim3(unsigned(f.own_b * f.stat_splits)), dim3(kThreads), 0, st,
                                      c.B, c.V, x, w, of, f.steps_v, f.stat_splits, b.part, b.picked));
@@ -1562,12 +1568,8 @@ int wide_backward(const Call& c, const Wide& f, const Plan& p, const Buffers& b,
                   const float* grad, const float* share, void* dx, int64_t lddx, void* dw, int64_t dsv, int64_t dsd,
                   hipStream_t st) {
   Operand<Bf16> x, w;
-  if (int rc = operands<Bf16>(c, p, b, &x, &w, st)) return rc;
+  if (int rc = operands<Bf16>(c, p, b, Rows{c.B, stats, grad, share, b.rows}, &x, &w, st)) return rc;
   const Labels of{c.labels, c.idx, c.n_labels, c.V};
-  const int64_t padded = f.steps_b * kStreamRows;
-  hipLaunchKernelGGL(k_wide_rows, dim3(unsigned(ceil_div(padded, 256))), dim3(256), 0, st, c.B, padded, of, stats, grad,
-                     share, b.rows);
-  HIP_TRY(hipGetLastError());
   Join<Bf16> join_dx{}, join_dw{};
   if (dx) {
     SGNN_WIDE(f.KD, hipLaunchKernelGGL((k_wide_grads<KD, false, false>), dim3(unsigned(f.own_b * f.dx_splits)),
