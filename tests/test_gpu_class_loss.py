@@ -507,3 +507,20 @@ def test_stacked_layer_with_thousands_of_classes(gpu_device):
         results.append((layer.W.detach().clone(), layer.Wt.detach().clone()))
     for a, b in zip(*results):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,D,V", [(5, 40, 3000), (30, 300, 700), (200, 100, 900), (300, 300, 5000)])
+def test_one_gradient_alone(gpu_device, dtype, B, D, V):
+    """Either operand's gradient by itself is the one that comes with the other's, bit for bit."""
+    x, w, labels = make(B, D, V, DTYPES[dtype], gpu_device, seed=B)
+    both = x.clone().requires_grad_(), w.clone().requires_grad_()
+    snn.class_cross_entropy(*both, labels).backward()
+    only_x, only_w = x.clone().requires_grad_(), w.clone().requires_grad_()
+    snn.class_cross_entropy(only_x, w, labels).backward()
+    snn.class_cross_entropy(x, only_w, labels).backward()
+    assert torch.equal(only_x.grad, both[0].grad) and torch.equal(only_w.grad, both[1].grad)
+    turned = w.t().contiguous().requires_grad_()         # stored by feature: the same values, the gradient likewise
+    snn.class_cross_entropy(x, turned.t(), labels).backward()
+    assert turned.grad.is_contiguous()
+    close(turned.grad.t(), both[1].grad.double(), reference(x, w, labels)["dw_bound"] * 2, "dweight by feature")
