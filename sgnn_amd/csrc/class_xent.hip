@@ -528,7 +528,8 @@ __global__ __launch_bounds__(256) void k_class_join(Join<T> first, Join<T> secon
 // second time mostly from the last-level cache), as it lies, and its gradient written once.  x
 // waits in LDS as bf16 planes; a wavefront takes 32 classes at a time straight from memory into the
 // matrix instructions' operand, splitting them in registers.  Both gradients are plain 32-bit
-// multiply-adds: 2 * rows of them per element of the weight.
+// multiply-adds: 2 * rows of them per element of the weight.  Losses of one row against 100003 classes of
+// 256 features in fp32: 26 us, 3.9 TB/s; with 512 or 1024 workgroups or 128 features loaded together 27 to 30.
 constexpr int kFewRows = 32;
 constexpr int kFewBlocks = 768;                  // workgroups: three per CU
 constexpr int kFewSteps = 4;                     // 16-feature steps loaded together
