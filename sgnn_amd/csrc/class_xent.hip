@@ -9,7 +9,10 @@
 //
 // All four products run on the bf16 matrix instructions (tile_product.h): bf16 operands as they
 // are, fp32 ones as three bf16 numbers each.  dz of bf16 operands is rounded to bf16 there
-// (relative 2^-8 per element at most, the half step that each result is rounded by, too).
+// (relative 2^-8 per element at most, the half step that each result is rounded by, too), but for the
+// label's element, the largest of its row and of nearly every class: that keeps 16 bits or more in both
+// gradients.  4096 x 256 against 50000 classes: dweight is off by 2.3e-5 of its norm before its own
+// rounding, with that element rounded like the others by 2.1e-4.
 //
 // Bound by the matrix unit.  2048 x 602 against 10007 classes in fp32 (24.7 GFLOP a product, six bf16
 // products each): statistics 175 us, dz 164, dx 169, dweight 204, that is 0.73 to 0.90 PFLOP/s of the
@@ -48,7 +51,7 @@ struct RowConst {
 };
 struct Rows {
   int64_t B;
-  const RowStat* stats;                          // NULL: not wanted
+  const RowStat* stats;                          // NULL: no more than the label is wanted, or nothing
   const float *grad, *share;
   RowConst out;
 };
@@ -88,7 +91,10 @@ __global__ __launch_bounds__(256) void k_class_operands(int D, int Dp, Source fi
   const int64_t r0 = block / across * 64;
   const int d0 = int(block % across) * 64, t = threadIdx.x;
   const T* in = static_cast<const T*>(src.in);
-  if (is_x && d0 == 0 && t < 64 && rows.stats) prepare_row(rows, r0 + t, of);
+  if (is_x && d0 == 0 && t < 64) {
+    if (rows.stats) prepare_row(rows, r0 + t, of);
+    else if (rows.out.label && r0 + t < rows.B) rows.out.label[r0 + t] = int(label_of(r0 + t, of.labels, of.idx, of.n_labels, of.V));
+  }
   const auto live = [&](int64_t r) {
     return r < src.rows && (!is_x || label_of(r, of.labels, of.idx, of.n_labels, of.V) >= 0);
   };
@@ -301,8 +307,8 @@ __global__ __launch_bounds__(1024) void k_class_mean(int64_t B, int64_t V, const
 // ------------------------------------------------------------------ backward
 // dz of the classes v0 .. v0 + 128 * tiles and all rows, [Bp][ldz]; rows and
 // classes beyond the last are 0.  `grad` NULL leaves the mean's factor to the gradients' last step.
-// The label's element dominates a row and is the one whose rounding to bf16 would be felt in dx:
-// what it loses is kept in rest[b] and joins dx in 32 bits.
+// The label's element dominates a row, and often its class, and is the one whose rounding to bf16 would be
+// felt: what it loses is kept in rest[b] and joins both gradients in 32 bits.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_class_dz(int64_t B, int64_t V, int Dp, Operand<T> x, Operand<T> w,
                                                        const int64_t* __restrict__ labels,
@@ -404,6 +410,69 @@ struct Product {
   int64_t plane, ldo;
   Direct<T> direct;
   unsigned blocks;                               // workgroups it takes: tiles_m * splits * tiles_n
+  // dweight in bf16: what the labels' elements lost by their rounding, `rest` of each of `rows` rows, at
+  // row label - first of the result
+  const float* rest;
+  const int* label;
+  int64_t rows, first;
+};
+
+// acc[m][n] += rest[b] * x[b][n] for the rows b whose label is class m, the element of dz that is nearly
+// all of a class's gradient, so that it keeps 16 bits: step by step of the reduction, whose rows of x are
+// in LDS.  A step's labels and rests are under way while the step before is multiplied.  Costs 4096 x 512
+// against 50000 classes 20 us of 270, 16384 x 512 against 500 (a label in every sixteen rows) 15 of 145 in all.
+struct RestOfLabels {
+  const Product<Bf16>& p;
+  int64_t m, end;                                // the wavefront's first class; the reduction's end
+  int n, lane;                                   // its first column in the tile
+  int label = -1, next_label = -1;
+  float rest = 0.f, next_rest = 0.f;
+  __device__ __forceinline__ void ahead(int64_t k) {
+    const int64_t b = k + lane;
+    const bool real = b < end && b < p.rows;
+    next_label = real ? p.label[b] : -1;
+    next_rest = real ? p.rest[b] : 0.f;
+  }
+  // waited for here, before the next stage's loads are on their way, which would be waited for, too
+  __device__ __forceinline__ void landed() {
+    asm volatile("" : "+v"(next_label), "+v"(next_rest));
+    label = next_label;
+    rest = next_rest;
+  }
+  __device__ __forceinline__ void behind(const char* x, Tile& acc) {
+    const int64_t at = label - (p.first + m);
+    const int in = label >= 0 && at >= 0 && at < 64 ? int(at) : -1;
+    const unsigned mine = to_bf16(rest);
+    const uint64_t hits = __ballot(in >= 0);
+    if (hits == 0) return;
+    for (int kk = 0; kk < Step<Bf16>::kDepth; kk += 16) {
+      unsigned h = unsigned(hits >> kk) & 0xffffu;
+      if (h == 0) continue;
+      // the operand classes x rows of sixteen rows, nearly all of it zeros
+      u32x4 rows[2] = {u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}};
+      for (; h != 0; h &= h - 1) {
+        const int r = __builtin_ctz(h);
+        const int to = __builtin_amdgcn_readlane(in, kk + r);
+        const unsigned value = unsigned(__builtin_amdgcn_readlane(int(mine), kk + r)) << (16 * (r & 1));
+        const unsigned here = (to & 31) == (lane & 31) && r >> 3 == lane >> 5 ? value : 0u;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) rows[i][w] |= i == to >> 5 && w == (r & 7) >> 1 ? here : 0u;
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        bf16x8 columns;
+        read_fragment<false>(x, n + 32 * j, kk, lane, columns);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          bf16x8 a;
+          __builtin_memcpy(&a, &rows[i], 16);
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, columns, acc[i][j], 0, 0, 0);
+        }
+      }
+    }
+  }
 };
 
 template <typename T, bool ADEEP>
@@ -417,7 +486,15 @@ __device__ __forceinline__ void form_product(const Product<T>& p, unsigned block
   const int64_t k0 = steps * split / p.splits * Step<T>::kDepth, k1 = steps * (split + 1) / p.splits * Step<T>::kDepth;
   Tile acc;
   clear(acc);
-  if (k0 < k1) multiply<T, ADEEP, false>(p.a, m0, p.b, n0, k0, k1, lds, acc);
+  if constexpr (!ADEEP && sizeof(T) == 2) {
+    RestOfLabels rest{p, m0 + wm, k1, wn, lane};
+    if (k0 < k1) {
+      rest.ahead(k0);
+      multiply<T, ADEEP, false>(p.a, m0, p.b, n0, k0, k1, lds, acc, rest);
+    }
+  } else {
+    if (k0 < k1) multiply<T, ADEEP, false>(p.a, m0, p.b, n0, k0, k1, lds, acc);
+  }
   if (!ADEEP && p.direct.out) {
     const Direct<T>& direct = p.direct;
     const float factor = direct.share ? direct.grad[0] * direct.share[0] : 1.f;
@@ -451,12 +528,14 @@ __device__ __forceinline__ void form_product(const Product<T>& p, unsigned block
     }
 }
 
-// Both gradients' products in one launch: 512 x 128 against 1000 classes in fp32 11 us, one after the
-// other 17 and a launch more; where either fills the card the same.
-template <typename T>
+// Both gradients' products in one launch where one of them leaves slots empty: 512 x 128 against 1000
+// classes in fp32 11 us, one after the other 17 and a launch more.  Where either fills the card, kernels of
+// their own: 4096 x 512 against 50000 classes in bf16, all of it, 1200 us, in one launch 1243; 2048 x 602
+// against 10007 in fp32 655 and 659.
+template <typename T, bool DX, bool DW>
 __global__ __launch_bounds__(kThreads) void k_class_products(Product<T> dx, Product<T> dw) {
   __shared__ __align__(128) char lds[kProductLds];
-  if (blockIdx.x < dx.blocks) form_product<T, true>(dx, blockIdx.x, lds);
+  if (!DW || (DX && blockIdx.x < dx.blocks)) form_product<T, true>(dx, blockIdx.x, lds);
   else form_product<T, false>(dw, blockIdx.x - dx.blocks, lds);
 }
 
@@ -1138,9 +1217,12 @@ __global__ __launch_bounds__(kGradThreads, 2) void k_wide_grads(int64_t owners, 
 #pragma unroll
       for (int i = 0; i < 16 * NB; ++i) weigh(i);
     }
+    bool with_label = false;
     if constexpr (BY_CLASS) {
       // rows whose label is among the owned classes: rare
-      for (uint64_t h = __ballot(label >= o0 && label < o0 + 32 * NB) >> (32 * sub) & 0xffffffffull; h != 0; h &= h - 1) {
+      uint64_t h = __ballot(label >= o0 && label < o0 + 32 * NB) >> (32 * sub) & 0xffffffffull;
+      with_label = h != 0;
+      for (; h != 0; h &= h - 1) {
         const int r = __builtin_ctzll(h);
         const int col = int(__shfl(label, 32 * sub + r) - o0);
         int mine = r - 4 * (lane >> 5);          // compared with constants
@@ -1172,7 +1254,26 @@ __global__ __launch_bounds__(kGradThreads, 2) void k_wide_grads(int64_t owners, 
     for (int j = 0; j < NB; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) p[j][e >> 3][e & 7] = static_cast<__bf16>(z[j][e]);
-    if constexpr (!kTurns) stream_gather_between<KD, NB>(tile, sub, here, p, acc, [](int) {});
+    // The label's element is nearly all of a class's gradient, and what rounding takes off it would be
+    // felt: a half step that holds one is multiplied by that, too.
+    bf16x8 off[NB][2];
+    if (BY_CLASS && with_label) {
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          off[j][e >> 3][e & 7] = static_cast<__bf16>(z[j][e] - static_cast<float>(p[j][e >> 3][e & 7]));
+    }
+    if constexpr (kTurns) {
+      if (BY_CLASS && with_label) stream_gather_between<KD, NB>(tile, sub, here, off, acc, [](int) {});
+    } else {
+      for (bool again = BY_CLASS && with_label;; again = false) {
+        stream_gather_between<KD, NB>(tile, sub, here, p, acc, [](int) {});
+        if (!again) break;
+#pragma unroll
+        for (int j = 0; j < NB; ++j) p[j][0] = off[j][0], p[j][1] = off[j][1];
+      }
+    }
   };
   const char* tile = lds;
   for (int64_t t = t0; t < t1; ++t) {
@@ -1362,6 +1463,7 @@ Buffers carve(const Plan& p, int64_t B, int64_t V, bool backward, void* base) {
     const size_t Np = size_t(p.tiles_d) * kTile;
     b.dz = c.take<char>(p.elem * p.Bp * p.piece);
     b.rest = c.take<float>(size_t(B));
+    if (p.elem == 2) b.rows.label = c.take<int>(size_t(B));
     b.dx = c.take<float>(size_t(p.dx_splits) * p.Bp * Np);
     b.dw = c.take<float>(size_t(p.dw_splits) * p.piece * Np);
   }
@@ -1506,7 +1608,7 @@ template <typename T>
 int backward(const Call& c, const Plan& p, const Buffers& b, const RowStat* stats, const float* grad,
              const float* share, void* dx, int64_t lddx, void* dw, int64_t dsv, int64_t dsd, hipStream_t st) {
   Operand<T> x, w;
-  if (int rc = operands<T>(c, p, b, Rows{}, &x, &w, st)) return rc;
+  if (int rc = operands<T>(c, p, b, Rows{c.B, nullptr, nullptr, nullptr, b.rows}, &x, &w, st)) return rc;
   const int64_t Np = int64_t(p.tiles_d) * kTile;
   T* const dz = reinterpret_cast<T*>(b.dz);
   const int depth = int(ceil_div(c.D, p.depth) * p.depth);
@@ -1521,20 +1623,30 @@ int backward(const Call& c, const Plan& p, const Buffers& b, const RowStat* stat
     Product<T> to_dx{}, to_dw{};
     if (dx)                                      // dx[b][d] += dz[b][v] . w[v][d]
       to_dx = Product<T>{a, Operand<T>{w.base + v0 * w.ld, w.ld, c.V - v0, w.cols}, width, p.tiles_d, p.dx_splits,
-                         v0 > 0 ? 1 : 0, b.dx, p.Bp * Np, Np, Direct<T>{}, unsigned(p.tiles_b * p.dx_splits * p.tiles_d)};
+                         v0 > 0 ? 1 : 0, b.dx, p.Bp * Np, Np, Direct<T>{}, unsigned(p.tiles_b * p.dx_splits * p.tiles_d), nullptr, nullptr, 0, 0};
     Join<T> join_dw{};
     if (dw) {                                    // dw[v][d] = dz[b][v] . x[b][d]
       const int64_t rows = c.V - v0 < width ? c.V - v0 : width;
       T* const out = static_cast<T*>(dw) + v0 * dsv;
       to_dw = Product<T>{a, x, p.Bp, p.tiles_d, p.dw_splits, 0, b.dw, p.piece * Np, Np, Direct<T>{},
-                         unsigned(tiles * p.dw_splits * p.tiles_d)};
+                         unsigned(tiles * p.dw_splits * p.tiles_d), b.rest, b.rows.label, c.B, v0};
       if (p.dw_splits == 1 && dsd == 1)
         to_dw.direct = Direct<T>{out, dsv, rows, int(c.D), share ? grad : nullptr, share};
       else
         join_dw = Join<T>{rows, int(c.D), p.dw_splits, b.dw, p.piece * Np, Np, share ? grad : nullptr, share, nullptr,
                           Labels{}, nullptr, 0, 0, out, dsv, dsd};
     }
-    hipLaunchKernelGGL((k_class_products<T>), dim3(to_dx.blocks + to_dw.blocks), dim3(kThreads), 0, st, to_dx, to_dw);
+    if (dx && dw && (to_dx.blocks < kSlots || to_dw.blocks < kSlots)) {
+      hipLaunchKernelGGL((k_class_products<T, true, true>), dim3(to_dx.blocks + to_dw.blocks), dim3(kThreads), 0, st,
+                         to_dx, to_dw);
+    } else {
+      if (dx) {
+        hipLaunchKernelGGL((k_class_products<T, true, false>), dim3(to_dx.blocks), dim3(kThreads), 0, st, to_dx, to_dw);
+        HIP_TRY(hipGetLastError());
+      }
+      if (dw)
+        hipLaunchKernelGGL((k_class_products<T, false, true>), dim3(to_dw.blocks), dim3(kThreads), 0, st, Product<T>{}, to_dw);
+    }
     HIP_TRY(hipGetLastError());
     Join<T> join_dx{};
     if (dx && v0 + p.piece >= c.V)               // all pieces are in

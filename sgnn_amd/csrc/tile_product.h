@@ -149,6 +149,9 @@ __device__ __forceinline__ void stage_operand(const Operand<T>& op, int64_t r0, 
   }
 }
 
+// byte of element (reduction row k, column m) of a staged flat operand of bf16
+__device__ __forceinline__ int flat_at(int k, int m) { return k * 256 + ((m >> 3) ^ ((k & 3) << 2)) * 16 + (m & 7) * 2; }
+
 // the operand of one 32 x 32 x 16 instruction: element `lane & 31` of the block at m0, eight
 // reduction indexes from k0 + 8 * (lane / 32)
 template <bool DEEP>
@@ -159,10 +162,10 @@ __device__ __forceinline__ void read_fragment(const char* lds, int m0, int k0, i
   } else {
     const int k = k0 + 8 * (lane >> 5) + ((lane & 15) >> 2);
     const int m = m0 + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-    const int at = ((m >> 3) ^ ((k & 3) << 2)) * 16 + (m & 7) * 2;       // k and k + 4 share k & 3
+    const char* at = lds + flat_at(k, m);                                // k and k + 4 share k & 3
     typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds + k * 256 + at));
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(lds + (k + 4) * 256 + at));
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 4 * 256));
     __builtin_memcpy(&out, &lo, 8);
     __builtin_memcpy(reinterpret_cast<char*>(&out) + 8, &hi, 8);
   }
@@ -236,10 +239,17 @@ __device__ __forceinline__ void multiply_sixteen(const SixteenPlanes& now, Tile&
 }
 
 // acc += A[m0 .., k0 .. k1] . B[n0 .., k0 .. k1]; k1 - k0 a multiple of the step.  `lds` holds two
-// stages of both operands; every wavefront has left them when this returns.
-template <typename T, bool ADEEP, bool BDEEP>
+// stages of both operands; every wavefront has left them when this returns.  bf16: `each` has its say
+// in every step: `landed` before the next step's loads, `ahead`(k of the next) among them, `behind`(B's
+// stage, acc) behind the products.
+struct Nothing {
+  __device__ __forceinline__ void landed() const {}
+  __device__ __forceinline__ void ahead(int64_t) const {}
+  __device__ __forceinline__ void behind(const char*, Tile&) const {}
+};
+template <typename T, bool ADEEP, bool BDEEP, typename Each = Nothing>
 __device__ __forceinline__ void multiply(const Operand<T>& A, int64_t m0, const Operand<T>& B, int64_t n0, int64_t k0,
-                                         int64_t k1, char* lds, Tile& acc) {
+                                         int64_t k1, char* lds, Tile& acc, Each&& each = Each{}) {
   constexpr int kDepth = Step<T>::kDepth;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
@@ -275,8 +285,12 @@ __device__ __forceinline__ void multiply(const Operand<T>& A, int64_t m0, const 
   }
   for (int64_t k = k0; k < k1; k += kDepth) {
     landed();                                    // this wavefront's part of the stage
+    each.landed();
     __syncthreads();                             // everybody's, and the other stage is free
-    if (k + kDepth < k1) stage(k + kDepth, cur ^ 1);
+    if (k + kDepth < k1) {
+      stage(k + kDepth, cur ^ 1);
+      each.ahead(k + kDepth);
+    }
     const char* a = lds + cur * 2 * kStageBytes;
 #pragma unroll
     for (int kk = 0; kk < kDepth; kk += 16) {
@@ -292,6 +306,7 @@ __device__ __forceinline__ void multiply(const Operand<T>& A, int64_t m0, const 
         for (int j = 0; j < 2; ++j)
           acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[i], fb[j], acc[i][j], 0, 0, 0);
     }
+    each.behind(a + kStageBytes, acc);
     cur ^= 1;
   }
   __syncthreads();

@@ -1,0 +1,56 @@
+"""``class_cross_entropy`` where it can go wrong beside its sizes: what the label's element of dz keeps,
+weights whose rows lie far apart, rows without a class, small and large heads through every kernel.
+
+Tolerances are those of ``test_gpu_class_loss``, but where a test says otherwise."""
+import pytest
+import torch
+from test_gpu_class_loss import DTYPES, HALF_STEP, U, check, close, make, reference  # noqa: F401
+
+from sgnn_amd import nn as snn
+
+pytestmark = pytest.mark.gpu
+
+
+def gradients(x, w, labels, idx=None, g=None):
+    """Both gradients of the mean (or of the rows' losses weighted by g)."""
+    xs, ws = x.detach().requires_grad_(), w.detach().requires_grad_()
+    if g is None:
+        snn.class_cross_entropy(xs, ws, labels, idx=idx).backward()
+    else:
+        (snn.class_cross_entropy(xs, ws, labels, idx=idx, reduction="none") * g).sum().backward()
+    return xs.grad, ws.grad
+
+
+@pytest.mark.parametrize("by_row", [False, True])
+@pytest.mark.parametrize("stored", ["by class", "by feature"])
+@pytest.mark.parametrize("B,D,V", [(300, 64, 100), (300, 100, 2000), (513, 192, 700), (300, 256, 300), (1500, 256, 5000),
+                                   (300, 300, 90), (2500, 320, 3000), (33, 257, 1000), (12000, 264, 12001)])
+def test_label_elements_in_the_weight_gradient(gpu_device, B, D, V, stored, by_row):
+    """bf16.  A class's gradient is mostly the label's elements of dz; they reach it with 16 bits (two bf16
+    numbers: half a step of half a step, 2^-16) or more, the other elements of dz with 8 (2^-8), and the
+    result is rounded once.  Bounds as in ``reference``, with 2^-16 in the place of 2^-8 for those
+    elements.  Logits in which the label stands out but is not certain, so that p - 1 is no bf16 number."""
+    x, w, labels = make(B, D, V, torch.bfloat16, gpu_device, seed=B + V)
+    labels[5] = -1
+    x = (x.float() + 2.5 * w.float()[labels.clamp_min(0)]).bfloat16()
+    g = torch.linspace(-1.0, 2.0, B, device=gpu_device) if by_row else None
+    live = labels >= 0
+    weight = torch.where(live, g.double() if by_row else torch.ones(B, device=gpu_device).double() / int(live.sum()),
+                         torch.zeros(B, device=gpu_device).double())[:, None]
+    xd, wd = x.double() * live[:, None], w.double()
+    z, size = xd @ wd.t(), xd.abs() @ wd.abs().t()
+    ez = ((6 * D + 20) * U * size).amax(1, keepdim=True)
+    p = torch.softmax(z, 1)
+    delta = 2 * ez + 4 * U * (1 + z.amax(1, keepdim=True) - z) + (V / 4 + 1100) * U
+    at = labels.clamp_min(0)[:, None]
+    one = torch.zeros_like(p).scatter_(1, at, 1.0)
+    dz = (p - one) * weight
+    keep = torch.full_like(p, 2.0 ** -8).scatter_(1, at, 2.0 ** -16)
+    edz = p * weight.abs() * torch.expm1(delta) + 4 * U * (p + one) * weight.abs() + keep * dz.abs()
+    want = dz.t() @ xd
+    bound = edz.t() @ xd.abs() + (6 * B + 600) * U * ((dz.abs() + edz).t() @ xd.abs())
+    bound = bound + HALF_STEP[torch.bfloat16] * (want.abs() + bound) + 1e-38
+    if stored == "by feature":
+        w = w.t().contiguous().t()
+    _, dw = gradients(x, w, labels, g=g)
+    close(dw, want, bound, "dweight")
