@@ -873,7 +873,7 @@ __device__ __forceinline__ void stage_stream(const Operand<Bf16>& op, int64_t r0
   constexpr int cpr = KD * 2;                    // chunks of a row
   const char* base = reinterpret_cast<const char*>(op.base + r0 * op.ld);              // uniform
   const int left = op.rows - r0 < kStreamRows ? int(op.rows - r0) : kStreamRows;       // at least 1
-  const unsigned pitch = unsigned(op.ld) * 2;
+  const unsigned pitch = unsigned(op.ld) * 2;    // 64 of them below 2^32 (weight_as_is)
 #pragma unroll
   for (int l = 0; l < stream_bytes<KD>() / 16 / (64 * WAVES); ++l) {
     const int first = (l * WAVES + wave) * 64, q = first + lane;
@@ -1540,21 +1540,23 @@ int check_call(const Call& c) {
   return SGNN_OK;
 }
 
-// A weight whose rows are whole steps and 16-byte aligned can be staged as it lies.
-bool weight_as_is(const Call& c, const Plan& p) {
+// A weight whose rows are whole steps and 16-byte aligned can be staged as it lies; for stage_stream,
+// whose offsets within a step have 32 bits, if they lie close enough together for that.
+bool weight_as_is(const Call& c, const Plan& p, bool streamed) {
   return c.sd == 1 && c.D % p.depth == 0 && size_t(c.sv) * p.elem % 16 == 0 &&
-         reinterpret_cast<uintptr_t>(c.w) % 16 == 0;
+         reinterpret_cast<uintptr_t>(c.w) % 16 == 0 &&
+         (!streamed || c.sv <= int64_t(UINT32_MAX) / (kStreamRows * int64_t(p.elem)));
 }
 
 template <typename T>
-int operands(const Call& c, const Plan& p, const Buffers& b, const Rows& rows, Operand<T>* x, Operand<T>* w,
-             hipStream_t st) {
+int operands(const Call& c, const Plan& p, const Buffers& b, const Rows& rows, bool streamed, Operand<T>* x,
+             Operand<T>* w, hipStream_t st) {
   const int across = p.Dp / 64;
   const Source sx{c.x, c.B, c.ldx, 1, b.x, ceil_div(c.B, 64) * across};
   Source sw{c.w, c.V, c.sv, c.sd, b.w, ceil_div(c.V, 64) * across};
   *x = Operand<T>{reinterpret_cast<const T*>(b.x), p.Dp, c.B, p.Dp};
   *w = Operand<T>{reinterpret_cast<const T*>(b.w), p.Dp, c.V, p.Dp};
-  if (weight_as_is(c, p)) {
+  if (weight_as_is(c, p, streamed)) {
     sw.blocks = 0;
     *w = Operand<T>{static_cast<const T*>(c.w), c.sv, c.V, c.D};
   }
@@ -1587,7 +1589,7 @@ template <typename T>
 int forward(const Call& c, const Plan& p, const Buffers& b, RowStat* stats, float* row_loss, float* loss,
             float* share, hipStream_t st) {
   Operand<T> x, w;
-  if (int rc = operands<T>(c, p, b, Rows{}, &x, &w, st)) return rc;
+  if (int rc = operands<T>(c, p, b, Rows{}, false, &x, &w, st)) return rc;
   const int depth = int(ceil_div(c.D, p.depth) * p.depth);
   hipLaunchKernelGGL((k_class_stats<T>), dim3(unsigned(p.tiles_b * p.stat_splits)), dim3(kThreads), 0, st, c.B, c.V,
                      depth, x, w, c.labels, c.idx, c.n_labels, p.tiles_v, p.stat_splits, b.part, b.picked);
@@ -1608,7 +1610,7 @@ template <typename T>
 int backward(const Call& c, const Plan& p, const Buffers& b, const RowStat* stats, const float* grad,
              const float* share, void* dx, int64_t lddx, void* dw, int64_t dsv, int64_t dsd, hipStream_t st) {
   Operand<T> x, w;
-  if (int rc = operands<T>(c, p, b, Rows{c.B, nullptr, nullptr, nullptr, b.rows}, &x, &w, st)) return rc;
+  if (int rc = operands<T>(c, p, b, Rows{c.B, nullptr, nullptr, nullptr, b.rows}, false, &x, &w, st)) return rc;
   const int64_t Np = int64_t(p.tiles_d) * kTile;
   T* const dz = reinterpret_cast<T*>(b.dz);
   const int depth = int(ceil_div(c.D, p.depth) * p.depth);
@@ -1669,7 +1671,7 @@ int backward(const Call& c, const Plan& p, const Buffers& b, const RowStat* stat
 int wide_forward(const Call& c, const Wide& f, const Plan& p, const Buffers& b, RowStat* stats, float* row_loss,
                  float* loss, float* share, hipStream_t st) {
   Operand<Bf16> x, w;
-  if (int rc = operands<Bf16>(c, p, b, Rows{}, &x, &w, st)) return rc;
+  if (int rc = operands<Bf16>(c, p, b, Rows{}, true, &x, &w, st)) return rc;
   const Labels of{c.labels, c.idx, c.n_labels, c.V};
   SGNN_WIDE(f.KD, hipLaunchKernelGGL((k_wide_stats<KD>), dim3(unsigned(f.own_b * f.stat_splits)), dim3(kThreads), 0, st,
                                      c.B, c.V, x, w, of, f.steps_v, f.stat_splits, b.part, b.picked));
@@ -1681,7 +1683,7 @@ int wide_backward(const Call& c, const Wide& f, const Plan& p, const Buffers& b,
                   const float* grad, const float* share, void* dx, int64_t lddx, void* dw, int64_t dsv, int64_t dsd,
                   hipStream_t st) {
   Operand<Bf16> x, w;
-  if (int rc = operands<Bf16>(c, p, b, Rows{c.B, stats, grad, share, b.rows}, &x, &w, st)) return rc;
+  if (int rc = operands<Bf16>(c, p, b, Rows{c.B, stats, grad, share, b.rows}, true, &x, &w, st)) return rc;
   const Labels of{c.labels, c.idx, c.n_labels, c.V};
   Join<Bf16> join_dx{}, join_dw{};
   if (dx) {

@@ -54,3 +54,19 @@ def test_label_elements_in_the_weight_gradient(gpu_device, B, D, V, stored, by_r
         w = w.t().contiguous().t()
     _, dw = gradients(x, w, labels, g=g)
     close(dw, want, bound, "dweight")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B", [5, 40])
+@pytest.mark.parametrize("D,V,stride", [(64, 96, 36_000_000), (256, 70, 1 << 26), (128, 96, 34_087_040),
+                                        (192, 96, 34_087_048), (320, 70, 36_000_000)])
+def test_classes_far_apart(gpu_device, dtype, B, D, V, stride):
+    """Rows of the weight so far apart that a step's offsets pass 32 bits: bit for bit the results of a
+    copy with its rows together.  (What lies between the rows is never touched.)"""
+    t = DTYPES[dtype]
+    x, w, labels = make(B, D, V, t, gpu_device, seed=D)
+    far = torch.empty_strided((V, D), (stride, 1), dtype=t, device=gpu_device)
+    far.copy_(w)
+    want, got = check(x, w, labels), check(x, far, labels)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
