@@ -2,9 +2,12 @@
 // exact splitting of fp32 and the inner loop of a 128 x 128 tile.
 //
 // bf16 operands go in as they are: their products are exact and summed in 32 bits.  An fp32 number
-// is the sum of three bf16 numbers (8 + 8 + 8 bits of its mantissa, cut off, so the sum is exact),
-// taken apart in registers on the way from LDS to the matrix instruction; of the nine products of
-// two numbers the three smallest, below 3 * 2^-24 of the whole, are left out.
+// is the sum of three bf16 numbers (8 bits of its mantissa cut off, the next 8 rounded to nearest, the
+// rest exactly), taken apart in registers on the way from LDS to the matrix instruction.  The second
+// is at most 2^-7, the third 2^-16 of the number's power of two, so of the nine products of two numbers
+// the three smallest, at most 2^-22 of the whole and of either sign, are left out.  (With the first
+// rounded, too, that would be 2^-24, for 4 % of the time and no visible difference in the results: the
+// sums' roundings are larger.)
 #pragma once
 #include "common.h"
 
@@ -30,7 +33,8 @@ template <typename T> __device__ __forceinline__ T narrow(float v);
 template <> __device__ __forceinline__ float narrow<float>(float v) { return v; }
 template <> __device__ __forceinline__ Bf16 narrow<Bf16>(float v) { return Bf16{to_bf16(v)}; }
 
-// v = a + b + c exactly, each a bf16 number; an infinity or NaN leaves a NaN behind
+// v = a + b + c exactly, each a bf16 number, 8 + 8 + 8 bits of its mantissa cut off: for products that
+// take all three.  An infinity or NaN leaves a NaN behind.
 __device__ __forceinline__ void split3(float v, float& a, float& b, float& c) {
   a = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
   const float r = v - a;
@@ -42,6 +46,19 @@ __device__ __forceinline__ unsigned high_halves(float lo, float hi) {
   return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
 }
 
+// two numbers as pairs of bf16 numbers, v = a + b + c exactly: a cut off, b rounded to nearest (cut off,
+// too, it would leave c twice as large and always of v's sign).  An infinity or NaN leaves a NaN behind.
+__device__ __forceinline__ void split_pair(float lo, float hi, unsigned& a, unsigned& b, unsigned& c) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  a = high_halves(lo, hi);
+  const float rl = lo - __uint_as_float(__float_as_uint(lo) & 0xffff0000u);
+  const float rh = hi - __uint_as_float(__float_as_uint(hi) & 0xffff0000u);
+  const bf16x2 rounded = __builtin_convertvector((f32x2{rl, rh}), bf16x2);
+  __builtin_memcpy(&b, &rounded, 4);
+  c = high_halves(rl - __uint_as_float(b << 16), rh - __uint_as_float(b & 0xffff0000u));
+}
+
 // bf16 numbers an element of type T is made of
 template <typename T> struct Planes { static constexpr int kCount = sizeof(T) == 4 ? 3 : 1; };
 
@@ -49,12 +66,11 @@ __device__ __forceinline__ void planes_of(const float (&v)[8], bf16x8 (&out)[3])
   u32x4 pl[3];
 #pragma unroll
   for (int e = 0; e < 8; e += 2) {
-    float a0, b0, c0, a1, b1, c1;
-    split3(v[e], a0, b0, c0);
-    split3(v[e + 1], a1, b1, c1);
-    pl[0][e / 2] = high_halves(a0, a1);
-    pl[1][e / 2] = high_halves(b0, b1);
-    pl[2][e / 2] = high_halves(c0, c1);
+    unsigned a, b, c;
+    split_pair(v[e], v[e + 1], a, b, c);
+    pl[0][e / 2] = a;
+    pl[1][e / 2] = b;
+    pl[2][e / 2] = c;
   }
 #pragma unroll
   for (int q = 0; q < 3; ++q) __builtin_memcpy(&out[q], &pl[q], 16);
@@ -211,10 +227,8 @@ __device__ __forceinline__ void read_sixteen(const char* stage, int kk, int wm, 
 // two neighbours of the 32 numbers a lane holds, to their planes
 __device__ __forceinline__ void take_apart(const Sixteen& v, int pair, SixteenPlanes& out) {
   const int x = pair >> 2, e = 2 * (pair & 3);
-  float a0, b0, c0, a1, b1, c1;
-  split3(v[x][e], a0, b0, c0);
-  split3(v[x][e + 1], a1, b1, c1);
-  unsigned a = high_halves(a0, a1), b = high_halves(b0, b1), c = high_halves(c0, c1);
+  unsigned a, b, c;
+  split_pair(v[x][e], v[x][e + 1], a, b, c);
   asm volatile("" : "+v"(a), "+v"(b), "+v"(c));  // now, not where it is used
   out[x][0][e / 2] = a;
   out[x][1][e / 2] = b;
