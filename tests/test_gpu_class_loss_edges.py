@@ -70,3 +70,27 @@ def test_classes_far_apart(gpu_device, dtype, B, D, V, stride):
     want, got = check(x, w, labels), check(x, far, labels)
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+def relative(got, want):
+    return ((got.double() - want).norm() / want.norm()).item()
+
+
+@pytest.mark.parametrize("B,D,V", [(5, 40, 3000), (30, 300, 700), (128, 64, 128), (200, 100, 900), (513, 602, 1000),
+                                   (300, 256, 5000), (12000, 40, 12001)])
+def test_fp32_is_as_exact_as_torch(gpu_device, B, D, V):
+    """Losses and gradients of fp32 operands are as far from the definition in 64 bits as those of torch's
+    operators in fp32.  The sums here run over six products where those run over one: with roundings of
+    either sign that is sqrt(6) = 2.5 times as far, 4 is allowed, and a rounding (2^-23) beside it.  With
+    16 bits of each operand (half of the six products) it would be 2^-17 at least, 30 times the roundings
+    of sums of these lengths."""
+    x, w, labels = make(B, D, V, torch.float32, gpu_device, seed=B)
+    dx, dw = gradients(x, w, labels)
+    rows = snn.class_cross_entropy(x, w, labels, reduction="none")
+    answers = []
+    for t in (torch.float32, torch.float64):
+        a, b = x.to(t).requires_grad_(), w.to(t).requires_grad_()
+        losses = torch.nn.functional.cross_entropy(a @ b.t(), labels, reduction="none")
+        answers.append((losses.detach(), *torch.autograd.grad(losses.mean(), (a, b))))
+    for got, plain, want, what in zip((rows, dx, dw), *answers, ("row losses", "dx", "dweight")):
+        assert relative(got, want) <= 4 * relative(plain, want) + 2.0 ** -23, what

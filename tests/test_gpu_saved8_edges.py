@@ -1,6 +1,7 @@
 """The 8-bit saved activations and the layer over them where they can go wrong beside their sizes."""
 import pytest
 import torch
+from test_gpu_saved8 import inputs
 
 from sgnn_amd import nn as snn
 
@@ -24,3 +25,26 @@ def test_products_of_two_numbers(gpu_device):
     snn.linear_saved_int8(x, w).backward(eye)
     want = v.double() * v.double()[3]
     assert bool(((x.grad[:, 0].double().cpu() - want).abs() <= 2.0 ** -22 * want).all())
+
+
+@pytest.mark.parametrize("slope", [0.0, 1.0, 0.2])
+@pytest.mark.parametrize("n,F,H", [(300, 100, 24), (4000, 602, 100), (70000, 64, 40), (9000, 256, 200)])
+def test_fp32_layer_is_as_exact_as_torch(gpu_device, n, F, H, slope):
+    """Output and input gradient in fp32 are as far from 64 bits as torch's products: four times at most
+    (sums over six products for one of theirs: sqrt(6) times the roundings) and a rounding."""
+    x = inputs(n, F, torch.float32, gpu_device, seed=n, spread=0.5)
+    g = torch.Generator().manual_seed(H)
+    w = (torch.randn(H, F, generator=g) / F ** 0.5).to(gpu_device)
+    grad = torch.randn(n, H, generator=g).to(gpu_device)
+    xs = x.clone().requires_grad_()
+    y = snn.linear_saved_int8(xs, w, slope=slope)
+    y.backward(grad)
+    s = torch.tensor(slope, dtype=torch.float32).double().item()
+
+    def layer(t):
+        a = x.to(t)
+        factor = torch.where(a > 0, torch.ones_like(a), torch.full_like(a, s))
+        return (a * factor) @ w.to(t).t(), (grad.to(t) @ w.to(t)) * factor
+    for got, plain, want in zip((y.detach(), xs.grad), layer(torch.float32), layer(torch.float64)):
+        off, usual = ((a.double() - want).norm() / want.norm() for a in (got, plain))
+        assert off <= 4 * usual + 2.0 ** -23
