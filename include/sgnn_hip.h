@@ -41,6 +41,7 @@ extern "C" {
 /* element types of the entry points that take more than fp32 */
 #define SGNN_F32               0
 #define SGNN_BF16              1
+#define SGNN_ALL_ROWS        256   /* or-ed to the type of the sgnn_class_xent entry points, see there */
 
 /* build flags */
 #define SGNN_STRIP_DIAG        1   /* drop (i,i) entries of the input first: model/SGNN.py:497-501 */
@@ -662,7 +663,9 @@ int sgnn_saved8_weight_grad(int dtype, int64_t n, int64_t F, int64_t H, const vo
  * along one of the two; dweight likewise (dsv, dsd).  `dtype` (SGNN_F32 or SGNN_BF16) holds for x,
  * weight, dx and dweight; losses, statistics and gradients of losses are fp32.  y(b) = labels[idx[b]]
  * when idx is given, else labels[b]; a row whose index or label is out of range has no class: its
- * loss is 0, it adds nothing to either gradient and does not count in the mean.
+ * loss is 0, it adds nothing to either gradient and does not count in the mean.  With SGNN_F32 |
+ * SGNN_ALL_ROWS as the type such a row is treated as by sgnn_softmax_xent_f32: its loss is 0, it counts
+ * in the mean and its dz_bv is g_b softmax(z_b)_v.
  *
  * forward: stats (3 floats a row, what the backward pass goes by: the largest z, the sum of
  *   exp(z - that), the label's z), row_loss; with `loss` also

@@ -26,6 +26,7 @@ ADAM_STATE_WORDS = 1026
 LOOPS_NONE, LOOPS_ADD, LOOPS_REMAINING = 0, 1, 2
 EPI_SCALE_ROW, EPI_SCALE_ROW2 = 0, 1
 F32, BF16 = 0, 1
+ALL_ROWS = 256                     # or-ed to F32 for the class loss
 SAVED8_GROUP = 32
 # tile-group operand state (sgnn_tilegroup_state_bytes): 32-bit words; the per-feature maxima follow the header
 TG_STATE_FLAG, TG_STATE_TINY, TG_STATE_TINY_LIMIT, TG_STATE_HEAD_WORDS = 1, 4, 6, 16

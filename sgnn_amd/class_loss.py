@@ -29,10 +29,10 @@ def _weight_layout(w):
 
 class _ClassXent(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, labels, idx, mean):
+    def forward(ctx, x, weight, labels, idx, mean, all_rows=False):
         x, (w, sv, sd) = unit_rows(x.detach()), _weight_layout(weight.detach())
         (B, D), V, dev = x.shape, w.shape[0], x.device
-        lib, dtype = _lib.load(), _lib.TYPES[x.dtype]
+        lib, dtype = _lib.load(), _lib.TYPES[x.dtype] | (_lib.ALL_ROWS if all_rows else 0)
         kept = torch.empty(4 * B + 1, dtype=torch.float32, device=dev)   # statistics, 1 / counted rows, row losses
         out = torch.empty(() if mean else (B,), dtype=torch.float32, device=dev)
         nbytes = lib.sgnn_class_xent_workspace_bytes(dtype, B, D, V, 0)
@@ -43,7 +43,7 @@ class _ClassXent(torch.autograd.Function):
                      sv, sd, labels.data_ptr(), labels.numel(), None if idx is None else idx.data_ptr(), at, rows, loss,
                      share, ws.data_ptr(), nbytes)
         ctx.save_for_backward(x, w, labels, idx, kept)
-        ctx.layout = (sv, sd, mean)
+        ctx.layout = (sv, sd, mean, dtype)
         return out
 
     @staticmethod
@@ -51,8 +51,8 @@ class _ClassXent(torch.autograd.Function):
     def backward(ctx, grad):
         x, w, labels, idx, kept = ctx.saved_tensors
         (B, D), V, dev = x.shape, w.shape[0], x.device
-        sv, sd, mean = ctx.layout
-        lib, dtype = _lib.load(), _lib.TYPES[x.dtype]
+        sv, sd, mean, dtype = ctx.layout
+        lib = _lib.load()
         grad = grad.contiguous()
         dx = torch.empty(B, D, dtype=x.dtype, device=dev) if ctx.needs_input_grad[0] else None
         dw, dsv, dsd = None, D, 1
@@ -68,7 +68,7 @@ class _ClassXent(torch.autograd.Function):
                      sv, sd, labels.data_ptr(), labels.numel(), None if idx is None else idx.data_ptr(), at,
                      grad.data_ptr(), at + 12 * B if mean else None, None if dx is None else dx.data_ptr(), D,
                      None if dw is None else dw.data_ptr(), dsv, dsd, ws.data_ptr(), nbytes)
-        return dx, dw, None, None, None
+        return dx, dw, None, None, None, None
 
 
 def _ids(t, what, device):
@@ -77,6 +77,23 @@ def _ids(t, what, device):
     if t.device != device:
         raise ValueError(f"{what} are on {t.device}, x on {device}")
     return t.contiguous()
+
+
+def checked_head(x, weight, labels, idx):
+    """``labels`` and ``idx`` as the kernels read them; a head that does not fit together is refused."""
+    if element_type(x, "x") != element_type(weight, "the weight"):
+        raise TypeError(f"x is {x.dtype}, the weight {weight.dtype}")
+    if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1] or x.shape[1] == 0 or weight.shape[0] == 0:
+        raise ValueError(f"need (B, D) rows and a (V, D) weight, got {tuple(x.shape)} and {tuple(weight.shape)}")
+    if weight.device != x.device:
+        raise ValueError(f"x is on {x.device}, the weight on {weight.device}")
+    labels = _ids(labels, "labels", x.device)
+    if idx is not None:
+        idx = _ids(idx, "idx", x.device)
+    rows = labels.numel() if idx is None else idx.numel()
+    if rows != x.shape[0]:
+        raise ValueError(f"{x.shape[0]} rows but {rows} {'labels' if idx is None else 'indices'}")
+    return labels, idx
 
 
 def class_cross_entropy(x, weight, labels, idx=None, reduction="mean"):
@@ -90,18 +107,7 @@ def class_cross_entropy(x, weight, labels, idx=None, reduction="mean"):
     in NaN or infinite."""
     if reduction not in ("mean", "none"):
         raise ValueError(f"reduction must be 'mean' or 'none', got {reduction!r}")
-    if element_type(x, "x") != element_type(weight, "the weight"):
-        raise TypeError(f"x is {x.dtype}, the weight {weight.dtype}")
-    if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1] or x.shape[1] == 0 or weight.shape[0] == 0:
-        raise ValueError(f"need (B, D) rows and a (V, D) weight, got {tuple(x.shape)} and {tuple(weight.shape)}")
-    if weight.device != x.device:
-        raise ValueError(f"x is on {x.device}, the weight on {weight.device}")
-    labels = _ids(labels, "labels", x.device)
-    if idx is not None:
-        idx = _ids(idx, "idx", x.device)
-    rows = labels.numel() if idx is None else idx.numel()
-    if rows != x.shape[0]:
-        raise ValueError(f"{x.shape[0]} rows but {rows} {'labels' if idx is None else 'indices'}")
+    labels, idx = checked_head(x, weight, labels, idx)
     if x.shape[0] == 0:                              # nothing counts: 0, with zero gradients
         nothing = x.float().sum(1) + weight[:0].float().sum()
         return nothing.sum() if reduction == "mean" else nothing

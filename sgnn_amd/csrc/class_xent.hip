@@ -36,7 +36,12 @@ __device__ __forceinline__ int64_t label_of(int64_t b, const int64_t* labels, co
 struct Labels {
   const int64_t *labels, *idx;
   int64_t n_labels, V;
+  bool all;                                      // rows without a class are rows like the others (fp32)
 };
+// does row b (of B or more) add to the gradients?
+__device__ __forceinline__ bool counts(int64_t b, int64_t B, const Labels& of) {
+  return b < B && (of.all || label_of(b, of.labels, of.idx, of.n_labels, of.V) >= 0);
+}
 
 struct RowStat { float m, s, picked; };          // what the backward pass needs of a row; picked = the label's logit
 
@@ -96,7 +101,7 @@ __global__ __launch_bounds__(256) void k_class_operands(int D, int Dp, Source fi
     else if (rows.out.label && r0 + t < rows.B) rows.out.label[r0 + t] = int(label_of(r0 + t, of.labels, of.idx, of.n_labels, of.V));
   }
   const auto live = [&](int64_t r) {
-    return r < src.rows && (!is_x || label_of(r, of.labels, of.idx, of.n_labels, of.V) >= 0);
+    return is_x ? counts(r, src.rows, of) : r < src.rows;
   };
   if (src.sd != 1) {
     for (int i = t; i < 64 * 64; i += 256) {
@@ -272,16 +277,14 @@ __global__ __launch_bounds__(256) void k_class_rows(int64_t B, int64_t V, int pa
 }
 
 // loss[0] = mean loss of the counted rows (0 if there are none), share[0] = 1 / their number.
-__global__ __launch_bounds__(1024) void k_class_mean(int64_t B, int64_t V, const float* __restrict__ row_loss,
-                                                     const int64_t* __restrict__ labels,
-                                                     const int64_t* __restrict__ idx, int64_t n_labels,
+__global__ __launch_bounds__(1024) void k_class_mean(int64_t B, Labels of, const float* __restrict__ row_loss,
                                                      float* __restrict__ loss, float* __restrict__ share) {
   __shared__ double s_sum[16];
   __shared__ int64_t s_count[16];
   double sum = 0.0;
   int64_t count = 0;
   for (int64_t b = threadIdx.x; b < B; b += 1024)
-    if (label_of(b, labels, idx, n_labels, V) >= 0) {
+    if (counts(b, B, of)) {                      // a row without a class has loss 0
       sum += double(row_loss[b]);
       ++count;
     }
@@ -310,16 +313,14 @@ __global__ __launch_bounds__(1024) void k_class_mean(int64_t B, int64_t V, const
 // The label's element dominates a row, and often its class, and is the one whose rounding to bf16 would be
 // felt: what it loses is kept in rest[b] and joins both gradients in 32 bits.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void k_class_dz(int64_t B, int64_t V, int Dp, Operand<T> x, Operand<T> w,
-                                                       const int64_t* __restrict__ labels,
-                                                       const int64_t* __restrict__ idx, int64_t n_labels,
+__global__ __launch_bounds__(kThreads) void k_class_dz(int64_t B, int Dp, Operand<T> x, Operand<T> w, Labels of,
                                                        const RowStat* __restrict__ stats,
                                                        const float* __restrict__ grad, float* __restrict__ rest,
                                                        int64_t v0, int tiles, T* __restrict__ dz, int64_t ldz) {
   __shared__ __align__(128) char lds[kProductLds];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wv = (wave >> 1) * 64, wb = (wave & 1) * 64;
-  const int64_t vt = v0 + int64_t(blockIdx.x % tiles) * kTile;
+  const int64_t V = of.V, vt = v0 + int64_t(blockIdx.x % tiles) * kTile;
   const int64_t b0 = int64_t(blockIdx.x / tiles) * kTile;
   Tile acc;
   clear(acc);
@@ -328,8 +329,9 @@ __global__ __launch_bounds__(kThreads) void k_class_dz(int64_t B, int64_t V, int
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const int64_t b = b0 + wb + 32 * j + (lane & 31);
-    const int64_t y = b < B ? label_of(b, labels, idx, n_labels, V) : -1;
-    const float g = y >= 0 ? (grad ? grad[b] : 1.f) : 0.f;
+    const int64_t y = b < B ? label_of(b, of.labels, of.idx, of.n_labels, V) : -1;
+    const bool live = y >= 0 || (of.all && b < B);
+    const float g = live ? (grad ? grad[b] : 1.f) : 0.f;
     const RowStat st = b < B ? stats[b] : RowStat{0.f, 1.f, 0.f};
     const float scale = g / st.s;
 #pragma unroll
@@ -347,12 +349,12 @@ __global__ __launch_bounds__(kThreads) void k_class_dz(int64_t B, int64_t V, int
             if constexpr (sizeof(T) == 2) rest[b] = d - widen(Bf16{to_bf16(d)});
           }
     }
-    if (vw + 64 > V || __any(y < 0)) {
+    if (vw + 64 > V || __any(!live)) {
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          if (y < 0 || vw + 32 * i + block_row(e, lane) >= V) acc[i][j][e] = 0.f;
+          if (!live || vw + 32 * i + block_row(e, lane) >= V) acc[i][j][e] = 0.f;
     }
   }
   T* out = dz + b0 * ldz + (vt - v0);
@@ -541,7 +543,7 @@ __global__ __launch_bounds__(kThreads) void k_class_products(Product<T> dx, Prod
 
 // out[r][d] = factor * (sum over the shares, in order, + rest[r] * weight[y(r)][d]), out at r * sr +
 // d * sd; factor = grad[0] * share[0] with `share`, grad[r] with `grad` alone, else 1; `rest` (dx in
-// bf16) may be NULL.  With `of` rows without a class are 0 whatever the weight holds.
+// bf16) may be NULL.  With `of` rows that do not count are 0 whatever the weight holds.
 template <typename T>
 struct Join {
   int64_t R;
@@ -579,7 +581,7 @@ __global__ __launch_bounds__(256) void k_class_join(Join<T> first, Join<T> secon
       const int64_t y = label_of(r, j.of.labels, j.of.idx, j.of.n_labels, j.of.V);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if (y < 0) v[e] = 0.f;
+        if (y < 0) v[e] = j.of.all ? v[e] : 0.f;
         else if (j.rest && d + e < j.D) v[e] += j.rest[r] * widen(j.weight[y * j.sv + (d + e) * j.sdw]);
       }
     }
@@ -625,7 +627,7 @@ __device__ __forceinline__ void few_stage(const Labels& of, int B, int D, int Dk
   constexpr int P = Planes<T>::kCount;
   for (int i = threadIdx.x; i < kFewRows * (Dk / 8); i += kThreads) {
     const int row = i / (Dk / 8), chunk = i - row * (Dk / 8), d = chunk * 8;
-    const bool live = row < B && label_of(row, of.labels, of.idx, of.n_labels, of.V) >= 0;
+    const bool live = counts(row, B, of);
     T v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = live && d + e < D ? x[row * ldx + d + e] : T{};
@@ -725,8 +727,9 @@ __global__ __launch_bounds__(kThreads) void k_few_dz(int B, int rows, int D, int
   few_stage<T>(of, B, D, Dk, x, ldx, few_lds);
   const int b = lane & 31;
   const int64_t y = b < B ? label_of(b, of.labels, of.idx, of.n_labels, of.V) : -1;
-  const RowStat st = y >= 0 ? stats[b] : RowStat{0.f, 1.f, 0.f};
-  const float g = y >= 0 ? (share ? grad[0] * share[0] : grad[b]) : 0.f;
+  const bool live = counts(b, B, of);
+  const RowStat st = live ? stats[b] : RowStat{0.f, 1.f, 0.f};
+  const float g = live ? (share ? grad[0] * share[0] : grad[b]) : 0.f;
   const float scale = g / st.s;
   for (int64_t v0 = (int64_t(blockIdx.x) * 4 + wave) * 32; v0 < V; v0 += int64_t(gridDim.x) * 128) {
     const f32x16 z = few_logits<T>(D, Dk, v0, V, w, sv, few_lds, lane);
@@ -734,7 +737,7 @@ __global__ __launch_bounds__(kThreads) void k_few_dz(int B, int rows, int D, int
     for (int e = 0; e < 16; ++e) {
       const int64_t v = v0 + block_row(e, lane);
       const float d = exp2_raw((z[e] - st.m) * kLog2e) * scale - (v == y ? g : 0.f);
-      if (b < rows && v < V) dz[v * rows + b] = y >= 0 ? d : 0.f;
+      if (b < rows && v < V) dz[v * rows + b] = live ? d : 0.f;
     }
   }
 }
@@ -752,8 +755,8 @@ __global__ __launch_bounds__(kThreads) void k_few_grads(int B, int D, int64_t V,
   const int d0 = (int(blockIdx.x) * 64 + lane) * VEC;
   const int left = D - d0;
   float xr[ROWS][VEC], dx[ROWS][VEC];
-  // bit b: row b has a class; the loads below do not wait for each other
-  const uint64_t live = __ballot(lane < B && label_of(lane, of.labels, of.idx, of.n_labels, of.V) >= 0);
+  // bit b: row b counts; the loads below do not wait for each other
+  const uint64_t live = __ballot(counts(lane, B, of));
 #pragma unroll
   for (int b = 0; b < ROWS; ++b)
 #pragma unroll
@@ -839,7 +842,7 @@ __global__ __launch_bounds__(kThreads) void k_few_join(int D, int rows, int spli
   if (q == 0 && d < D) {
 #pragma unroll
     for (int z = 1; z < 8; ++z) s += joined[z][c];
-    dx[b * lddx + d] = label_of(b, of.labels, of.idx, of.n_labels, of.V) >= 0 ? narrow<T>(s) : T{};
+    dx[b * lddx + d] = counts(b, b + 1, of) ? narrow<T>(s) : T{};
   }
 }
 
@@ -1515,6 +1518,8 @@ struct Call {
   const int64_t* labels;
   int64_t n_labels;
   const int64_t* idx;
+  bool all;
+  Labels of() const { return {labels, idx, n_labels, V, all}; }
 };
 
 // One launch takes fewer than 2^32 threads: a wavefront a row, a workgroup of 256 for 64 x 64 of the
@@ -1530,6 +1535,7 @@ const char* too_large(int64_t B, int64_t D, int64_t V) {
 int check_call(const Call& c) {
   using sgnn::fail;
   if (c.dtype != SGNN_F32 && c.dtype != SGNN_BF16) return fail(SGNN_ERR_INVALID, "unknown element type");
+  if (c.all && c.dtype != SGNN_F32) return fail(SGNN_ERR_UNSUPPORTED, "rows without a class count in fp32 only");
   if (c.B <= 0 || c.D <= 0 || c.V <= 0) return fail(SGNN_ERR_INVALID, "need B > 0, D > 0, V > 0");
   if (const char* why = too_large(c.B, c.D, c.V)) return fail(SGNN_ERR_UNSUPPORTED, why);
   if (c.ldx < c.D) return fail(SGNN_ERR_INVALID, "row stride smaller than the width");
@@ -1561,7 +1567,7 @@ int operands(const Call& c, const Plan& p, const Buffers& b, const Rows& rows, b
     *w = Operand<T>{static_cast<const T*>(c.w), c.sv, c.V, c.D};
   }
   hipLaunchKernelGGL((k_class_operands<T>), dim3(unsigned(sx.blocks + sw.blocks)), dim3(256), 0, st, int(c.D), p.Dp, sx,
-                     sw, Labels{c.labels, c.idx, c.n_labels, c.V}, rows);
+                     sw, c.of(), rows);
   HIP_TRY(hipGetLastError());
   return SGNN_OK;
 }
@@ -1572,8 +1578,7 @@ int finish_forward(const Call& c, int parts, const Buffers& b, RowStat* stats, f
                      c.labels, c.idx, c.n_labels, stats, row_loss);
   HIP_TRY(hipGetLastError());
   if (loss) {
-    hipLaunchKernelGGL(k_class_mean, dim3(1), dim3(1024), 0, st, c.B, c.V, row_loss, c.labels, c.idx, c.n_labels, loss,
-                       share);
+    hipLaunchKernelGGL(k_class_mean, dim3(1), dim3(1024), 0, st, c.B, c.of(), row_loss, loss, share);
     HIP_TRY(hipGetLastError());
   }
   return SGNN_OK;
@@ -1618,8 +1623,8 @@ int backward(const Call& c, const Plan& p, const Buffers& b, const RowStat* stat
     const int64_t left = ceil_div(c.V - v0, kTile);
     const int tiles = int(left < p.piece / kTile ? left : p.piece / kTile);
     const int64_t width = int64_t(tiles) * kTile;
-    hipLaunchKernelGGL((k_class_dz<T>), dim3(unsigned(p.tiles_b * tiles)), dim3(kThreads), 0, st, c.B, c.V, depth, x, w,
-                       c.labels, c.idx, c.n_labels, stats, share ? nullptr : grad, b.rest, v0, tiles, dz, p.piece);
+    hipLaunchKernelGGL((k_class_dz<T>), dim3(unsigned(p.tiles_b * tiles)), dim3(kThreads), 0, st, c.B, depth, x, w,
+                       c.of(), stats, share ? nullptr : grad, b.rest, v0, tiles, dz, p.piece);
     HIP_TRY(hipGetLastError());
     const Operand<T> a{dz, p.piece, p.Bp, p.piece};
     Product<T> to_dx{}, to_dw{};
@@ -1653,7 +1658,7 @@ int backward(const Call& c, const Plan& p, const Buffers& b, const RowStat* stat
     Join<T> join_dx{};
     if (dx && v0 + p.piece >= c.V)               // all pieces are in
       join_dx = Join<T>{c.B, int(c.D), p.dx_splits, b.dx, p.Bp * Np, Np, share ? grad : nullptr, share,
-                        sizeof(T) == 2 ? b.rest : nullptr, Labels{c.labels, c.idx, c.n_labels, c.V},
+                        sizeof(T) == 2 ? b.rest : nullptr, c.of(),
                         static_cast<const T*>(c.w), c.sv, c.sd, static_cast<T*>(dx), lddx, int64_t(1)};
     if (int rc = launch_joins(join_dx, join_dw, st)) return rc;
   }
@@ -1672,7 +1677,7 @@ int wide_forward(const Call& c, const Wide& f, const Plan& p, const Buffers& b, 
                  float* loss, float* share, hipStream_t st) {
   Operand<Bf16> x, w;
   if (int rc = operands<Bf16>(c, p, b, Rows{}, true, &x, &w, st)) return rc;
-  const Labels of{c.labels, c.idx, c.n_labels, c.V};
+  const Labels of = c.of();
   SGNN_WIDE(f.KD, hipLaunchKernelGGL((k_wide_stats<KD>), dim3(unsigned(f.own_b * f.stat_splits)), dim3(kThreads), 0, st,
                                      c.B, c.V, x, w, of, f.steps_v, f.stat_splits, b.part, b.picked));
   HIP_TRY(hipGetLastError());
@@ -1684,7 +1689,7 @@ int wide_backward(const Call& c, const Wide& f, const Plan& p, const Buffers& b,
                   hipStream_t st) {
   Operand<Bf16> x, w;
   if (int rc = operands<Bf16>(c, p, b, Rows{c.B, stats, grad, share, b.rows}, true, &x, &w, st)) return rc;
-  const Labels of{c.labels, c.idx, c.n_labels, c.V};
+  const Labels of = c.of();
   Join<Bf16> join_dx{}, join_dw{};
   if (dx) {
     SGNN_WIDE(f.KD, hipLaunchKernelGGL((k_wide_grads<KD, false, false>), dim3(unsigned(f.own_b * f.dx_splits)),
@@ -1717,7 +1722,7 @@ int wide_backward(const Call& c, const Wide& f, const Plan& p, const Buffers& b,
 template <typename T>
 int few_forward(const Call& c, const Few& f, const Buffers& b, RowStat* stats, float* row_loss, float* loss,
                 float* share, hipStream_t st) {
-  const Labels of{c.labels, c.idx, c.n_labels, c.V};
+  const Labels of = c.of();
   if (int rc = allow_lds(reinterpret_cast<const void*>(&k_few_stats<T>), f.lds)) return rc;
   hipLaunchKernelGGL((k_few_stats<T>), dim3(f.blocks), dim3(kThreads), f.lds, st, int(c.B), int(c.D), f.Dk, c.V,
                      static_cast<const T*>(c.x), c.ldx, static_cast<const T*>(c.w), c.sv, of, b.part, b.picked);
@@ -1728,7 +1733,7 @@ int few_forward(const Call& c, const Few& f, const Buffers& b, RowStat* stats, f
 template <typename T>
 int few_backward(const Call& c, const Few& f, const Buffers& b, const RowStat* stats, const float* grad,
                  const float* share, void* dx, int64_t lddx, void* dw, int64_t dsv, int64_t dsd, hipStream_t st) {
-  const Labels of{c.labels, c.idx, c.n_labels, c.V};
+  const Labels of = c.of();
   const T* x = static_cast<const T*>(c.x);
   const T* w = static_cast<const T*>(c.w);
   if (int rc = allow_lds(reinterpret_cast<const void*>(&k_few_dz<T>), f.lds)) return rc;
@@ -1758,6 +1763,7 @@ int few_backward(const Call& c, const Few& f, const Buffers& b, const RowStat* s
 }  // namespace
 
 extern "C" size_t sgnn_class_xent_workspace_bytes(int dtype, int64_t B, int64_t D, int64_t V, int backward) {
+  dtype &= ~SGNN_ALL_ROWS;
   if (B <= 0 || D <= 0 || V <= 0 || (dtype != SGNN_F32 && dtype != SGNN_BF16) || too_large(B, D, V)) return 0;
   // the weight's layout is not known here: enough for either way
   const size_t whole = carve(make_plan(dtype, B, D, V), B, V, backward != 0, nullptr).bytes;
@@ -1774,7 +1780,8 @@ extern "C" int sgnn_class_xent_forward(int dtype, int64_t B, int64_t D, int64_t 
                                        float* loss, float* share, void* workspace, size_t workspace_bytes,
                                        void* stream) {
   using sgnn::fail;
-  const Call c{dtype, B, D, V, x, ldx, weight, sv, sd, labels, n_labels, idx};
+  const Call c{dtype & ~SGNN_ALL_ROWS, B, D, V, x, ldx, weight, sv, sd, labels, n_labels, idx, (dtype & SGNN_ALL_ROWS) != 0};
+  dtype = c.dtype;
   if (int rc = check_call(c)) return rc;
   if (!stats || !row_loss || !workspace || (loss && !share)) return fail(SGNN_ERR_INVALID, "null pointer");
   if (workspace_bytes < sgnn_class_xent_workspace_bytes(dtype, B, D, V, 0))
@@ -1800,7 +1807,8 @@ extern "C" int sgnn_class_xent_backward(int dtype, int64_t B, int64_t D, int64_t
                                         const float* share, void* dx, int64_t lddx, void* dweight, int64_t dsv,
                                         int64_t dsd, void* workspace, size_t workspace_bytes, void* stream) {
   using sgnn::fail;
-  const Call c{dtype, B, D, V, x, ldx, weight, sv, sd, labels, n_labels, idx};
+  const Call c{dtype & ~SGNN_ALL_ROWS, B, D, V, x, ldx, weight, sv, sd, labels, n_labels, idx, (dtype & SGNN_ALL_ROWS) != 0};
+  dtype = c.dtype;
   if (int rc = check_call(c)) return rc;
   if (!stats || !grad || !workspace) return fail(SGNN_ERR_INVALID, "null pointer");
   if (dx && lddx < D) return fail(SGNN_ERR_INVALID, "row stride smaller than the width");

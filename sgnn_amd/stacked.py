@@ -61,7 +61,7 @@ import torch.nn.functional as Fn
 
 from . import _lib
 from . import utils as prop
-from .class_loss import class_cross_entropy
+from .class_loss import _ClassXent, checked_head
 
 
 class Func(torch.nn.Module):
@@ -320,7 +320,9 @@ def _head_cross_entropy(E, Wt, labels, idx, unit=False):
     if (E.is_cuda and E.dtype == torch.float32 and E.dim() == 2 and Wt.dtype == torch.float32
             and labels.dtype == torch.int64 and labels.dim() == 1 and E.shape[0] > 0
             and Wt.shape[1] >= _PIECEWISE_CLASSES):
-        return class_cross_entropy(E, Wt.t(), labels, idx)
+        # as _SoftmaxXent takes rows without a class: they count in the mean
+        all_rows = labels.is_contiguous() and E.shape[0] * Wt.shape[1] <= _FUSED_LOSS_MAX
+        return _ClassXent.apply(E, Wt.t(), *checked_head(E, Wt.t(), labels, idx), True, all_rows)
     return _cross_entropy(E.matmul(Wt), labels, idx, unit)
 
 

@@ -94,3 +94,60 @@ def test_fp32_is_as_exact_as_torch(gpu_device, B, D, V):
         answers.append((losses.detach(), *torch.autograd.grad(losses.mean(), (a, b))))
     for got, plain, want, what in zip((rows, dx, dw), *answers, ("row losses", "dx", "dweight")):
         assert relative(got, want) <= 4 * relative(plain, want) + 2.0 ** -23, what
+
+
+@pytest.mark.parametrize("unit", [False, True])
+@pytest.mark.parametrize("B,D,V", [(64, 128, 4096), (300, 33, 5001), (64, 128, 4095)])
+def test_stacked_head_with_rows_without_a_class(gpu_device, B, D, V, unit):
+    """The label head of the stacked training treats labels and indices out of range alike on either side of
+    the class count from which it runs over the classes in pieces: they add nothing to the loss, count in
+    the mean, and dz = softmax / B.  Loss and gradients against that in 64 bits, with the bounds of
+    ``reference`` for rows of weight 1 / B (whose own dz is p / B alone: a share of the same bound)."""
+    from sgnn_amd.stacked import _head_cross_entropy
+    x, w, labels = make(B, D, V, torch.float32, gpu_device, seed=B, nodes=B + 9)
+    labels[:5] = torch.tensor([-1, V, -100, 2 ** 40, V - 1], device=gpu_device)
+    idx = torch.arange(B, device=gpu_device)
+    idx[7], idx[8] = -1, B + 9
+    E, Wt = x.clone().requires_grad_(), w.t().contiguous().requires_grad_()
+    loss = _head_cross_entropy(E, Wt, labels, idx, unit=unit)
+    loss.backward()
+    dead = torch.tensor([0, 1, 2, 3, 7, 8], device=gpu_device)
+    known = labels.clone()
+    known[:4] = 0
+    inside = idx.clone()
+    inside[7:9] = 0
+    ref = reference(x, w, known, inside)             # every row with a class
+    p = torch.softmax(x.double() @ w.double().t(), 1)
+    dz = p.clone()
+    alive = torch.ones(B, dtype=torch.bool, device=gpu_device)
+    alive[dead] = False
+    dz[torch.arange(B, device=gpu_device)[alive], labels[idx[alive]]] -= 1
+    dz /= B
+    close(loss.detach(), ref["loss"][alive].sum() / B, ref["loss_bound"].mean() + 1e-30, "mean loss")
+    close(E.grad, dz @ w.double(), ref["dx_bound"], "dE")
+    close(Wt.grad.t(), dz.t() @ x.double(), ref["dw_bound"], "dWt")
+
+
+@pytest.mark.parametrize("B,D,V", [(5, 40, 300), (30, 64, 700), (200, 48, 500)])
+def test_rows_without_a_class_that_count(gpu_device, B, D, V):
+    """The same through every kernel of fp32 operands, bit for bit the results of the rows' losses for rows
+    with a class; and the call is refused in bf16, where no caller needs it."""
+    from sgnn_amd._lib import SgnnHipError
+    from sgnn_amd.class_loss import _ClassXent
+    x, w, labels = make(B, D, V, torch.float32, gpu_device, seed=D)
+    labels[1], labels[3] = -1, V
+    xs, ws = x.clone().requires_grad_(), w.clone().requires_grad_()
+    rows = _ClassXent.apply(xs, ws, labels, None, False, True)
+    assert torch.equal(rows.detach(), snn.class_cross_entropy(x, w, labels, reduction="none"))
+    rows.sum().backward()
+    p = torch.softmax(x.double() @ w.double().t(), 1)
+    for r in range(B):
+        if r not in (1, 3):
+            p[r, labels[r]] -= 1
+    known = labels.clone()
+    known[1] = known[3] = 0
+    ref = reference(x, w, known, g=torch.ones(B, device=gpu_device))
+    close(xs.grad, p @ w.double(), ref["dx_bound"], "dx")
+    close(ws.grad, p.t() @ x.double(), ref["dw_bound"], "dweight")
+    with pytest.raises(SgnnHipError):
+        _ClassXent.apply(x.bfloat16(), w.bfloat16(), labels, None, True, True)
