@@ -79,8 +79,17 @@ def _ids(t, what, device):
     return t.contiguous()
 
 
-def checked_head(x, weight, labels, idx):
-    """``labels`` and ``idx`` as the kernels read them; a head that does not fit together is refused."""
+def class_cross_entropy(x, weight, labels, idx=None, reduction="mean"):
+    """Cross-entropy of ``x @ weight.T`` (``x`` B x D, ``weight`` V x D, both float32 or both
+    bfloat16) against ``labels[idx]`` (``labels`` if ``idx`` is None; int64), in float32.
+
+    A row whose index or label is out of range (-1, say) has no class: its loss and its part of
+    either gradient are 0.  ``reduction="mean"`` is the mean over the other rows (0 if there are
+    none), ``"none"`` the loss of each row.  ``weight`` may be a transposed view (``Wt.t()``); its
+    gradient comes in the same layout.  An infinite or NaN element makes the losses it takes part
+    in NaN or infinite."""
+    if reduction not in ("mean", "none"):
+        raise ValueError(f"reduction must be 'mean' or 'none', got {reduction!r}")
     if element_type(x, "x") != element_type(weight, "the weight"):
         raise TypeError(f"x is {x.dtype}, the weight {weight.dtype}")
     if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1] or x.shape[1] == 0 or weight.shape[0] == 0:
@@ -93,21 +102,6 @@ def checked_head(x, weight, labels, idx):
     rows = labels.numel() if idx is None else idx.numel()
     if rows != x.shape[0]:
         raise ValueError(f"{x.shape[0]} rows but {rows} {'labels' if idx is None else 'indices'}")
-    return labels, idx
-
-
-def class_cross_entropy(x, weight, labels, idx=None, reduction="mean"):
-    """Cross-entropy of ``x @ weight.T`` (``x`` B x D, ``weight`` V x D, both float32 or both
-    bfloat16) against ``labels[idx]`` (``labels`` if ``idx`` is None; int64), in float32.
-
-    A row whose index or label is out of range (-1, say) has no class: its loss and its part of
-    either gradient are 0.  ``reduction="mean"`` is the mean over the other rows (0 if there are
-    none), ``"none"`` the loss of each row.  ``weight`` may be a transposed view (``Wt.t()``); its
-    gradient comes in the same layout.  An infinite or NaN element makes the losses it takes part
-    in NaN or infinite."""
-    if reduction not in ("mean", "none"):
-        raise ValueError(f"reduction must be 'mean' or 'none', got {reduction!r}")
-    labels, idx = checked_head(x, weight, labels, idx)
     if x.shape[0] == 0:                              # nothing counts: 0, with zero gradients
         nothing = x.float().sum(1) + weight[:0].float().sum()
         return nothing.sum() if reduction == "mean" else nothing

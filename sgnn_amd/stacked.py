@@ -61,7 +61,7 @@ import torch.nn.functional as Fn
 
 from . import _lib
 from . import utils as prop
-from .class_loss import _ClassXent, checked_head
+from .class_loss import _ClassXent
 
 
 class Func(torch.nn.Module):
@@ -310,6 +310,21 @@ class _HeadXent(torch.autograd.Function):
 _PIECEWISE_CLASSES = 4096
 
 
+def _in_pieces(E, Wt, labels, idx):
+    """Does the class loss take this head?  Heads beyond its sizes (65536 features, say) and whatever it
+    does not read as it is go by the stock product, as all others do."""
+    if not (E.is_cuda and E.dtype == torch.float32 and E.dim() == 2 and Wt.dtype == torch.float32
+            and Wt.device == E.device and E.shape[1] == Wt.shape[0] and Wt.shape[1] >= _PIECEWISE_CLASSES):
+        return False
+    rows = labels if idx is None else idx            # longer than the batch: the first of them
+    if rows.numel() < E.shape[0] or labels.numel() == 0:
+        return False
+    if any(t.dtype != torch.int64 or t.dim() != 1 or t.device != E.device for t in (labels, rows)):
+        return False
+    # no workspace: a size that the kernels refuse
+    return _lib.load().sgnn_class_xent_workspace_bytes(_lib.F32, E.shape[0], E.shape[1], Wt.shape[1], 1) > 0
+
+
 def _head_cross_entropy(E, Wt, labels, idx, unit=False):
     """``cross_entropy(E @ Wt, labels[idx])``."""
     if (E.is_cuda and E.dtype == torch.float32 and E.dim() == 2 and Wt.dtype == torch.float32 and Wt.stride(1) == 1
@@ -317,12 +332,10 @@ def _head_cross_entropy(E, Wt, labels, idx, unit=False):
             and E.shape[1] <= 256 and Wt.shape[1] <= 64
             and 4 * (E.shape[1] * Wt.shape[1] + 8 * E.shape[1] + 8 * Wt.shape[1]) <= 65536):
         return _HeadXent.apply(E, Wt, labels, idx, unit)
-    if (E.is_cuda and E.dtype == torch.float32 and E.dim() == 2 and Wt.dtype == torch.float32
-            and labels.dtype == torch.int64 and labels.dim() == 1 and E.shape[0] > 0
-            and Wt.shape[1] >= _PIECEWISE_CLASSES):
+    if _in_pieces(E, Wt, labels, idx):
         # as _SoftmaxXent takes rows without a class: they count in the mean
         all_rows = labels.is_contiguous() and E.shape[0] * Wt.shape[1] <= _FUSED_LOSS_MAX
-        return _ClassXent.apply(E, Wt.t(), *checked_head(E, Wt.t(), labels, idx), True, all_rows)
+        return _ClassXent.apply(E, Wt.t(), labels.contiguous(), None if idx is None else idx.contiguous(), True, all_rows)
     return _cross_entropy(E.matmul(Wt), labels, idx, unit)
 
 

@@ -151,3 +151,23 @@ def test_rows_without_a_class_that_count(gpu_device, B, D, V):
     close(ws.grad, p.t() @ x.double(), ref["dw_bound"], "dweight")
     with pytest.raises(SgnnHipError):
         _ClassXent.apply(x.bfloat16(), w.bfloat16(), labels, None, True, True)
+
+
+def test_stacked_head_refuses_nothing_it_took(gpu_device):
+    """Heads of thousands of classes with more features than the class loss takes, and labels or indices
+    longer than the batch (the first of them count): the loss of the stock product, as with fewer classes."""
+    from sgnn_amd.stacked import _cross_entropy, _head_cross_entropy
+    g = torch.Generator(gpu_device).manual_seed(0)
+    E = torch.randn(4, 65600, device=gpu_device, generator=g, requires_grad=True)
+    Wt = torch.randn(65600, 4100, device=gpu_device, generator=g) / 256
+    labels = torch.tensor([3, 4099, 0, 17, 5, 6], device=gpu_device)
+    loss = _head_cross_entropy(E, Wt, labels, None)
+    want = _cross_entropy(E.matmul(Wt), labels, None)
+    assert torch.equal(loss, want)
+    assert torch.equal(torch.autograd.grad(loss, E)[0], torch.autograd.grad(want, E)[0])
+    E, Wt = E[:, :40].detach(), Wt[:40].contiguous()
+    want = _cross_entropy(E.matmul(Wt), labels[:4], None)
+    assert torch.allclose(_head_cross_entropy(E, Wt, labels, None), want, rtol=1e-5, atol=0)
+    idx = torch.tensor([5, 4, 1, 0, 2, 2, 3], device=gpu_device)
+    want = _cross_entropy(E.matmul(Wt), labels, idx[:4])
+    assert torch.allclose(_head_cross_entropy(E, Wt, labels, idx), want, rtol=1e-5, atol=0)
