@@ -302,19 +302,29 @@ class _HeadXent(torch.autograd.Function):
         return dE * grad_loss, dWt * grad_loss, None, None, None
 
 
-# From this many classes on the loss runs over the classes in pieces instead of forming the batch's
-# logits and their gradient.  Loss and both gradients, replayed from a graph, logits formed / in
-# pieces: 64 rows of 64 features 32 / 53 us at 1024 classes, 62 / 58 at 4096, 190 / 82 at 16384;
-# 4096 rows of 128, 95 / 98, 251 / 177 and 927 / 591 us; 16384 rows of 256, 344 / 305, 1045 / 1046
-# and 4159 / 3933 us, with two arrays of rows x classes fewer in memory.
-_PIECEWISE_CLASSES = 4096
+def _piecewise_classes(B, D):
+    """From how many classes on the loss of B rows of D features runs over the classes in pieces instead of
+    forming the batch's logits and their gradient.
+
+    Loss and both gradients, replayed from a graph, logits formed / in pieces, us: 64 rows of 128 features
+    65 / 60 at 4096 classes, 197 / 83 at 16384; of 256, 65 / 76 at 4096, 98 / 86 at 6000; of 602, 122 / 134
+    at 8192, 224 / 176 at 16384; of 1000, 235 / 262 at 16384, 528 / 445 at 32768; of 1433, 1074 / 1128 at
+    65536.  512 rows of 256, 95 / 102 at 4096, 145 / 117 at 6000; of 1433, 376 / 389 at 8192, 723 / 702 at
+    16384.  4096 rows of 602, 567 / 533 at 4096; of 1433, 1115 / 1145 at 4096, 1751 / 1709 at 6000.  Few
+    rows of many features are few workgroups with a long way each; with many rows the two are close, and
+    two arrays of rows x classes are fewer in memory."""
+    if D <= 150:
+        return 4096
+    if D > 1024 and B < 128:
+        return math.inf
+    return max(4096, 4 * D if B >= 2048 else 5000, 22 * D * math.sqrt(64 / max(B, 64)))
 
 
 def _in_pieces(E, Wt, labels, idx):
     """Does the class loss take this head?  Heads beyond its sizes (65536 features, say) and whatever it
     does not read as it is go by the stock product, as all others do."""
     if not (E.is_cuda and E.dtype == torch.float32 and E.dim() == 2 and Wt.dtype == torch.float32
-            and Wt.device == E.device and E.shape[1] == Wt.shape[0] and Wt.shape[1] >= _PIECEWISE_CLASSES):
+            and Wt.device == E.device and E.shape[1] == Wt.shape[0] and Wt.shape[1] >= _piecewise_classes(*E.shape)):
         return False
     rows = labels if idx is None else idx            # longer than the batch: the first of them
     if rows.numel() < E.shape[0] or labels.numel() == 0:

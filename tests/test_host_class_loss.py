@@ -63,3 +63,13 @@ def test_python_layer_needs_gpu_tensors():
     from sgnn_amd import nn
     with pytest.raises(ValueError):
         nn.class_cross_entropy(torch.randn(3, 8), torch.randn(70, 8), torch.zeros(3, dtype=torch.int64))
+
+
+@pytest.mark.parametrize("B,D,V,pieces", [
+    (64, 128, 4096, True), (64, 128, 4095, False), (300, 33, 5001, True), (64, 256, 4096, False), (64, 256, 6000, True),
+    (64, 602, 8192, False), (64, 602, 16384, True), (32, 1433, 65536, False), (512, 256, 4096, False),
+    (512, 1433, 8192, False), (512, 1433, 16384, True), (4096, 1433, 4096, False), (4096, 602, 4096, True),
+])
+def test_stacked_heads_in_pieces_where_that_is_faster(B, D, V, pieces):
+    from sgnn_amd.stacked import _piecewise_classes
+    assert (V >= _piecewise_classes(B, D)) is pieces
