@@ -1156,7 +1156,23 @@ __global__ __launch_bounds__(kGradThreads, 2) void k_wide_grads(int64_t owners, 
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[d][j][e] = 0.f;
   float shift[NB] = {};
-  bool any_large = false;
+  bool any_large = false, wild = false;          // wild: an owned class holds an infinity or NaN
+  if constexpr (BY_CLASS) {
+    unsigned lo = 0, hi = 0;                     // the largest magnitudes of either half of the words
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+      for (int k = 0; k < KD; ++k) {
+        u32x4 w;
+        __builtin_memcpy(&w, &own[j][k], 16);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          lo = max(lo, w[q] & 0x7fffu);
+          hi = max(hi, w[q] & 0x7fff0000u);
+        }
+      }
+    wild = __any(lo >= 0x7f80u || hi >= 0x7f800000u);
+  }
   if constexpr (!BY_CLASS) {
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
@@ -1222,6 +1238,17 @@ __global__ __launch_bounds__(kGradThreads, 2) void k_wide_grads(int64_t owners, 
     }
     bool with_label = false;
     if constexpr (BY_CLASS) {
+      // 0 x infinity in rows without a class and beyond the last, whose shift is infinite: p is 0 there
+      if (wild) {
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const f32x4 its_shift = shifts(e);
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) z[j][e + q] = its_shift[q] == INFINITY ? 0.f : z[j][e + q];
+        }
+      }
       // rows whose label is among the owned classes: rare
       uint64_t h = __ballot(label >= o0 && label < o0 + 32 * NB) >> (32 * sub) & 0xffffffffull;
       with_label = h != 0;

@@ -171,3 +171,24 @@ def test_stacked_head_refuses_nothing_it_took(gpu_device):
     idx = torch.tensor([5, 4, 1, 0, 2, 2, 3], device=gpu_device)
     want = _cross_entropy(E.matmul(Wt), labels, idx[:4])
     assert torch.allclose(_head_cross_entropy(E, Wt, labels, idx), want, rtol=1e-5, atol=0)
+
+
+@pytest.mark.parametrize("by_row", [False, True])
+@pytest.mark.parametrize("B,D,V", [(7, 40, 90), (200, 48, 150), (130, 64, 300), (200, 100, 2000), (70, 192, 100),
+                                   (300, 256, 300), (100, 300, 200)])
+def test_masked_classes_and_rows_without_a_class(gpu_device, B, D, V, by_row):
+    """bf16.  Classes masked by an infinite weight (p is 0 in every row that counts) beside rows without a
+    class, the last among them: the weight's gradient is that of the other classes, 0 in the masked ones."""
+    x, w, labels = make(B, D, V, torch.bfloat16, gpu_device, seed=B)
+    x[:, 0] = x[:, 0].abs() + 1
+    keep = V - 10
+    labels %= keep
+    labels[2], labels[B // 2], labels[B - 1] = -1, V, -1
+    masked = w.clone()
+    masked[keep:, 0] = -float("inf")
+    g = torch.linspace(0.5, 1.5, B, device=gpu_device) if by_row else None
+    _, dw = gradients(x, masked, labels, g=g)
+    labels[B // 2] = -1
+    ref = reference(x, w[:keep], labels, g=g)
+    close(dw[:keep], ref["dw"], ref["dw_bound"], "dweight")
+    assert bool((dw[keep:] == 0).all())
