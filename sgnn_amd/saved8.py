@@ -16,6 +16,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _lib
 from ._lib import TYPES, element_type
@@ -196,7 +197,7 @@ def linear_saved_int8(x, weight, slope=1.0):
     input but the 8-bit codes for the backward pass.  The output and ``x``'s gradient are those of
     the full activation; the weight's gradient is formed from the codes (off by half a step of
     their group at most, element by element).  An infinite or NaN element makes its row's outputs
-    NaN."""
+    NaN.  Neither forward-mode nor second derivatives: autograd refuses both."""
     code = element_type(x, "the input")
     if element_type(weight, "the weight") != code:
         raise TypeError(f"the input is {x.dtype}, the weight {weight.dtype}")
@@ -205,6 +206,8 @@ def linear_saved_int8(x, weight, slope=1.0):
     if weight.device != x.device:
         raise ValueError(f"the input is on {x.device}, the weight on {weight.device}")
     slope = checked_slope(slope)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+    # an operand with a forward-mode tangent, too: autograd refuses it there, here it would be lost
+    if (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)
+            or any(unpack_dual(t).tangent is not None for t in (x, weight))):
         return _LinearSaved.apply(x, weight, slope)
     return _linear(x, weight, slope)

@@ -48,3 +48,19 @@ def test_fp32_layer_is_as_exact_as_torch(gpu_device, n, F, H, slope):
     for got, plain, want in zip((y.detach(), xs.grad), layer(torch.float32), layer(torch.float64)):
         off, usual = ((a.double() - want).norm() / want.norm() for a in (got, plain))
         assert off <= 4 * usual + 2.0 ** -23
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(gpu_device, grad):
+    """A forward-mode derivative is refused whether or not an operand requires a gradient, never lost."""
+    import torch.autograd.forward_ad as forward_ad
+    x, w = torch.randn(5, 8, device=gpu_device), torch.randn(3, 8, device=gpu_device, requires_grad=grad)
+    for dual in (0, 1):
+        with forward_ad.dual_level():
+            args = [x, w]
+            args[dual] = forward_ad.make_dual(args[dual], torch.ones_like(args[dual]))
+            with pytest.raises(RuntimeError, match="forward"):
+                snn.linear_saved_int8(*args)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward"):
+                snn.linear_saved_int8(*args)
+    assert snn.linear_saved_int8(x, w.detach()).grad_fn is None
