@@ -126,10 +126,11 @@ class SavedInt8:
         return dW
 
     def input_grad(self, grad):
-        """``grad * act'(x)``: the gradient of the activation's input from that of its output."""
-        grad = self._grad(grad, self.shape[1], "the activation's gradient")
+        """``grad * act'(x)``: the gradient of the activation's input from that of its output, a
+        tensor of its own."""
+        given, grad = grad, self._grad(grad, self.shape[1], "the activation's gradient")
         if self.slope == 1.0:
-            return grad
+            return grad.clone() if grad.data_ptr() == given.data_ptr() else grad
         n, F = self.shape
         out = torch.empty(n, F, dtype=grad.dtype, device=self.device)
         _lib.call_on(self.device, _lib.load().sgnn_saved8_input_grad, TYPES[grad.dtype], n, F, self.codes.data_ptr(),

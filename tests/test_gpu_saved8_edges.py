@@ -64,3 +64,16 @@ def test_forward_mode_is_refused(gpu_device, grad):
             with torch.no_grad(), pytest.raises(RuntimeError, match="forward"):
                 snn.linear_saved_int8(*args)
     assert snn.linear_saved_int8(x, w.detach()).grad_fn is None
+
+
+@pytest.mark.parametrize("slope", [0.0, 1.0, 0.2])
+def test_input_grad_is_a_tensor_of_its_own(gpu_device, slope):
+    """Writing to the result leaves the gradient that it was made of alone, whatever the slope."""
+    saved = snn.save_int8(inputs(20, 40, torch.float32, gpu_device, seed=1), slope)
+    wide = torch.randn(20, 50, device=gpu_device)
+    for grad in (torch.randn(20, 40, device=gpu_device), wide[:, 3:43], wide[:1, :40].expand(20, 40)):
+        before = grad.clone()
+        dx = saved.input_grad(grad)
+        assert slope != 1.0 or torch.equal(dx, grad)
+        dx.add_(1.0)
+        assert torch.equal(grad, before)
