@@ -192,3 +192,46 @@ def test_masked_classes_and_rows_without_a_class(gpu_device, B, D, V, by_row):
     ref = reference(x, w[:keep], labels, g=g)
     close(dw[:keep], ref["dw"], ref["dw_bound"], "dweight")
     assert bool((dw[keep:] == 0).all())
+
+
+# up to 32 rows (bf16: 16), rows in registers (bf16 up to 256 features), tiles, tiles in several pieces
+EVERY_WAY = [(5, 40, 300), (16, 100, 500), (30, 300, 400), (150, 64, 400), (150, 300, 400), (12000, 264, 12001)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("stored", ["by class", "by feature"])
+@pytest.mark.parametrize("B,D,V", EVERY_WAY)
+def test_row_gradients_every_way(gpu_device, dtype, B, D, V, stored):
+    """A gradient of its own for every row, some of them 0 or negative, through every kernel."""
+    x, w, labels = make(B, D, V, DTYPES[dtype], gpu_device, seed=B + 1)
+    labels[B // 3] = -1
+    g = torch.randn(B, generator=torch.Generator().manual_seed(B)).to(gpu_device)
+    g[B // 2] = 0.0
+    if stored == "by feature":
+        w = w.t().contiguous().t()
+    dx, dw = gradients(x, w, labels, g=g)
+    ref = reference(x, w, labels, g=g)
+    close(dx, ref["dx"], ref["dx_bound"], "dx")
+    close(dw, ref["dw"], ref["dw_bound"], "dweight")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("stored", ["by class", "by feature"])
+@pytest.mark.parametrize("B,D,V", EVERY_WAY)
+def test_rows_without_a_class_every_way(gpu_device, dtype, B, D, V, stored):
+    """Labels and indices out of range whose rows hold NaN and infinities, a repeated index, the last row
+    among them: losses and gradients are those of the other rows."""
+    x, w, labels = make(B, D, V, DTYPES[dtype], gpu_device, seed=B + 2, nodes=B + 4)
+    labels[:2] = torch.tensor([-1, V], device=gpu_device)
+    idx = torch.arange(B, device=gpu_device) + 2
+    idx[1], idx[3], idx[B - 1] = 0, -1, B + 4
+    idx[2] = idx[4]
+    if B > 5:
+        idx[B // 2] = 1
+    dead = [1, 3, B - 1] + ([B // 2] if B > 5 else [])
+    for k, r in enumerate(dead):
+        x[r] = (float("nan"), float("inf"), -float("inf"))[k % 3]
+    if stored == "by feature":
+        w = w.t().contiguous().t()
+    dx, dw, loss = check(x, w, labels, idx)
+    assert bool((dx[dead] == 0).all()) and bool(torch.isfinite(dw).all()) and bool(torch.isfinite(loss))
