@@ -530,10 +530,11 @@ __device__ __forceinline__ void form_product(const Product<T>& p, unsigned block
     }
 }
 
-// Both gradients' products in one launch where one of them leaves slots empty: 512 x 128 against 1000
-// classes in fp32 11 us, one after the other 17 and a launch more.  Where either fills the card, kernels of
-// their own: 4096 x 512 against 50000 classes in bf16, all of it, 1200 us, in one launch 1243; 2048 x 602
-// against 10007 in fp32 655 and 659.
+// Both gradients' products in one launch: 512 x 128 against 1000 classes in fp32 11 us, one after the
+// other 17 and a launch more; 4096 x 128 against 50000, all of it, 1491 us and 1510.  Not so in bf16 where
+// neither leaves half the slots empty: there kernels of their own, in which dx does without dweight's steps
+// for the labels (in one kernel they cost it 60 us): 4096 x 512 against 50000 1193 us, in one launch 1229;
+// 1777 x 700 against 10007 211 and 215.
 template <typename T, bool DX, bool DW>
 __global__ __launch_bounds__(kThreads) void k_class_products(Product<T> dx, Product<T> dw) {
   __shared__ __align__(128) char lds[kProductLds];
@@ -1670,17 +1671,19 @@ int backward(const Call& c, const Plan& p, const Buffers& b, const RowStat* stat
         join_dw = Join<T>{rows, int(c.D), p.dw_splits, b.dw, p.piece * Np, Np, share ? grad : nullptr, share, nullptr,
                           Labels{}, nullptr, 0, 0, out, dsv, dsd};
     }
-    if (dx && dw && (to_dx.blocks < kSlots || to_dw.blocks < kSlots)) {
-      hipLaunchKernelGGL((k_class_products<T, true, true>), dim3(to_dx.blocks + to_dw.blocks), dim3(kThreads), 0, st,
-                         to_dx, to_dw);
-    } else {
-      if (dx) {
+    bool together = true;
+    if constexpr (sizeof(T) == 2) {
+      together = dx && dw && (to_dx.blocks < kSlots / 2 || to_dw.blocks < kSlots / 2);
+      if (!together && dx) {
         hipLaunchKernelGGL((k_class_products<T, true, false>), dim3(to_dx.blocks), dim3(kThreads), 0, st, to_dx, to_dw);
         HIP_TRY(hipGetLastError());
       }
-      if (dw)
+      if (!together && dw)
         hipLaunchKernelGGL((k_class_products<T, false, true>), dim3(to_dw.blocks), dim3(kThreads), 0, st, Product<T>{}, to_dw);
     }
+    if (together)
+      hipLaunchKernelGGL((k_class_products<T, true, true>), dim3(to_dx.blocks + to_dw.blocks), dim3(kThreads), 0, st, to_dx,
+                         to_dw);
     HIP_TRY(hipGetLastError());
     Join<T> join_dx{};
     if (dx && v0 + p.piece >= c.V)               // all pieces are in
