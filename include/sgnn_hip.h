@@ -623,8 +623,8 @@ int sgnn_head_xent_f32(int64_t B, int64_t D, int64_t C, const float* E, int64_t 
  *                |a| <= 128 * 2^s; code < 0 exactly where x > 0 is false (NaN groups too); with
  *                slope 0 negative codes stand for 0.
  * An element is off by at most half its group's step.  `dtype` is SGNN_F32 or SGNN_BF16 and holds
- * for x, y, weight, out, grad, dx and dW alike (bf16 activations that the slope moved are
- * rounded before the product); each result is rounded once, to nearest even.
+ * for x, y, weight, out, grad, dx and dW alike (bf16 activations that the slope moved
+ * enter the product with 16 bits, as two bf16 numbers); each result is rounded once, to nearest even.
  *
  * sgnn_save8            x -> codes and steps.
  * sgnn_saved8_linear    y = a . weight^T (weight H x F, row stride ldw) and, with codes and steps, those

@@ -485,8 +485,10 @@ __device__ __forceinline__ void lin_planes(const float (&v)[8], bf16x8 (&out)[1]
 
 // y[r][h] for 128 rows and 32 * NB units a workgroup; `codes` NULL: nothing is kept.  SPLIT, for few
 // rows: 32 rows a workgroup, whose wavefronts take turns at the steps of the features, each with a
-// piece of the weight of its own, and add their sums up in the end, in order.
-template <typename T, int NB, bool SPLIT>
+// piece of the weight of its own, and add their sums up in the end, in order.  MOVED, for bf16 whose slope
+// is neither 0 nor 1: activations are two bf16 numbers each in the product (169343 x 128, 256 units, forward
+// and backward 172 us; with one 170, and at slope 0.2 the output moves by 1.0e-3 of its norm).
+template <typename T, int NB, bool SPLIT, bool MOVED>
 __global__ __launch_bounds__(256) void k_linear8(int64_t n, int F, int H, const T* __restrict__ x, int64_t ldx,
                                                  const T* __restrict__ w, int64_t ldw, float slope,
                                                  uint8_t* __restrict__ codes, uint8_t* __restrict__ steps,
@@ -561,8 +563,15 @@ __global__ __launch_bounds__(256) void k_linear8(int64_t n, int F, int H, const 
         save_group(a, plain, r < n, half, codes + r * (int64_t(groups) * kGroup) + f, steps + r * groups + (f >> 5));
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        bf16x8 fa[P];
+        bf16x8 fa[P], off;
         lin_planes(a[s], fa);
+        if constexpr (MOVED) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float d = a[s][e] - static_cast<float>(fa[0][e]);
+            off[e] = static_cast<__bf16>(fabsf(d) < INFINITY ? d : 0.f);       // infinities have said it all
+          }
+        }
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
           const int row = 32 * j + (lane & 31), c = 4 * g + 2 * s + half;
@@ -572,6 +581,7 @@ __global__ __launch_bounds__(256) void k_linear8(int64_t n, int F, int H, const 
             fb[q] = *reinterpret_cast<const bf16x8*>(lds + (q * kUnits + row) * (kLinStep * 2) +
                                                      ((c ^ spread_128(row)) << 4));
           multiply_planes<P>(fa, fb, acc[j]);
+          if constexpr (MOVED) acc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(off, fb[0], acc[j], 0, 0, 0);
         }
       }
     }
@@ -878,22 +888,26 @@ int check_linear(int dtype, int64_t n, int64_t F, int64_t H, float slope, const 
 template <typename T>
 int launch_linear(int64_t n, int64_t F, int64_t H, const void* x, int64_t ldx, const void* w, int64_t ldw, float slope,
                   uint8_t* codes, uint8_t* steps, void* y, int64_t ldy, hipStream_t st) {
-#define SGNN_LIN8(NB, SPLIT)                                                                                         \
-  hipLaunchKernelGGL((k_linear8<T, NB, SPLIT>), dim3(unsigned((n + (SPLIT ? 31 : 127)) / (SPLIT ? 32 : 128)),        \
+#define SGNN_LIN8_AS(NB, SPLIT, MOVED)                                                                               \
+  hipLaunchKernelGGL((k_linear8<T, NB, SPLIT, MOVED>), dim3(unsigned((n + (SPLIT ? 31 : 127)) / (SPLIT ? 32 : 128)),        \
                                                      unsigned((H + 32 * NB - 1) / (32 * NB))),                       \
                      dim3(256), 0, st, n, int(F), int(H), static_cast<const T*>(x), ldx, static_cast<const T*>(w),   \
                      ldw, slope, codes, steps, static_cast<T*>(y), ldy)
+#define SGNN_LIN8(NB, SPLIT)                                                                                         \
+  if (sizeof(T) == 2 && slope != 0.f && slope != 1.f) SGNN_LIN8_AS(NB, SPLIT, (sizeof(T) == 2));                     \
+  else SGNN_LIN8_AS(NB, SPLIT, false)
   // Few rows are bound by the wait for one load after the other along the features, which four
   // wavefronts share; more rows than fill the card gain nothing by it.  fp32, together / split, at 8192,
   // 16384 and 32768 rows: 1433 features, 16 units 64 / 24, 64 / 32, 67 / 62 us; 500, 64: 33 / 15, 35 / 27,
   // 37 / 51 us; 602, 128 (two workgroups for the same rows): 51 / 30, 53 / 57, 55 / 108 us.  A single step
   // has nothing to share.
   const bool split = F > kLinStep && (n + 31) / 32 * ((H + 63) / 64) <= 512;
-  if (H <= 32) {
-    if (split) SGNN_LIN8(1, true); else SGNN_LIN8(1, false);
-  } else if (split) SGNN_LIN8(2, true);
-  else if (H <= 64) SGNN_LIN8(2, false);
-  else SGNN_LIN8(4, false);
+  if (H <= 32 && split) { SGNN_LIN8(1, true); }
+  else if (H <= 32) { SGNN_LIN8(1, false); }
+  else if (split) { SGNN_LIN8(2, true); }
+  else if (H <= 64) { SGNN_LIN8(2, false); }
+  else { SGNN_LIN8(4, false); }
+#undef SGNN_LIN8_AS
 #undef SGNN_LIN8
   HIP_TRY(hipGetLastError());
   return SGNN_OK;

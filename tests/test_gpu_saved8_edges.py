@@ -91,3 +91,34 @@ def test_fp32_weight_gradient_is_as_exact_as_torch(gpu_device, n, F, H, slope):
     want = grad.double().t() @ value.double()
     off, usual = ((a.double() - want).norm() / want.norm() for a in (saved.weight_grad(grad), grad.t() @ value))
     assert off <= 4 * usual + 2.0 ** -23
+
+
+@pytest.mark.parametrize("slope", [0.0, 0.2, 0.9, 1.0])
+@pytest.mark.parametrize("n,F,H", [(3, 7, 33), (130, 31, 64), (400, 90, 24), (66000, 40, 20), (9001, 70, 200), (500, 300, 16)])
+def test_bf16_activations_in_the_product(gpu_device, n, F, H, slope):
+    """Activations that the slope moves are no bf16 numbers any more; they enter the product with 16 bits (two
+    bf16 numbers: half a step of half a step, 2^-16).  The output is off by that, by its sum of up to two
+    products a feature in 32 bits (2^-23 an addition) and by its own rounding, half a step of 2^-8."""
+    x = inputs(n, F, torch.bfloat16, gpu_device, seed=n, spread=0.5)
+    w = (torch.randn(H, F, generator=torch.Generator().manual_seed(H)) / F ** 0.5).to(gpu_device, torch.bfloat16)
+    xd, wd = x.double(), w.double()
+    act = torch.where(xd > 0, xd, torch.tensor(slope, dtype=torch.float32).double().item() * xd)
+    want = act @ wd.t()
+    off = (2.0 ** -16 + (2 * F + 8) * 2.0 ** -23) * (act.abs() @ wd.abs().t())
+    y = snn.linear_saved_int8(x, w, slope=slope).double()
+    assert bool(((y - want).abs() <= off + 2.0 ** -8 * (want.abs() + off) + 2.0 ** -134).all())
+
+
+@pytest.mark.parametrize("slope", [0.0, 0.2, 1.0])
+def test_infinite_bf16_activations(gpu_device, slope):
+    """In bf16 an infinity stays one on the way to the output, and what is beside it is what it was."""
+    x = inputs(70, 40, torch.bfloat16, gpu_device, seed=2)
+    w = (torch.randn(30, 40, generator=torch.Generator().manual_seed(1)) / 6 + 0.01).to(gpu_device, torch.bfloat16)
+    before = snn.linear_saved_int8(x, w, slope=slope)
+    x[5, 3], x[60, 39] = float("inf"), -float("inf")
+    y = snn.linear_saved_int8(x, w, slope=slope)
+    assert torch.equal(y[5].float(), float("inf") * torch.sign(w[:, 3].float()))
+    if slope:
+        assert torch.equal(y[60].float(), -float("inf") * torch.sign(w[:, 39].float()))
+    beside = [r for r in range(70) if r not in (5, 60)]
+    assert torch.equal(y[beside], before[beside])
