@@ -235,3 +235,29 @@ def test_rows_without_a_class_every_way(gpu_device, dtype, B, D, V, stored):
         w = w.t().contiguous().t()
     dx, dw, loss = check(x, w, labels, idx)
     assert bool((dx[dead] == 0).all()) and bool(torch.isfinite(dw).all()) and bool(torch.isfinite(loss))
+
+
+@pytest.mark.parametrize("dtype,B", [("bf16", 4), ("bf16", 70), ("f32", 4), ("f32", 70)])
+def test_weights_of_more_than_2_to_the_31_elements(gpu_device, dtype, B):
+    """8.5 million classes of 256 features.  All but 300 of them, at both ends and around element 2^31, are
+    masked by a large negative weight on a feature that is 1 (p is 0, exactly): losses and gradients are
+    those of the 300."""
+    t = DTYPES[dtype]
+    V, D = 8_500_000, 256
+    at = torch.cat([torch.arange(100), torch.arange(100) + 2 ** 31 // D - 50, torch.arange(100) + V - 100]).to(gpu_device)
+    x, w, labels = make(B, D, 300, t, gpu_device, seed=B)
+    x[:, 0], w[:, 0] = 1.0, 0.0
+    big = torch.zeros(V, D, dtype=t, device=gpu_device)
+    big[:, 0] = -2.0 ** 20
+    big[at] = w
+    labels[0] = 299
+    ref = reference(x, w, labels)
+    dx, dw = gradients(x, big, at[labels])
+    # a masked class adds an exact 0, so the sums' roundings are those of 300 classes and of joining up to 768
+    # workgroups' shares: within the (V / 4 + 1100) u of the bound for V = 300
+    rows = snn.class_cross_entropy(x, big, at[labels], reduction="none")
+    close(rows, ref["loss"], ref["loss_bound"], "row losses")
+    close(dx, ref["dx"], ref["dx_bound"], "dx")
+    close(dw[at], ref["dw"], ref["dw_bound"], "dweight")
+    dw[at] = 0
+    assert not bool(dw.any())

@@ -122,3 +122,39 @@ def test_infinite_bf16_activations(gpu_device, slope):
         assert torch.equal(y[60].float(), -float("inf") * torch.sign(w[:, 39].float()))
     beside = [r for r in range(70) if r not in (5, 60)]
     assert torch.equal(y[beside], before[beside])
+
+
+@pytest.mark.parametrize("slope", [0.2, 1.0])
+def test_activations_of_more_than_2_to_the_31_elements(gpu_device, slope):
+    """2.2 million rows of 1000 features in bf16: codes, values, outputs and gradients of the rows at the end
+    and around element 2^31 are those of these rows alone."""
+    n, F, H = 2_200_000, 1000, 8
+    x = torch.randn(n, F, device=gpu_device, dtype=torch.bfloat16)
+    w = torch.randn(H, F, device=gpu_device).bfloat16() / 32
+    grad = torch.randn(n, H, device=gpu_device).bfloat16()
+    parts = [slice(2 ** 31 // F - 40, 2 ** 31 // F + 40), slice(n - 70, n)]
+    saved = snn.save_int8(x, slope)
+    value = saved.restore()
+    act = saved.input_grad(x)
+    xs = x.requires_grad_()
+    y = snn.linear_saved_int8(xs, w, slope=slope)
+    (dx,) = torch.autograd.grad(y, xs, grad)
+    for at in parts:
+        own = x[at].detach().clone()
+        alone = snn.save_int8(own, slope)
+        assert torch.equal(saved.codes[at], alone.codes) and torch.equal(saved.steps[at], alone.steps)
+        assert torch.equal(value[at], alone.restore()) and torch.equal(act[at], alone.input_grad(own))
+        own.requires_grad_()
+        z = snn.linear_saved_int8(own, w, slope=slope)
+        # few rows share the features between wavefronts, so their sums have another order: (2 F + 8)
+        # additions of 2^-23 on either side and two roundings of half a step
+        near = 2 * (2 * F + 8) * 2.0 ** -23 * 2 * (own.detach().float().abs() @ w.float().abs().t()) + 2.0 ** -7 * z.abs()
+        assert bool(((y[at] - z).abs() <= near).all())
+        assert torch.equal(dx[at], torch.autograd.grad(z, own, grad[at])[0])
+    only = torch.zeros_like(grad)
+    for at in parts:
+        only[at] = grad[at]
+    want = sum(grad[at].double().t() @ value[at].double() for at in parts)
+    size = sum(grad[at].double().abs().t() @ value[at].double().abs() for at in parts)
+    got = saved.weight_grad(only).double()
+    assert bool(((got - want).abs() <= (3 * 150 + 1032) * 2.0 ** -23 * size + 2.0 ** -8 * want.abs()).all())
