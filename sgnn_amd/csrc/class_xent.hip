@@ -15,8 +15,8 @@
 // rounding, with that element rounded like the others by 2.1e-4.
 //
 // Bound by the matrix unit.  2048 x 602 against 10007 classes in fp32 (24.7 GFLOP a product, six bf16
-// products each): statistics 175 us, dz 164, dx 169, dweight 204, that is 0.73 to 0.90 PFLOP/s of the
-// 1.04 that a library product of bf16 matrices reaches.
+// products each): statistics 156 us, dz 148, the gradients' products 322 together, that is 0.92 to 1.00
+// PFLOP/s of the 1.04 (8192^3) to 1.34 (16384^3) that a library product of bf16 matrices reaches.
 #include "tile_product.h"
 
 namespace {
@@ -857,8 +857,8 @@ __global__ __launch_bounds__(kThreads) void k_few_join(int D, int rows, int spli
 //   owner x, stream weight:  statistics;  dx^T = weight^T . p
 //   owner weight, stream x:  dweight^T = x^T . dz
 // The step's rows are permuted within LDS so that neither way of reading meets bank conflicts.
-// 4096 x 256 against 50000 classes: statistics 118 us (0.89 PFLOP/s), dx 185 and dweight 243 us with their
-// own logits (1.13 and 0.86); 257 features, by the tiles with dz in memory, 967 us instead of 546.
+// 4096 x 256 against 50000 classes: statistics 105 us (1.00 PFLOP/s), dx 174 and dweight 225 us with their
+// own logits (1.21 and 0.93), 507 in all; 257 features, by the tiles with dz in memory, 983.
 constexpr int kOwnRows = 256;                    // of a workgroup: NB blocks of 32 a wavefront
 constexpr int kStreamRows = 64;                  // of a step
 
@@ -1125,7 +1125,8 @@ __device__ __forceinline__ void stream_gather_between(const char* tile, int sub,
 // (in dweight here; dx takes it in its last step).  The sums go to part[split][owned row][KD * 16] in
 // 32 bits or, with `out` (dweight from one split), times the mean's factor to where they belong.
 // A wavefront owns 32 rows: 64 (half the LDS reads, but one wavefront a SIMD instead of two) took
-// 58 + 58 us instead of 56 + 52 us at 1777 x 100 x 30011, and spilled at 256 features.
+// 58 + 58 us instead of 56 + 52 us at 1777 x 100 x 30011, and spilled at 256 features, where dweight's
+// kernel keeps 6 registers in scratch as it is (21 and 292 us with a factor for every row).
 constexpr int kGradThreads = 512;
 
 template <int KD, bool BY_CLASS, bool PER_ROW>

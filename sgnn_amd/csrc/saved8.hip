@@ -124,7 +124,7 @@ __device__ __forceinline__ void store_row(T* p, int left, const T (&v)[V]) {
 
 // A workgroup owns `rows` whole rows; `per_row` = lanes a row takes (a multiple of a group's
 // lanes, so that a group never leaves its wavefront's aligned block of lanes).
-// Bound by memory: 232965 x 256 fp32 saved in 71 us (301 MB, 4.2 TB/s) and restored in 60 us (5.0; a
+// Bound by memory: 232965 x 256 fp32 saved in 70 us (301 MB, 4.3 TB/s) and restored in 59 us (5.1; a
 // copy reaches 5.1).
 constexpr int kEltThreads = 256;
 
@@ -225,7 +225,7 @@ __global__ __launch_bounds__(kEltThreads) void k_input_grad8(int64_t n, int F, c
 // bf16 numbers (8 + 8 + 8 bits of its mantissa, cut off, not rounded, so the sum is exact), which
 // makes every product exact and the sums those of 32-bit arithmetic; bf16 grad takes one plane.
 // Chunks go to the workspace and are added in chunk order by a second launch.
-// Measured with its sum on 232965 x 602 fp32, 128 units: 147 us (codes and grad are 260 MB, 51 us; the
+// Measured with its sum on 232965 x 602 fp32, 128 units: 143 us (codes and grad are 260 MB, 51 us; the
 // matrix instructions of three planes 65 us, decoding and splitting as much again).  Two workgroups
 // of eight wavefronts on a compute unit take turns at these; at one, 227 us.  Staging one step
 // ahead into a second buffer saves a barrier a step and gains nothing (140 us instead of 137 without
@@ -438,7 +438,7 @@ __global__ __launch_bounds__(256) void k_weight_grad_sum8(int F, int64_t total, 
 // 0-3 and 8-11 of sixteen in the first half of the wavefront, the others in the second, so that a
 // load takes whole 32-byte pieces of a row.  The weight is split into bf16 planes on its way to LDS,
 // 64 features (of x, or units of grad) at a time, and serves the workgroup's rows.  Measured on
-// 232965 x 256 fp32 with 64 units: y and the codes 103 us (3.5 TB/s of the 360 MB it moves), dx 108 us
+// 232965 x 256 fp32 with 64 units: y and the codes 104 us (3.5 TB/s of the 360 MB it moves), dx 111 us
 // (in pieces of 32 bytes, without the way through LDS, 118 us);
 // with 64 rows a wavefront, so that a piece of the weight read from LDS serves two products, 114 and
 // 129 us: half the wavefronts wait for the same loads.

@@ -86,7 +86,7 @@ class SGConv(_GraphConvBase):
     only the linear map runs per forward, as in torch_geometric.
 
     ``checkpoint="int8"`` keeps the linear map's input for the backward pass in 8 bits
-    (``linear_saved_int8``)."""
+    (``linear_saved_int8``, whose outputs are NaN where an input is infinite)."""
 
     def __init__(self, in_channels, out_channels, K=1, cached=False, add_self_loops=True, bias=True,
                  reorder=True, checkpoint=None):
@@ -120,7 +120,8 @@ class SGConv(_GraphConvBase):
 class GCNConv(_GraphConvBase):
     """``A_hat (x W^T) + b`` — torch_geometric.nn.GCNConv as used at model/GCN.py:9-10.
 
-    ``checkpoint="int8"`` keeps the layer's input for the backward pass in 8 bits.  ``input_slope``
+    ``checkpoint="int8"`` keeps the layer's input for the backward pass in 8 bits
+    (``linear_saved_int8``, whose outputs are NaN where an input is infinite).  ``input_slope``
     folds the activation in front of the layer (model/GCN.py:15) into it: the layer takes the
     pre-activation and applies ``x if x > 0 else input_slope * x`` itself (1: none, 0: ReLU), so
     that nothing else of it has to be kept."""

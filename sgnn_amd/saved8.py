@@ -145,7 +145,8 @@ def _empty(n, F, device):
 
 
 def save_int8(x, slope=1.0):
-    """``x if x > 0 else slope * x`` in 8 bits (``slope`` 1: no activation, 0: ReLU)."""
+    """``x if x > 0 else slope * x`` in 8 bits (``slope`` 1: no activation, 0: ReLU).  A part of a backward
+    pass of one's own: neither it nor what is made of it is differentiable."""
     code = element_type(x, "the activation")
     if x.dim() != 2 or x.shape[1] == 0:
         raise ValueError(f"the activation must be a matrix with at least one column, got {tuple(x.shape)}")
@@ -198,7 +199,7 @@ def linear_saved_int8(x, weight, slope=1.0):
     input but the 8-bit codes for the backward pass.  The output and ``x``'s gradient are those of
     the full activation; the weight's gradient is formed from the codes (off by half a step of
     their group at most, element by element).  An infinite or NaN element makes its row's outputs
-    NaN.  Neither forward-mode nor second derivatives: autograd refuses both."""
+    NaN (in bfloat16 an infinity may stay one).  Neither forward-mode nor second derivatives: autograd refuses both."""
     code = element_type(x, "the input")
     if element_type(weight, "the weight") != code:
         raise TypeError(f"the input is {x.dtype}, the weight {weight.dtype}")
