@@ -87,7 +87,7 @@ def class_cross_entropy(x, weight, labels, idx=None, reduction="mean"):
     either gradient are 0.  ``reduction="mean"`` is the mean over the other rows (0 if there are
     none), ``"none"`` the loss of each row.  ``weight`` may be a transposed view (``Wt.t()``); its
     gradient comes in the same layout.  An infinite or NaN element makes the losses it takes part
-    in NaN or infinite."""
+    in NaN or infinite; in bfloat16 a class whose logit is -infinity has p = 0 instead."""
     if reduction not in ("mean", "none"):
         raise ValueError(f"reduction must be 'mean' or 'none', got {reduction!r}")
     if element_type(x, "x") != element_type(weight, "the weight"):

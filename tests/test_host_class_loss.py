@@ -73,3 +73,15 @@ def test_python_layer_needs_gpu_tensors():
 def test_stacked_heads_in_pieces_where_that_is_faster(B, D, V, pieces):
     from sgnn_amd.stacked import _piecewise_classes
     assert (V >= _piecewise_classes(B, D)) is pieces
+
+
+def test_rows_that_count_without_a_class_are_asked_for_in_the_type():
+    """SGNN_ALL_ROWS goes with fp32 alone; sizes and refusals are those of fp32 otherwise."""
+    from sgnn_amd._lib import ALL_ROWS, BF16, F32
+    lib = _lib()
+    for back in (0, 1):
+        assert (lib.sgnn_class_xent_workspace_bytes(F32 | ALL_ROWS, 100, 50, 5000, back)
+                == lib.sgnn_class_xent_workspace_bytes(F32, 100, 50, 5000, back) > 0)
+    assert forward(lib, dtype=BF16 | ALL_ROWS) == -4 and b"fp32 only" in lib.sgnn_last_error()
+    assert forward(lib, dtype=F32 | ALL_ROWS, B=0) == -1 and b"B > 0" in lib.sgnn_last_error()
+    assert forward(lib, dtype=2 | ALL_ROWS) == -1 and b"type" in lib.sgnn_last_error()
