@@ -158,3 +158,28 @@ def test_activations_of_more_than_2_to_the_31_elements(gpu_device, slope):
     size = sum(grad[at].double().abs().t() @ value[at].double().abs() for at in parts)
     got = saved.weight_grad(only).double()
     assert bool(((got - want).abs() <= (3 * 150 + 1032) * 2.0 ** -23 * size + 2.0 ** -8 * want.abs()).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("slope", [1.5, 7.0])
+def test_slopes_beyond_one(gpu_device, dtype, slope):
+    """Output and input gradient with a slope that enlarges: sums in 32 bits of up to six products a term,
+    the sum's error times the slope, one rounding (half a step of 2^-24 or 2^-8) of the result; bf16
+    activations with 16 bits."""
+    n, F, H = 700, 90, 40
+    x = inputs(n, F, dtype, gpu_device, seed=5, spread=0.5).requires_grad_()
+    g = torch.Generator().manual_seed(6)
+    w = (torch.randn(H, F, generator=g) / 9).to(gpu_device, dtype)
+    grad = torch.randn(n, H, generator=g).to(gpu_device, dtype)
+    half = 2.0 ** -24 if dtype == torch.float32 else 2.0 ** -8
+    y = snn.linear_saved_int8(x, w, slope=slope)
+    y.backward(grad)
+    xd, wd, gd = x.detach().double(), w.double(), grad.double()
+    factor = torch.where(xd > 0, torch.ones_like(xd), torch.full_like(xd, slope))
+    act = factor * xd
+    off = (2.0 ** -16 * (half > 2.0 ** -20) + 2.0 ** -24 + (6 * F + 20) * 2.0 ** -23) * (act.abs() @ wd.abs().t())
+    want = act @ wd.t()
+    assert bool(((y.detach().double() - want).abs() <= off + half * (want.abs() + off)).all())
+    want = (gd @ wd) * factor
+    off = (6 * H + 21) * 2.0 ** -23 * (gd.abs() @ wd.abs()) * factor
+    assert bool(((x.grad.double() - want).abs() <= off + half * (want.abs() + off)).all())
